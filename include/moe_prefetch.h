@@ -38,6 +38,11 @@
  *                           the reference's cache path stops at one token, 0007:114)
  *   moe_combine             the sum over k of the weighted expert rows (0009:697-703, order per 0009:355)
  *   moe_quant_rows          ggml's quantize_row_q8_K of the activations, in the form the matrix cores read
+ *   moe_route_scored        build_moe_ffn's other gatings: sigmoid scores, a selection bias, expert groups, weights
+ *                           renormalised or not and scaled (un-vendored upstream)
+ *   moe_block_norm          the norm before ffn_gate_inp, the norm after the block, the residual add and its scale
+ *                           (un-vendored upstream; the reference's lookahead names that norm, 0010:382-403)
+ *   moe_sample              llama.cpp's sampler chain over one row of logits per sequence (un-vendored upstream)
  * No counterpart in the reference: moe_host_alloc/free (the reference pins the model buffer
  * through ggml's CUDA_Host buffer type), moe_synth_* (seeded synthetic weights and inputs).
  */
@@ -66,6 +71,7 @@ extern "C" {
 
 #define MOE_DTYPE_F32  0    /* activation element types */
 #define MOE_DTYPE_BF16 1
+#define MOE_DTYPE_F16  2   /* moe_route_scored, moe_block_norm and moe_sample only */
 
 const char *moe_last_error(void);   /* message of the last failure on this thread */
 int moe_abi_version(void);
@@ -668,6 +674,130 @@ int moe_combine(const float *pair_rows, int n_tok, int K, int H, float *out, int
 #define MOE_BATCH_HOST_MAX_TOKENS 64
 int moe_decode_batch(moe_cache *c, const float *x, const float *bias, float *out, int n_tok, int32_t *ids_host,
                      void *stream);
+
+/* ---- around the expert products ----------------------------------------------
+ * Routing by scores, the norms on both sides of a block, and sampling.  The
+ * three calls below launch on `stream`, allocate nothing, keep nothing between
+ * calls and use no workspace: calls on several streams or threads at once and
+ * calls captured into HIP graphs are fine as long as their outputs are apart.
+ * Their pointers are of the current device.  Rows may lie apart: a row stride
+ * counts elements and is at least the row's length.  No alignment is asked for
+ * beyond the element's own; rows of 16-byte aligned vectors run faster. */
+
+/* The K experts of each token from its router logits:
+ *   s_e = sigmoid(l_e)  or  exp(l_e - max) / sum exp(l - max)
+ *   v_e = s_e + bias_e                                          (selection only)
+ *   with n_groups > 1 the experts form n_groups runs of E / n_groups; a group's
+ *   score is the sum of its best group_best v_e, and the top_groups best groups stay
+ *   ids = the K largest v_e left, the largest first; the lower id, or group, on a tie
+ *   w_k = scale * s_{ids[k]} / (renormalize ? sum of the K scores : 1)
+ * Scores and selection are computed in 64 bits, w rounded once.  An expert whose
+ * logit is -inf or NaN, or whose v_e is, is switched off: it scores 0 and is chosen,
+ * lower ids first and with weight 0, only where fewer than K experts are left, so
+ * that ids always holds K different experts.  (A group's switched-off experts do
+ * not count for its score; w is 0 where the sum is.)  A logit of +inf takes its row's
+ * whole softmax, shared by all such logits. */
+#define MOE_SCORE_SOFTMAX 0
+#define MOE_SCORE_SIGMOID 1
+#define MOE_ROUTE_SCORED_MAX_E 1024
+#define MOE_ROUTE_SCORED_MAX_K 64
+typedef struct {
+    const void *logits;       /* dev [n_tok][E], MOE_DTYPE_*, rows logits_stride apart */
+    int64_t logits_stride;
+    int32_t logits_type;
+    int32_t n_tok, E, K;      /* E <= MOE_ROUTE_SCORED_MAX_E, K <= min(E, MOE_ROUTE_SCORED_MAX_K); n_tok may be 0 */
+    int32_t score;            /* MOE_SCORE_* */
+    int32_t renormalize;
+    int32_t n_groups;         /* 1..64, divides E */
+    int32_t top_groups;       /* 1..n_groups, top_groups * (E / n_groups) >= K */
+    int32_t group_best;       /* 1 or 2, <= E / n_groups */
+    float scale;
+    const float *bias;        /* dev [E] or NULL */
+    const int32_t *table;     /* dev [E] or NULL: expert -> slot, as in moe_route */
+    int32_t dummy;            /* slot written when table is NULL */
+    int32_t *ids;             /* dev out [n_tok][K] */
+    float *w;                 /* dev out [n_tok][K] */
+    int32_t *slots;           /* dev out [n_tok][K] or NULL */
+    float *scores;            /* dev out [n_tok][E] s_e, or NULL */
+} moe_route_scored_desc;
+int moe_route_scored(const moe_route_scored_desc *d, void *stream);
+
+/* The residual stream between two blocks, per token:
+ *   b = sum of the token's n_sum branch rows, in order
+ *   p = N(b; post_weight, post_bias), or b without a post-norm
+ *   r = x + scale * act(gate) * p, or x without a branch
+ *   y = N(r; weight, bias)
+ *   N(z; g, c) = (z - mean z) / sqrt(mean (z - mean z)^2 + eps) * (g + weight_offset) + c    MOE_NORM_LAYER
+ *                z / sqrt(mean z^2 + eps) * (g + weight_offset) + c                          MOE_NORM_RMS
+ * in 32 bits; r is rounded to x's type where it is stored, y comes from the
+ * unrounded r.  Either r or y may overwrite x (same rows and type); no other
+ * overlap is allowed.  At least one of r and y is given. */
+#define MOE_NORM_RMS   0
+#define MOE_NORM_LAYER 1
+#define MOE_GATE_PLAIN   0
+#define MOE_GATE_SIGMOID 1
+#define MOE_BLOCK_NORM_MAX_H 16384
+typedef struct {
+    int32_t n_tok, H;         /* H <= MOE_BLOCK_NORM_MAX_H; n_tok may be 0 */
+    int32_t kind;             /* MOE_NORM_* */
+    const void *x;            /* dev [n_tok][H], x_type, rows x_stride apart */
+    int64_t x_stride;
+    int32_t x_type;           /* MOE_DTYPE_*: x's and r's */
+    const void *branch;       /* dev [n_tok][n_sum][H] or NULL, branch_type (MOE_DTYPE_F32 or x_type); a token's
+                                 rows branch_stride * n_sum apart, its n_sum rows branch_stride apart */
+    int64_t branch_stride;
+    int32_t branch_type, n_sum;
+    const void *gate;         /* dev or NULL, gate_type (MOE_DTYPE_F32 or x_type): element (t, h) at
+                                 t * gate_row_stride + h * gate_col_stride (0 or 1); gate_row_stride 0: one row
+                                 for every token */
+    int64_t gate_row_stride;
+    int32_t gate_col_stride, gate_type, gate_act;   /* MOE_GATE_* */
+    float scale, weight_offset, eps, post_eps;
+    const void *weight, *bias;            /* dev [H] or NULL (1 and 0; the offset applies to a given weight), weight_type */
+    const void *post_weight, *post_bias;  /* dev [H] or NULL, weight_type */
+    int32_t weight_type;      /* MOE_DTYPE_F32 or x_type */
+    int32_t post;             /* 1: norm after the block */
+    void *residual;           /* dev out [n_tok][H] r or NULL, x_type */
+    int64_t residual_stride;
+    void *y;                  /* dev out [n_tok][H] or NULL */
+    int64_t y_stride;
+    int32_t y_type;           /* MOE_DTYPE_F32 or x_type */
+} moe_block_norm_desc;
+int moe_block_norm(const moe_block_norm_desc *d, void *stream);
+
+/* The next token of each row of logits, from a given uniform number u in [0, 1):
+ *   e_i = exp((l_i - max l) / temperature), the tokens in descending order of l_i, the lower index first on a tie
+ *   top_k   the first top_k of them
+ *   top_p   of those the shortest run from the front whose mass is at least top_p of theirs
+ *   min_p   of those the ones with e_i >= min_p
+ *   token   the first of what is left whose running mass exceeds u times the mass of what is left
+ *   prob    its share of that mass
+ * A temperature that is not above 0 takes the first of the order (prob 1).  top_k
+ * outside 1..V-1, top_p not below 1 and min_p not above 0 cut nothing; a NaN among
+ * them cuts nothing; the first of the order always stays.  Logits of -inf and NaN
+ * are switched off; a row with nothing else gives token -1 and prob 0.  (Logits of
+ * +inf share a row's whole mass.)  u outside [0, 1) or NaN counts as the nearest end
+ * (NaN as 0).  Masses are integers of 62 - ceil(log2 V) fractional bits of exp computed
+ * in 64 bits, so sums are exact in any order: the same row gives the same token in any
+ * batch. */
+#define MOE_SAMPLE_MAX_V (1 << 20)
+typedef struct {
+    const void *logits;       /* dev [n_tok][V], MOE_DTYPE_*, rows logits_stride apart */
+    int64_t logits_stride;
+    int32_t logits_type;
+    int32_t n_tok, V;         /* V <= MOE_SAMPLE_MAX_V; n_tok may be 0 */
+    const float *u;           /* dev [n_tok] */
+    const float *temperature; /* dev [n_tok] or NULL: temperature_all */
+    const int32_t *top_k;     /* dev [n_tok] or NULL: top_k_all */
+    const float *top_p;       /* dev [n_tok] or NULL: top_p_all */
+    const float *min_p;       /* dev [n_tok] or NULL: min_p_all */
+    float temperature_all;
+    int32_t top_k_all;
+    float top_p_all, min_p_all;
+    int32_t *tokens;          /* dev out [n_tok] */
+    float *probs;             /* dev out [n_tok] or NULL */
+} moe_sample_desc;
+int moe_sample(const moe_sample_desc *d, void *stream);
 
 /* ---- slab pool behind the Python ExpertCache ------------------------------- */
 typedef struct moe_pool moe_pool;

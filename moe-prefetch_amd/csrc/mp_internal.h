@@ -309,6 +309,46 @@ hipError_t static_scratch(void **ptr);
 hipError_t launch_swiglu_quant(const float *y2, int P, int I, float *h_out, int n_h, uint16_t *q16, float *dx,
                                uint16_t *bs16, hipStream_t st);
 
+// Operators around the expert products; the fields are those of the descriptors of the same name in
+// moe_prefetch.h, checked by the caller.  Element types there and here: 0 f32, 1 bf16, 2 fp16.
+struct ScoredArgs {
+    const void *logits;
+    int64_t ld;
+    int type, n_tok, E, K, score, renorm, groups, top_groups, group_best;
+    float scale;
+    const float *bias;
+    const int32_t *table;
+    int32_t dummy;
+    int32_t *ids;
+    float *w;
+    int32_t *slots;
+    float *scores;
+};
+hipError_t launch_route_scored(const ScoredArgs &a, hipStream_t st);
+
+struct NormArgs {
+    int n_tok, H, kind, post, x_type, b_type, n_sum, gate_type, gate_act, w_type, y_type;
+    const void *x, *branch, *gate, *w, *c, *pw, *pc;
+    void *r, *y;
+    int64_t ldx, ldb, ldr, ldy, gate_row;
+    int gate_col;
+    float scale, offset, eps, post_eps;
+};
+hipError_t launch_block_norm(const NormArgs &a, hipStream_t st);
+
+struct SampleArgs {
+    const void *logits;
+    int64_t ld;
+    int type, n_tok, V;
+    const float *u, *temp, *top_p, *min_p;
+    const int32_t *top_k;
+    float temp_all, top_p_all, min_p_all;
+    int top_k_all;
+    int32_t *tokens;
+    float *probs;
+};
+hipError_t launch_sample(const SampleArgs &a, hipStream_t st);
+
 // ev (optional): [logits start, logits end, select start, select end]
 hipError_t launch_route(const RouteLaunch &l, hipStream_t st, hipEvent_t *ev = nullptr);
 hipError_t launch_experts(const ExpertArgs &a, hipStream_t st);

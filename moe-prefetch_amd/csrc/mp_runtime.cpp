@@ -3999,6 +3999,131 @@ int moe_decode_batch(moe_cache *c, const float *x, const float *bias, float *out
     return cache_step(c);
 }
 
+// ---- around the expert products -----------------------------------------------
+static bool dtype_ok(int t) { return t == MOE_DTYPE_F32 || t == MOE_DTYPE_BF16 || t == MOE_DTYPE_F16; }
+static bool aligned_to(const void *p, int type) { return (uintptr_t)p % (type == MOE_DTYPE_F32 ? 4 : 2) == 0; }
+
+// a scored routing's rule, apart from its buffers
+static int scored_check(const moe_route_scored_desc *d) {
+    if (d->E < 1 || d->E > MOE_ROUTE_SCORED_MAX_E)
+        return fail(MOE_ERR_ARG, "moe_route_scored: n_experts %d must be 1..%d", d->E, MOE_ROUTE_SCORED_MAX_E);
+    if (d->K < 1 || d->K > d->E || d->K > MOE_ROUTE_SCORED_MAX_K)
+        return fail(MOE_ERR_ARG, "moe_route_scored: n_expert_used %d must be 1..%d", d->K,
+                    std::min(d->E, (int32_t)MOE_ROUTE_SCORED_MAX_K));
+    if (d->score != MOE_SCORE_SOFTMAX && d->score != MOE_SCORE_SIGMOID)
+        return fail(MOE_ERR_ARG, "moe_route_scored: score %d unsupported", d->score);
+    if (d->n_groups < 1 || d->n_groups > 64 || d->E % d->n_groups)
+        return fail(MOE_ERR_ARG, "moe_route_scored: n_groups %d must be 1..64 and divide %d", d->n_groups, d->E);
+    const int m = d->E / d->n_groups;
+    if (d->top_groups < 1 || d->top_groups > d->n_groups || (int64_t)d->top_groups * m < d->K)
+        return fail(MOE_ERR_ARG, "moe_route_scored: top_groups %d must be 1..%d and hold %d experts", d->top_groups,
+                    d->n_groups, d->K);
+    if (d->group_best < 1 || d->group_best > 2 || d->group_best > m)
+        return fail(MOE_ERR_ARG, "moe_route_scored: group_best %d must be 1 or 2 and at most %d", d->group_best, m);
+    if (!(d->scale - d->scale == 0.0f)) return fail(MOE_ERR_ARG, "moe_route_scored: scale is not finite");
+    return MOE_OK;
+}
+
+int moe_route_scored(const moe_route_scored_desc *d, void *stream) {
+    if (!d) return fail(MOE_ERR_ARG, "moe_route_scored: null argument");
+    const int r = scored_check(d);
+    if (r != MOE_OK) return r;
+    if (d->n_tok < 0) return fail(MOE_ERR_ARG, "moe_route_scored: n_tok %d out of range", d->n_tok);
+    if (!dtype_ok(d->logits_type)) return fail(MOE_ERR_ARG, "moe_route_scored: logits_type %d unsupported", d->logits_type);
+    if (d->n_tok == 0) return MOE_OK;
+    if (!d->logits || !d->ids || !d->w) return fail(MOE_ERR_ARG, "moe_route_scored: null argument");
+    if (d->logits_stride < d->E)
+        return fail(MOE_ERR_ARG, "moe_route_scored: logits_stride %lld below n_experts", (long long)d->logits_stride);
+    if (!aligned_to(d->logits, d->logits_type) ||
+        ((uintptr_t)d->bias | (uintptr_t)d->table | (uintptr_t)d->ids | (uintptr_t)d->w | (uintptr_t)d->slots |
+         (uintptr_t)d->scores) % 4)
+        return fail(MOE_ERR_ARG, "moe_route_scored: misaligned pointer");
+    mp::ScoredArgs a{};
+    a.logits = d->logits; a.ld = d->logits_stride; a.type = d->logits_type;
+    a.n_tok = d->n_tok; a.E = d->E; a.K = d->K; a.score = d->score; a.renorm = d->renormalize;
+    a.groups = d->n_groups; a.top_groups = d->top_groups; a.group_best = d->group_best; a.scale = d->scale;
+    a.bias = d->bias; a.table = d->table; a.dummy = d->dummy;
+    a.ids = d->ids; a.w = d->w; a.slots = d->slots; a.scores = d->scores;
+    HIPCHK(mp::launch_route_scored(a, (hipStream_t)stream));
+    return MOE_OK;
+}
+
+int moe_block_norm(const moe_block_norm_desc *d, void *stream) {
+    if (!d) return fail(MOE_ERR_ARG, "moe_block_norm: null argument");
+    if (d->n_tok < 0) return fail(MOE_ERR_ARG, "moe_block_norm: n_tok %d out of range", d->n_tok);
+    if (d->H < 1 || d->H > MOE_BLOCK_NORM_MAX_H)
+        return fail(MOE_ERR_ARG, "moe_block_norm: hidden size %d must be 1..%d", d->H, MOE_BLOCK_NORM_MAX_H);
+    if (d->kind != MOE_NORM_RMS && d->kind != MOE_NORM_LAYER)
+        return fail(MOE_ERR_ARG, "moe_block_norm: kind %d unsupported", d->kind);
+    if (!dtype_ok(d->x_type)) return fail(MOE_ERR_ARG, "moe_block_norm: x_type %d unsupported", d->x_type);
+    auto of_x = [&](int t) { return t == MOE_DTYPE_F32 || t == d->x_type; };
+    if (!of_x(d->branch_type) || !of_x(d->gate_type) || !of_x(d->weight_type) || !of_x(d->y_type))
+        return fail(MOE_ERR_ARG, "moe_block_norm: branch, gate, weights and y are f32 or of x's type");
+    if (d->gate_act != MOE_GATE_PLAIN && d->gate_act != MOE_GATE_SIGMOID)
+        return fail(MOE_ERR_ARG, "moe_block_norm: gate_act %d unsupported", d->gate_act);
+    if (d->gate_col_stride != 0 && d->gate_col_stride != 1)
+        return fail(MOE_ERR_ARG, "moe_block_norm: gate_col_stride %d must be 0 or 1", d->gate_col_stride);
+    if (!(d->eps >= 0.0f) || !(d->post_eps >= 0.0f) || !(d->scale - d->scale == 0.0f) ||
+        !(d->weight_offset - d->weight_offset == 0.0f))
+        return fail(MOE_ERR_ARG, "moe_block_norm: eps below 0, or scale or weight_offset not finite");
+    if (!d->branch && (d->gate || d->post)) return fail(MOE_ERR_ARG, "moe_block_norm: a gate or post-norm without a branch");
+    if (d->branch && (d->n_sum < 1 || d->n_sum > MOE_ROUTE_SCORED_MAX_K))
+        return fail(MOE_ERR_ARG, "moe_block_norm: n_sum %d must be 1..%d", d->n_sum, MOE_ROUTE_SCORED_MAX_K);
+    if (!d->post && (d->post_weight || d->post_bias))
+        return fail(MOE_ERR_ARG, "moe_block_norm: post-norm weights without a post-norm");
+    if (d->n_tok == 0) return MOE_OK;
+    if (!d->x || (!d->residual && !d->y)) return fail(MOE_ERR_ARG, "moe_block_norm: null argument");
+    if (d->residual && d->residual == d->y) return fail(MOE_ERR_ARG, "moe_block_norm: residual and y are the same memory");
+    if ((d->residual == d->x && d->residual_stride != d->x_stride) ||
+        (d->y == d->x && (d->y_stride != d->x_stride || d->y_type != d->x_type)))
+        return fail(MOE_ERR_ARG, "moe_block_norm: an output over x needs x's stride and type");
+    if (d->x_stride < d->H || (d->branch && d->branch_stride < d->H) || (d->residual && d->residual_stride < d->H) ||
+        (d->y && d->y_stride < d->H))
+        return fail(MOE_ERR_ARG, "moe_block_norm: a row stride below the hidden size");
+    if (d->gate && (d->gate_row_stride < 0 || (d->gate_row_stride && d->gate_col_stride && d->gate_row_stride < d->H)))
+        return fail(MOE_ERR_ARG, "moe_block_norm: gate_row_stride %lld", (long long)d->gate_row_stride);
+    if (!aligned_to(d->x, d->x_type) || !aligned_to(d->branch, d->branch_type) || !aligned_to(d->gate, d->gate_type) ||
+        !aligned_to(d->weight, d->weight_type) || !aligned_to(d->bias, d->weight_type) ||
+        !aligned_to(d->post_weight, d->weight_type) || !aligned_to(d->post_bias, d->weight_type) ||
+        !aligned_to(d->residual, d->x_type) || !aligned_to(d->y, d->y_type))
+        return fail(MOE_ERR_ARG, "moe_block_norm: misaligned pointer");
+    mp::NormArgs a{};
+    a.n_tok = d->n_tok; a.H = d->H; a.kind = d->kind; a.post = d->post != 0;
+    a.x_type = d->x_type; a.b_type = d->branch_type; a.gate_type = d->gate_type; a.w_type = d->weight_type;
+    a.y_type = d->y_type; a.n_sum = d->n_sum; a.gate_act = d->gate_act;
+    a.x = d->x; a.branch = d->branch; a.gate = d->gate;
+    a.w = d->weight; a.c = d->bias; a.pw = d->post_weight; a.pc = d->post_bias;
+    a.r = d->residual; a.y = d->y;
+    a.ldx = d->x_stride; a.ldb = d->branch_stride; a.ldr = d->residual_stride; a.ldy = d->y_stride;
+    a.gate_row = d->gate_row_stride; a.gate_col = d->gate_col_stride;
+    a.scale = d->scale; a.offset = d->weight_offset; a.eps = d->eps; a.post_eps = d->post_eps;
+    HIPCHK(mp::launch_block_norm(a, (hipStream_t)stream));
+    return MOE_OK;
+}
+
+int moe_sample(const moe_sample_desc *d, void *stream) {
+    if (!d) return fail(MOE_ERR_ARG, "moe_sample: null argument");
+    if (d->n_tok < 0) return fail(MOE_ERR_ARG, "moe_sample: n_tok %d out of range", d->n_tok);
+    if (d->V < 1 || d->V > MOE_SAMPLE_MAX_V)
+        return fail(MOE_ERR_ARG, "moe_sample: vocabulary %d must be 1..%d", d->V, MOE_SAMPLE_MAX_V);
+    if (!dtype_ok(d->logits_type)) return fail(MOE_ERR_ARG, "moe_sample: logits_type %d unsupported", d->logits_type);
+    if (d->n_tok == 0) return MOE_OK;
+    if (!d->logits || !d->u || !d->tokens) return fail(MOE_ERR_ARG, "moe_sample: null argument");
+    if (d->logits_stride < d->V)
+        return fail(MOE_ERR_ARG, "moe_sample: logits_stride %lld below the vocabulary", (long long)d->logits_stride);
+    if (!aligned_to(d->logits, d->logits_type) ||
+        ((uintptr_t)d->u | (uintptr_t)d->temperature | (uintptr_t)d->top_k | (uintptr_t)d->top_p | (uintptr_t)d->min_p |
+         (uintptr_t)d->tokens | (uintptr_t)d->probs) % 4)
+        return fail(MOE_ERR_ARG, "moe_sample: misaligned pointer");
+    mp::SampleArgs a{};
+    a.logits = d->logits; a.ld = d->logits_stride; a.type = d->logits_type; a.n_tok = d->n_tok; a.V = d->V;
+    a.u = d->u; a.temp = d->temperature; a.top_k = d->top_k; a.top_p = d->top_p; a.min_p = d->min_p;
+    a.temp_all = d->temperature_all; a.top_k_all = d->top_k_all; a.top_p_all = d->top_p_all; a.min_p_all = d->min_p_all;
+    a.tokens = d->tokens; a.probs = d->probs;
+    HIPCHK(mp::launch_sample(a, (hipStream_t)stream));
+    return MOE_OK;
+}
+
 // ---- slab pool --------------------------------------------------------------
 int moe_pool_create(int n_layers, int capacity, size_t bytes_per_expert, int device, moe_pool **out) {
     if (!out || n_layers <= 0 || capacity <= 0 || bytes_per_expert == 0) return fail(MOE_ERR_ARG, "bad arguments");

@@ -4,12 +4,20 @@ Drop-in surfaces of the reference's Python prototypes:
   ExpertCache      (src/prefetch_engine.py)
   ExpertPredictor  (src/predictor.py)
 The engine itself (the llama-moecache runtime and the expert kernels) is
-MoeCache; all of it calls libmoeprefetch.so through its C ABI.
+MoeCache; around its expert products stand ScoredRouter, BlockNorm and
+Sampler (block.py); all of it calls libmoeprefetch.so through its C ABI.
 """
 from ._lib import MoeError, TYPE_Q4K, TYPE_Q6K, lib
 from .engine import MoeCache, parse_slot_profile
 from .predictor import ExpertPredictor
 from .prefetch_engine import ExpertCache
 
-__all__ = ["ExpertCache", "ExpertPredictor", "MoeCache", "MoeError", "TYPE_Q4K", "TYPE_Q6K",
-           "lib", "parse_slot_profile"]
+__all__ = ["BlockNorm", "ExpertCache", "ExpertPredictor", "MoeCache", "MoeError", "Sampler", "ScoredRouter",
+           "TYPE_Q4K", "TYPE_Q6K", "lib", "parse_slot_profile"]
+
+
+def __getattr__(name):                # these need torch, which the rest of the package does not import
+    if name in ("BlockNorm", "Sampler", "ScoredRouter"):
+        from . import block
+        return getattr(block, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -12,7 +12,10 @@ LIB_PATH = os.path.join(HERE, "libmoeprefetch.so")
 MOE_OK = 0
 MOE_ERR_ARG, MOE_ERR_HIP, MOE_ERR_NOMEM, MOE_ERR_STATE = -1, -2, -3, -4
 TYPE_Q4K, TYPE_Q6K = 12, 14
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+SCORE = {"softmax": 0, "sigmoid": 1}
+NORM = {"rms": 0, "layer": 1}
+GATE_ACT = {None: 0, "sigmoid": 1}
 # the static workspace of moe_grouped_experts_static (MOE_GROUPED_STATIC_SCRATCH_BYTES)
 GROUPED_STATIC_SCRATCH_BYTES = 16 << 20
 ADMIT = {"off": 0, "heat": 1, "window": 2}
@@ -20,6 +23,7 @@ PUBLISH = {"fifo": 0, "sorted": 1, "live": 2}
 
 P = ctypes.c_void_p
 I32 = ctypes.c_int32
+I64 = ctypes.c_int64
 U64 = ctypes.c_uint64
 F32 = ctypes.c_float
 SZ = ctypes.c_size_t
@@ -51,6 +55,28 @@ class GroupedDesc(ctypes.Structure):
                 ("store", P), ("expert_bytes", U64), ("n_store", I32),
                 ("out", P), ("accumulate", I32), ("pair_out", P), ("h_out", P), ("workspace", P),
                 ("kernel_ms", P), ("shared", P)]
+
+
+class RouteScoredDesc(ctypes.Structure):
+    _fields_ = [("logits", P), ("logits_stride", I64), ("logits_type", I32), ("n_tok", I32), ("E", I32), ("K", I32),
+                ("score", I32), ("renormalize", I32), ("n_groups", I32), ("top_groups", I32), ("group_best", I32),
+                ("scale", F32), ("bias", P), ("table", P), ("dummy", I32), ("ids", P), ("w", P), ("slots", P),
+                ("scores", P)]
+
+
+class BlockNormDesc(ctypes.Structure):
+    _fields_ = [("n_tok", I32), ("H", I32), ("kind", I32), ("x", P), ("x_stride", I64), ("x_type", I32),
+                ("branch", P), ("branch_stride", I64), ("branch_type", I32), ("n_sum", I32),
+                ("gate", P), ("gate_row_stride", I64), ("gate_col_stride", I32), ("gate_type", I32), ("gate_act", I32),
+                ("scale", F32), ("weight_offset", F32), ("eps", F32), ("post_eps", F32),
+                ("weight", P), ("bias", P), ("post_weight", P), ("post_bias", P), ("weight_type", I32), ("post", I32),
+                ("residual", P), ("residual_stride", I64), ("y", P), ("y_stride", I64), ("y_type", I32)]
+
+
+class SampleDesc(ctypes.Structure):
+    _fields_ = [("logits", P), ("logits_stride", I64), ("logits_type", I32), ("n_tok", I32), ("V", I32), ("u", P),
+                ("temperature", P), ("top_k", P), ("top_p", P), ("min_p", P), ("temperature_all", F32),
+                ("top_k_all", I32), ("top_p_all", F32), ("min_p_all", F32), ("tokens", P), ("probs", P)]
 
 
 class CacheConfig(ctypes.Structure):
@@ -228,6 +254,9 @@ SIGNATURES = {
     "moe_grouped_experts": (ctypes.c_int, [ctypes.POINTER(GroupedDesc), P]),
     "moe_grouped_plan": (ctypes.c_int, [ctypes.c_int] * 8 + [P]),
     "moe_grouped_experts_static": (ctypes.c_int, [ctypes.POINTER(GroupedDesc), P]),
+    "moe_route_scored": (ctypes.c_int, [ctypes.POINTER(RouteScoredDesc), P]),
+    "moe_block_norm": (ctypes.c_int, [ctypes.POINTER(BlockNormDesc), P]),
+    "moe_sample": (ctypes.c_int, [ctypes.POINTER(SampleDesc), P]),
     "moe_combine": (ctypes.c_int, [P, ctypes.c_int, ctypes.c_int, ctypes.c_int, P, ctypes.c_int, P]),
     "moe_pool_create": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, SZ, ctypes.c_int, ctypes.POINTER(P)]),
     "moe_pool_destroy": (ctypes.c_int, [P]),
