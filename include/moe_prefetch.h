@@ -677,9 +677,9 @@ int moe_decode_batch(moe_cache *c, const float *x, const float *bias, float *out
 
 /* ---- around the expert products ----------------------------------------------
  * Routing by scores, the norms on both sides of a block, and sampling.  The
- * three calls below launch on `stream`, allocate nothing, keep nothing between
- * calls and use no workspace: calls on several streams or threads at once and
- * calls captured into HIP graphs are fine as long as their outputs are apart.
+ * three calls below launch on `stream`, allocate nothing and keep nothing between
+ * calls: calls on several streams or threads at once and calls captured into HIP
+ * graphs are fine as long as their outputs, and moe_sample's workspaces, are apart.
  * Their pointers are of the current device.  Rows may lie apart: a row stride
  * counts elements and is at least the row's length.  No alignment is asked for
  * beyond the element's own; rows of 16-byte aligned vectors run faster. */
@@ -697,6 +697,7 @@ int moe_decode_batch(moe_cache *c, const float *x, const float *bias, float *out
  * that ids always holds K different experts.  (A group's switched-off experts do
  * not count for its score; w is 0 where the sum is.)  A logit of +inf takes its row's
  * whole softmax, shared by all such logits. */
+#define MOE_BLOCK_MAX_TOKENS (1 << 20)
 #define MOE_SCORE_SOFTMAX 0
 #define MOE_SCORE_SIGMOID 1
 #define MOE_ROUTE_SCORED_MAX_E 1024
@@ -705,7 +706,8 @@ typedef struct {
     const void *logits;       /* dev [n_tok][E], MOE_DTYPE_*, rows logits_stride apart */
     int64_t logits_stride;
     int32_t logits_type;
-    int32_t n_tok, E, K;      /* E <= MOE_ROUTE_SCORED_MAX_E, K <= min(E, MOE_ROUTE_SCORED_MAX_K); n_tok may be 0 */
+    int32_t n_tok, E, K;      /* n_tok 0..MOE_BLOCK_MAX_TOKENS, E <= MOE_ROUTE_SCORED_MAX_E,
+                                 K <= min(E, MOE_ROUTE_SCORED_MAX_K) */
     int32_t score;            /* MOE_SCORE_* */
     int32_t renormalize;
     int32_t n_groups;         /* 1..64, divides E */
@@ -738,7 +740,7 @@ int moe_route_scored(const moe_route_scored_desc *d, void *stream);
 #define MOE_GATE_SIGMOID 1
 #define MOE_BLOCK_NORM_MAX_H 16384
 typedef struct {
-    int32_t n_tok, H;         /* H <= MOE_BLOCK_NORM_MAX_H; n_tok may be 0 */
+    int32_t n_tok, H;         /* n_tok 0..MOE_BLOCK_MAX_TOKENS, H <= MOE_BLOCK_NORM_MAX_H */
     int32_t kind;             /* MOE_NORM_* */
     const void *x;            /* dev [n_tok][H], x_type, rows x_stride apart */
     int64_t x_stride;
@@ -776,16 +778,16 @@ int moe_block_norm(const moe_block_norm_desc *d, void *stream);
  * outside 1..V-1, top_p not below 1 and min_p not above 0 cut nothing; a NaN among
  * them cuts nothing; the first of the order always stays.  Logits of -inf and NaN
  * are switched off; a row with nothing else gives token -1 and prob 0.  (Logits of
- * +inf share a row's whole mass.)  u outside [0, 1) or NaN counts as the nearest end
- * (NaN as 0).  Masses are integers of 62 - ceil(log2 V) fractional bits of exp computed
- * in 64 bits, so sums are exact in any order: the same row gives the same token in any
- * batch. */
+ * +inf share a row's whole mass.)  u of 1 and above counts as the largest number
+ * below 1, u below 0 and NaN as 0.  Masses and their sums are computed in 64 bits, in an order that the row
+ * alone decides: the same row gives the same token in any batch. */
 #define MOE_SAMPLE_MAX_V (1 << 20)
+#define MOE_SAMPLE_MAX_TOKENS 65535
 typedef struct {
     const void *logits;       /* dev [n_tok][V], MOE_DTYPE_*, rows logits_stride apart */
     int64_t logits_stride;
     int32_t logits_type;
-    int32_t n_tok, V;         /* V <= MOE_SAMPLE_MAX_V; n_tok may be 0 */
+    int32_t n_tok, V;         /* n_tok 0..MOE_SAMPLE_MAX_TOKENS, V <= MOE_SAMPLE_MAX_V */
     const float *u;           /* dev [n_tok] */
     const float *temperature; /* dev [n_tok] or NULL: temperature_all */
     const int32_t *top_k;     /* dev [n_tok] or NULL: top_k_all */
@@ -796,7 +798,9 @@ typedef struct {
     float top_p_all, min_p_all;
     int32_t *tokens;          /* dev out [n_tok] */
     float *probs;             /* dev out [n_tok] or NULL */
+    void *workspace;          /* dev, moe_sample_workspace_bytes(), 8-byte aligned; nothing in it outlives the call */
 } moe_sample_desc;
+size_t moe_sample_workspace_bytes(int n_tok, int V);
 int moe_sample(const moe_sample_desc *d, void *stream);
 
 /* ---- slab pool behind the Python ExpertCache ------------------------------- */

@@ -346,8 +346,11 @@ struct SampleArgs {
     int top_k_all;
     int32_t *tokens;
     float *probs;
+    int slices, cap, keep;      // set by the launcher, and the workspace's parts
+    void *heads, *lists;
 };
-hipError_t launch_sample(const SampleArgs &a, hipStream_t st);
+size_t sample_ws_bytes(int n_tok, int V);
+hipError_t launch_sample(SampleArgs a, void *ws, hipStream_t st);
 
 // ev (optional): [logits start, logits end, select start, select end]
 hipError_t launch_route(const RouteLaunch &l, hipStream_t st, hipEvent_t *ev = nullptr);

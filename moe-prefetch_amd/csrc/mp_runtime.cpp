@@ -4028,7 +4028,8 @@ int moe_route_scored(const moe_route_scored_desc *d, void *stream) {
     if (!d) return fail(MOE_ERR_ARG, "moe_route_scored: null argument");
     const int r = scored_check(d);
     if (r != MOE_OK) return r;
-    if (d->n_tok < 0) return fail(MOE_ERR_ARG, "moe_route_scored: n_tok %d out of range", d->n_tok);
+    if (d->n_tok < 0 || d->n_tok > MOE_BLOCK_MAX_TOKENS)
+        return fail(MOE_ERR_ARG, "moe_route_scored: n_tok %d out of range", d->n_tok);
     if (!dtype_ok(d->logits_type)) return fail(MOE_ERR_ARG, "moe_route_scored: logits_type %d unsupported", d->logits_type);
     if (d->n_tok == 0) return MOE_OK;
     if (!d->logits || !d->ids || !d->w) return fail(MOE_ERR_ARG, "moe_route_scored: null argument");
@@ -4050,7 +4051,8 @@ int moe_route_scored(const moe_route_scored_desc *d, void *stream) {
 
 int moe_block_norm(const moe_block_norm_desc *d, void *stream) {
     if (!d) return fail(MOE_ERR_ARG, "moe_block_norm: null argument");
-    if (d->n_tok < 0) return fail(MOE_ERR_ARG, "moe_block_norm: n_tok %d out of range", d->n_tok);
+    if (d->n_tok < 0 || d->n_tok > MOE_BLOCK_MAX_TOKENS)
+        return fail(MOE_ERR_ARG, "moe_block_norm: n_tok %d out of range", d->n_tok);
     if (d->H < 1 || d->H > MOE_BLOCK_NORM_MAX_H)
         return fail(MOE_ERR_ARG, "moe_block_norm: hidden size %d must be 1..%d", d->H, MOE_BLOCK_NORM_MAX_H);
     if (d->kind != MOE_NORM_RMS && d->kind != MOE_NORM_LAYER)
@@ -4101,26 +4103,31 @@ int moe_block_norm(const moe_block_norm_desc *d, void *stream) {
     return MOE_OK;
 }
 
+size_t moe_sample_workspace_bytes(int n_tok, int V) {
+    return n_tok < 1 || V < 1 || V > MOE_SAMPLE_MAX_V ? 0 : mp::sample_ws_bytes(n_tok, V);
+}
+
 int moe_sample(const moe_sample_desc *d, void *stream) {
     if (!d) return fail(MOE_ERR_ARG, "moe_sample: null argument");
-    if (d->n_tok < 0) return fail(MOE_ERR_ARG, "moe_sample: n_tok %d out of range", d->n_tok);
+    if (d->n_tok < 0 || d->n_tok > MOE_SAMPLE_MAX_TOKENS)
+        return fail(MOE_ERR_ARG, "moe_sample: n_tok %d out of range", d->n_tok);
     if (d->V < 1 || d->V > MOE_SAMPLE_MAX_V)
         return fail(MOE_ERR_ARG, "moe_sample: vocabulary %d must be 1..%d", d->V, MOE_SAMPLE_MAX_V);
     if (!dtype_ok(d->logits_type)) return fail(MOE_ERR_ARG, "moe_sample: logits_type %d unsupported", d->logits_type);
     if (d->n_tok == 0) return MOE_OK;
-    if (!d->logits || !d->u || !d->tokens) return fail(MOE_ERR_ARG, "moe_sample: null argument");
+    if (!d->logits || !d->u || !d->tokens || !d->workspace) return fail(MOE_ERR_ARG, "moe_sample: null argument");
     if (d->logits_stride < d->V)
         return fail(MOE_ERR_ARG, "moe_sample: logits_stride %lld below the vocabulary", (long long)d->logits_stride);
     if (!aligned_to(d->logits, d->logits_type) ||
         ((uintptr_t)d->u | (uintptr_t)d->temperature | (uintptr_t)d->top_k | (uintptr_t)d->top_p | (uintptr_t)d->min_p |
-         (uintptr_t)d->tokens | (uintptr_t)d->probs) % 4)
+         (uintptr_t)d->tokens | (uintptr_t)d->probs) % 4 || (uintptr_t)d->workspace % 8)
         return fail(MOE_ERR_ARG, "moe_sample: misaligned pointer");
     mp::SampleArgs a{};
     a.logits = d->logits; a.ld = d->logits_stride; a.type = d->logits_type; a.n_tok = d->n_tok; a.V = d->V;
     a.u = d->u; a.temp = d->temperature; a.top_k = d->top_k; a.top_p = d->top_p; a.min_p = d->min_p;
     a.temp_all = d->temperature_all; a.top_k_all = d->top_k_all; a.top_p_all = d->top_p_all; a.min_p_all = d->min_p_all;
     a.tokens = d->tokens; a.probs = d->probs;
-    HIPCHK(mp::launch_sample(a, (hipStream_t)stream));
+    HIPCHK(mp::launch_sample(a, d->workspace, (hipStream_t)stream));
     return MOE_OK;
 }
 

@@ -76,7 +76,7 @@ class BlockNormDesc(ctypes.Structure):
 class SampleDesc(ctypes.Structure):
     _fields_ = [("logits", P), ("logits_stride", I64), ("logits_type", I32), ("n_tok", I32), ("V", I32), ("u", P),
                 ("temperature", P), ("top_k", P), ("top_p", P), ("min_p", P), ("temperature_all", F32),
-                ("top_k_all", I32), ("top_p_all", F32), ("min_p_all", F32), ("tokens", P), ("probs", P)]
+                ("top_k_all", I32), ("top_p_all", F32), ("min_p_all", F32), ("tokens", P), ("probs", P), ("workspace", P)]
 
 
 class CacheConfig(ctypes.Structure):
@@ -256,6 +256,7 @@ SIGNATURES = {
     "moe_grouped_experts_static": (ctypes.c_int, [ctypes.POINTER(GroupedDesc), P]),
     "moe_route_scored": (ctypes.c_int, [ctypes.POINTER(RouteScoredDesc), P]),
     "moe_block_norm": (ctypes.c_int, [ctypes.POINTER(BlockNormDesc), P]),
+    "moe_sample_workspace_bytes": (SZ, [ctypes.c_int, ctypes.c_int]),
     "moe_sample": (ctypes.c_int, [ctypes.POINTER(SampleDesc), P]),
     "moe_combine": (ctypes.c_int, [P, ctypes.c_int, ctypes.c_int, ctypes.c_int, P, ctypes.c_int, P]),
     "moe_pool_create": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, SZ, ctypes.c_int, ctypes.POINTER(P)]),

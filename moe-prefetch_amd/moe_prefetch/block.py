@@ -289,5 +289,7 @@ class Sampler:
         tokens = _out(tokens, (T,), torch.int32, dev, "tokens", stream)
         probs = _out(probs, (T,), f32, dev, "probs", stream)
         d.tokens, d.probs = tokens.data_ptr(), probs.data_ptr()
+        ws = _empty((lib().moe_sample_workspace_bytes(T, self.V),), torch.uint8, dev, stream)
+        d.workspace = ws.data_ptr()
         _call(lib().moe_sample, d, dev, stream, "moe_sample")
         return tokens, probs

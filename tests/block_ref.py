@@ -128,7 +128,7 @@ def sample(l, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
             e = e[:max(1, int((e >= mp).sum()))]
         c = np.cumsum(e)
         uu = float(np.float32(u[t]))
-        uu = uu if uu > 0 else 0.0
-        j = min(int(np.searchsorted(c, uu * c[-1], side="right")), int((e > 0).sum()) - 1)
+        uu = min(uu, 1.0 - 2.0 ** -24) if uu > 0 else 0.0
+        j = int(np.searchsorted(c, uu * c[-1], side="right"))
         tokens[t], probs[t] = order[j], e[j] / c[-1]
     return tokens, probs

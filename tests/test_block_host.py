@@ -27,7 +27,7 @@ def scored(**kw):
     dict(E=0), dict(E=1025), dict(K=0), dict(K=65), dict(E=5, K=6), dict(score=2), dict(n_groups=0), dict(n_groups=65),
     dict(n_groups=5), dict(top_groups=0), dict(top_groups=2), dict(n_groups=16, top_groups=1), dict(group_best=0),
     dict(group_best=3), dict(n_groups=64, top_groups=64, group_best=2), dict(scale=float("inf")),
-    dict(scale=float("nan")), dict(n_tok=-1), dict(logits_type=3), dict(logits=None), dict(ids=None), dict(w=None),
+    dict(scale=float("nan")), dict(n_tok=-1), dict(n_tok=(1 << 20) + 1), dict(logits_type=3), dict(logits=None), dict(ids=None), dict(w=None),
     dict(logits_stride=63), dict(logits=PTR + 2), dict(logits_type=1, logits=PTR + 1), dict(ids=PTR + 2),
     dict(bias=PTR + 1), dict(table=PTR + 2), dict(slots=PTR + 3), dict(scores=PTR + 1)])
 def test_scored_refusals(bad):
@@ -44,7 +44,7 @@ def norm(**kw):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(n_tok=-1), dict(H=0), dict(H=16385), dict(kind=2), dict(x_type=3), dict(branch_type=2), dict(gate_type=2),
+    dict(n_tok=-1), dict(n_tok=(1 << 20) + 1), dict(H=0), dict(H=16385), dict(kind=2), dict(x_type=3), dict(branch_type=2), dict(gate_type=2),
     dict(weight_type=2), dict(y_type=2), dict(gate_act=2), dict(gate_col_stride=2), dict(eps=-1.0),
     dict(eps=float("nan")), dict(post_eps=-1.0), dict(scale=float("inf")), dict(weight_offset=float("nan")),
     dict(branch=None, gate=PTR), dict(branch=None, post=1), dict(n_sum=0), dict(n_sum=65), dict(post_weight=PTR),
@@ -60,16 +60,16 @@ def test_norm_refusals(bad):
 
 def sample(**kw):
     d = dict(logits=PTR, logits_stride=100, logits_type=0, n_tok=2, V=100, u=PTR, temperature_all=1.0, top_p_all=1.0,
-             tokens=PTR)
+             tokens=PTR, workspace=PTR)
     d.update(kw)
     return L.moe_sample(ctypes.byref(_lib.SampleDesc(**d)), None)
 
 
 @pytest.mark.parametrize("bad", [
-    dict(n_tok=-1), dict(V=0), dict(V=(1 << 20) + 1), dict(logits_type=-1), dict(logits=None), dict(u=None),
+    dict(n_tok=-1), dict(n_tok=65536), dict(V=0), dict(V=(1 << 20) + 1), dict(logits_type=-1), dict(logits=None), dict(u=None),
     dict(tokens=None), dict(logits_stride=99), dict(logits=PTR + 2), dict(logits_type=2, logits=PTR + 1),
     dict(u=PTR + 1), dict(temperature=PTR + 2), dict(top_k=PTR + 2), dict(top_p=PTR + 2), dict(min_p=PTR + 2),
-    dict(tokens=PTR + 2), dict(probs=PTR + 2)])
+    dict(tokens=PTR + 2), dict(probs=PTR + 2), dict(workspace=None), dict(workspace=PTR + 4)])
 def test_sample_refusals(bad):
     assert sample(**bad) == _lib.MOE_ERR_ARG
     assert b"moe_sample" in L.moe_last_error()
