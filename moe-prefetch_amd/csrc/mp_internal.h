@@ -347,7 +347,8 @@ struct SampleArgs {
     int32_t *tokens;
     float *probs;
     int slices, cap, keep;      // set by the launcher, and the workspace's parts
-    void *heads, *lists;
+    void *heads, *lists, *rest;
+    uint32_t *n_rest;
 };
 size_t sample_ws_bytes(int n_tok, int V);
 hipError_t launch_sample(SampleArgs a, void *ws, hipStream_t st);

@@ -1,5 +1,19 @@
 // mp_sample.hip -- the next token of a row of logits (moe_sample): temperature,
 // top-k, top-p, min-p and the draw from a given uniform number.
+//
+// With e_i = exp((l_i - max) / temperature) and the tokens in descending order (the
+// lower index first), every cut keeps a front part of that order, and the draw takes
+// the first token whose running mass exceeds u times the mass kept.  So what is
+// needed is a front part of the order long enough to decide, and the whole row's
+// mass where top-k does not bound it; the row itself is read once:
+//   1 slice   one wave per 4,096 logits of a row, in registers: the maximum, the
+//             candidates (every logit from a bound on) and, if the mass counts, its sum
+//   2 pick    one workgroup per row: the order is complete down to the highest of
+//             the slices' bounds; sorts that, cuts, draws
+//   3 rest    rows that step 2 could not decide (a flat distribution: the cut or the
+//             draw lies behind the candidates): a histogram of counts and masses by
+//             several workgroups, the last of which reads the one bin that matters.
+//             Rows of one value or nearly so end in a radix search (locate).
 #include <hip/hip_runtime.h>
 
 #include "mp_device.h"
@@ -10,7 +24,28 @@ namespace mp {
 
 constexpr int SMP_THREADS = 1024, SMP_WAVES = SMP_THREADS / 64;
 constexpr int SMP_BINS = 2048;
-constexpr int SMP_LIST = 2048;                        // candidates that one row's workgroup sorts
+constexpr int SMP_LIST = 2048;                        // tokens that a workgroup sorts
+constexpr int SLICE_WAVES = 4, SLICE_EPT = 64, SLICE = 64 * SLICE_EPT, SLICES_MAX = 256;
+constexpr int REST_PARTS = 8, REST_GRID = 256;
+
+// 2^(j / 64), rounded to the nearest
+__constant__ double EXP_TAB[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
 
 // 2^(y / 64) for y <= 0 in 64 bits, within 2^-50: 64 powers from a table, e^x to x^5
 // on |x| <= ln 2 / 128 (the next term is below 4e-17).  y below -64000 counts as that, and so does a NaN.
@@ -29,9 +64,6 @@ __device__ inline double exp64(double y, const double *tab) {
     const uint64_t b = __builtin_bit_cast(uint64_t, tab[i & 63] * p);
     return __builtin_bit_cast(double, b + ((uint64_t)(int64_t)(i >> 6) << 52));
 }
-__device__ inline void exp64_table(double *tab) {     // by the first 64 threads
-    if (threadIdx.x < 64) tab[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
-}
 
 // f32 in the order of unsigned integers (-0 as +0)
 __device__ inline uint32_t sort_key(float v) {
@@ -39,235 +71,17 @@ __device__ inline uint32_t sort_key(float v) {
     return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 __device__ inline float key_value(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
-constexpr uint32_t KEY_NONE = 0x007fffffu;            // of -inf; NaN is read as -inf
+constexpr uint32_t KEY_NONE = 0x007fffffu;            // of -inf
+// an entry of the order: the larger comes first
+__device__ inline uint64_t entry(float v, uint32_t i) { return ((uint64_t)sort_key(v) << 32) | (uint32_t)~i; }
+__device__ inline uint32_t entry_key(uint64_t e) { return (uint32_t)(e >> 32); }
+__device__ inline int32_t entry_token(uint64_t e) { return (int32_t)~(uint32_t)e; }
 
 struct SampleCuts {
     float temp, top_p, min_p;
     int top_k;
     double u;                                         // in [0, 1)
 };
-
-struct SampleShared {
-    uint32_t cnt[SMP_BINS];
-    uint64_t mass[SMP_BINS];
-    uint64_t wm[SMP_WAVES];
-    uint32_t wc[SMP_WAVES];
-    uint64_t found_m;
-    uint32_t found_c, found_bin;
-};
-
-// A row's masses: e = exp((value - max) / temperature), as integers of `shift` fractional bits where
-// sums of any order have to agree
-struct Mass {
-    double vmax, c;                                   // c = 64 / (temperature ln 2)
-    const double *tab;
-    int shift;
-    __device__ double e(uint32_t key) const {
-        const double v = (double)key_value(key);
-        if (vmax == INFINITY) return v == INFINITY ? 1.0 : 0.0;
-        return v == vmax ? 1.0 : exp64((v - vmax) * c, tab);
-    }
-    __device__ uint64_t fixed(uint32_t key) const { return (uint64_t)(ldexp(e(key), shift) + 0.5); }
-};
-
-template <int T>
-struct Row {
-    const typename Elem<T>::raw *l;
-    int V;
-    template <class F>
-    __device__ void each(F f) const {                 // f(key) of every token that is on
-        for (int i = threadIdx.x; i < V; i += SMP_THREADS) {
-            const uint32_t k = key(i);
-            if (k > KEY_NONE) f(k);
-        }
-    }
-    __device__ uint32_t key(int i) const {
-        const float v = Elem<T>::load(l[i]);
-        return v != v ? KEY_NONE : sort_key(v);
-    }
-};
-
-__device__ inline uint64_t shfl_up_u64(uint64_t v, int o) {
-    const uint32_t lo = __shfl_up((uint32_t)v, o, 64), hi = __shfl_up((uint32_t)(v >> 32), o, 64);
-    return ((uint64_t)hi << 32) | lo;
-}
-
-__device__ inline uint64_t block_sum_u64(uint64_t v, SampleShared &s) {
-    const int lane = threadIdx.x & 63;
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t lo = __shfl_xor((uint32_t)v, o, 64), hi = __shfl_xor((uint32_t)(v >> 32), o, 64);
-        v += ((uint64_t)hi << 32) | lo;
-    }
-    __syncthreads();
-    if (lane == 0) s.wm[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t t = 0;
-    for (int w = 0; w < SMP_WAVES; ++w) t += s.wm[w];
-    return t;
-}
-
-// The key at which the running count (by_mass 0) or mass (1) of the tokens in
-// descending order first reaches target >= 1, and the count and mass before it:
-// three levels of 11, 11 and 10 key bits.
-struct Cut {
-    uint32_t key, n_before;
-    uint64_t m_before;
-};
-template <int T>
-__device__ Cut locate(const Row<T> &row, const Mass &ms, bool by_mass, uint64_t target, SampleShared &s) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    Cut c{0, 0, 0};
-    for (int level = 0; level < 3; ++level) {
-        const int sh = level == 0 ? 21 : level == 1 ? 10 : 0;
-        const uint32_t mask = level == 2 ? 1023u : 2047u;
-        const int up = level == 0 ? 31 : level == 1 ? 21 : 10;     // bits above: fixed by the levels before
-        const uint32_t fixed_bits = c.key;
-        __syncthreads();
-        for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { s.cnt[i] = 0; s.mass[i] = 0; }
-        __syncthreads();
-        row.each([&](uint32_t k) {
-            if (level && (k >> up) != (fixed_bits >> up)) return;
-            const uint32_t b = (k >> sh) & mask;
-            atomicAdd(&s.cnt[b], 1u);
-            atomicAdd((unsigned long long *)&s.mass[b], (unsigned long long)ms.fixed(k));
-        });
-        __syncthreads();
-        // thread t: bins 2047 - 2t and the next lower; inclusive scan from the highest bin down
-        const int b0 = SMP_BINS - 1 - 2 * tid;
-        const uint32_t c0 = s.cnt[b0], c1 = s.cnt[b0 - 1];
-        const uint64_t m0 = s.mass[b0], m1 = s.mass[b0 - 1];
-        uint32_t cs = c0 + c1;
-        uint64_t msum = m0 + m1;
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t uc = __shfl_up(cs, o, 64);
-            const uint64_t um = shfl_up_u64(msum, o);
-            if (lane >= o) { cs += uc; msum += um; }
-        }
-        if (lane == 63) { s.wc[wave] = cs; s.wm[wave] = msum; }
-        __syncthreads();
-        uint32_t cb = c.n_before + cs - (c0 + c1);
-        uint64_t mb = c.m_before + msum - (m0 + m1);
-        for (int w = 0; w < wave; ++w) { cb += s.wc[w]; mb += s.wm[w]; }
-        const uint64_t before = by_mass ? mb : cb, mid = before + (by_mass ? m0 : c0), end = mid + (by_mass ? m1 : c1);
-        if (before < target && target <= end) {
-            const bool first = target <= mid;
-            s.found_bin = (uint32_t)(first ? b0 : b0 - 1);
-            s.found_c = first ? cb : cb + c0;
-            s.found_m = first ? mb : mb + m0;
-        }
-        __syncthreads();
-        c.key = fixed_bits | (s.found_bin << sh);
-        c.n_before = s.found_c;
-        c.m_before = s.found_m;
-    }
-    return c;
-}
-
-// The row's token from the whole row, in any case: what the candidates cannot decide.
-template <int T>
-__device__ void sample_row(const SampleArgs &a, int64_t tok, uint32_t kmax, const SampleCuts &cut, const Mass &ms,
-                           SampleShared &s) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Row<T> row{(const typename Elem<T>::raw *)a.logits + tok * a.ld, a.V};
-    uint64_t total;
-    uint32_t cut_key = 0;
-    bool all = true;                                  // nothing was cut by count yet
-    if (cut.top_k > 0 && cut.top_k < a.V) {
-        uint64_t on = 0;
-        row.each([&](uint32_t) { ++on; });
-        on = block_sum_u64(on, s);
-        if ((uint64_t)cut.top_k < on) {
-            const Cut c = locate(row, ms, false, (uint64_t)cut.top_k, s);
-            cut_key = c.key;
-            total = c.m_before + ((uint32_t)cut.top_k - c.n_before) * ms.fixed(c.key);
-            all = false;
-        }
-    }
-    if (all) {
-        uint64_t sum = 0;
-        row.each([&](uint32_t k) { sum += ms.fixed(k); });
-        total = block_sum_u64(sum, s);
-    }
-    if (cut.top_p < 1.0f) {
-        const double want = ceil((double)fmaxf(cut.top_p, 0.0f) * (double)total);
-        const uint64_t m = want >= (double)total ? total : max((uint64_t)want, (uint64_t)1);
-        const Cut c = locate(row, ms, true, m, s);
-        const uint64_t f = ms.fixed(c.key);
-        cut_key = c.key;
-        total = c.m_before + (m - c.m_before + f - 1) / f * f;
-    }
-    if (cut.min_p > 0.0f) {
-        // the lowest key with e >= min_p, 64 ways a step
-        uint32_t lo = KEY_NONE, hi = kmax;
-        if (cut.min_p > 1.0f) {
-            total = ms.fixed(kmax);
-        } else {
-            while (hi - lo > 1) {
-                const uint32_t mid = lo + (uint32_t)(((uint64_t)(hi - lo) * (uint32_t)(lane + 1)) >> 6);
-                const uint64_t ge = __ballot(mid >= hi || (mid > lo && ms.e(mid) >= (double)cut.min_p));
-                const int f = __ffsll((unsigned long long)ge) - 1;      // lane 63's mid is hi
-                const uint32_t nhi = __shfl(mid, f, 64);
-                const uint32_t nlo = f ? __shfl(mid, f - 1, 64) : lo;
-                lo = nlo;
-                hi = nhi;
-            }
-            if (hi > cut_key) {
-                uint64_t sum = 0;
-                row.each([&](uint32_t k) { if (k >= hi) sum += ms.fixed(k); });
-                total = block_sum_u64(sum, s);
-            }
-        }
-    }
-    const uint64_t t = min((uint64_t)(cut.u * (double)total), total - 1);
-    const Cut c = locate(row, ms, true, t + 1, s);
-    const uint32_t key = c.key, place = (uint32_t)((t - c.m_before) / ms.fixed(key)) + 1;
-    const double prob = ldexp(ms.e(key), ms.shift) / (double)total;
-    // the place-th token of that key, by index: wave w holds a run of the row
-    const int seg = (a.V + SMP_WAVES - 1) / SMP_WAVES;
-    const int i0 = wave * seg, i1 = min(i0 + seg, a.V);
-    uint32_t n = 0;
-    for (int i = i0; i < i1; i += 64) n += (uint32_t)__popcll(__ballot(i + lane < i1 && row.key(min(i + lane, a.V - 1)) == key));
-    __syncthreads();
-    if (lane == 0) s.wc[wave] = n;
-    __syncthreads();
-    uint32_t before = 0;
-    for (int w = 0; w < wave; ++w) before += s.wc[w];
-    if (before >= place || before + n < place) return;
-    for (int i = i0; i < i1; i += 64) {
-        uint64_t m = __ballot(i + lane < i1 && row.key(min(i + lane, a.V - 1)) == key);
-        const uint32_t c = (uint32_t)__popcll(m);
-        if (before + c >= place) {
-            for (uint32_t r = before + 1; r < place; ++r) m &= m - 1;
-            if (lane == 0) {
-                a.tokens[tok] = i + __ffsll((unsigned long long)m) - 1;
-                if (a.probs) a.probs[tok] = (float)prob;
-            }
-            return;
-        }
-        before += c;
-    }
-}
-
-// ---------------------------------------------------------------------------
-// Two launches.  The first reads the logits once, a workgroup per run of
-// SLICE of a row: its maximum, its mass where the row's whole mass counts, and its
-// candidates -- every logit from a bound on, which is the R-th largest of the
-// threads' maxima, so that about SLICE_KEEP / S of them are kept whatever the
-// values are.  The second, a workgroup per row, has the row's order complete down to
-// the highest of the bounds, sorts that and cuts and draws; what needs more than
-// these candidates is worked out from the whole row (sample_row).
-constexpr int SLICE_THREADS = 256, SLICE_EPT = 64, SLICE = SLICE_THREADS * SLICE_EPT;
-constexpr int SLICE_KEEP = 320;
-static_assert(SMP_LIST >= 2 * SLICE_KEEP, "a row's candidates");
-
-struct SliceHead {
-    double mass;                                      // sum of exp((l - vmax) / temperature), 0 if not needed
-    float vmax;                                       // of the logits that are on, -inf if none is
-    uint32_t bound;                                   // every key of the slice from here on is in its list
-    uint32_t n;                                       // candidates
-    uint32_t at;                                      // greedy rows: the lowest index of vmax
-};
-
 __device__ inline SampleCuts load_cuts(const SampleArgs &a, int64_t tok) {
     SampleCuts c;
     c.temp = a.temp ? a.temp[tok] : a.temp_all;
@@ -278,37 +92,66 @@ __device__ inline SampleCuts load_cuts(const SampleArgs &a, int64_t tok) {
     c.u = u > 0.0f ? (double)fminf(u, 0x1.fffffep-1f) : 0.0;
     return c;
 }
+__device__ inline double exp64_scale(float temp) { return 64.0 / (0.6931471805599453094 * (double)temp); }
 
+// A row's masses, and as integers of `shift` fractional bits where sums of any order have to agree
+struct Mass {
+    double vmax, c;                                   // e = 2^((value - vmax) c / 64)
+    const double *tab;
+    int shift;
+    __device__ double e(uint32_t key) const {
+        const double v = (double)key_value(key);
+        if (vmax == INFINITY) return v == INFINITY ? 1.0 : 0.0;
+        return exp64((v - vmax) * c, tab);
+    }
+    __device__ uint64_t fixed(uint32_t key) const { return (uint64_t)(ldexp(e(key), shift) + 0.5); }
+};
+__device__ inline Mass row_mass(const SampleArgs &a, float vmax, float temp, const double *tab) {
+    return {(double)vmax, exp64_scale(temp), tab, 62 - (a.V > 1 ? 32 - __clz(a.V - 1) : 0)};
+}
+
+// ---------------------------------------------------------------------------
+// 1: slices
+
+struct SliceHead {
+    double mass;                                      // sum of exp((l - vmax) / temperature), 0 if not needed
+    float vmax;                                       // of the logits that are on, -inf if none is
+    uint32_t bound;                                   // every key of the slice from here on is in its list
+    uint32_t n;                                       // candidates
+    uint32_t at;                                      // greedy rows: the lowest index of vmax
+};
+
+// Chunks of 64 lanes x 16 bytes go to a row's slices in turn, so that neighbouring
+// likely tokens spread over them.  The bound is the value that about `keep` lanes' maxima
+// reach (a bisection; any value would do); should more than `cap` logits lie above it, a higher one.
 template <int T>
-__global__ __launch_bounds__(SLICE_THREADS) void sample_slice_kernel(SampleArgs a) {
+__global__ __launch_bounds__(64 * SLICE_WAVES) void sample_slice_kernel(SampleArgs a) {
     typedef typename Elem<T>::raw raw;
     constexpr int VEC = 16 / sizeof(raw), NV = SLICE_EPT / VEC;
-    __shared__ __attribute__((aligned(16))) float s_max[SLICE_THREADS];
-    __shared__ double s_sum[SLICE_THREADS / 64];
     __shared__ double s_tab[64];
-    __shared__ uint32_t s_at[SLICE_THREADS / 64];
-    __shared__ uint32_t s_n;
-    __shared__ float s_bound;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t tok = blockIdx.x / a.slices;
-    const int slice = blockIdx.x % a.slices, base = slice * SLICE;
-    const SampleCuts cut = load_cuts(a, tok);
-    const raw *l = (const raw *)a.logits + tok * a.ld + base;
-    const int n_el = min(SLICE, a.V - base);
-    exp64_table(s_tab);
-    if (tid == 0) s_n = 0;
+    const int lane = threadIdx.x & 63;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.n_rest = 0;
+    const int64_t id = (int64_t)blockIdx.x * SLICE_WAVES + (threadIdx.x >> 6);
+    const bool live = id < (int64_t)a.n_tok * a.slices;
+    const int64_t tok = live ? id / a.slices : 0;
+    const int slice = (int)(id - tok * a.slices);
+    const raw *l = (const raw *)a.logits + tok * a.ld;
     float v[SLICE_EPT];
-    if ((uintptr_t)l % 16 == 0) {
+    const int i0 = (slice * 64 + lane) * VEC, step = a.slices * 64 * VEC;      // vector j at i0 + j step
+    if (!live) {
+#pragma unroll
+        for (int j = 0; j < SLICE_EPT; ++j) v[j] = -INFINITY;
+    } else if ((uintptr_t)l % 16 == 0) {
         uint4 q[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int i = (SLICE_THREADS * j + tid) * VEC;
-            if (i + VEC <= n_el) {
+            const int i = i0 + j * step;
+            if (i + VEC <= a.V) {
                 q[j] = *(const uint4 *)(l + i);
             } else {
                 raw t[VEC];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) t[e] = i + e < n_el ? l[i + e] : Elem<T>::store(-INFINITY);
+                for (int e = 0; e < VEC; ++e) t[e] = i + e < a.V ? l[i + e] : Elem<T>::store(-INFINITY);
                 __builtin_memcpy(&q[j], t, 16);
             }
         }
@@ -322,106 +165,508 @@ __global__ __launch_bounds__(SLICE_THREADS) void sample_slice_kernel(SampleArgs 
     } else {
 #pragma unroll
         for (int j = 0; j < SLICE_EPT; ++j) {
-            const int i = (SLICE_THREADS * (j / VEC) + tid) * VEC + j % VEC;
-            v[j] = i < n_el ? Elem<T>::load(l[i]) : -INFINITY;
+            const int i = i0 + (j / VEC) * step + j % VEC;
+            v[j] = i < a.V ? Elem<T>::load(l[i]) : -INFINITY;
         }
     }
+    const SampleCuts cut = load_cuts(a, tok);
+    if (threadIdx.x < 64) s_tab[threadIdx.x] = EXP_TAB[threadIdx.x];
+    __syncthreads();
+    if (!live) return;
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < SLICE_EPT; ++j) m = fmaxf(m, v[j]);       // passes over a NaN
-    s_max[tid] = m;
-    __syncthreads();
-    float vmax = -INFINITY;
-    {
-        const float4 q = ((const float4 *)s_max)[lane];
-        vmax = wave_max(fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)));
-    }
+    const float vmax = wave_max(m);
     SliceHead h{};
     h.vmax = vmax;
-    SliceHead *head = (SliceHead *)a.heads + blockIdx.x;
+    SliceHead *head = (SliceHead *)a.heads + id;
     if (!(cut.temp > 0.0f)) {
         uint32_t at = 0xffffffffu;
 #pragma unroll
         for (int j = SLICE_EPT - 1; j >= 0; --j)
-            if (v[j] == vmax) at = (uint32_t)((SLICE_THREADS * (j / VEC) + tid) * VEC + j % VEC);
+            if (v[j] == vmax) at = (uint32_t)(i0 + (j / VEC) * step + j % VEC);
         for (int o = 32; o > 0; o >>= 1) at = min(at, (uint32_t)__shfl_xor(at, o, 64));
-        if (lane == 0) s_at[wave] = at;
-        __syncthreads();
-        if (tid == 0) {
-            for (int w = 0; w < SLICE_THREADS / 64; ++w) h.at = w ? min(h.at, s_at[w]) : s_at[0];
-            h.at += (uint32_t)base;
-            *head = h;
-        }
+        h.at = at;
+        if (lane == 0) *head = h;
         return;
     }
-    const bool by_k = cut.top_k > 0 && cut.top_k < a.V;
-    if (!by_k) {                                      // the row's whole mass counts
-        const double c = 64.0 / (0.6931471805599453094 * (double)cut.temp), vm = (double)vmax;
-        double sum = 0.0;
+    if (!(cut.top_k > 0 && cut.top_k < a.V)) {        // the row's whole mass counts
+        const double c = exp64_scale(cut.temp), vm = (double)vmax;
+        double sum[4] = {};
 #pragma unroll
-        for (int j = 0; j < SLICE_EPT; ++j) sum += exp64(((double)v[j] - vm) * c, s_tab);
-        for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-        if (lane == 0) s_sum[wave] = sum;
+        for (int j = 0; j < SLICE_EPT; ++j) sum[j & 3] += exp64(((double)v[j] - vm) * c, s_tab);
+        double t = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
+        h.mass = t;
     }
-    // the R-th largest of the threads' maxima
-    int rank = 0;
-    for (int i = 0; i < SLICE_THREADS; i += 4) {
-        const float4 q = *(const float4 *)&s_max[i];
-        rank += (q.x > m) || (q.x == m && i < tid);
-        rank += (q.y > m) || (q.y == m && i + 1 < tid);
-        rank += (q.z > m) || (q.z == m && i + 2 < tid);
-        rank += (q.w > m) || (q.w == m && i + 3 < tid);
-    }
-    if (rank == a.keep - 1) s_bound = m;
-    __syncthreads();
-    const float bound = s_bound;
-    uint64_t *list = (uint64_t *)a.lists + (size_t)blockIdx.x * a.cap;
-    if (m >= bound)
-#pragma unroll
-        for (int j = 0; j < SLICE_EPT; ++j)
-            if (v[j] >= bound && v[j] > -INFINITY) {
-                const uint32_t at = atomicAdd(&s_n, 1u);
-                const uint32_t i = (uint32_t)(base + (SLICE_THREADS * (j / VEC) + tid) * VEC + j % VEC);
-                if (at < (uint32_t)a.cap) list[at] = ((uint64_t)sort_key(v[j]) << 32) | (uint32_t)~i;
+    uint64_t *list = (uint64_t *)a.lists + (size_t)id * a.cap;
+    const uint32_t mk = sort_key(m), top = (uint32_t)__builtin_amdgcn_readfirstlane((int)sort_key(vmax));
+    int keep = a.keep;
+    for (;;) {
+        uint32_t lo = KEY_NONE, hi = top;             // at least keep lanes reach lo
+        if (keep > 1 && vmax > -INFINITY) {
+            for (int it = 0; it < 20 && hi > lo; ++it) {
+                const uint32_t mid = hi - (hi - lo) / 2;
+                const int c = __popcll(__ballot(mk >= mid));
+                if (c >= keep) lo = mid;
+                else hi = mid - 1;
+                if (c == keep) break;
             }
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 0; !by_k && w < SLICE_THREADS / 64; ++w) h.mass += s_sum[w];
-        h.n = min(s_n, (uint32_t)a.cap);
-        h.bound = s_n > (uint32_t)a.cap ? 0xffffffffu : bound == -INFINITY ? 0u : sort_key(bound);
-        *head = h;
+        } else {
+            lo = top;
+        }
+        const float bound = key_value(lo);
+        uint32_t n = 0;
+#pragma unroll
+        for (int j = 0; j < SLICE_EPT; ++j) {
+            const bool in = v[j] >= bound && v[j] > -INFINITY;
+            const uint64_t b = __ballot(in);
+            if (b) {
+                const uint32_t p = n + (uint32_t)__popcll(b & ((1ull << lane) - 1));
+                if (in && p < (uint32_t)a.cap) list[p] = entry(v[j], (uint32_t)(i0 + (j / VEC) * step + j % VEC));
+                n += (uint32_t)__popcll(b);
+            }
+        }
+        h.n = n;
+        h.bound = lo > KEY_NONE ? lo : 0;
+        if (n <= (uint32_t)a.cap) break;
+        if (keep <= 1) {                              // more equal maxima than that
+            h.n = 0;
+            h.bound = 0xffffffffu;
+            break;
+        }
+        keep = keep / 4;
     }
+    if (lane == 0) *head = h;
 }
 
+// ---------------------------------------------------------------------------
+// the order of up to SMP_LIST entries, and running sums over it
+
 struct SampleList {
-    uint64_t raw[SMP_LIST], sorted[SMP_LIST];         // key << 32 | ~index: descending order, the lower index first
-    double wsum[SMP_WAVES];
-    uint32_t n, cut, by_p, by_min, at;
-    double total;
+    uint64_t raw[SMP_LIST], sorted[SMP_LIST];
+    uint32_t n;
 };
-union SampleLds {
-    SampleShared row;
+// sorted[0 .. n) = raw[0 .. n) in descending order (the entries differ): each entry's rank, four lanes counting
+__device__ inline void sort_list(SampleList &s, int n) {
+    __syncthreads();
+    for (int i0 = 0; i0 < n; i0 += SMP_THREADS / 4) {
+        const int i = i0 + ((int)threadIdx.x >> 2);
+        const uint64_t mine = s.raw[min(i, n - 1)];
+        int rank = 0;
+        for (int j = threadIdx.x & 3; j < n; j += 4) rank += s.raw[j] > mine;
+        rank += dpp_i<DPP_XOR1>(rank);
+        rank += dpp_i<DPP_XOR2>(rank);
+        if ((threadIdx.x & 3) == 0 && i < n) s.sorted[rank] = mine;
+    }
+    __syncthreads();
+}
+
+__device__ inline uint64_t shfl_up_u64(uint64_t v, int o) {
+    const uint32_t lo = __shfl_up((uint32_t)v, o, 64), hi = __shfl_up((uint32_t)(v >> 32), o, 64);
+    return ((uint64_t)hi << 32) | lo;
+}
+__device__ inline double shfl_up_t(double v, int o) { return __shfl_up(v, o, 64); }
+__device__ inline uint64_t shfl_up_t(uint64_t v, int o) { return shfl_up_u64(v, o); }
+// the sum of v over the threads before this one, in a fixed order
+template <class N>
+__device__ inline N block_before(N v, N *s_w) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    N run = v;
+    for (int o = 1; o < 64; o <<= 1) {
+        const N up = shfl_up_t(run, o);
+        if (lane >= o) run += up;
+    }
+    __syncthreads();
+    if (lane == 63) s_w[wave] = run;
+    __syncthreads();
+    N before = 0;
+    for (int w = 0; w < wave; ++w) before += s_w[w];
+    N prev = shfl_up_t(run, 1);
+    return before + (lane ? prev : (N)0);
+}
+
+// ---------------------------------------------------------------------------
+// 3: whole rows
+
+struct SampleShared {
+    uint32_t cnt[SMP_BINS];
+    uint64_t mass[SMP_BINS];
+    uint64_t wm[SMP_WAVES];
+    uint64_t wc[SMP_WAVES];
+    uint64_t found_m, found_e;
+    uint32_t found_c, found_bin, last;
     SampleList list;
 };
 
 template <int T>
-__global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) {
-    __shared__ SampleLds s;
+struct Row {
+    typedef typename Elem<T>::raw raw;
+    const raw *l;
+    int V;
+    __device__ float at(int i) const { return Elem<T>::load(l[i]); }
+    // f(value, index) of every token that is on, of [i0, i1) (i0 a multiple of 8)
+    template <class F>
+    __device__ void each(int i0, int i1, F f) const {
+        constexpr int VEC = 16 / sizeof(raw), U = 4;
+        if ((uintptr_t)l % 16 == 0) {
+            int i = i0 + (int)threadIdx.x * VEC;
+            for (; i + (U - 1) * SMP_THREADS * VEC + VEC <= i1; i += U * SMP_THREADS * VEC) {
+                uint4 q[U];
+#pragma unroll
+                for (int k = 0; k < U; ++k) q[k] = *(const uint4 *)(l + i + k * SMP_THREADS * VEC);
+#pragma unroll
+                for (int k = 0; k < U; ++k) some(q[k], i + k * SMP_THREADS * VEC, f);
+            }
+            for (; i + VEC <= i1; i += SMP_THREADS * VEC) some(*(const uint4 *)(l + i), i, f);
+            for (int j = i; j < min(i + VEC, i1); ++j) {
+                const float v = at(j);
+                if (v > -INFINITY) f(v, j);
+            }
+        } else {
+            for (int i = i0 + (int)threadIdx.x; i < i1; i += SMP_THREADS) {
+                const float v = at(i);
+                if (v > -INFINITY) f(v, i);
+            }
+        }
+    }
+    template <class F>
+    __device__ void each(F f) const { each(0, V, f); }
+
+private:
+    template <class F>
+    __device__ void some(uint4 q, int i, F f) const {
+        constexpr int VEC = 16 / sizeof(raw);
+        raw t[VEC];
+        __builtin_memcpy(t, &q, 16);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float v = Elem<T>::load(t[e]);
+            if (v > -INFINITY) f(v, i + e);
+        }
+    }
+};
+
+__device__ inline uint64_t block_sum_u64(uint64_t v, SampleShared &s) {
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t lo = __shfl_xor((uint32_t)v, o, 64), hi = __shfl_xor((uint32_t)(v >> 32), o, 64);
+        v += ((uint64_t)hi << 32) | lo;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.wm[threadIdx.x >> 6] = v;
+    __syncthreads();
+    uint64_t t = 0;
+    for (int w = 0; w < SMP_WAVES; ++w) t += s.wm[w];
+    return t;
+}
+
+// Where the running count or mass of the order first reaches a target >= 1: the
+// key there, the count and mass before it (before its first equal), and the token, or -1 if it is
+// yet to be looked up among the equal ones.
+struct Cut {
+    uint32_t key;
+    int32_t token;
+    uint64_t n_before, m_before;
+};
+
+// by a radix search: three levels of 11, 11 and 10 key bits, whatever the values are
+template <int T>
+struct RadixSearch {
+    const Row<T> &row;
+    const Mass &ms;
+    SampleShared &s;
+    __device__ void totals(uint64_t &n, uint64_t &m) const {
+        uint64_t c = 0, sum = 0;
+        row.each([&](float v, int) { ++c; sum += ms.fixed(sort_key(v)); });
+        n = block_sum_u64(c, s);
+        m = block_sum_u64(sum, s);
+    }
+    __device__ uint64_t mass_from(uint32_t key) const {
+        uint64_t sum = 0;
+        row.each([&](float v, int) { const uint32_t k = sort_key(v); if (k >= key) sum += ms.fixed(k); });
+        return block_sum_u64(sum, s);
+    }
+    __device__ Cut find(bool by_mass, uint64_t target) const {
+        const int tid = threadIdx.x;
+        Cut c{0, -1, 0, 0};
+        for (int level = 0; level < 3; ++level) {
+            const int sh = level == 0 ? 21 : level == 1 ? 10 : 0;
+            const uint32_t mask = level == 2 ? 1023u : 2047u;
+            const int up = level == 1 ? 21 : 10;      // bits above: fixed by the levels before
+            const uint32_t fixed_bits = c.key;
+            __syncthreads();
+            for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { s.cnt[i] = 0; s.mass[i] = 0; }
+            __syncthreads();
+            row.each([&](float v, int) {
+                const uint32_t k = sort_key(v);
+                if (level && (k >> up) != (fixed_bits >> up)) return;
+                const uint32_t b = mask - ((k >> sh) & mask);      // bin 0: the largest
+                atomicAdd(&s.cnt[b], 1u);
+                atomicAdd((unsigned long long *)&s.mass[b], (unsigned long long)ms.fixed(k));
+            });
+            __syncthreads();
+            find_bin(s, by_mass, target, c.n_before, c.m_before);
+            c.key = fixed_bits | ((mask - s.found_bin) << sh);
+            c.n_before = s.found_c;
+            c.m_before = s.found_m;
+        }
+        return c;
+    }
+    // the bin that holds the target, and the count and mass before it
+    static __device__ void find_bin(SampleShared &s, bool by_mass, uint64_t target, uint64_t n0, uint64_t m0) {
+        const int b = 2 * (int)threadIdx.x;
+        const uint64_t c0 = s.cnt[b], c1 = s.cnt[b + 1], q0 = s.mass[b], q1 = s.mass[b + 1];
+        const uint64_t cb = n0 + block_before<uint64_t>(c0 + c1, s.wc), mb = m0 + block_before<uint64_t>(q0 + q1, s.wm);
+        const uint64_t before = by_mass ? mb : cb, mid = before + (by_mass ? q0 : c0), end = mid + (by_mass ? q1 : c1);
+        if (before < target && target <= end) {
+            const bool first = target <= mid;
+            s.found_bin = (uint32_t)(first ? b : b + 1);
+            s.found_c = (uint32_t)(first ? cb : cb + c0);
+            s.found_m = first ? mb : mb + q0;
+        }
+        __syncthreads();
+    }
+};
+
+// by a histogram of the row over bins of equal width below the maximum (s.cnt, s.mass), and the sorted
+// entries of the one bin that holds the target
+__device__ inline int bin_of(float v, float vmax, float per) { return (int)fminf((vmax - v) * per, (float)(SMP_BINS - 1)); }
+// bins of 1/64 of a factor of two: 2,048 span 32 of them, and of 152k logits spread like a normal
+// distribution's with a deviation of 1 the fullest holds about 660
+__device__ inline float bins_per(float temp) { return (float)fmin(64.0 / (0.6931471805599453094 * (double)temp), 1e30); }
+
+template <int T>
+struct BinSearch {
+    const Row<T> &row;
+    const Mass &ms;
+    SampleShared &s;
+    float vmax, per;
+    uint64_t n_all, m_all;
+    bool &full;                                       // a bin holds more entries than can be sorted
+    __device__ void totals(uint64_t &n, uint64_t &m) const { n = n_all; m = m_all; }
+    __device__ uint64_t mass_from(uint32_t key) const {
+        const int b = bin_of(key_value(key), vmax, per);
+        uint64_t sum = 0;
+        for (int i = threadIdx.x; i < b; i += SMP_THREADS) sum += s.mass[i];
+        row.each([&](float v, int) {
+            const uint32_t k = sort_key(v);
+            if (k >= key && bin_of(v, vmax, per) == b) sum += ms.fixed(k);
+        });
+        return block_sum_u64(sum, s);
+    }
+    __device__ Cut find(bool by_mass, uint64_t target) const {
+        __syncthreads();
+        RadixSearch<T>::find_bin(s, by_mass, target, 0, 0);
+        const int b = (int)s.found_bin, n = (int)s.cnt[b];
+        uint64_t nb = s.found_c, mb = s.found_m;
+        if (n > SMP_LIST) {
+            full = true;
+            return Cut{0, -1, 0, 0};
+        }
+        if (threadIdx.x == 0) s.list.n = 0;
+        __syncthreads();
+        row.each([&](float v, int i) {
+            if (bin_of(v, vmax, per) == b) s.list.raw[atomicAdd(&s.list.n, 1u)] = entry(v, (uint32_t)i);
+        });
+        sort_list(s.list, n);
+        const int j = 2 * (int)threadIdx.x;
+        const uint64_t q0 = j < n ? ms.fixed(entry_key(s.list.sorted[j])) : 0;
+        const uint64_t q1 = j + 1 < n ? ms.fixed(entry_key(s.list.sorted[j + 1])) : 0;
+        mb += block_before<uint64_t>(q0 + q1, s.wm);
+        nb += (uint64_t)j;
+        const uint64_t before = by_mass ? mb : nb, mid = before + (by_mass ? q0 : (uint64_t)(j < n)),
+                       end = mid + (by_mass ? q1 : (uint64_t)(j + 1 < n));
+        if (before < target && target <= end) {
+            const bool first = target <= mid;
+            s.found_e = s.list.sorted[first ? j : j + 1];
+            s.found_c = (uint32_t)(first ? nb : nb + 1);
+            s.found_m = first ? mb : mb + q0;
+        }
+        __syncthreads();
+        return Cut{entry_key(s.found_e), entry_token(s.found_e), s.found_c, s.found_m};
+    }
+};
+
+// The row's token by a search over the whole row.  A cut's n_before and m_before may stand before the first of the
+// equal keys (a radix search) or right before the token itself: (target - before) counts on from there either way.
+template <int T, class Search>
+__device__ bool sample_row(const SampleArgs &a, int64_t tok, uint32_t kmax, const SampleCuts &cut, const Mass &ms,
+                           const Row<T> &row, const Search &search, const bool &full, SampleShared &s) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t on, total;
+    search.totals(on, total);
+    uint32_t cut_key = 0;
+    if (cut.top_k > 0 && cut.top_k < a.V && (uint64_t)cut.top_k < on) {
+        const Cut c = search.find(false, (uint64_t)cut.top_k);
+        if (full) return false;
+        cut_key = c.key;
+        total = c.m_before + ((uint64_t)cut.top_k - c.n_before) * ms.fixed(c.key);
+    }
+    if (cut.top_p < 1.0f) {
+        const double want = ceil((double)fmaxf(cut.top_p, 0.0f) * (double)total);
+        const uint64_t m = want >= (double)total ? total : max((uint64_t)want, (uint64_t)1);
+        const Cut c = search.find(true, m);
+        if (full) return false;
+        const uint64_t f = ms.fixed(c.key);
+        cut_key = c.key;
+        total = c.m_before + (m - c.m_before + f - 1) / f * f;
+    }
+    if (cut.min_p > 1.0f) {
+        total = ms.fixed(kmax);
+    } else if (cut.min_p > 0.0f) {
+        // the lowest key with e >= min_p, 64 ways a step
+        uint32_t lo = KEY_NONE, hi = kmax;
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (uint32_t)(((uint64_t)(hi - lo) * (uint32_t)(lane + 1)) >> 6);
+            const uint64_t ge = __ballot(mid >= hi || (mid > lo && ms.e(mid) >= (double)cut.min_p));
+            const int f = __ffsll((unsigned long long)ge) - 1;      // lane 63's mid is hi
+            const uint32_t nhi = __shfl(mid, f, 64);
+            const uint32_t nlo = f ? __shfl(mid, f - 1, 64) : lo;
+            lo = nlo;
+            hi = nhi;
+        }
+        if (hi > cut_key) total = search.mass_from(hi);
+    }
+    const uint64_t t = min((uint64_t)(cut.u * (double)total), total - 1);
+    const Cut c = search.find(true, t + 1);
+    if (full) return false;
+    const float prob = (float)(ldexp(ms.e(c.key), ms.shift) / (double)total);
+    if (c.token >= 0) {
+        if (threadIdx.x == 0) {
+            a.tokens[tok] = c.token;
+            if (a.probs) a.probs[tok] = prob;
+        }
+        return true;
+    }
+    // the place-th token of that key, by index: wave w holds a run of the row
+    const uint32_t place = (uint32_t)((t - c.m_before) / ms.fixed(c.key)) + 1;
+    const float value = key_value(c.key);
+    const int seg = (a.V + SMP_WAVES - 1) / SMP_WAVES;
+    const int i0 = wave * seg, i1 = min(i0 + seg, a.V);
+    uint32_t n = 0;
+    for (int i = i0; i < i1; i += 64) n += (uint32_t)__popcll(__ballot(i + lane < i1 && row.at(min(i + lane, a.V - 1)) == value));
+    __syncthreads();
+    if (lane == 0) s.wc[wave] = n;
+    __syncthreads();
+    uint32_t before = 0;
+    for (int w = 0; w < wave; ++w) before += (uint32_t)s.wc[w];
+    if (before >= place || before + n < place) return true;
+    for (int i = i0; i < i1; i += 64) {
+        uint64_t m = __ballot(i + lane < i1 && row.at(min(i + lane, a.V - 1)) == value);
+        const uint32_t k = (uint32_t)__popcll(m);
+        if (before + k >= place) {
+            for (uint32_t r = before + 1; r < place; ++r) m &= m - 1;
+            if (lane == 0) {
+                a.tokens[tok] = i + __ffsll((unsigned long long)m) - 1;
+                if (a.probs) a.probs[tok] = prob;
+            }
+            return true;
+        }
+        before += k;
+    }
+    return true;
+}
+
+// what step 2 hands to step 3
+struct RestRow {
+    uint64_t mass[SMP_BINS];
+    uint32_t cnt[SMP_BINS];
+    int64_t tok;
+    float vmax;
+    uint32_t parts;                                   // finished
+};
+
+// A fixed number of workgroups take the parts of the undecided rows in turn; the one
+// that finishes a row's last part decides the row.  No workgroup waits for another.
+template <int T>
+__global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) {
+    __shared__ SampleShared s;
     __shared__ double s_tab[64];
-    __shared__ SliceHead s_head[64];
+    const int tid = threadIdx.x;
+    const uint32_t n = *a.n_rest;
+    if (blockIdx.x >= n * REST_PARTS) return;
+    if (tid < 64) s_tab[tid] = EXP_TAB[tid];
+    for (uint32_t task = blockIdx.x; task < n * REST_PARTS; task += gridDim.x) {
+        RestRow &r = ((RestRow *)a.rest)[task / REST_PARTS];
+        const int part = (int)(task % REST_PARTS);
+        const int64_t tok = r.tok;
+        const float vmax = r.vmax;
+        const SampleCuts cut = load_cuts(a, tok);
+        const Row<T> row{(const typename Elem<T>::raw *)a.logits + tok * a.ld, a.V};
+        const Mass ms = row_mass(a, vmax, cut.temp, s_tab);
+        const float per = bins_per(cut.temp);
+        const int run = ((a.V + REST_PARTS - 1) / REST_PARTS + 7) / 8 * 8;
+        __syncthreads();
+        for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { s.cnt[i] = 0; s.mass[i] = 0; }
+        __syncthreads();
+        if (vmax < INFINITY)
+            row.each(min(part * run, a.V), min((part + 1) * run, a.V), [&](float v, int) {
+                const int b = bin_of(v, vmax, per);
+                atomicAdd(&s.cnt[b], 1u);
+                atomicAdd((unsigned long long *)&s.mass[b], (unsigned long long)ms.fixed(sort_key(v)));
+            });
+        __syncthreads();
+        for (int i = tid; i < SMP_BINS; i += SMP_THREADS)
+            if (s.cnt[i]) {
+                __hip_atomic_fetch_add(&r.cnt[i], s.cnt[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_fetch_add(&r.mass[i], s.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        __threadfence();
+        __syncthreads();
+        if (tid == 0)
+            s.last = __hip_atomic_fetch_add(&r.parts, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == REST_PARTS - 1;
+        __syncthreads();
+        if (!s.last) continue;
+        __threadfence();
+        uint64_t c = 0, m = 0;
+        for (int i = tid; i < SMP_BINS; i += SMP_THREADS) {
+            s.cnt[i] = __hip_atomic_load(&r.cnt[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s.mass[i] = __hip_atomic_load(&r.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            c += s.cnt[i];
+            m += s.mass[i];
+        }
+        c = block_sum_u64(c, s);
+        m = block_sum_u64(m, s);
+        bool full = vmax == INFINITY;
+        const uint32_t kmax = sort_key(vmax);
+        if (!full) sample_row(a, tok, kmax, cut, ms, row, BinSearch<T>{row, ms, s, vmax, per, c, m, full}, full, s);
+        if (full) {
+            const bool no = false;
+            sample_row(a, tok, kmax, cut, ms, row, RadixSearch<T>{row, ms, s}, no, s);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 2: one workgroup per row
+
+struct PickLds {
+    SampleList list;
+    double wsum[SMP_WAVES], total;
+    uint32_t by_p, by_min, at, rest;
+    SliceHead head[SLICES_MAX];
+    double tab[64];
+};
+
+template <int T>
+__global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) {
+    __shared__ PickLds s;
     const int64_t tok = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x;
     const SampleCuts cut = load_cuts(a, tok);
     const SliceHead *heads = (const SliceHead *)a.heads + tok * a.slices;
-    exp64_table(s_tab);
-    if (tid < a.slices) s_head[tid] = heads[tid];
-    if (tid == 0) s.list.n = 0;
+    if (tid < 64) s.tab[tid] = EXP_TAB[tid];
+    if (tid < a.slices) s.head[tid] = heads[tid];
+    if (tid == 0) {
+        s.list.n = 0;
+        s.by_p = s.by_min = s.at = 0xffffffffu;
+    }
     __syncthreads();
     float vmax = -INFINITY;
     uint32_t bound = 0;
     for (int i = 0; i < a.slices; ++i) {
-        vmax = fmaxf(vmax, s_head[i].vmax);
-        bound = max(bound, s_head[i].bound);
+        vmax = fmaxf(vmax, s.head[i].vmax);
+        bound = max(bound, s.head[i].bound);
     }
     if (vmax == -INFINITY) {                          // nothing is on
         if (tid == 0) {
@@ -432,160 +677,150 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) 
     }
     if (!(cut.temp > 0.0f)) {
         if (tid == 0) {
-            int i = 0;
-            while (s_head[i].vmax != vmax) ++i;
-            a.tokens[tok] = (int32_t)s_head[i].at;
+            uint32_t at = 0xffffffffu;
+            for (int i = 0; i < a.slices; ++i)
+                if (s.head[i].vmax == vmax) at = min(at, s.head[i].at);
+            a.tokens[tok] = (int32_t)at;
             if (a.probs) a.probs[tok] = 1.0f;
         }
         return;
     }
-    const Mass ms{(double)vmax, 64.0 / (0.6931471805599453094 * (double)cut.temp), s_tab,
-                  62 - (a.V > 1 ? 32 - __clz(a.V - 1) : 0)};
-    const uint32_t kmax = sort_key(vmax);
+    const Mass ms = row_mass(a, vmax, cut.temp, s.tab);
     const bool by_k = cut.top_k > 0 && cut.top_k < a.V;
     for (int i = tid; i < a.slices * a.cap; i += SMP_THREADS) {
-        const int sl = i / a.cap, j = i % a.cap;
-        if (j >= (int)s_head[sl].n) continue;
+        const int sl = i / a.cap, j = i - sl * a.cap;
+        if (j >= (int)s.head[sl].n) continue;
         const uint64_t e = ((const uint64_t *)a.lists)[(size_t)(tok * a.slices) * a.cap + i];
-        if ((uint32_t)(e >> 32) < bound) continue;
+        if (entry_key(e) < bound) continue;
         const uint32_t at = atomicAdd(&s.list.n, 1u);
         if (at < SMP_LIST) s.list.raw[at] = e;
     }
     __syncthreads();
     const int n = (int)s.list.n;
-    bool done = vmax < INFINITY && n > 0 && n <= SMP_LIST;
-    __syncthreads();
-    if (done) {
-        // sorted by rank: the entries differ
-        for (int i = tid; i < n; i += SMP_THREADS) {
-            const uint64_t mine = s.list.raw[i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += s.list.raw[j] > mine;
-            s.list.sorted[rank] = mine;
-        }
+    if (vmax < INFINITY && n > 0 && n <= SMP_LIST) {
         if (tid == 0) {
-            s.list.cut = s.list.by_p = s.list.by_min = s.list.at = 0xffffffffu;
             double total = 0.0;
             if (!by_k)
                 for (int i = 0; i < a.slices; ++i)
-                    if (s_head[i].vmax > -INFINITY)
-                        total += s_head[i].mass * exp64(((double)s_head[i].vmax - ms.vmax) * ms.c, s_tab);
-            s.list.total = total;
+                    if (s.head[i].vmax > -INFINITY) total += s.head[i].mass * exp64(((double)s.head[i].vmax - ms.vmax) * ms.c, s.tab);
+            s.total = total;
         }
-        __syncthreads();
+        sort_list(s.list, n);
         // running masses: thread t has entries 2t and 2t + 1
         const int j0 = 2 * tid, j1 = j0 + 1;
-        const double e0 = j0 < n ? ms.e((uint32_t)(s.list.sorted[j0] >> 32)) : 0.0;
-        const double e1 = j1 < n ? ms.e((uint32_t)(s.list.sorted[j1] >> 32)) : 0.0;
-        double run = e0 + e1;
-        for (int o = 1; o < 64; o <<= 1) {
-            const double up = __shfl_up(run, o, 64);
-            if (lane >= o) run += up;
+        const double e0 = j0 < n ? ms.e(entry_key(s.list.sorted[j0])) : 0.0;
+        const double e1 = j1 < n ? ms.e(entry_key(s.list.sorted[j1])) : 0.0;
+        const double c0 = block_before<double>(e0 + e1, s.wsum) + e0, c1 = c0 + e1;
+        uint32_t kept = (uint32_t)n;                  // how many of the sorted entries stay
+        bool open = bound != 0;                       // tokens behind them may stay, too
+        bool sure = true;                             // the mass that top-p shares is known
+        if (by_k && cut.top_k <= n) {
+            kept = (uint32_t)cut.top_k;
+            open = false;
+        } else if (by_k && open) {
+            sure = false;
         }
-        if (lane == 63) s.list.wsum[wave] = run;
-        __syncthreads();
-        double before = 0.0;
-        for (int w = 0; w < wave; ++w) before += s.list.wsum[w];
-        const double c1 = before + run, c0 = c1 - e1;
-        const bool whole = bound == 0;                // the candidates are all the row has
-        uint32_t kept = (uint32_t)n;                  // how many of the sorted stay, if that is known
-        bool open = !whole;                           // tokens behind the candidates may stay, too
-        double total = s.list.total;
-        if (by_k) {
-            if (cut.top_k <= n) {
-                kept = (uint32_t)cut.top_k;
-                open = false;
-            }
-            done = !open;
-            if (j0 == (int)kept - 1) s.list.total = c0;
-            if (j1 == (int)kept - 1) s.list.total = c1;
+        if (!open) {                                  // all that stays is at hand
+            if (j0 == (int)kept - 1) s.total = c0;
+            if (j1 == (int)kept - 1) s.total = c1;
             __syncthreads();
-            total = s.list.total;
-        } else if (whole) {
-            if (j0 == n - 1) s.list.total = c0;
-            if (j1 == n - 1) s.list.total = c1;
-            __syncthreads();
-            total = s.list.total;
         }
-        if (cut.top_p < 1.0f) {
-            const double want = (double)fmaxf(cut.top_p, 0.0f) * total;
-            if (j0 < (int)kept && c0 >= want) atomicMin(&s.list.by_p, (uint32_t)j0);
-            if (j1 < (int)kept && c1 >= want) atomicMin(&s.list.by_p, (uint32_t)j1);
+        if (cut.top_p < 1.0f && sure) {
+            const double want = (double)fmaxf(cut.top_p, 0.0f) * s.total;
+            if (j0 < (int)kept && c0 >= want) atomicMin(&s.by_p, (uint32_t)j0);
+            if (j1 < (int)kept && c1 >= want) atomicMin(&s.by_p, (uint32_t)j1);
             __syncthreads();
-            const uint32_t f = s.list.by_p;
-            if (f < kept) { kept = f + 1; open = false; }
+            if (s.by_p < kept) { kept = s.by_p + 1; open = false; }
         }
         if (cut.min_p > 0.0f) {
-            if (j0 < (int)kept && !(e0 >= (double)cut.min_p)) atomicMin(&s.list.by_min, (uint32_t)j0);
-            if (j1 < (int)kept && !(e1 >= (double)cut.min_p)) atomicMin(&s.list.by_min, (uint32_t)j1);
+            if (j0 < (int)kept && !(e0 >= (double)cut.min_p)) atomicMin(&s.by_min, (uint32_t)j0);
+            if (j1 < (int)kept && !(e1 >= (double)cut.min_p)) atomicMin(&s.by_min, (uint32_t)j1);
             __syncthreads();
-            const uint32_t f = s.list.by_min;
-            if (f < kept) { kept = max(f, 1u); open = false; }
+            // (behind an undecided top-k, top-p may keep fewer than min-p does)
+            if (s.by_min < kept && (sure || !(cut.top_p < 1.0f))) { kept = max(s.by_min, 1u); open = false; sure = true; }
         }
-        if (done && !(open && (cut.top_p < 1.0f || cut.min_p > 0.0f))) {
+        if (sure && !(open && (cut.top_p < 1.0f || cut.min_p > 0.0f))) {
             __syncthreads();
             if (!open) {
-                if (j0 == (int)kept - 1) s.list.total = c0;
-                if (j1 == (int)kept - 1) s.list.total = c1;
+                if (j0 == (int)kept - 1) s.total = c0;
+                if (j1 == (int)kept - 1) s.total = c1;
             }
             __syncthreads();
-            total = s.list.total;
-            const double t = cut.u * total;
-            if (j0 < (int)kept && c0 > t) atomicMin(&s.list.at, (uint32_t)j0);
-            if (j1 < (int)kept && c1 > t) atomicMin(&s.list.at, (uint32_t)j1);
+            const double t = cut.u * s.total;
+            if (j0 < (int)kept && c0 > t) atomicMin(&s.at, (uint32_t)j0);
+            if (j1 < (int)kept && c1 > t) atomicMin(&s.at, (uint32_t)j1);
             __syncthreads();
-            const uint32_t at = s.list.at;
-            done = at != 0xffffffffu;
-            if (done && (j0 == (int)at || j1 == (int)at)) {
-                a.tokens[tok] = (int32_t)~(uint32_t)s.list.sorted[at];
-                if (a.probs) a.probs[tok] = (float)((j0 == (int)at ? e0 : e1) / total);
+            const uint32_t at = s.at;
+            if (j0 == (int)at || j1 == (int)at) {
+                a.tokens[tok] = entry_token(s.list.sorted[at]);
+                if (a.probs) a.probs[tok] = (float)((j0 == (int)at ? e0 : e1) / s.total);
             }
-        } else {
-            done = false;
+            if (at != 0xffffffffu) return;
         }
     }
-    if (done) return;
+    // undecided: step 3
+    if (tid == 0) s.rest = atomicAdd(a.n_rest, 1u);
     __syncthreads();
-    sample_row<T>(a, tok, kmax, cut, ms, s.row);
+    RestRow &r = ((RestRow *)a.rest)[s.rest];
+    for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { r.cnt[i] = 0; r.mass[i] = 0; }
+    if (tid == 0) {
+        r.tok = tok;
+        r.vmax = vmax;
+        r.parts = 0;
+    }
 }
 
-// slices of a row, candidates a slice keeps room for, and the rank of its bound
+// ---------------------------------------------------------------------------
+// slices of a row, candidates that a slice has room for, and lanes above its bound
 struct SamplePlan {
     int slices, cap, keep;
 };
 static SamplePlan sample_plan(int V) {
     SamplePlan p;
     p.slices = (V + SLICE - 1) / SLICE;
-    // of SLICE_THREADS maxima over runs of random values, those above the value that x of them exceed on
-    // average: 1 - exp(-x / threads)
-    const double want = (double)SLICE_KEEP / p.slices;
-    p.keep = (int)ceil(SLICE_THREADS * (1.0 - exp(-want / SLICE_THREADS)));
-    p.keep = p.keep < 8 ? 8 : p.keep;
-    p.cap = (2 * (int)want + 64 + 15) / 16 * 16;
+    const int want = p.slices >= 64 ? 8 : p.slices >= 25 ? 16 : 400 / p.slices;
+    // of 64 maxima over runs of random values, those above the value that `want` of all exceed
+    p.keep = (int)ceil(64.0 * (1.0 - exp(-want / 64.0)));
+    p.cap = (2 * want + 32 + 15) / 16 * 16;
     return p;
 }
 
-size_t sample_ws_bytes(int n_tok, int V) {
+struct SampleWs {
+    size_t lists, heads, rest, n_rest, total;
+};
+static SampleWs sample_ws(int n_tok, int V) {
     const SamplePlan p = sample_plan(V);
-    return (size_t)n_tok * p.slices * (sizeof(SliceHead) + 8 * (size_t)p.cap);
+    SampleWs w;
+    size_t o = 0;
+    w.lists = o; o += (size_t)n_tok * p.slices * 8 * p.cap;
+    w.heads = o; o += (size_t)n_tok * p.slices * sizeof(SliceHead);
+    w.rest = o; o += (size_t)n_tok * sizeof(RestRow);
+    w.n_rest = o; o += 8;
+    w.total = o;
+    return w;
 }
+size_t sample_ws_bytes(int n_tok, int V) { return sample_ws(n_tok, V).total; }
 
 template <int T>
 static hipError_t launch_sample_t(const SampleArgs &a, hipStream_t st) {
-    hipLaunchKernelGGL(sample_slice_kernel<T>, dim3((unsigned)a.n_tok * (unsigned)a.slices), dim3(SLICE_THREADS), 0, st, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    const int64_t waves = (int64_t)a.n_tok * a.slices;
+    hipLaunchKernelGGL(sample_slice_kernel<T>, dim3((unsigned)((waves + SLICE_WAVES - 1) / SLICE_WAVES)),
+                       dim3(64 * SLICE_WAVES), 0, st, a);
     hipLaunchKernelGGL(sample_pick_kernel<T>, dim3((unsigned)a.n_tok), dim3(SMP_THREADS), 0, st, a);
+    hipLaunchKernelGGL(sample_rest_kernel<T>, dim3(REST_GRID), dim3(SMP_THREADS), 0, st, a);
     return hipGetLastError();
 }
 
 hipError_t launch_sample(SampleArgs a, void *ws, hipStream_t st) {
     const SamplePlan p = sample_plan(a.V);
+    const SampleWs w = sample_ws(a.n_tok, a.V);
     a.slices = p.slices;
     a.cap = p.cap;
     a.keep = p.keep;
-    a.lists = ws;
-    a.heads = (uint8_t *)ws + (size_t)a.n_tok * p.slices * 8 * p.cap;
+    a.lists = (uint8_t *)ws + w.lists;
+    a.heads = (uint8_t *)ws + w.heads;
+    a.rest = (uint8_t *)ws + w.rest;
+    a.n_rest = (uint32_t *)((uint8_t *)ws + w.n_rest);
     return a.type == T_F32 ? launch_sample_t<T_F32>(a, st)
          : a.type == T_BF16 ? launch_sample_t<T_BF16>(a, st) : launch_sample_t<T_F16>(a, st);
 }
