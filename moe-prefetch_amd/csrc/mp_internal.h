@@ -346,7 +346,7 @@ struct SampleArgs {
     int top_k_all;
     int32_t *tokens;
     float *probs;
-    int slices, cap, keep;      // set by the launcher, and the workspace's parts
+    int slices, cap, cap_log, keep;     // set by the launcher, and the workspace's parts
     void *heads, *lists, *rest;
     uint32_t *n_rest;
 };

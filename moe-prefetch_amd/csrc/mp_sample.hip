@@ -22,9 +22,11 @@
 
 namespace mp {
 
-constexpr int SMP_THREADS = 1024, SMP_WAVES = SMP_THREADS / 64;
+constexpr int SMP_THREADS = 512, SMP_WAVES = SMP_THREADS / 64;
 constexpr int SMP_BINS = 2048;
 constexpr int SMP_LIST = 2048;                        // tokens that a workgroup sorts
+constexpr int SMP_PER = SMP_LIST / SMP_THREADS;       // of them, or of the bins, to a thread
+static_assert(SMP_BINS == SMP_LIST, "bins and tokens to a thread");
 constexpr int SLICE_WAVES = 4, SLICE_EPT = 64, SLICE = 64 * SLICE_EPT, SLICES_MAX = 256;
 constexpr int REST_PARTS = 8, REST_GRID = 256;
 
@@ -125,7 +127,7 @@ struct SliceHead {
 // likely tokens spread over them.  The bound is the value that about `keep` lanes' maxima
 // reach (a bisection; any value would do); should more than `cap` logits lie above it, a higher one.
 template <int T>
-__global__ __launch_bounds__(64 * SLICE_WAVES) void sample_slice_kernel(SampleArgs a) {
+__global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(SampleArgs a) {
     typedef typename Elem<T>::raw raw;
     constexpr int VEC = 16 / sizeof(raw), NV = SLICE_EPT / VEC;
     __shared__ double s_tab[64];
@@ -179,32 +181,22 @@ __global__ __launch_bounds__(64 * SLICE_WAVES) void sample_slice_kernel(SampleAr
     const float vmax = wave_max(m);
     SliceHead h{};
     h.vmax = vmax;
-    SliceHead *head = (SliceHead *)a.heads + id;
-    if (!(cut.temp > 0.0f)) {
-        uint32_t at = 0xffffffffu;
-#pragma unroll
-        for (int j = SLICE_EPT - 1; j >= 0; --j)
-            if (v[j] == vmax) at = (uint32_t)(i0 + (j / VEC) * step + j % VEC);
-        for (int o = 32; o > 0; o >>= 1) at = min(at, (uint32_t)__shfl_xor(at, o, 64));
-        h.at = at;
-        if (lane == 0) *head = h;
-        return;
-    }
-    if (!(cut.top_k > 0 && cut.top_k < a.V)) {        // the row's whole mass counts
+    const bool greedy = !(cut.temp > 0.0f);
+    if (!greedy && !(cut.top_k > 0 && cut.top_k < a.V)) {         // the row's whole mass counts
         const double c = exp64_scale(cut.temp), vm = (double)vmax;
-        double sum[4] = {};
+        double sum[2] = {};
 #pragma unroll
-        for (int j = 0; j < SLICE_EPT; ++j) sum[j & 3] += exp64(((double)v[j] - vm) * c, s_tab);
-        double t = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        for (int j = 0; j < SLICE_EPT; ++j) sum[j & 1] += exp64(((double)v[j] - vm) * c, s_tab);
+        double t = sum[0] + sum[1];
         for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
         h.mass = t;
     }
     uint64_t *list = (uint64_t *)a.lists + (size_t)id * a.cap;
     const uint32_t mk = sort_key(m), top = (uint32_t)__builtin_amdgcn_readfirstlane((int)sort_key(vmax));
-    int keep = a.keep;
+    int keep = greedy ? 1 : a.keep;
     for (;;) {
         uint32_t lo = KEY_NONE, hi = top;             // at least keep lanes reach lo
-        if (keep > 1 && vmax > -INFINITY) {
+        if (keep > 1) {
             for (int it = 0; it < 20 && hi > lo; ++it) {
                 const uint32_t mid = hi - (hi - lo) / 2;
                 const int c = __popcll(__ballot(mk >= mid));
@@ -215,21 +207,41 @@ __global__ __launch_bounds__(64 * SLICE_WAVES) void sample_slice_kernel(SampleAr
         } else {
             lo = top;
         }
-        const float bound = key_value(lo);
-        uint32_t n = 0;
+        // the lane's logits from the bound on, the last in bit 0 (all that are on above a bound of -inf)
+        const float bound = lo > KEY_NONE ? key_value(lo) : -__FLT_MAX__;
+        uint64_t in = 0;
 #pragma unroll
-        for (int j = 0; j < SLICE_EPT; ++j) {
-            const bool in = v[j] >= bound && v[j] > -INFINITY;
-            const uint64_t b = __ballot(in);
-            if (b) {
-                const uint32_t p = n + (uint32_t)__popcll(b & ((1ull << lane) - 1));
-                if (in && p < (uint32_t)a.cap) list[p] = entry(v[j], (uint32_t)(i0 + (j / VEC) * step + j % VEC));
-                n += (uint32_t)__popcll(b);
-            }
+        for (int half = 0; half < 2; ++half) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w = 2 * w + (v[32 * half + j] >= bound);
+            in = (in << 32) | w;
         }
-        h.n = n;
+        int n = __popcll(in);
+        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+        if (greedy) {
+            const int j = __clzll((long long)in);
+            uint32_t at = in ? (uint32_t)(i0 + (j / VEC) * step + j % VEC) : 0xffffffffu;
+            for (int o = 32; o > 0; o >>= 1) at = min(at, (uint32_t)__shfl_xor(at, o, 64));
+            h.at = at;
+            break;
+        }
+        h.n = (uint32_t)n;
         h.bound = lo > KEY_NONE ? lo : 0;
-        if (n <= (uint32_t)a.cap) break;
+        if (n <= a.cap) {
+            // few lanes have any: their values are read again rather than picked from 64 registers
+            uint32_t p = 0;
+            for (uint64_t b = __ballot(in != 0); b; b = __ballot(in != 0)) {
+                if (in) {
+                    const int j = __clzll((long long)in);
+                    const uint32_t i = (uint32_t)(i0 + (j / VEC) * step + j % VEC);
+                    list[p + (uint32_t)__popcll(b & ((1ull << lane) - 1))] = entry(Elem<T>::load(l[i]), i);
+                    in &= ~(0x8000000000000000ull >> j);
+                }
+                p += (uint32_t)__popcll(b);
+            }
+            break;
+        }
         if (keep <= 1) {                              // more equal maxima than that
             h.n = 0;
             h.bound = 0xffffffffu;
@@ -237,7 +249,7 @@ __global__ __launch_bounds__(64 * SLICE_WAVES) void sample_slice_kernel(SampleAr
         }
         keep = keep / 4;
     }
-    if (lane == 0) *head = h;
+    if (lane == 0) ((SliceHead *)a.heads)[id] = h;
 }
 
 // ---------------------------------------------------------------------------
@@ -247,18 +259,40 @@ struct SampleList {
     uint64_t raw[SMP_LIST], sorted[SMP_LIST];
     uint32_t n;
 };
-// sorted[0 .. n) = raw[0 .. n) in descending order (the entries differ): each entry's rank, four lanes counting
+// sorted[0 .. n) = raw[0 .. n) in descending order (the entries differ).  Up to 256 entries by each one's rank, four lanes
+// counting; more by a bitonic network, whose strides below 64 stay within a wave's 128 entries and need no barrier.
 __device__ inline void sort_list(SampleList &s, int n) {
+    const int tid = threadIdx.x;
     __syncthreads();
-    for (int i0 = 0; i0 < n; i0 += SMP_THREADS / 4) {
-        const int i = i0 + ((int)threadIdx.x >> 2);
-        const uint64_t mine = s.raw[min(i, n - 1)];
-        int rank = 0;
-        for (int j = threadIdx.x & 3; j < n; j += 4) rank += s.raw[j] > mine;
-        rank += dpp_i<DPP_XOR1>(rank);
-        rank += dpp_i<DPP_XOR2>(rank);
-        if ((threadIdx.x & 3) == 0 && i < n) s.sorted[rank] = mine;
+    if (n <= 256) {
+        for (int i0 = 0; i0 < n; i0 += SMP_THREADS / 4) {
+            const int i = i0 + (tid >> 2);
+            const uint64_t mine = s.raw[min(i, n - 1)];
+            int rank = 0;
+            for (int j = tid & 3; j < n; j += 4) rank += s.raw[j] > mine;
+            rank += dpp_i<DPP_XOR1>(rank);
+            rank += dpp_i<DPP_XOR2>(rank);
+            if ((tid & 3) == 0 && i < n) s.sorted[rank] = mine;
+        }
+        __syncthreads();
+        return;
     }
+    const int m = 1 << (32 - __clz(n - 1));           // 512, 1024 or 2048
+    for (int i = tid; i < m; i += SMP_THREADS) s.sorted[i] = i < n ? s.raw[i] : 0;
+    __syncthreads();
+    for (int k = 2; k <= m; k <<= 1)
+        for (int d = k / 2; d > 0; d >>= 1) {
+            for (int p = tid; p < m / 2; p += SMP_THREADS) {
+                const int i = 2 * p - (p & (d - 1));  // pairs (i, i + d)
+                const uint64_t x = s.sorted[i], y = s.sorted[i + d];
+                if ((x < y) == ((i & k) == 0)) {
+                    s.sorted[i] = y;
+                    s.sorted[i + d] = x;
+                }
+            }
+            if (d >= 128 || (d == 1 && k >= 128)) __syncthreads();
+            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
     __syncthreads();
 }
 
@@ -306,22 +340,36 @@ struct Row {
     int V;
     __device__ float at(int i) const { return Elem<T>::load(l[i]); }
     // f(value, index) of every token that is on, of [i0, i1) (i0 a multiple of 8)
-    template <class F>
-    __device__ void each(int i0, int i1, F f) const {
-        constexpr int VEC = 16 / sizeof(raw), U = 4;
+    // U vectors of 16 bytes in flight to a thread: 8 (64 KiB) for a plain comparison
+    template <int U, class F>
+    __device__ inline void each(int i0, int i1, F f) const {
+        constexpr int VEC = 16 / sizeof(raw);
         if ((uintptr_t)l % 16 == 0) {
             int i = i0 + (int)threadIdx.x * VEC;
-            for (; i + (U - 1) * SMP_THREADS * VEC + VEC <= i1; i += U * SMP_THREADS * VEC) {
+            for (; i < i1; i += U * SMP_THREADS * VEC) {
                 uint4 q[U];
 #pragma unroll
-                for (int k = 0; k < U; ++k) q[k] = *(const uint4 *)(l + i + k * SMP_THREADS * VEC);
+                for (int k = 0; k < U; ++k) {
+                    const int j = i + k * SMP_THREADS * VEC;
+                    if (j + VEC <= i1) {
+                        q[k] = *(const uint4 *)(l + j);
+                    } else {
+                        raw t[VEC];
 #pragma unroll
-                for (int k = 0; k < U; ++k) some(q[k], i + k * SMP_THREADS * VEC, f);
-            }
-            for (; i + VEC <= i1; i += SMP_THREADS * VEC) some(*(const uint4 *)(l + i), i, f);
-            for (int j = i; j < min(i + VEC, i1); ++j) {
-                const float v = at(j);
-                if (v > -INFINITY) f(v, j);
+                        for (int e = 0; e < VEC; ++e) t[e] = j + e < i1 ? l[j + e] : Elem<T>::store(-INFINITY);
+                        __builtin_memcpy(&q[k], t, 16);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    raw t[VEC];
+                    __builtin_memcpy(t, &q[k], 16);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float v = Elem<T>::load(t[e]);
+                        if (v > -INFINITY) f(v, i + k * SMP_THREADS * VEC + e);
+                    }
+                }
             }
         } else {
             for (int i = i0 + (int)threadIdx.x; i < i1; i += SMP_THREADS) {
@@ -330,21 +378,8 @@ struct Row {
             }
         }
     }
-    template <class F>
-    __device__ void each(F f) const { each(0, V, f); }
-
-private:
-    template <class F>
-    __device__ void some(uint4 q, int i, F f) const {
-        constexpr int VEC = 16 / sizeof(raw);
-        raw t[VEC];
-        __builtin_memcpy(t, &q, 16);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float v = Elem<T>::load(t[e]);
-            if (v > -INFINITY) f(v, i + e);
-        }
-    }
+    template <int U, class F>
+    __device__ inline void each(F f) const { each<U>(0, V, f); }
 };
 
 __device__ inline uint64_t block_sum_u64(uint64_t v, SampleShared &s) {
@@ -363,6 +398,7 @@ __device__ inline uint64_t block_sum_u64(uint64_t v, SampleShared &s) {
 // Where the running count or mass of the order first reaches a target >= 1: the
 // key there, the count and mass before it (before its first equal), and the token, or -1 if it is
 // yet to be looked up among the equal ones.
+constexpr int32_t CUT_FULL = -2;                      // as token: more entries in the bin than can be sorted
 struct Cut {
     uint32_t key;
     int32_t token;
@@ -372,18 +408,18 @@ struct Cut {
 // by a radix search: three levels of 11, 11 and 10 key bits, whatever the values are
 template <int T>
 struct RadixSearch {
-    const Row<T> &row;
-    const Mass &ms;
+    Row<T> row;
+    Mass ms;
     SampleShared &s;
     __device__ void totals(uint64_t &n, uint64_t &m) const {
         uint64_t c = 0, sum = 0;
-        row.each([&](float v, int) { ++c; sum += ms.fixed(sort_key(v)); });
+        row.template each<1>([&](float v, int) { ++c; sum += ms.fixed(sort_key(v)); });
         n = block_sum_u64(c, s);
         m = block_sum_u64(sum, s);
     }
     __device__ uint64_t mass_from(uint32_t key) const {
         uint64_t sum = 0;
-        row.each([&](float v, int) { const uint32_t k = sort_key(v); if (k >= key) sum += ms.fixed(k); });
+        row.template each<1>([&](float v, int) { const uint32_t k = sort_key(v); if (k >= key) sum += ms.fixed(k); });
         return block_sum_u64(sum, s);
     }
     __device__ Cut find(bool by_mass, uint64_t target) const {
@@ -397,7 +433,7 @@ struct RadixSearch {
             __syncthreads();
             for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { s.cnt[i] = 0; s.mass[i] = 0; }
             __syncthreads();
-            row.each([&](float v, int) {
+            row.template each<1>([&](float v, int) {
                 const uint32_t k = sort_key(v);
                 if (level && (k >> up) != (fixed_bits >> up)) return;
                 const uint32_t b = mask - ((k >> sh) & mask);      // bin 0: the largest
@@ -414,15 +450,20 @@ struct RadixSearch {
     }
     // the bin that holds the target, and the count and mass before it
     static __device__ void find_bin(SampleShared &s, bool by_mass, uint64_t target, uint64_t n0, uint64_t m0) {
-        const int b = 2 * (int)threadIdx.x;
-        const uint64_t c0 = s.cnt[b], c1 = s.cnt[b + 1], q0 = s.mass[b], q1 = s.mass[b + 1];
-        const uint64_t cb = n0 + block_before<uint64_t>(c0 + c1, s.wc), mb = m0 + block_before<uint64_t>(q0 + q1, s.wm);
-        const uint64_t before = by_mass ? mb : cb, mid = before + (by_mass ? q0 : c0), end = mid + (by_mass ? q1 : c1);
-        if (before < target && target <= end) {
-            const bool first = target <= mid;
-            s.found_bin = (uint32_t)(first ? b : b + 1);
-            s.found_c = (uint32_t)(first ? cb : cb + c0);
-            s.found_m = first ? mb : mb + q0;
+        const int b = SMP_PER * (int)threadIdx.x;
+        uint64_t c = 0, m = 0;
+        for (int j = 0; j < SMP_PER; ++j) { c += s.cnt[b + j]; m += s.mass[b + j]; }
+        c = n0 + block_before<uint64_t>(c, s.wc);
+        m = m0 + block_before<uint64_t>(m, s.wm);
+        for (int j = 0; j < SMP_PER; ++j) {
+            const uint64_t before = by_mass ? m : c, end = before + (by_mass ? s.mass[b + j] : s.cnt[b + j]);
+            if (before < target && target <= end) {
+                s.found_bin = (uint32_t)(b + j);
+                s.found_c = (uint32_t)c;
+                s.found_m = m;
+            }
+            c += s.cnt[b + j];
+            m += s.mass[b + j];
         }
         __syncthreads();
     }
@@ -437,18 +478,17 @@ __device__ inline float bins_per(float temp) { return (float)fmin(64.0 / (0.6931
 
 template <int T>
 struct BinSearch {
-    const Row<T> &row;
-    const Mass &ms;
+    Row<T> row;
+    Mass ms;
     SampleShared &s;
     float vmax, per;
     uint64_t n_all, m_all;
-    bool &full;                                       // a bin holds more entries than can be sorted
     __device__ void totals(uint64_t &n, uint64_t &m) const { n = n_all; m = m_all; }
     __device__ uint64_t mass_from(uint32_t key) const {
         const int b = bin_of(key_value(key), vmax, per);
         uint64_t sum = 0;
         for (int i = threadIdx.x; i < b; i += SMP_THREADS) sum += s.mass[i];
-        row.each([&](float v, int) {
+        row.template each<1>([&](float v, int) {
             const uint32_t k = sort_key(v);
             if (k >= key && bin_of(v, vmax, per) == b) sum += ms.fixed(k);
         });
@@ -459,28 +499,27 @@ struct BinSearch {
         RadixSearch<T>::find_bin(s, by_mass, target, 0, 0);
         const int b = (int)s.found_bin, n = (int)s.cnt[b];
         uint64_t nb = s.found_c, mb = s.found_m;
-        if (n > SMP_LIST) {
-            full = true;
-            return Cut{0, -1, 0, 0};
-        }
+        if (n > SMP_LIST) return Cut{0, CUT_FULL, 0, 0};
         if (threadIdx.x == 0) s.list.n = 0;
         __syncthreads();
-        row.each([&](float v, int i) {
+        row.template each<8>([&](float v, int i) {
             if (bin_of(v, vmax, per) == b) s.list.raw[atomicAdd(&s.list.n, 1u)] = entry(v, (uint32_t)i);
         });
         sort_list(s.list, n);
-        const int j = 2 * (int)threadIdx.x;
-        const uint64_t q0 = j < n ? ms.fixed(entry_key(s.list.sorted[j])) : 0;
-        const uint64_t q1 = j + 1 < n ? ms.fixed(entry_key(s.list.sorted[j + 1])) : 0;
-        mb += block_before<uint64_t>(q0 + q1, s.wm);
-        nb += (uint64_t)j;
-        const uint64_t before = by_mass ? mb : nb, mid = before + (by_mass ? q0 : (uint64_t)(j < n)),
-                       end = mid + (by_mass ? q1 : (uint64_t)(j + 1 < n));
-        if (before < target && target <= end) {
-            const bool first = target <= mid;
-            s.found_e = s.list.sorted[first ? j : j + 1];
-            s.found_c = (uint32_t)(first ? nb : nb + 1);
-            s.found_m = first ? mb : mb + q0;
+        const int j0 = SMP_PER * (int)threadIdx.x;
+        uint64_t q[SMP_PER], m = 0;
+        for (int j = 0; j < SMP_PER; ++j) m += q[j] = j0 + j < n ? ms.fixed(entry_key(s.list.sorted[j0 + j])) : 0;
+        mb += block_before<uint64_t>(m, s.wm);
+        nb += (uint64_t)j0;
+        for (int j = 0; j < SMP_PER && j0 + j < n; ++j) {
+            const uint64_t before = by_mass ? mb : nb;
+            if (before < target && target <= before + (by_mass ? q[j] : 1)) {
+                s.found_e = s.list.sorted[j0 + j];
+                s.found_c = (uint32_t)nb;
+                s.found_m = mb;
+            }
+            mb += q[j];
+            ++nb;
         }
         __syncthreads();
         return Cut{entry_key(s.found_e), entry_token(s.found_e), s.found_c, s.found_m};
@@ -490,46 +529,52 @@ struct BinSearch {
 // The row's token by a search over the whole row.  A cut's n_before and m_before may stand before the first of the
 // equal keys (a radix search) or right before the token itself: (target - before) counts on from there either way.
 template <int T, class Search>
-__device__ bool sample_row(const SampleArgs &a, int64_t tok, uint32_t kmax, const SampleCuts &cut, const Mass &ms,
-                           const Row<T> &row, const Search &search, const bool &full, SampleShared &s) {
+__device__ inline bool sample_row(const SampleArgs &a, int64_t tok, uint32_t kmax, const SampleCuts &cut, const Search search,
+                                  SampleShared &s) {
+    const Row<T> row = search.row;
+    const Mass ms = search.ms;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t on, total;
+    uint64_t on, total, t = 0;
     search.totals(on, total);
     uint32_t cut_key = 0;
-    if (cut.top_k > 0 && cut.top_k < a.V && (uint64_t)cut.top_k < on) {
-        const Cut c = search.find(false, (uint64_t)cut.top_k);
-        if (full) return false;
-        cut_key = c.key;
-        total = c.m_before + ((uint64_t)cut.top_k - c.n_before) * ms.fixed(c.key);
-    }
-    if (cut.top_p < 1.0f) {
-        const double want = ceil((double)fmaxf(cut.top_p, 0.0f) * (double)total);
-        const uint64_t m = want >= (double)total ? total : max((uint64_t)want, (uint64_t)1);
-        const Cut c = search.find(true, m);
-        if (full) return false;
-        const uint64_t f = ms.fixed(c.key);
-        cut_key = c.key;
-        total = c.m_before + (m - c.m_before + f - 1) / f * f;
-    }
-    if (cut.min_p > 1.0f) {
-        total = ms.fixed(kmax);
-    } else if (cut.min_p > 0.0f) {
-        // the lowest key with e >= min_p, 64 ways a step
-        uint32_t lo = KEY_NONE, hi = kmax;
-        while (hi - lo > 1) {
-            const uint32_t mid = lo + (uint32_t)(((uint64_t)(hi - lo) * (uint32_t)(lane + 1)) >> 6);
-            const uint64_t ge = __ballot(mid >= hi || (mid > lo && ms.e(mid) >= (double)cut.min_p));
-            const int f = __ffsll((unsigned long long)ge) - 1;      // lane 63's mid is hi
-            const uint32_t nhi = __shfl(mid, f, 64);
-            const uint32_t nlo = f ? __shfl(mid, f - 1, 64) : lo;
-            lo = nlo;
-            hi = nhi;
+    Cut c{};
+    for (int step = 0; step < 3; ++step) {            // top-k, top-p, the draw
+        uint64_t target;
+        if (step == 0) {
+            if (!(cut.top_k > 0 && cut.top_k < a.V && (uint64_t)cut.top_k < on)) continue;
+            target = (uint64_t)cut.top_k;
+        } else if (step == 1) {
+            if (!(cut.top_p < 1.0f)) continue;
+            const double want = ceil((double)fmaxf(cut.top_p, 0.0f) * (double)total);
+            target = want >= (double)total ? total : max((uint64_t)want, (uint64_t)1);
+        } else {
+            if (cut.min_p > 1.0f) {
+                total = ms.fixed(kmax);
+            } else if (cut.min_p > 0.0f) {
+                // the lowest key with e >= min_p, 64 ways a step
+                uint32_t lo = KEY_NONE, hi = kmax;
+                while (hi - lo > 1) {
+                    const uint32_t mid = lo + (uint32_t)(((uint64_t)(hi - lo) * (uint32_t)(lane + 1)) >> 6);
+                    const uint64_t ge = __ballot(mid >= hi || (mid > lo && ms.e(mid) >= (double)cut.min_p));
+                    const int f = __ffsll((unsigned long long)ge) - 1;      // lane 63's mid is hi
+                    const uint32_t nhi = __shfl(mid, f, 64);
+                    const uint32_t nlo = f ? __shfl(mid, f - 1, 64) : lo;
+                    lo = nlo;
+                    hi = nhi;
+                }
+                if (hi > cut_key) total = search.mass_from(hi);
+            }
+            t = min((uint64_t)(cut.u * (double)total), total - 1);
+            target = t + 1;
         }
-        if (hi > cut_key) total = search.mass_from(hi);
+        c = search.find(step > 0, target);
+        if (c.token == CUT_FULL) return false;
+        const uint64_t f = ms.fixed(c.key);
+        if (step < 2) {
+            cut_key = c.key;
+            total = c.m_before + (step == 0 ? (target - c.n_before) * f : (target - c.m_before + f - 1) / f * f);
+        }
     }
-    const uint64_t t = min((uint64_t)(cut.u * (double)total), total - 1);
-    const Cut c = search.find(true, t + 1);
-    if (full) return false;
     const float prob = (float)(ldexp(ms.e(c.key), ms.shift) / (double)total);
     if (c.token >= 0) {
         if (threadIdx.x == 0) {
@@ -600,7 +645,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
         for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { s.cnt[i] = 0; s.mass[i] = 0; }
         __syncthreads();
         if (vmax < INFINITY)
-            row.each(min(part * run, a.V), min((part + 1) * run, a.V), [&](float v, int) {
+            row.template each<1>(min(part * run, a.V), min((part + 1) * run, a.V), [&](float v, int) {
                 const int b = bin_of(v, vmax, per);
                 atomicAdd(&s.cnt[b], 1u);
                 atomicAdd((unsigned long long *)&s.mass[b], (unsigned long long)ms.fixed(sort_key(v)));
@@ -627,13 +672,9 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
         }
         c = block_sum_u64(c, s);
         m = block_sum_u64(m, s);
-        bool full = vmax == INFINITY;
         const uint32_t kmax = sort_key(vmax);
-        if (!full) sample_row(a, tok, kmax, cut, ms, row, BinSearch<T>{row, ms, s, vmax, per, c, m, full}, full, s);
-        if (full) {
-            const bool no = false;
-            sample_row(a, tok, kmax, cut, ms, row, RadixSearch<T>{row, ms, s}, no, s);
-        }
+        if (vmax == INFINITY || !sample_row<T>(a, tok, kmax, cut, BinSearch<T>{row, ms, s, vmax, per, c, m}, s))
+            sample_row<T>(a, tok, kmax, cut, RadixSearch<T>{row, ms, s}, s);
     }
 }
 
@@ -644,7 +685,6 @@ struct PickLds {
     SampleList list;
     double wsum[SMP_WAVES], total;
     uint32_t by_p, by_min, at, rest;
-    SliceHead head[SLICES_MAX];
     double tab[64];
 };
 
@@ -652,22 +692,41 @@ template <int T>
 __global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) {
     __shared__ PickLds s;
     const int64_t tok = blockIdx.x;
-    const int tid = threadIdx.x;
-    const SampleCuts cut = load_cuts(a, tok);
+    const int tid = threadIdx.x, lane = tid & 63;
     const SliceHead *heads = (const SliceHead *)a.heads + tok * a.slices;
+    const uint64_t *lists = (const uint64_t *)a.lists + (size_t)(tok * a.slices) * a.cap;
+    // every load first: each wave the heads of all slices, each thread its places in the slices' lists (what lies
+    // behind a list's end is read and left out)
+    constexpr int HEADS = SLICES_MAX / 64, FIRST = 8;
+    SliceHead hd[HEADS];
+    uint64_t en[FIRST];
+    uint32_t en_n[FIRST];
+    const int places = a.slices << a.cap_log;
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i)
+        if (lane + 64 * i < a.slices) hd[i] = heads[lane + 64 * i];
+        else hd[i] = SliceHead{0.0, -INFINITY, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < FIRST; ++i) {
+        const int p = tid + SMP_THREADS * i;
+        en_n[i] = p < places ? heads[p >> a.cap_log].n : 0;
+        en[i] = p < places ? lists[p] : 0;
+    }
+    const SampleCuts cut = load_cuts(a, tok);
     if (tid < 64) s.tab[tid] = EXP_TAB[tid];
-    if (tid < a.slices) s.head[tid] = heads[tid];
     if (tid == 0) {
         s.list.n = 0;
         s.by_p = s.by_min = s.at = 0xffffffffu;
     }
-    __syncthreads();
     float vmax = -INFINITY;
     uint32_t bound = 0;
-    for (int i = 0; i < a.slices; ++i) {
-        vmax = fmaxf(vmax, s.head[i].vmax);
-        bound = max(bound, s.head[i].bound);
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        vmax = fmaxf(vmax, hd[i].vmax);
+        bound = max(bound, hd[i].bound);
     }
+    vmax = wave_max(vmax);
+    for (int o = 32; o > 0; o >>= 1) bound = max(bound, (uint32_t)__shfl_xor(bound, o, 64));
     if (vmax == -INFINITY) {                          // nothing is on
         if (tid == 0) {
             a.tokens[tok] = -1;
@@ -676,10 +735,12 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) 
         return;
     }
     if (!(cut.temp > 0.0f)) {
+        uint32_t at = 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i)
+            if (hd[i].vmax == vmax) at = min(at, hd[i].at);
+        for (int o = 32; o > 0; o >>= 1) at = min(at, (uint32_t)__shfl_xor(at, o, 64));
         if (tid == 0) {
-            uint32_t at = 0xffffffffu;
-            for (int i = 0; i < a.slices; ++i)
-                if (s.head[i].vmax == vmax) at = min(at, s.head[i].at);
             a.tokens[tok] = (int32_t)at;
             if (a.probs) a.probs[tok] = 1.0f;
         }
@@ -687,30 +748,46 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) 
     }
     const Mass ms = row_mass(a, vmax, cut.temp, s.tab);
     const bool by_k = cut.top_k > 0 && cut.top_k < a.V;
-    for (int i = tid; i < a.slices * a.cap; i += SMP_THREADS) {
-        const int sl = i / a.cap, j = i - sl * a.cap;
-        if (j >= (int)s.head[sl].n) continue;
-        const uint64_t e = ((const uint64_t *)a.lists)[(size_t)(tok * a.slices) * a.cap + i];
-        if (entry_key(e) < bound) continue;
+    __syncthreads();
+    auto take = [&](uint64_t e) {
         const uint32_t at = atomicAdd(&s.list.n, 1u);
         if (at < SMP_LIST) s.list.raw[at] = e;
+    };
+    const uint32_t in_list = (1u << a.cap_log) - 1;
+#pragma unroll
+    for (int i = 0; i < FIRST; ++i) {
+        const int p = tid + SMP_THREADS * i;
+        if (((uint32_t)p & in_list) < en_n[i] && entry_key(en[i]) >= bound) take(en[i]);
+    }
+    for (int p = tid + SMP_THREADS * FIRST; p < places; p += SMP_THREADS)
+        if (((uint32_t)p & in_list) < heads[p >> a.cap_log].n) {
+            const uint64_t e = lists[p];
+            if (entry_key(e) >= bound) take(e);
+        }
+    if (tid < 64 && !by_k) {
+        double total = 0.0;
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i)
+            if (hd[i].vmax > -INFINITY) total += hd[i].mass * exp64(((double)hd[i].vmax - ms.vmax) * ms.c, s.tab);
+        for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, 64);
+        if (tid == 0) s.total = total;
     }
     __syncthreads();
     const int n = (int)s.list.n;
     if (vmax < INFINITY && n > 0 && n <= SMP_LIST) {
-        if (tid == 0) {
-            double total = 0.0;
-            if (!by_k)
-                for (int i = 0; i < a.slices; ++i)
-                    if (s.head[i].vmax > -INFINITY) total += s.head[i].mass * exp64(((double)s.head[i].vmax - ms.vmax) * ms.c, s.tab);
-            s.total = total;
-        }
         sort_list(s.list, n);
-        // running masses: thread t has entries 2t and 2t + 1
-        const int j0 = 2 * tid, j1 = j0 + 1;
-        const double e0 = j0 < n ? ms.e(entry_key(s.list.sorted[j0])) : 0.0;
-        const double e1 = j1 < n ? ms.e(entry_key(s.list.sorted[j1])) : 0.0;
-        const double c0 = block_before<double>(e0 + e1, s.wsum) + e0, c1 = c0 + e1;
+        // running masses, SMP_PER entries to a thread
+        const int j0 = SMP_PER * tid;
+        double e[SMP_PER], c[SMP_PER], sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < SMP_PER; ++j) {
+            e[j] = 0.0;
+            if (j0 + j < n) e[j] = ms.e(entry_key(s.list.sorted[j0 + j]));
+            sum += e[j];
+        }
+        double run = block_before<double>(sum, s.wsum);
+#pragma unroll
+        for (int j = 0; j < SMP_PER; ++j) c[j] = run += e[j];
         uint32_t kept = (uint32_t)n;                  // how many of the sorted entries stay
         bool open = bound != 0;                       // tokens behind them may stay, too
         bool sure = true;                             // the mass that top-p shares is known
@@ -720,41 +797,40 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) 
         } else if (by_k && open) {
             sure = false;
         }
-        if (!open) {                                  // all that stays is at hand
-            if (j0 == (int)kept - 1) s.total = c0;
-            if (j1 == (int)kept - 1) s.total = c1;
+        auto first_of = [&](uint32_t *at, auto pred) {      // the first kept entry with pred, or kept and above
+#pragma unroll
+            for (int j = SMP_PER - 1; j >= 0; --j)
+                if (j0 + j < (int)kept && pred(j)) atomicMin(at, (uint32_t)(j0 + j));
             __syncthreads();
-        }
+            return *at;
+        };
+        auto total_of_kept = [&]() {
+#pragma unroll
+            for (int j = 0; j < SMP_PER; ++j)
+                if (j0 + j == (int)kept - 1) s.total = c[j];
+            __syncthreads();
+        };
+        if (!open) total_of_kept();                   // all that stays is at hand
         if (cut.top_p < 1.0f && sure) {
             const double want = (double)fmaxf(cut.top_p, 0.0f) * s.total;
-            if (j0 < (int)kept && c0 >= want) atomicMin(&s.by_p, (uint32_t)j0);
-            if (j1 < (int)kept && c1 >= want) atomicMin(&s.by_p, (uint32_t)j1);
-            __syncthreads();
-            if (s.by_p < kept) { kept = s.by_p + 1; open = false; }
+            const uint32_t f = first_of(&s.by_p, [&](int j) { return c[j] >= want; });
+            if (f < kept) { kept = f + 1; open = false; }
         }
-        if (cut.min_p > 0.0f) {
-            if (j0 < (int)kept && !(e0 >= (double)cut.min_p)) atomicMin(&s.by_min, (uint32_t)j0);
-            if (j1 < (int)kept && !(e1 >= (double)cut.min_p)) atomicMin(&s.by_min, (uint32_t)j1);
-            __syncthreads();
-            // (behind an undecided top-k, top-p may keep fewer than min-p does)
-            if (s.by_min < kept && (sure || !(cut.top_p < 1.0f))) { kept = max(s.by_min, 1u); open = false; sure = true; }
+        // (behind an undecided top-k, top-p may keep fewer than min-p does)
+        if (cut.min_p > 0.0f && (sure || !(cut.top_p < 1.0f))) {
+            const uint32_t f = first_of(&s.by_min, [&](int j) { return !(e[j] >= (double)cut.min_p); });
+            if (f < kept) { kept = max(f, 1u); open = false; sure = true; }
         }
         if (sure && !(open && (cut.top_p < 1.0f || cut.min_p > 0.0f))) {
-            __syncthreads();
-            if (!open) {
-                if (j0 == (int)kept - 1) s.total = c0;
-                if (j1 == (int)kept - 1) s.total = c1;
-            }
-            __syncthreads();
-            const double t = cut.u * s.total;
-            if (j0 < (int)kept && c0 > t) atomicMin(&s.at, (uint32_t)j0);
-            if (j1 < (int)kept && c1 > t) atomicMin(&s.at, (uint32_t)j1);
-            __syncthreads();
-            const uint32_t at = s.at;
-            if (j0 == (int)at || j1 == (int)at) {
-                a.tokens[tok] = entry_token(s.list.sorted[at]);
-                if (a.probs) a.probs[tok] = (float)((j0 == (int)at ? e0 : e1) / s.total);
-            }
+            if (!open) total_of_kept();
+            const double t = cut.u * s.total, total = s.total;
+            const uint32_t at = first_of(&s.at, [&](int j) { return c[j] > t; });
+#pragma unroll
+            for (int j = 0; j < SMP_PER; ++j)
+                if (j0 + j == (int)at) {
+                    a.tokens[tok] = entry_token(s.list.sorted[at]);
+                    if (a.probs) a.probs[tok] = (float)(e[j] / total);
+                }
             if (at != 0xffffffffu) return;
         }
     }
@@ -773,7 +849,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) 
 // ---------------------------------------------------------------------------
 // slices of a row, candidates that a slice has room for, and lanes above its bound
 struct SamplePlan {
-    int slices, cap, keep;
+    int slices, cap_log, keep;
 };
 static SamplePlan sample_plan(int V) {
     SamplePlan p;
@@ -781,7 +857,8 @@ static SamplePlan sample_plan(int V) {
     const int want = p.slices >= 64 ? 8 : p.slices >= 25 ? 16 : 400 / p.slices;
     // of 64 maxima over runs of random values, those above the value that `want` of all exceed
     p.keep = (int)ceil(64.0 * (1.0 - exp(-want / 64.0)));
-    p.cap = (2 * want + 32 + 15) / 16 * 16;
+    p.cap_log = 5;
+    while ((1 << p.cap_log) < want + want / 2 + 24) ++p.cap_log;
     return p;
 }
 
@@ -792,7 +869,7 @@ static SampleWs sample_ws(int n_tok, int V) {
     const SamplePlan p = sample_plan(V);
     SampleWs w;
     size_t o = 0;
-    w.lists = o; o += (size_t)n_tok * p.slices * 8 * p.cap;
+    w.lists = o; o += (size_t)n_tok * p.slices << (p.cap_log + 3);
     w.heads = o; o += (size_t)n_tok * p.slices * sizeof(SliceHead);
     w.rest = o; o += (size_t)n_tok * sizeof(RestRow);
     w.n_rest = o; o += 8;
@@ -807,7 +884,7 @@ static hipError_t launch_sample_t(const SampleArgs &a, hipStream_t st) {
     hipLaunchKernelGGL(sample_slice_kernel<T>, dim3((unsigned)((waves + SLICE_WAVES - 1) / SLICE_WAVES)),
                        dim3(64 * SLICE_WAVES), 0, st, a);
     hipLaunchKernelGGL(sample_pick_kernel<T>, dim3((unsigned)a.n_tok), dim3(SMP_THREADS), 0, st, a);
-    hipLaunchKernelGGL(sample_rest_kernel<T>, dim3(REST_GRID), dim3(SMP_THREADS), 0, st, a);
+    hipLaunchKernelGGL(sample_rest_kernel<T>, dim3((unsigned)min((int64_t)REST_GRID, (int64_t)a.n_tok * REST_PARTS)), dim3(SMP_THREADS), 0, st, a);
     return hipGetLastError();
 }
 
@@ -815,7 +892,8 @@ hipError_t launch_sample(SampleArgs a, void *ws, hipStream_t st) {
     const SamplePlan p = sample_plan(a.V);
     const SampleWs w = sample_ws(a.n_tok, a.V);
     a.slices = p.slices;
-    a.cap = p.cap;
+    a.cap_log = p.cap_log;
+    a.cap = 1 << p.cap_log;
     a.keep = p.keep;
     a.lists = (uint8_t *)ws + w.lists;
     a.heads = (uint8_t *)ws + w.heads;
