@@ -28,7 +28,7 @@ constexpr int SMP_LIST = 2048;                        // tokens that a workgroup
 constexpr int SMP_PER = SMP_LIST / SMP_THREADS;       // of them, or of the bins, to a thread
 static_assert(SMP_BINS == SMP_LIST, "bins and tokens to a thread");
 constexpr int SLICE_WAVES = 4, SLICE_EPT = 64, SLICE = 64 * SLICE_EPT, SLICES_MAX = 256;
-constexpr int REST_PARTS = 8, REST_GRID = 256;
+constexpr int REST_PARTS = 16, REST_GRID = 256;
 
 // 2^(j / 64), rounded to the nearest
 __constant__ double EXP_TAB[64] = {
@@ -256,20 +256,28 @@ __global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(Sampl
 // the order of up to SMP_LIST entries, and running sums over it
 
 struct SampleList {
-    uint64_t raw[SMP_LIST], sorted[SMP_LIST];
+    __attribute__((aligned(16))) uint64_t raw[SMP_LIST], sorted[SMP_LIST];
     uint32_t n;
 };
-// sorted[0 .. n) = raw[0 .. n) in descending order (the entries differ).  Up to 256 entries by each one's rank, four lanes
-// counting; more by a bitonic network, whose strides below 64 stay within a wave's 128 entries and need no barrier.
+// sorted[0 .. n) = raw[0 .. n) in descending order (the entries differ).  Up to 1,024 entries by each one's rank, four lanes
+// counting (348 entries: 1 us against 9 of the network, whose every step waits for LDS); more by a bitonic network, whose strides below 64 stay within a wave's 128 entries and need no barrier.
 __device__ inline void sort_list(SampleList &s, int n) {
     const int tid = threadIdx.x;
     __syncthreads();
-    if (n <= 256) {
+    if (n <= 1024) {
+        for (int i = n + tid; i < (n + 31) / 32 * 32; i += SMP_THREADS) s.raw[i] = 0;
+        __syncthreads();
         for (int i0 = 0; i0 < n; i0 += SMP_THREADS / 4) {
             const int i = i0 + (tid >> 2);
             const uint64_t mine = s.raw[min(i, n - 1)];
             int rank = 0;
-            for (int j = tid & 3; j < n; j += 4) rank += s.raw[j] > mine;
+            for (int j = 2 * (tid & 3); j < n; j += 32) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 8) {
+                    const ulonglong2 q = *(const ulonglong2 *)&s.raw[j + k];
+                    rank += (q.x > mine) + (q.y > mine);
+                }
+            }
             rank += dpp_i<DPP_XOR1>(rank);
             rank += dpp_i<DPP_XOR2>(rank);
             if ((tid & 3) == 0 && i < n) s.sorted[rank] = mine;
@@ -296,28 +304,33 @@ __device__ inline void sort_list(SampleList &s, int n) {
     __syncthreads();
 }
 
-__device__ inline uint64_t shfl_up_u64(uint64_t v, int o) {
-    const uint32_t lo = __shfl_up((uint32_t)v, o, 64), hi = __shfl_up((uint32_t)(v >> 32), o, 64);
-    return ((uint64_t)hi << 32) | lo;
+template <int CTRL, int ROWS, int BANKS, class N>
+__device__ inline N scan_step(N v) {                  // v plus the lane's that CTRL names, where it is one
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, BANKS, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, BANKS, false);
+    return v + __builtin_bit_cast(N, ((uint64_t)hi << 32) | lo);
 }
-__device__ inline double shfl_up_t(double v, int o) { return __shfl_up(v, o, 64); }
-__device__ inline uint64_t shfl_up_t(uint64_t v, int o) { return shfl_up_u64(v, o); }
-// the sum of v over the threads before this one, in a fixed order
+// the sums of a wave's 64-bit values up to each lane, in a fixed order
 template <class N>
-__device__ inline N block_before(N v, N *s_w) {
+__device__ inline N wave_scan(N v) {
+    v = scan_step<0x111, 0xf, 0xf>(v);                // row_shr 1, 2, 4, 8, then the rows' last lanes
+    v = scan_step<0x112, 0xf, 0xf>(v);
+    v = scan_step<0x114, 0xf, 0xe>(v);
+    v = scan_step<0x118, 0xf, 0xc>(v);
+    v = scan_step<0x142, 0xa, 0xf>(v);
+    return scan_step<0x143, 0xc, 0xf>(v);
+}
+// the sum of v over the threads before this one
+__device__ inline uint64_t block_before(uint64_t v, uint64_t *s_w) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    N run = v;
-    for (int o = 1; o < 64; o <<= 1) {
-        const N up = shfl_up_t(run, o);
-        if (lane >= o) run += up;
-    }
+    const uint64_t run = wave_scan(v);
     __syncthreads();
     if (lane == 63) s_w[wave] = run;
     __syncthreads();
-    N before = 0;
+    uint64_t before = run - v;
     for (int w = 0; w < wave; ++w) before += s_w[w];
-    N prev = shfl_up_t(run, 1);
-    return before + (lane ? prev : (N)0);
+    return before;
 }
 
 // ---------------------------------------------------------------------------
@@ -340,36 +353,23 @@ struct Row {
     int V;
     __device__ float at(int i) const { return Elem<T>::load(l[i]); }
     // f(value, index) of every token that is on, of [i0, i1) (i0 a multiple of 8)
-    // U vectors of 16 bytes in flight to a thread: 8 (64 KiB) for a plain comparison
-    template <int U, class F>
+    // (the next vector is on its way while one is worked on)
+    template <class F>
     __device__ inline void each(int i0, int i1, F f) const {
         constexpr int VEC = 16 / sizeof(raw);
         if ((uintptr_t)l % 16 == 0) {
             int i = i0 + (int)threadIdx.x * VEC;
-            for (; i < i1; i += U * SMP_THREADS * VEC) {
-                uint4 q[U];
+            uint4 q = vec(i, i1);
+            for (; i < i1; i += SMP_THREADS * VEC) {
+                const uint4 next = vec(i + SMP_THREADS * VEC, i1);
+                raw t[VEC];
+                __builtin_memcpy(t, &q, 16);
 #pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    const int j = i + k * SMP_THREADS * VEC;
-                    if (j + VEC <= i1) {
-                        q[k] = *(const uint4 *)(l + j);
-                    } else {
-                        raw t[VEC];
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) t[e] = j + e < i1 ? l[j + e] : Elem<T>::store(-INFINITY);
-                        __builtin_memcpy(&q[k], t, 16);
-                    }
+                for (int e = 0; e < VEC; ++e) {
+                    const float v = Elem<T>::load(t[e]);
+                    if (v > -INFINITY) f(v, i + e);
                 }
-#pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    raw t[VEC];
-                    __builtin_memcpy(t, &q[k], 16);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float v = Elem<T>::load(t[e]);
-                        if (v > -INFINITY) f(v, i + k * SMP_THREADS * VEC + e);
-                    }
-                }
+                q = next;
             }
         } else {
             for (int i = i0 + (int)threadIdx.x; i < i1; i += SMP_THREADS) {
@@ -378,17 +378,67 @@ struct Row {
             }
         }
     }
-    template <int U, class F>
-    __device__ inline void each(F f) const { each<U>(0, V, f); }
+    template <class F>
+    __device__ inline void each(F f) const { each(0, V, f); }
+    // f(value, index) of the few tokens of [from, to]: 64 tokens to a thread at a time become a mask (three
+    // instructions each; a branch for each took 170 clocks), whose values are read again
+    template <class F>
+    __device__ inline void among(float from, float to, F f) const {
+        constexpr int VEC = 16 / sizeof(raw), NV = 64 / VEC;
+        const bool vectors = (uintptr_t)l % 16 == 0;
+        const int step = vectors ? SMP_THREADS * VEC : SMP_THREADS, group = vectors ? VEC : 1;
+        for (int i0 = (int)threadIdx.x * group; i0 < V; i0 += 64 / group * step) {
+            uint64_t in = 0;
+            if (vectors) {
+                uint4 q[NV];
+#pragma unroll
+                for (int k = 0; k < NV; ++k) q[k] = vec(i0 + k * step, V);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t w = 0;
+#pragma unroll
+                    for (int k = half * NV / 2; k < (half + 1) * NV / 2; ++k) {
+                        raw t[VEC];
+                        __builtin_memcpy(t, &q[k], 16);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            const float v = Elem<T>::load(t[e]);
+                            w = 2 * w + (__builtin_amdgcn_fmed3f(v, from, to) == v);
+                        }
+                    }
+                    in = (in << 32) | w;
+                }
+            } else {
+                for (int k = 0; k < 64; ++k) {
+                    const int i = i0 + k * step;
+                    const float v = i < V ? at(i) : -INFINITY;
+                    in = 2 * in + (v >= from && v <= to);
+                }
+            }
+            for (; in; in &= ~(0x8000000000000000ull >> __clzll((long long)in))) {
+                const int k = __clzll((long long)in), i = i0 + k / group * step + k % group;
+                f(at(i), i);
+            }
+        }
+    }
+
+private:
+    __device__ inline uint4 vec(int i, int i1) const {            // -inf from i1 on
+        constexpr int VEC = 16 / sizeof(raw);
+        if (i + VEC <= i1) return *(const uint4 *)(l + i);
+        uint4 q;
+        raw t[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) t[e] = i + e < i1 ? l[i + e] : Elem<T>::store(-INFINITY);
+        __builtin_memcpy(&q, t, 16);
+        return q;
+    }
 };
 
-__device__ inline uint64_t block_sum_u64(uint64_t v, SampleShared &s) {
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t lo = __shfl_xor((uint32_t)v, o, 64), hi = __shfl_xor((uint32_t)(v >> 32), o, 64);
-        v += ((uint64_t)hi << 32) | lo;
-    }
+__device__ inline uint64_t block_sum(uint64_t v, SampleShared &s) {
+    const uint64_t run = wave_scan(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s.wm[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) s.wm[threadIdx.x >> 6] = run;
     __syncthreads();
     uint64_t t = 0;
     for (int w = 0; w < SMP_WAVES; ++w) t += s.wm[w];
@@ -413,14 +463,14 @@ struct RadixSearch {
     SampleShared &s;
     __device__ void totals(uint64_t &n, uint64_t &m) const {
         uint64_t c = 0, sum = 0;
-        row.template each<1>([&](float v, int) { ++c; sum += ms.fixed(sort_key(v)); });
-        n = block_sum_u64(c, s);
-        m = block_sum_u64(sum, s);
+        row.each([&](float v, int) { ++c; sum += ms.fixed(sort_key(v)); });
+        n = block_sum(c, s);
+        m = block_sum(sum, s);
     }
     __device__ uint64_t mass_from(uint32_t key) const {
         uint64_t sum = 0;
-        row.template each<1>([&](float v, int) { const uint32_t k = sort_key(v); if (k >= key) sum += ms.fixed(k); });
-        return block_sum_u64(sum, s);
+        row.each([&](float v, int) { const uint32_t k = sort_key(v); if (k >= key) sum += ms.fixed(k); });
+        return block_sum(sum, s);
     }
     __device__ Cut find(bool by_mass, uint64_t target) const {
         const int tid = threadIdx.x;
@@ -433,7 +483,7 @@ struct RadixSearch {
             __syncthreads();
             for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { s.cnt[i] = 0; s.mass[i] = 0; }
             __syncthreads();
-            row.template each<1>([&](float v, int) {
+            row.each([&](float v, int) {
                 const uint32_t k = sort_key(v);
                 if (level && (k >> up) != (fixed_bits >> up)) return;
                 const uint32_t b = mask - ((k >> sh) & mask);      // bin 0: the largest
@@ -453,8 +503,8 @@ struct RadixSearch {
         const int b = SMP_PER * (int)threadIdx.x;
         uint64_t c = 0, m = 0;
         for (int j = 0; j < SMP_PER; ++j) { c += s.cnt[b + j]; m += s.mass[b + j]; }
-        c = n0 + block_before<uint64_t>(c, s.wc);
-        m = m0 + block_before<uint64_t>(m, s.wm);
+        c = n0 + block_before(c, s.wc);
+        m = m0 + block_before(m, s.wm);
         for (int j = 0; j < SMP_PER; ++j) {
             const uint64_t before = by_mass ? m : c, end = before + (by_mass ? s.mass[b + j] : s.cnt[b + j]);
             if (before < target && target <= end) {
@@ -476,6 +526,21 @@ __device__ inline int bin_of(float v, float vmax, float per) { return (int)fminf
 // distribution's with a deviation of 1 the fullest holds about 660
 __device__ inline float bins_per(float temp) { return (float)fmin(64.0 / (0.6931471805599453094 * (double)temp), 1e30); }
 
+// The lowest key above lo with pred, which holds from some key up to hi on: 64 ways a step.
+template <class F>
+__device__ inline uint32_t lowest_key(uint32_t lo, uint32_t hi, F pred) {
+    const int lane = threadIdx.x & 63;
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (uint32_t)(((uint64_t)(hi - lo) * (uint32_t)(lane + 1)) >> 6);
+        const uint64_t b = __ballot(mid >= hi || (mid > lo && pred(mid)));
+        const int f = __ffsll((unsigned long long)b) - 1;         // lane 63's mid is hi
+        const uint32_t nhi = (uint32_t)__builtin_amdgcn_readlane((int)mid, f);
+        if (f) lo = (uint32_t)__builtin_amdgcn_readlane((int)mid, f - 1);
+        hi = nhi;
+    }
+    return hi;
+}
+
 template <int T>
 struct BinSearch {
     Row<T> row;
@@ -488,11 +553,11 @@ struct BinSearch {
         const int b = bin_of(key_value(key), vmax, per);
         uint64_t sum = 0;
         for (int i = threadIdx.x; i < b; i += SMP_THREADS) sum += s.mass[i];
-        row.template each<1>([&](float v, int) {
+        row.each([&](float v, int) {
             const uint32_t k = sort_key(v);
             if (k >= key && bin_of(v, vmax, per) == b) sum += ms.fixed(k);
         });
-        return block_sum_u64(sum, s);
+        return block_sum(sum, s);
     }
     __device__ Cut find(bool by_mass, uint64_t target) const {
         __syncthreads();
@@ -502,14 +567,16 @@ struct BinSearch {
         if (n > SMP_LIST) return Cut{0, CUT_FULL, 0, 0};
         if (threadIdx.x == 0) s.list.n = 0;
         __syncthreads();
-        row.template each<8>([&](float v, int i) {
-            if (bin_of(v, vmax, per) == b) s.list.raw[atomicAdd(&s.list.n, 1u)] = entry(v, (uint32_t)i);
-        });
+        // the bin's values, so that the pass over the row only compares
+        const uint32_t kmax = sort_key(vmax);
+        const float from = key_value(lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return bin_of(key_value(k), vmax, per) <= b; }));
+        const uint32_t above = b == 0 ? kmax + 1 : lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return bin_of(key_value(k), vmax, per) < b; });
+        row.among(from, key_value(above - 1), [&](float v, int i) { s.list.raw[atomicAdd(&s.list.n, 1u)] = entry(v, (uint32_t)i); });
         sort_list(s.list, n);
         const int j0 = SMP_PER * (int)threadIdx.x;
         uint64_t q[SMP_PER], m = 0;
         for (int j = 0; j < SMP_PER; ++j) m += q[j] = j0 + j < n ? ms.fixed(entry_key(s.list.sorted[j0 + j])) : 0;
-        mb += block_before<uint64_t>(m, s.wm);
+        mb += block_before(m, s.wm);
         nb += (uint64_t)j0;
         for (int j = 0; j < SMP_PER && j0 + j < n; ++j) {
             const uint64_t before = by_mass ? mb : nb;
@@ -551,17 +618,7 @@ __device__ inline bool sample_row(const SampleArgs &a, int64_t tok, uint32_t kma
             if (cut.min_p > 1.0f) {
                 total = ms.fixed(kmax);
             } else if (cut.min_p > 0.0f) {
-                // the lowest key with e >= min_p, 64 ways a step
-                uint32_t lo = KEY_NONE, hi = kmax;
-                while (hi - lo > 1) {
-                    const uint32_t mid = lo + (uint32_t)(((uint64_t)(hi - lo) * (uint32_t)(lane + 1)) >> 6);
-                    const uint64_t ge = __ballot(mid >= hi || (mid > lo && ms.e(mid) >= (double)cut.min_p));
-                    const int f = __ffsll((unsigned long long)ge) - 1;      // lane 63's mid is hi
-                    const uint32_t nhi = __shfl(mid, f, 64);
-                    const uint32_t nlo = f ? __shfl(mid, f - 1, 64) : lo;
-                    lo = nlo;
-                    hi = nhi;
-                }
+                const uint32_t hi = lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return ms.e(k) >= (double)cut.min_p; });
                 if (hi > cut_key) total = search.mass_from(hi);
             }
             t = min((uint64_t)(cut.u * (double)total), total - 1);
@@ -645,7 +702,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
         for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { s.cnt[i] = 0; s.mass[i] = 0; }
         __syncthreads();
         if (vmax < INFINITY)
-            row.template each<1>(min(part * run, a.V), min((part + 1) * run, a.V), [&](float v, int) {
+            row.each(min(part * run, a.V), min((part + 1) * run, a.V), [&](float v, int) {
                 const int b = bin_of(v, vmax, per);
                 atomicAdd(&s.cnt[b], 1u);
                 atomicAdd((unsigned long long *)&s.mass[b], (unsigned long long)ms.fixed(sort_key(v)));
@@ -670,8 +727,8 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
             c += s.cnt[i];
             m += s.mass[i];
         }
-        c = block_sum_u64(c, s);
-        m = block_sum_u64(m, s);
+        c = block_sum(c, s);
+        m = block_sum(m, s);
         const uint32_t kmax = sort_key(vmax);
         if (vmax == INFINITY || !sample_row<T>(a, tok, kmax, cut, BinSearch<T>{row, ms, s, vmax, per, c, m}, s))
             sample_row<T>(a, tok, kmax, cut, RadixSearch<T>{row, ms, s}, s);
@@ -681,15 +738,170 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
 // ---------------------------------------------------------------------------
 // 2: one workgroup per row
 
+constexpr int PICK_WAVES = 4, PICK_THREADS = 64 * PICK_WAVES, PICK_PER = 8, PICK_MAX = 64 * PICK_PER;
 struct PickLds {
-    SampleList list;
-    double wsum[SMP_WAVES], total;
-    uint32_t by_p, by_min, at, rest;
+    uint64_t list[SMP_LIST];                          // candidates, in no order
+    uint64_t order[PICK_MAX];                         // the front of the order
+    double cum[PICK_MAX];                             // and its running masses
     double tab[64];
+    uint32_t n, rest;
 };
 
+__device__ inline uint64_t lane_u64(uint64_t v, int l) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
+}
+__device__ inline void wave_lds() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }    // a wave's LDS accesses stay in order
+
+// All four waves read the candidates; the first one decides, without a barrier: up to 512 candidates in
+// its registers, of which it sorts the next up to 64 at a time (bounded by a bisection) until
+// the cuts and the draw fall within what is sorted.  Returns whether they did.
+__device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCuts &cut, const Mass &ms, uint32_t bound,
+                                double mass, PickLds &s) {
+    const int lane = threadIdx.x & 63;
+    const bool by_k = cut.top_k > 0 && cut.top_k < a.V;
+    int n = (int)s.n;
+    if (n == 0 || n > SMP_LIST || ms.vmax == INFINITY) return false;
+    bool open = bound != 0;                           // tokens behind the candidates may stay, too
+    uint64_t x[PICK_PER];
+    if (n <= PICK_MAX) {
+#pragma unroll
+        for (int j = 0; j < PICK_PER; ++j) x[j] = 64 * j + lane < n ? s.list[64 * j + lane] : 0;
+    } else {                                          // the largest 512 of them
+        uint64_t lo = 0, hi = ~0ull;                  // more than 512 reach lo, at most 512 reach hi
+        while (hi - lo > 1) {
+            const uint64_t mid = lo + (hi - lo) / 2;
+            int c = 0;
+            for (int j = lane; j < n; j += 64) c += s.list[j] >= mid;
+            for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+            if (c > PICK_MAX) lo = mid;
+            else hi = mid;
+            if (c == PICK_MAX) break;
+        }
+        int c = 0;
+        for (int j0 = 0; j0 < n; j0 += 64) {          // moved to the front: never past where they are read
+            const uint64_t e = j0 + lane < n ? s.list[j0 + lane] : 0;
+            const uint64_t b = __ballot(e >= hi);
+            wave_lds();
+            if (e >= hi) s.list[c + __popcll(b & ((1ull << lane) - 1))] = e;
+            wave_lds();
+            c += __popcll(b);
+        }
+        n = c;
+        open = true;
+#pragma unroll
+        for (int j = 0; j < PICK_PER; ++j) x[j] = 64 * j + lane < n ? s.list[64 * j + lane] : 0;
+    }
+    int have = 0;                                     // sorted so far
+    double sum = 0.0;                                 // their mass
+    uint64_t below = ~0ull;                           // those left are below
+    auto extend = [&]() {                             // sorts the next
+        int c = n - have;
+        uint64_t from = 1;
+        if (c > 64) {
+            // more than 64 of those left reach lo, at most 64 reach hi
+            uint64_t lo = (uint64_t)bound << 32, hi = min(below, (uint64_t)(sort_key((float)ms.vmax) + 1) << 32);
+            for (;;) {
+                const uint64_t mid = lo + (hi - lo) / 2;
+                c = 0;
+#pragma unroll
+                for (int j = 0; j < PICK_PER; ++j) c += __popcll(__ballot(x[j] >= mid));
+                if (c > 64) lo = mid;
+                else hi = mid;
+                if (hi - lo == 1 || (c <= 64 && c >= 40)) break;
+            }
+            from = hi;
+        }
+        c = 0;
+#pragma unroll
+        for (int j = 0; j < PICK_PER; ++j) {
+            const bool in = x[j] >= from;
+            const uint64_t b = __ballot(in);
+            if (in) s.order[have + c + __popcll(b & ((1ull << lane) - 1))] = x[j];
+            if (in) x[j] = 0;                         // taken
+            c += __popcll(b);
+        }
+        wave_lds();
+        const uint64_t mine = lane < c ? s.order[have + lane] : 0;
+        int rank = 0;
+#pragma unroll 16
+        for (int l = 0; l < 64; ++l) rank += lane_u64(mine, l) > mine;
+        wave_lds();
+        if (lane < c) s.order[have + rank] = mine;
+        wave_lds();
+        const uint64_t sorted = lane < c ? s.order[have + lane] : 0;
+        const double run = sum + wave_scan(lane < c ? ms.e(entry_key(sorted)) : 0.0);
+        if (lane < c) s.cum[have + lane] = run;
+        wave_lds();
+        sum = s.cum[have + c - 1];
+        below = from;
+        have += c;
+    };
+    // the first of [0, to) with pred, or to
+    auto first_of = [&](int to, auto pred) {
+        for (int j0 = 0; j0 < to; j0 += 64) {
+            const uint64_t b = __ballot(j0 + lane < to && pred(min(j0 + lane, to - 1)));
+            if (b) return j0 + __ffsll((unsigned long long)b) - 1;
+        }
+        return to;
+    };
+    auto low = [&](int j) { return !(ms.e(entry_key(s.order[j])) >= (double)cut.min_p); };
+    const double top_p = (double)fmaxf(cut.top_p, 0.0f);
+    const bool with_p = cut.top_p < 1.0f, with_min = cut.min_p > 0.0f;
+    int kept;                                         // how many of the order stay
+    double total = mass;
+    if (by_k || !open) {
+        const int k = by_k ? min(cut.top_k, n) : n;
+        while (have < k) extend();
+        kept = k;
+        if (!by_k || cut.top_k <= n || !open) {
+            total = s.cum[k - 1];
+            open = false;
+        } else if (with_p) {
+            return false;                             // a share of an unknown mass
+        }
+    } else {
+        // all candidates together may not reach far enough
+        double all = 0.0;
+        bool low_one = false;
+#pragma unroll
+        for (int j = 0; j < PICK_PER; ++j) {
+            const double e = x[j] ? ms.e(entry_key(x[j])) : 0.0;
+            all += e;
+            low_one |= x[j] && !(e >= (double)cut.min_p);
+        }
+        for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o, 64);
+        const double reach = with_p || with_min ? top_p * total : cut.u * total;
+        if (all * (1.0 + 1e-12) < reach && !(with_min && __ballot(low_one))) return false;
+        do extend();
+        while (have < n && !(with_p && sum >= top_p * total) && !(with_min && low(have - 1)) &&
+               !(!with_p && !with_min && sum > cut.u * total));
+        kept = have;
+    }
+    if (with_p) {
+        const double want = top_p * total;
+        const int f = first_of(kept, [&](int j) { return s.cum[j] >= want; });
+        if (f < kept) { kept = f + 1; open = false; }
+    }
+    if (with_min) {
+        const int f = first_of(kept, low);
+        if (f < kept) { kept = max(f, 1); open = false; }
+    }
+    if (open && (with_p || with_min || by_k)) return false;
+    if (!open) total = s.cum[kept - 1];
+    const double t = cut.u * total;
+    const int at = first_of(kept, [&](int j) { return s.cum[j] > t; });
+    if (at == kept) return false;                     // behind the candidates
+    if (lane == 0) {
+        const uint64_t e = s.order[at];
+        a.tokens[tok] = entry_token(e);
+        if (a.probs) a.probs[tok] = (float)(ms.e(entry_key(e)) / total);
+    }
+    return true;
+}
+
 template <int T>
-__global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) {
+__global__ __launch_bounds__(PICK_THREADS) void sample_pick_kernel(SampleArgs a) {
     __shared__ PickLds s;
     const int64_t tok = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -708,16 +920,13 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) 
         else hd[i] = SliceHead{0.0, -INFINITY, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < FIRST; ++i) {
-        const int p = tid + SMP_THREADS * i;
+        const int p = tid + PICK_THREADS * i;
         en_n[i] = p < places ? heads[p >> a.cap_log].n : 0;
         en[i] = p < places ? lists[p] : 0;
     }
     const SampleCuts cut = load_cuts(a, tok);
     if (tid < 64) s.tab[tid] = EXP_TAB[tid];
-    if (tid == 0) {
-        s.list.n = 0;
-        s.by_p = s.by_min = s.at = 0xffffffffu;
-    }
+    if (tid == 0) s.n = 0;
     float vmax = -INFINITY;
     uint32_t bound = 0;
 #pragma unroll
@@ -747,98 +956,42 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pick_kernel(SampleArgs a) 
         return;
     }
     const Mass ms = row_mass(a, vmax, cut.temp, s.tab);
-    const bool by_k = cut.top_k > 0 && cut.top_k < a.V;
     __syncthreads();
-    auto take = [&](uint64_t e) {
-        const uint32_t at = atomicAdd(&s.list.n, 1u);
-        if (at < SMP_LIST) s.list.raw[at] = e;
+    auto take = [&](bool in, uint64_t e) {            // one place in the list for a wave's at a time
+        const uint64_t b = __ballot(in);
+        if (!b) return;
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&s.n, (uint32_t)__popcll(b));
+        at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(b & ((1ull << lane) - 1));
+        if (in && at < SMP_LIST) s.list[at] = e;
     };
     const uint32_t in_list = (1u << a.cap_log) - 1;
 #pragma unroll
     for (int i = 0; i < FIRST; ++i) {
-        const int p = tid + SMP_THREADS * i;
-        if (((uint32_t)p & in_list) < en_n[i] && entry_key(en[i]) >= bound) take(en[i]);
+        const int p = tid + PICK_THREADS * i;
+        take(((uint32_t)p & in_list) < en_n[i] && entry_key(en[i]) >= bound, en[i]);
     }
-    for (int p = tid + SMP_THREADS * FIRST; p < places; p += SMP_THREADS)
-        if (((uint32_t)p & in_list) < heads[p >> a.cap_log].n) {
-            const uint64_t e = lists[p];
-            if (entry_key(e) >= bound) take(e);
-        }
-    if (tid < 64 && !by_k) {
-        double total = 0.0;
-#pragma unroll
-        for (int i = 0; i < HEADS; ++i)
-            if (hd[i].vmax > -INFINITY) total += hd[i].mass * exp64(((double)hd[i].vmax - ms.vmax) * ms.c, s.tab);
-        for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, 64);
-        if (tid == 0) s.total = total;
+    for (int p0 = PICK_THREADS * FIRST; p0 < places; p0 += PICK_THREADS) {
+        const int p = min(p0 + tid, places - 1);
+        const uint64_t e = lists[p];
+        take(p0 + tid < places && ((uint32_t)p & in_list) < heads[p >> a.cap_log].n && entry_key(e) >= bound, e);
     }
     __syncthreads();
-    const int n = (int)s.list.n;
-    if (vmax < INFINITY && n > 0 && n <= SMP_LIST) {
-        sort_list(s.list, n);
-        // running masses, SMP_PER entries to a thread
-        const int j0 = SMP_PER * tid;
-        double e[SMP_PER], c[SMP_PER], sum = 0.0;
+    if (tid < 64) {
+        double mass = 0.0;                            // of the row, where it counts
+        if (!(cut.top_k > 0 && cut.top_k < a.V)) {
 #pragma unroll
-        for (int j = 0; j < SMP_PER; ++j) {
-            e[j] = 0.0;
-            if (j0 + j < n) e[j] = ms.e(entry_key(s.list.sorted[j0 + j]));
-            sum += e[j];
+            for (int i = 0; i < HEADS; ++i)
+                if (hd[i].vmax > -INFINITY) mass += hd[i].mass * exp64(((double)hd[i].vmax - ms.vmax) * ms.c, s.tab);
+            for (int o = 1; o < 64; o <<= 1) mass += __shfl_xor(mass, o, 64);
         }
-        double run = block_before<double>(sum, s.wsum);
-#pragma unroll
-        for (int j = 0; j < SMP_PER; ++j) c[j] = run += e[j];
-        uint32_t kept = (uint32_t)n;                  // how many of the sorted entries stay
-        bool open = bound != 0;                       // tokens behind them may stay, too
-        bool sure = true;                             // the mass that top-p shares is known
-        if (by_k && cut.top_k <= n) {
-            kept = (uint32_t)cut.top_k;
-            open = false;
-        } else if (by_k && open) {
-            sure = false;
-        }
-        auto first_of = [&](uint32_t *at, auto pred) {      // the first kept entry with pred, or kept and above
-#pragma unroll
-            for (int j = SMP_PER - 1; j >= 0; --j)
-                if (j0 + j < (int)kept && pred(j)) atomicMin(at, (uint32_t)(j0 + j));
-            __syncthreads();
-            return *at;
-        };
-        auto total_of_kept = [&]() {
-#pragma unroll
-            for (int j = 0; j < SMP_PER; ++j)
-                if (j0 + j == (int)kept - 1) s.total = c[j];
-            __syncthreads();
-        };
-        if (!open) total_of_kept();                   // all that stays is at hand
-        if (cut.top_p < 1.0f && sure) {
-            const double want = (double)fmaxf(cut.top_p, 0.0f) * s.total;
-            const uint32_t f = first_of(&s.by_p, [&](int j) { return c[j] >= want; });
-            if (f < kept) { kept = f + 1; open = false; }
-        }
-        // (behind an undecided top-k, top-p may keep fewer than min-p does)
-        if (cut.min_p > 0.0f && (sure || !(cut.top_p < 1.0f))) {
-            const uint32_t f = first_of(&s.by_min, [&](int j) { return !(e[j] >= (double)cut.min_p); });
-            if (f < kept) { kept = max(f, 1u); open = false; sure = true; }
-        }
-        if (sure && !(open && (cut.top_p < 1.0f || cut.min_p > 0.0f))) {
-            if (!open) total_of_kept();
-            const double t = cut.u * s.total, total = s.total;
-            const uint32_t at = first_of(&s.at, [&](int j) { return c[j] > t; });
-#pragma unroll
-            for (int j = 0; j < SMP_PER; ++j)
-                if (j0 + j == (int)at) {
-                    a.tokens[tok] = entry_token(s.list.sorted[at]);
-                    if (a.probs) a.probs[tok] = (float)(e[j] / total);
-                }
-            if (at != 0xffffffffu) return;
-        }
+        const bool done = pick_row(a, tok, cut, ms, bound, mass, s);
+        if (lane == 0) s.rest = done ? 0xffffffffu : atomicAdd(a.n_rest, 1u);
     }
-    // undecided: step 3
-    if (tid == 0) s.rest = atomicAdd(a.n_rest, 1u);
     __syncthreads();
-    RestRow &r = ((RestRow *)a.rest)[s.rest];
-    for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { r.cnt[i] = 0; r.mass[i] = 0; }
+    if (s.rest == 0xffffffffu) return;
+    RestRow &r = ((RestRow *)a.rest)[s.rest];         // undecided: step 3
+    for (int i = tid; i < SMP_BINS; i += PICK_THREADS) { r.cnt[i] = 0; r.mass[i] = 0; }
     if (tid == 0) {
         r.tok = tok;
         r.vmax = vmax;
@@ -857,8 +1010,8 @@ static SamplePlan sample_plan(int V) {
     const int want = p.slices >= 64 ? 8 : p.slices >= 25 ? 16 : 400 / p.slices;
     // of 64 maxima over runs of random values, those above the value that `want` of all exceed
     p.keep = (int)ceil(64.0 * (1.0 - exp(-want / 64.0)));
-    p.cap_log = 5;
-    while ((1 << p.cap_log) < want + want / 2 + 24) ++p.cap_log;
+    p.cap_log = 4;
+    while ((1 << p.cap_log) < want + want / 4) ++p.cap_log;
     return p;
 }
 
@@ -883,7 +1036,7 @@ static hipError_t launch_sample_t(const SampleArgs &a, hipStream_t st) {
     const int64_t waves = (int64_t)a.n_tok * a.slices;
     hipLaunchKernelGGL(sample_slice_kernel<T>, dim3((unsigned)((waves + SLICE_WAVES - 1) / SLICE_WAVES)),
                        dim3(64 * SLICE_WAVES), 0, st, a);
-    hipLaunchKernelGGL(sample_pick_kernel<T>, dim3((unsigned)a.n_tok), dim3(SMP_THREADS), 0, st, a);
+    hipLaunchKernelGGL(sample_pick_kernel<T>, dim3((unsigned)a.n_tok), dim3(PICK_THREADS), 0, st, a);
     hipLaunchKernelGGL(sample_rest_kernel<T>, dim3((unsigned)min((int64_t)REST_GRID, (int64_t)a.n_tok * REST_PARTS)), dim3(SMP_THREADS), 0, st, a);
     return hipGetLastError();
 }
