@@ -1,5 +1,12 @@
 // mp_scored.hip -- routing by scores (moe_route_scored): softmax or sigmoid, a
 // selection bias, expert groups, top-k, renormalised and scaled weights.
+//
+// One wave per token; lane j holds experts NV j .. NV j + NV - 1, so that of two
+// equal values the one on the lower lane, or earlier on the same lane, has the
+// lower id.  Scores and selection values are f64: two experts' order, and a
+// group's, has to be that of the definition however near they are.  The K best
+// come out in K rounds of a wave maximum over the lanes' best; a round compares the
+// upper words and looks at the lower ones only where two lanes agree in them.
 #include <hip/hip_runtime.h>
 
 #include "mp_device.h"
@@ -22,14 +29,7 @@ __device__ inline double lane_d(double v, int l) {
     const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l);
     return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
-// maximum and sum over the wave, the same bits on every lane
-__device__ inline double wave_max_d(double v) {
-    v = fmax(v, dpp_d<DPP_XOR1>(v));
-    v = fmax(v, dpp_d<DPP_XOR2>(v));
-    v = fmax(v, dpp_d<DPP_HALF_MIRROR>(v));
-    v = fmax(v, dpp_d<DPP_MIRROR>(v));
-    return fmax(fmax(lane_d(v, 0), lane_d(v, 16)), fmax(lane_d(v, 32), lane_d(v, 48)));
-}
+// sum over the wave, the same bits on every lane
 __device__ inline double wave_sum_d(double v) {
     v = v + dpp_d<DPP_XOR1>(v);
     v = v + dpp_d<DPP_XOR2>(v);
@@ -37,36 +37,93 @@ __device__ inline double wave_sum_d(double v) {
     v = v + dpp_d<DPP_MIRROR>(v);
     return (lane_d(v, 0) + lane_d(v, 16)) + (lane_d(v, 32) + lane_d(v, 48));
 }
+// e^x for x <= 0 in 64 bits, within 2^-52: e^r to r^13 on |r| <= ln 2 / 2 (the next term is
+// below 5e-18) times a power of two, down to 0
+__device__ inline double exp_d(double x) {
+    constexpr double MAGIC = 6755399441055744.0;      // 1.5 * 2^52: adding it rounds to a whole number
+    x = fmax(x, -800.0);
+    const double m = fma(x, 1.4426950408889634074, MAGIC);
+    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, m);
+    const double f = m - MAGIC;
+    const double r = fma(f, -1.9082149292705877e-10, fma(f, -0.693147180369123816490, x));   // ln 2 in two parts
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, r, 1.0 / 479001600.0);
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, n);
+}
 
-// One wave per token; lane j holds experts NV j .. NV j + NV - 1, so that of two
-// equal values the one on the lower lane, or lower on the same lane, has the
-// lower id.  K rounds take the largest value left.
+// The order of selection values as that of unsigned 64-bit numbers: above 1 for every number but NaN, 1 for an
+// expert switched off, 0 for none.
+constexpr uint64_t KEY_OFF = 1;
+__device__ inline uint64_t value_key(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);     // -0 as +0
+    return b ^ ((b >> 63) ? ~0ull : 1ull << 63);
+}
+
+// the best two of a group that spans `lanes` (a power of two) neighbouring lanes, on each of them
+__device__ inline void best_two(double &b0, double &b1, double c0, double c1) {
+    b1 = fmax(fmin(b0, c0), fmax(b1, c1));
+    b0 = fmax(b0, c0);
+}
+__device__ inline void group_best_two(double &b0, double &b1, int lanes) {
+    // quads hold one pair after two steps, eights after three: the mirrors reach another's
+    if (lanes > 1) best_two(b0, b1, dpp_d<DPP_XOR1>(b0), dpp_d<DPP_XOR1>(b1));
+    if (lanes > 2) best_two(b0, b1, dpp_d<DPP_XOR2>(b0), dpp_d<DPP_XOR2>(b1));
+    if (lanes > 4) best_two(b0, b1, dpp_d<DPP_HALF_MIRROR>(b0), dpp_d<DPP_HALF_MIRROR>(b1));
+    if (lanes > 8) best_two(b0, b1, dpp_d<DPP_MIRROR>(b0), dpp_d<DPP_MIRROR>(b1));
+    if (lanes > 16) best_two(b0, b1, __shfl_xor(b0, 16, 64), __shfl_xor(b1, 16, 64));
+}
+
 template <int T, int NV>
 __global__ __launch_bounds__(64 * SCORED_WAVES) void route_scored_kernel(ScoredArgs a) {
-    __shared__ double s_s[SCORED_WAVES][64 * NV];     // scores (0: switched off)
-    __shared__ double s_v[SCORED_WAVES][64 * NV];     // selection values
+    __shared__ double s_s[SCORED_WAVES][64 * NV];     // scores
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row = (int64_t)blockIdx.x * SCORED_WAVES + wave;
-    const bool live = row < a.n_tok;
-    const int64_t tok = live ? row : a.n_tok - 1;
-    const typename Elem<T>::raw *l = (const typename Elem<T>::raw *)a.logits + tok * a.ld;
+    if (row >= a.n_tok) return;                       // (a wave's LDS is its own: no barrier)
+    const int64_t tok = row;
+    typedef typename Elem<T>::raw raw;
+    const raw *l = (const raw *)a.logits + tok * a.ld;
     double s[NV], v[NV];
     bool on[NV];
-    double m = -INFINITY;
+    float x[NV], bias[NV];
+    if (a.vec) {
+        struct alignas(sizeof(raw) * NV > 16 ? 16 : sizeof(raw) * NV) Vec { raw v[NV]; };
+        struct alignas(NV > 4 ? 16 : 4 * NV) Vec4 { float v[NV]; };
+        const bool in = NV * lane < a.E;
+        const Vec q = in ? ((const Vec *)l)[lane] : Vec{};
+        const Vec4 b = in && a.bias ? ((const Vec4 *)a.bias)[lane] : Vec4{};
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int e = NV * lane + j;
-        const float x = e < a.E ? Elem<T>::load(l[e]) : -INFINITY;
-        on[j] = x > -INFINITY;                        // false for a NaN
-        s[j] = on[j] ? (double)x : -INFINITY;
-        m = fmax(m, s[j]);
+        for (int j = 0; j < NV; ++j) { x[j] = in ? Elem<T>::load(q.v[j]) : -INFINITY; bias[j] = b.v[j]; }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = NV * lane + j;
+            x[j] = e < a.E ? Elem<T>::load(l[e]) : -INFINITY;
+            bias[j] = e < a.E && a.bias ? a.bias[e] : 0.0f;
+        }
     }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) on[j] = x[j] > -INFINITY;        // false for a NaN
     if (a.score == 0) {
-        m = wave_max_d(m);
+        float mf = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) mf = fmaxf(mf, x[j]);        // passes over a NaN
+        mf = wave_max(mf);
         double sum = 0.0;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            s[j] = !on[j] ? 0.0 : m == INFINITY ? (s[j] == INFINITY ? 1.0 : 0.0) : exp(s[j] - m);
+            s[j] = !on[j] ? 0.0 : mf == INFINITY ? (x[j] == INFINITY ? 1.0 : 0.0) : exp_d((double)x[j] - (double)mf);
             sum += s[j];
         }
         sum = wave_sum_d(sum);
@@ -74,91 +131,144 @@ __global__ __launch_bounds__(64 * SCORED_WAVES) void route_scored_kernel(ScoredA
         for (int j = 0; j < NV; ++j) s[j] = on[j] ? s[j] / sum : 0.0;
     } else {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) s[j] = on[j] ? 1.0 / (1.0 + exp(-s[j])) : 0.0;
+        for (int j = 0; j < NV; ++j) {
+            const double e = exp_d(-fabs((double)x[j]));
+            s[j] = on[j] ? (x[j] < 0.0f ? e : 1.0) / (1.0 + e) : 0.0;
+        }
     }
-    if (a.scores && live)
+    if (a.scores)
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (NV * lane + j < a.E) a.scores[tok * a.E + NV * lane + j] = (float)s[j];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int e = NV * lane + j;
-        v[j] = on[j] && a.bias ? s[j] + (double)a.bias[e] : s[j];
-        if (!on[j] || !(v[j] > -INFINITY)) v[j] = -INFINITY;
-        s_s[wave][e] = v[j] > -INFINITY ? s[j] : 0.0;
-        s_v[wave][e] = v[j];
+        v[j] = on[j] ? s[j] + (double)bias[j] : -INFINITY;
+        if (!(v[j] > -INFINITY)) v[j] = -INFINITY;
+        s_s[wave][NV * lane + j] = s[j];
     }
-    __syncthreads();
     if (a.groups > 1) {
         const int n = a.E / a.groups;
-        double gs = -INFINITY;                        // lane g: group g's score
-        if (lane < a.groups) {
+        if (a.group_lanes) {                          // a group is group_lanes whole lanes
             double b0 = -INFINITY, b1 = -INFINITY;
-            for (int i = 0; i < n; ++i) {
-                const double u = s_v[wave][lane * n + i];
-                b1 = u > b0 ? b0 : fmax(b1, u);
-                b0 = fmax(b0, u);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                b1 = fmax(fmin(b0, v[j]), b1);
+                b0 = fmax(b0, v[j]);
             }
-            gs = a.group_best == 2 && b1 > -INFINITY ? b0 + b1 : b0;
-        }
-        int rank = 0;
-        for (int g = 0; g < a.groups; ++g) {
-            const double o = lane_d(gs, g);
-            rank += o > gs || (o == gs && g < lane);
-        }
-        const uint64_t keep = __ballot(lane < a.groups && rank < a.top_groups);
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (!(keep >> (min(NV * lane + j, a.E - 1) / n) & 1)) {
-                v[j] = -INFINITY;
-                s_s[wave][NV * lane + j] = 0.0;
+            group_best_two(b0, b1, a.group_lanes);
+            const double gs = a.group_best == 2 && b1 > -INFINITY ? b0 + b1 : b0;
+            const int mine = lane / a.group_lanes;
+            int rank = 0;
+            for (int g = 0; g < a.groups; ++g) {
+                const double o = lane_d(gs, g * a.group_lanes);
+                rank += o > gs || (o == gs && g < mine);
             }
+            const bool stay = rank < a.top_groups;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (!stay) v[j] = -INFINITY;
+        } else {                                      // lane g looks through group g's values
+            double *sv = s_s[wave];                   // (the scores are put back below)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int j = 0; j < NV; ++j) sv[NV * lane + j] = v[j];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            double b0 = -INFINITY, b1 = -INFINITY;
+            if (lane < a.groups)
+                for (int i = 0; i < n; ++i) {
+                    const double u = sv[lane * n + i];
+                    b1 = fmax(fmin(b0, u), b1);
+                    b0 = fmax(b0, u);
+                }
+            const double gs = a.group_best == 2 && b1 > -INFINITY ? b0 + b1 : b0;
+            int rank = 0;
+            for (int g = 0; g < a.groups; ++g) {
+                const double o = lane_d(gs, g);
+                rank += o > gs || (o == gs && g < lane);
+            }
+            const uint64_t keep = __ballot(lane < a.groups && rank < a.top_groups);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int e = NV * lane + j;
+                if (!(keep >> (min(e, a.E - 1) / n) & 1)) v[j] = -INFINITY;
+                sv[e] = s[j];
+            }
+        }
     }
-    uint32_t taken = 0;
+    // each lane's values in order, equal ones in that of their ids
+    uint64_t k[NV];
+    int id[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-        if (NV * lane + j >= a.E) taken |= 1u << j;
-    int id = 0;
-    for (int k = 0; k < a.K; ++k) {
-        double b = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (!(taken >> j & 1)) b = fmax(b, v[j]);
-        const double M = wave_max_d(b);
-        // M = -inf: only experts switched off are left, every lane that has one holds it
-        const bool mine = taken != (1u << NV) - 1u && b == M;
-        const int win = __ffsll((unsigned long long)__ballot(mine)) - 1;
-        int j0 = 0;
-#pragma unroll
-        for (int j = NV - 1; j >= 0; --j)
-            if (!(taken >> j & 1) && v[j] == M) j0 = j;
-        const int e = NV * win + __builtin_amdgcn_readlane(j0, win);
-        if (lane == win) taken |= 1u << j0;
-        if (lane == k) id = e;
+    for (int j = 0; j < NV; ++j) {
+        id[j] = NV * lane + j;
+        k[j] = id[j] >= a.E ? 0 : v[j] > -INFINITY ? value_key(v[j]) : KEY_OFF;
     }
-    __syncthreads();
-    double w = lane < a.K ? s_s[wave][id] : 0.0;
+#pragma unroll
+    for (int i = 1; i < NV; ++i)
+#pragma unroll
+        for (int j = i; j > 0; --j)
+            if (k[j] > k[j - 1]) {
+                const uint64_t t = k[j];
+                k[j] = k[j - 1];
+                k[j - 1] = t;
+                const int u = id[j];
+                id[j] = id[j - 1];
+                id[j - 1] = u;
+            }
+    int my_id = 0;
+    bool my_on = false;
+    for (int r = 0; r < a.K; ++r) {
+        const uint32_t hi = (uint32_t)(k[0] >> 32);
+        const uint32_t M = wave_max_u32_bcast(hi);
+        uint64_t who = __ballot(hi == M);
+        if (who & (who - 1)) {                        // (uniform) two lanes or more agree in the upper word
+            const uint32_t lo = hi == M ? (uint32_t)k[0] : 0;
+            const uint32_t L = wave_max_u32_bcast(lo);
+            who = __ballot(hi == M && lo == L);
+        }
+        const int win = __ffsll((unsigned long long)who) - 1;
+        const int e = __builtin_amdgcn_readlane(id[0], win);
+        if (lane == r) {
+            my_id = e;
+            my_on = M != 0;                           // a key above KEY_OFF has an upper word
+        }
+        const bool pop = lane == win;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            k[j] = pop ? (j + 1 < NV ? k[j + 1] : 0) : k[j];
+            id[j] = pop && j + 1 < NV ? id[j + 1] : id[j];
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    double w = lane < a.K && my_on ? s_s[wave][my_id] : 0.0;
     if (a.renorm) {
         const double sum = wave_sum_d(w);
         w = sum > 0.0 ? w / sum : 0.0;
     }
-    if (live && lane < a.K) {
+    if (lane < a.K) {
         const int64_t o = tok * a.K + lane;
-        a.ids[o] = id;
+        a.ids[o] = my_id;
         a.w[o] = (float)((double)a.scale * w);
-        if (a.slots) a.slots[o] = a.table ? a.table[id] : a.dummy;
+        if (a.slots) a.slots[o] = a.table ? a.table[my_id] : a.dummy;
     }
 }
 
+template <int T, int NV>
+static hipError_t launch_scored_n(ScoredArgs a, hipStream_t st) {
+    const int size = T == T_F32 ? 4 : 2, vec = size * NV < 16 ? size * NV : 16, vecb = 4 * NV < 16 ? 4 * NV : 16;
+    a.vec = a.E % NV == 0 && (uintptr_t)a.logits % vec == 0 && a.ld * size % vec == 0 && (uintptr_t)a.bias % vecb == 0;
+    const int n = a.E / a.groups, lanes = n / NV;
+    a.group_lanes = n % NV == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+    hipLaunchKernelGGL((route_scored_kernel<T, NV>), dim3((unsigned)((a.n_tok + SCORED_WAVES - 1) / SCORED_WAVES)),
+                       dim3(64 * SCORED_WAVES), 0, st, a);
+    return hipGetLastError();
+}
 template <int T>
 static hipError_t launch_scored_t(const ScoredArgs &a, hipStream_t st) {
-    const dim3 grid((unsigned)((a.n_tok + (int64_t)SCORED_WAVES - 1) / SCORED_WAVES)), block(64 * SCORED_WAVES);
-    if (a.E <= 64) hipLaunchKernelGGL((route_scored_kernel<T, 1>), grid, block, 0, st, a);
-    else if (a.E <= 128) hipLaunchKernelGGL((route_scored_kernel<T, 2>), grid, block, 0, st, a);
-    else if (a.E <= 256) hipLaunchKernelGGL((route_scored_kernel<T, 4>), grid, block, 0, st, a);
-    else if (a.E <= 512) hipLaunchKernelGGL((route_scored_kernel<T, 8>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((route_scored_kernel<T, 16>), grid, block, 0, st, a);
-    return hipGetLastError();
+    return a.E <= 64 ? launch_scored_n<T, 1>(a, st) : a.E <= 128 ? launch_scored_n<T, 2>(a, st)
+         : a.E <= 256 ? launch_scored_n<T, 4>(a, st) : a.E <= 512 ? launch_scored_n<T, 8>(a, st)
+                      : launch_scored_n<T, 16>(a, st);
 }
 
 hipError_t launch_route_scored(const ScoredArgs &a, hipStream_t st) {
