@@ -5,6 +5,7 @@ module never falls back to anything else: a missing library raises.
 """
 import ctypes
 import os
+import struct as _struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmoeprefetch.so")
@@ -16,6 +17,7 @@ DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 SCORE = {"softmax": 0, "sigmoid": 1}
 NORM = {"rms": 0, "layer": 1}
 GATE_ACT = {None: 0, "sigmoid": 1}
+SAMPLE_MAX_TOKENS = 65535          # MOE_SAMPLE_MAX_TOKENS
 # the static workspace of moe_grouped_experts_static (MOE_GROUPED_STATIC_SCRATCH_BYTES)
 GROUPED_STATIC_SCRATCH_BYTES = 16 << 20
 ADMIT = {"off": 0, "heat": 1, "window": 2}
@@ -284,6 +286,20 @@ def lib():
             f.argtypes = args
         _lib = L
     return _lib
+
+
+def packed(struct):
+    """(pack, place): pack(*values) gives the bytes of a descriptor, its fields in order; place maps their names."""
+    code = {P: "P", I32: "i", I64: "q", U64: "Q", F32: "f"}
+    fmt = "@" + "".join(code[t] for _, t in struct._fields_) + "0P"
+    assert _struct.calcsize(fmt) == ctypes.sizeof(struct)
+    return _struct.Struct(fmt).pack, {n: i for i, (n, _) in enumerate(struct._fields_)}
+
+
+def entry(name):
+    """An entry point that takes its descriptor as bytes: a call from Python then packs once instead of setting fields."""
+    lib()
+    return ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, P)((name, _lib))
 
 
 def check(rc, what=""):

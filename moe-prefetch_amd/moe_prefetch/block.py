@@ -11,16 +11,20 @@ may be used from several streams and threads at once.  A call launches on `strea
 None: the tensors' device's current stream), does not synchronise, and can be captured into a graph.  Tensors are
 on one GPU; a call on another device than the current one makes it current for its length.  Outputs that are not
 given are allocated on the call's stream.  Inference only: no gradients.
-"""
-import ctypes
 
+A decode step makes these calls in every layer, so a call is short on the host too: one pass over its arguments, its
+descriptor packed at once (about 3 us before the launch itself).
+"""
 import torch
 
 from . import _lib
-from ._lib import check, lib
+from ._lib import MoeError, check, lib
 
+_F32, _I32 = torch.float32, torch.int32
 DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
-_RAW_STREAM = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _dtype(t, what):
@@ -30,19 +34,26 @@ def _dtype(t, what):
     return d
 
 
-def _on(t, dev, what):
-    if t.device != dev or t.device.type != "cuda":
-        raise ValueError(f"{what} is on {t.device}, not on a GPU" if t.device.type != "cuda"
-                         else f"{what} is on {t.device}, the call's other tensors on {dev}")
+def _place(t, dev, what):
+    if t.device.type != "cuda":
+        raise ValueError(f"{what} is on {t.device}, not on a GPU")
+    raise ValueError(f"{what} is on {t.device}, the call's other tensors on cuda:{dev}")
+
+
+def _on_gpu(t, what):
+    """The index of t's GPU."""
+    dev = t.get_device()
+    if dev < 0 or not t.is_cuda:
+        _place(t, dev, what)
+    return dev
 
 
 def _vec(t, n, dtype, dev, what):
-    """A contiguous vector of n elements: its address, or None."""
-    if t is None:
-        return None
-    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    """The address of a contiguous vector of n elements."""
+    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} vector of {n}, not {t.dtype} {tuple(t.shape)}")
-    _on(t, dev, what)
+    if t.get_device() != dev:
+        _place(t, dev, what)
     return t.data_ptr()
 
 
@@ -54,39 +65,48 @@ def _empty(shape, dtype, dev, stream):
         return torch.empty(shape, dtype=dtype, device=dev)
 
 
-def _out(t, shape, dtype, dev, what, stream=None):
-    if t is None:
-        return _empty(shape, dtype, dev, stream)
-    if t.dtype is not dtype or tuple(t.shape) != shape or not t.is_contiguous():
+def _out(t, shape, dtype, dev, what):
+    """The address of a given output."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous {dtype} {shape}, not {t.dtype} {tuple(t.shape)}")
-    _on(t, dev, what)
-    return t
+    if t.get_device() != dev:
+        _place(t, dev, what)
+    return t.data_ptr()
 
 
-def _rows(t, n, dev, what):
-    """[rows][n] with unit column stride: its row stride."""
-    if t.dim() != 2 or t.shape[1] != n or (n > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what} must be [tokens][{n}] with its columns next to each other, "
-                         f"not {tuple(t.shape)} with strides {t.stride()}")
-    _on(t, dev, what)
-    ld = t.stride(0)
-    if t.shape[0] <= 1:
+def _rows(t, rows, n, dev, what):
+    """The row stride of [rows][n] with unit column stride."""
+    if t.shape != (rows, n):
+        raise ValueError(f"{what} must be [{rows}][{n}], not {tuple(t.shape)}")
+    if t.get_device() != dev:
+        _place(t, dev, what)
+    ld, one = t.stride()
+    if one != 1 and n > 1:
+        raise ValueError(f"the columns of {what} must be next to each other, not {t.stride()} apart")
+    if rows <= 1:
         return n                                      # one row: its stride is not used
     if ld < n:
         raise ValueError(f"the rows of {what} overlap (row stride {ld})")
     return ld
 
 
+def _first(t, n, what):
+    """(rows, row stride, device) of a call's first tensor [rows][n]."""
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be [tokens][{n}], not {tuple(t.shape)}")
+    dev, rows = _on_gpu(t, what), t.shape[0]
+    return rows, _rows(t, rows, n, dev, what), dev
+
+
 def _call(fn, desc, dev, stream, what):
-    if stream is None:
-        raw = _RAW_STREAM(dev.index) if _RAW_STREAM else torch.cuda.current_stream(dev).cuda_stream
-    else:
-        raw = stream if isinstance(stream, int) else stream.cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        check(fn(ctypes.byref(desc), raw), what)
+    raw = _raw_stream(dev) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
+    if _device() == dev:
+        rc = fn(desc, raw)
     else:
         with torch.cuda.device(dev):
-            check(fn(ctypes.byref(desc), raw), what)
+            rc = fn(desc, raw)
+    if rc:
+        check(rc, what)
 
 
 class ScoredRouter:
@@ -103,12 +123,13 @@ class ScoredRouter:
             raise ValueError(f"score must be one of {sorted(_lib.SCORE)}, not {score!r}")
         self.E, self.K, self.bias = int(n_experts), int(n_expert_used), bias
         top = n_groups if top_groups is None else top_groups
-        self._desc = _lib.RouteScoredDesc(n_tok=0, E=self.E, K=self.K, score=_lib.SCORE[score],
-                                          renormalize=int(bool(renormalize)), n_groups=int(n_groups),
-                                          top_groups=int(top), group_best=int(group_best), scale=float(scale))
+        self._rule = (self.E, self.K, _lib.SCORE[score], int(bool(renormalize)), int(n_groups), int(top), int(group_best),
+                      float(scale))
         if bias is not None:
-            _vec(bias, self.E, torch.float32, bias.device, "bias")
-        check(lib().moe_route_scored(ctypes.byref(self._desc), None), "moe_route_scored")   # the rule alone: n_tok 0
+            _vec(bias, self.E, _F32, bias.get_device(), "bias")
+        self._pack, self._fn = _lib.packed(_lib.RouteScoredDesc)[0], _lib.entry("moe_route_scored")
+        none = self._pack(0, 0, 0, 0, *self._rule, 0, 0, 0, 0, 0, 0, 0)     # the rule alone: no tokens
+        check(self._fn(none, None), "moe_route_scored")
 
     def __call__(self, logits, ids=None, w=None, table=None, dummy=None, slots=None, scores=None, stream=None):
         """logits [tokens][n_experts] f32, bf16 or fp16 -> ids [tokens][K] int32, w [tokens][K] f32.
@@ -116,24 +137,21 @@ class ScoredRouter:
         slots (int32 [tokens][K]) receives table[ids] (table: int32 [n_experts]) or dummy (n_experts unless given)
         without a table; scores (f32 [tokens][n_experts]) receives every expert's score.
         """
-        dev = logits.device
-        d = _lib.RouteScoredDesc.from_buffer_copy(self._desc)
-        d.logits_type = _dtype(logits, "logits")
-        d.logits_stride = _rows(logits, self.E, dev, "logits")
-        T = logits.shape[0]
-        ids = _out(ids, (T, self.K), torch.int32, dev, "ids", stream)
-        w = _out(w, (T, self.K), torch.float32, dev, "w", stream)
-        d.logits, d.n_tok, d.ids, d.w = logits.data_ptr(), T, ids.data_ptr(), w.data_ptr()
-        if self.bias is not None:
-            d.bias = _vec(self.bias, self.E, torch.float32, dev, "bias")
-        if table is not None:
-            d.table = _vec(table, self.E, torch.int32, dev, "table")
-        d.dummy = self.E if dummy is None else dummy
-        if slots is not None:
-            d.slots = _out(slots, (T, self.K), torch.int32, dev, "slots").data_ptr()
-        if scores is not None:
-            d.scores = _out(scores, (T, self.E), torch.float32, dev, "scores").data_ptr()
-        _call(lib().moe_route_scored, d, dev, stream, "moe_route_scored")
+        E, K = self.E, self.K
+        T, ld, dev = _first(logits, E, "logits")
+        out = (T, K)
+        if ids is None:
+            ids = _empty(out, _I32, dev, stream)
+        if w is None:
+            w = _empty(out, _F32, dev, stream)
+        bias = self.bias
+        desc = self._pack(logits.data_ptr(), ld, _dtype(logits, "logits"), T, *self._rule,
+                          0 if bias is None else _vec(bias, E, _F32, dev, "bias"),
+                          0 if table is None else _vec(table, E, _I32, dev, "table"), E if dummy is None else dummy,
+                          _out(ids, out, _I32, dev, "ids"), _out(w, out, _F32, dev, "w"),
+                          0 if slots is None else _out(slots, out, _I32, dev, "slots"),
+                          0 if scores is None else _out(scores, (T, E), _F32, dev, "scores"))
+        _call(self._fn, desc, dev, stream, "moe_route_scored")
         return ids, w
 
 
@@ -152,26 +170,25 @@ class BlockNorm:
         if gate_act not in _lib.GATE_ACT:
             raise ValueError(f"gate_act must be None or 'sigmoid', not {gate_act!r}")
         self.H = int(hidden)
-        self.post = (post_weight is not None or post_bias is not None) if post is None else bool(post)
+        self.post = int((post_weight is not None or post_bias is not None) if post is None else bool(post))
         if not self.post and (post_weight is not None or post_bias is not None):
             raise ValueError("post-norm weights without a post-norm")
         self.weights = (weight, bias, post_weight, post_bias)
         given = [t for t in self.weights if t is not None]
         if len({t.dtype for t in given}) > 1:
             raise ValueError("the weights must be of one dtype")
-        self.w_dtype = given[0].dtype if given else torch.float32
-        self.w_dev = given[0].device if given else None
-        d = _lib.BlockNormDesc(n_tok=0, H=self.H, kind=_lib.NORM[kind], gate_act=_lib.GATE_ACT[gate_act],
-                               scale=float(scale), weight_offset=float(weight_offset), eps=float(eps),
-                               post_eps=float(eps if post_eps is None else post_eps))
+        self.kind, self.act = _lib.NORM[kind], _lib.GATE_ACT[gate_act]
+        self._rule = (float(scale), float(weight_offset), float(eps), float(eps if post_eps is None else post_eps))
+        self._pack, self._fn = _lib.packed(_lib.BlockNormDesc)[0], _lib.entry("moe_block_norm")
+        none = self._pack(0, self.H, self.kind, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, self.act, *self._rule, *[0] * 11)
+        check(self._fn(none, None), "moe_block_norm")                       # the rule alone: no tokens
+        self.w_dev, w_type = None, 0
         if given:
-            _dtype(given[0], "weight")
-        check(lib().moe_block_norm(ctypes.byref(d), None), "moe_block_norm")        # the rule alone: n_tok 0
+            w_type, self.w_dev = _dtype(given[0], "weight"), _on_gpu(given[0], "weight")
         names = ("weight", "bias", "post_weight", "post_bias")
-        for name, t in zip(names, self.weights):
-            if t is not None:
-                setattr(d, name, _vec(t, self.H, self.w_dtype, self.w_dev, name))
-        self._desc = d
+        ptr = [0 if t is None else _vec(t, self.H, given[0].dtype, self.w_dev, n) for n, t in zip(names, self.weights)]
+        self._w_post = (*ptr, w_type, self.post)
+        self._w = (ptr[0], ptr[1], 0, 0, w_type, 0)                         # of a call without a branch
 
     def __call__(self, x, branch=None, gate=None, out=None, residual=None, out_dtype=None, stream=None):
         """x [tokens][hidden] f32, bf16 or fp16; branch [tokens][hidden] or [tokens][n][hidden] (its n rows are
@@ -181,69 +198,52 @@ class BlockNorm:
         out receives y (of out_dtype: x's, unless given, or f32), residual receives r (x's dtype); residual=x updates
         the stream in place.  Without a branch r is x and nothing is written for it unless residual is given.
         """
-        dev, H = x.device, self.H
-        d = _lib.BlockNormDesc.from_buffer_copy(self._desc)
-        d.x_type = _dtype(x, "x")
-        d.x_stride = _rows(x, H, dev, "x")
-        T = x.shape[0]
-        d.n_tok, d.x = T, x.data_ptr()
-        if self.w_dev is not None:
-            if self.w_dev != dev:
-                raise ValueError(f"the weights are on {self.w_dev}, x on {dev}")
-            d.weight_type = DTYPES[self.w_dtype]
-        if branch is not None:
-            d.branch_type = _dtype(branch, "branch")
-            d.post = int(self.post)
-            if branch.dim() == 3:
-                n = branch.shape[1]
-                if branch.shape[0] != T or branch.shape[2] != H or not branch.is_contiguous():
-                    raise ValueError(f"branch must be contiguous [{T}][n][{H}], not {tuple(branch.shape)}")
-                _on(branch, dev, "branch")
-                d.branch_stride, d.n_sum = H, n
-            else:
-                d.branch_stride, d.n_sum = _rows(branch, H, dev, "branch"), 1
-                if branch.shape[0] != T:
-                    raise ValueError(f"branch has {branch.shape[0]} rows, x {T}")
-            d.branch = branch.data_ptr()
-        if gate is not None:
-            self._gate(d, gate, T, dev)
-        if residual is None and branch is not None:
-            residual = _empty((T, H), x.dtype, dev, stream)
+        H = self.H
+        T, ld, dev = _first(x, H, "x")
+        dtype = x.dtype
+        if self.w_dev is not None and self.w_dev != dev:
+            raise ValueError(f"the weights are on cuda:{self.w_dev}, x on cuda:{dev}")
+        if branch is None:
+            b = (0, 0, 0, 0)
+        elif branch.dim() == 3:
+            n = branch.shape[1]
+            b = (_out(branch, (T, n, H), branch.dtype, dev, "branch"), H, _dtype(branch, "branch"), n)
+        else:
+            b = (branch.data_ptr(), _rows(branch, T, H, dev, "branch"), _dtype(branch, "branch"), 1)
         if residual is not None:
-            if residual.dtype is not x.dtype or residual.shape[0] != T:
-                raise ValueError(f"residual must be {x.dtype} [{T}][{H}]")
-            d.residual_stride = _rows(residual, H, dev, "residual")
-            d.residual = residual.data_ptr()
+            if residual.dtype is not dtype:
+                raise ValueError(f"residual must be {dtype}, as x is, not {residual.dtype}")
+            r = (residual.data_ptr(), _rows(residual, T, H, dev, "residual"))
+        elif branch is not None:
+            residual = _empty((T, H), dtype, dev, stream)
+            r = (residual.data_ptr(), H)
+        else:
+            r = (0, 0)
         if out is None:
-            out = _empty((T, H), x.dtype if out_dtype is None else out_dtype, dev, stream)
-        elif out.shape[0] != T or (out_dtype is not None and out.dtype is not out_dtype):
-            raise ValueError(f"out must be {out_dtype or out.dtype} [{T}][{H}]")
-        d.y_type = _dtype(out, "out")
-        d.y_stride = _rows(out, H, dev, "out")
-        d.y = out.data_ptr()
-        _call(lib().moe_block_norm, d, dev, stream, "moe_block_norm")
+            out = _empty((T, H), dtype if out_dtype is None else out_dtype, dev, stream)
+        elif out_dtype is not None and out.dtype is not out_dtype:
+            raise ValueError(f"out is {out.dtype}, not {out_dtype}")
+        desc = self._pack(T, H, self.kind, x.data_ptr(), ld, _dtype(x, "x"), *b,
+                          *((0, 0, 0, 0) if gate is None else self._gate(gate, T, dev)), self.act, *self._rule,
+                          *(self._w if branch is None else self._w_post), *r, out.data_ptr(),
+                          _rows(out, T, H, dev, "out"), _dtype(out, "out"))
+        _call(self._fn, desc, dev, stream, "moe_block_norm")
         return out, x if residual is None else residual
 
-    def _gate(self, d, gate, T, dev):
-        H = self.H
-        _on(gate, dev, "gate")
-        d.gate_type = _dtype(gate, "gate")
-        shape = tuple(gate.shape)
+    def _gate(self, gate, T, dev):
+        """(address, row stride, column stride, type)"""
+        H, shape, at, kind = self.H, tuple(gate.shape), gate.data_ptr(), _dtype(gate, "gate")
+        if gate.get_device() != dev:
+            _place(gate, dev, "gate")
         if shape == (H,):
-            row, col = 0, 1
-        elif shape == (T,) or shape == (T, 1):
-            row, col = 1, 0
+            if gate.stride(0) == 1 or H == 1:
+                return at, 0, 1, kind
         elif shape == (T, H):
-            row, col = H, 1
-        else:
-            raise ValueError(f"gate must be [{T}], [{T}][1], [{H}] or [{T}][{H}], not {shape}")
-        if col and H > 1 and gate.stride(-1) != 1:
-            raise ValueError(f"the columns of gate must be next to each other, not {gate.stride()}")
-        if row and T > 1:
-            row = gate.stride(0)
-            if row < (H if col else 1):
-                raise ValueError(f"the rows of gate overlap (row stride {row})")
-        d.gate, d.gate_row_stride, d.gate_col_stride = gate.data_ptr(), row, col
+            return at, _rows(gate, T, H, dev, "gate"), 1, kind
+        elif shape == (T,) or shape == (T, 1):
+            if T <= 1 or gate.stride(0) >= 1:
+                return at, gate.stride(0) if T > 1 else 1, 0, kind
+        raise ValueError(f"gate must be [{T}], [{T}][1], [{H}] or [{T}][{H}], not {shape} with strides {gate.stride()}")
 
 
 class Sampler:
@@ -251,8 +251,10 @@ class Sampler:
 
     def __init__(self, vocab):
         self.V = int(vocab)
-        self._desc = _lib.SampleDesc(n_tok=0, V=self.V, temperature_all=1.0, top_k_all=0, top_p_all=1.0, min_p_all=0.0)
-        check(lib().moe_sample(ctypes.byref(self._desc), None), "moe_sample")       # the size alone: n_tok 0
+        self._pack, self._fn = _lib.packed(_lib.SampleDesc)[0], _lib.entry("moe_sample")
+        none = self._pack(0, 0, 0, 0, self.V, 0, 0, 0, 0, 0, 1.0, 0, 1.0, 0.0, 0, 0, 0)
+        check(self._fn(none, None), "moe_sample")                           # the size alone: no tokens
+        self._ws = {}                                                       # tokens -> workspace bytes
 
     def __call__(self, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, probs=None,
                  stream=None):
@@ -262,34 +264,39 @@ class Sampler:
         temperature, top_p, min_p (f32) and top_k (int32): a number for every row, a tensor [tokens], or None
         (temperature 1, nothing cut).  A temperature of 0 takes the largest logit.
         """
-        dev = logits.device
-        d = _lib.SampleDesc.from_buffer_copy(self._desc)
-        d.logits_type = _dtype(logits, "logits")
-        d.logits_stride = _rows(logits, self.V, dev, "logits")
-        T = logits.shape[0]
-        d.logits, d.n_tok = logits.data_ptr(), T
-        f32 = torch.float32
-        d.u = _vec(u, T, f32, dev, "u")
-        if isinstance(temperature, torch.Tensor):
-            d.temperature = _vec(temperature, T, f32, dev, "temperature")
+        V = self.V
+        T, ld, dev = _first(logits, V, "logits")
+        Tensor = torch.Tensor
+        t_row = k_row = p_row = m_row = 0
+        t_all, k_all, p_all, m_all = 1.0, 0, 1.0, 0.0
+        if isinstance(temperature, Tensor):
+            t_row = _vec(temperature, T, _F32, dev, "temperature")
         elif temperature is not None:
-            d.temperature_all = temperature
-        if isinstance(top_k, torch.Tensor):
-            d.top_k = _vec(top_k, T, torch.int32, dev, "top_k")
+            t_all = temperature
+        if isinstance(top_k, Tensor):
+            k_row = _vec(top_k, T, _I32, dev, "top_k")
         elif top_k is not None:
-            d.top_k_all = top_k
-        if isinstance(top_p, torch.Tensor):
-            d.top_p = _vec(top_p, T, f32, dev, "top_p")
+            k_all = top_k
+        if isinstance(top_p, Tensor):
+            p_row = _vec(top_p, T, _F32, dev, "top_p")
         elif top_p is not None:
-            d.top_p_all = top_p
-        if isinstance(min_p, torch.Tensor):
-            d.min_p = _vec(min_p, T, f32, dev, "min_p")
+            p_all = top_p
+        if isinstance(min_p, Tensor):
+            m_row = _vec(min_p, T, _F32, dev, "min_p")
         elif min_p is not None:
-            d.min_p_all = min_p
-        tokens = _out(tokens, (T,), torch.int32, dev, "tokens", stream)
-        probs = _out(probs, (T,), f32, dev, "probs", stream)
-        d.tokens, d.probs = tokens.data_ptr(), probs.data_ptr()
-        ws = _empty((lib().moe_sample_workspace_bytes(T, self.V),), torch.uint8, dev, stream)
-        d.workspace = ws.data_ptr()
-        _call(lib().moe_sample, d, dev, stream, "moe_sample")
+            m_all = min_p
+        if tokens is None:
+            tokens = _empty((T,), _I32, dev, stream)
+        if probs is None:
+            probs = _empty((T,), _F32, dev, stream)
+        size = self._ws.get(T)
+        if size is None:
+            if T > _lib.SAMPLE_MAX_TOKENS:
+                raise MoeError(f"moe_sample: n_tok {T} out of range")
+            size = self._ws[T] = lib().moe_sample_workspace_bytes(T, V)
+        ws = _empty((size,), torch.uint8, dev, stream)
+        desc = self._pack(logits.data_ptr(), ld, _dtype(logits, "logits"), T, V, _vec(u, T, _F32, dev, "u"), t_row, k_row,
+                          p_row, m_row, t_all, k_all, p_all, m_all, _out(tokens, (T,), _I32, dev, "tokens"),
+                          _out(probs, (T,), _F32, dev, "probs"), ws.data_ptr())
+        _call(self._fn, desc, dev, stream, "moe_sample")
         return tokens, probs

@@ -100,6 +100,14 @@ def test_descriptors_match_the_header(tmp_path, name, struct):
     assert [getattr(struct, f).offset for f in fields] + [ctypes.sizeof(struct)] == want
 
 
+@pytest.mark.parametrize("struct", [_lib.RouteScoredDesc, _lib.BlockNormDesc, _lib.SampleDesc])
+def test_packed_descriptors(struct):
+    pack, place = _lib.packed(struct)
+    values = [7 * i + 3 for i in range(len(place))]
+    d = struct.from_buffer_copy(pack(*values))
+    assert [getattr(d, n) for n in place] == values
+
+
 def test_rules_are_refused_where_they_are_made():
     with pytest.raises(MoeError, match="n_experts"):
         ScoredRouter(2000, 8)
