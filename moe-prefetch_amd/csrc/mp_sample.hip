@@ -145,6 +145,11 @@ __global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(Sampl
         for (int j = 0; j < SLICE_EPT; ++j) v[j] = -INFINITY;
     } else if ((uintptr_t)l % 16 == 0) {
         uint4 q[NV];
+        const bool whole = (NV - 1) * step + (slice + 1) * 64 * VEC <= a.V;    // every vector of the slice
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) q[j] = *(const uint4 *)(l + i0 + j * step);
+        } else {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int i = i0 + j * step;
@@ -156,6 +161,7 @@ __global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(Sampl
                 for (int e = 0; e < VEC; ++e) t[e] = i + e < a.V ? l[i + e] : Elem<T>::store(-INFINITY);
                 __builtin_memcpy(&q[j], t, 16);
             }
+        }
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -193,9 +199,10 @@ __global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(Sampl
     }
     uint64_t *list = (uint64_t *)a.lists + (size_t)id * a.cap;
     const uint32_t mk = sort_key(m), top = (uint32_t)__builtin_amdgcn_readfirstlane((int)sort_key(vmax));
+    const uint32_t low = ~wave_max_u32_bcast(~mk);    // the least of the lanes' maxima
     int keep = greedy ? 1 : a.keep;
     for (;;) {
-        uint32_t lo = KEY_NONE, hi = top;             // at least keep lanes reach lo
+        uint32_t lo = low, hi = top;                  // at least keep lanes reach lo
         if (keep > 1) {
             for (int it = 0; it < 20 && hi > lo; ++it) {
                 const uint32_t mid = hi - (hi - lo) / 2;
