@@ -255,6 +255,14 @@ int moe_cache_set_router(moe_cache *c, int layer, const float *W_dev);
  * the layer's expert_bytes; NULL removes it).  Decoding adds it with weight 1
  * after the routed experts; the cache never evicts or counts it. */
 int moe_cache_set_shared(moe_cache *c, int layer, const void *expert, size_t expert_bytes);
+/* Route `layer` by scores (moe_route_scored; of `rule` the score, renormalize,
+ * n_groups, top_groups, group_best, scale and bias count, its E and K are the
+ * cache's, and the bias is read at every call) instead of by softmax and top-k;
+ * NULL returns to that.  Such a layer decodes through moe_decode_batch, one token
+ * too: moe_decode_token and moe_decode_layer, whose launches route by softmax,
+ * refuse a cache that has one (MOE_ERR_STATE).  Not with a cache prior. */
+typedef struct moe_route_scored_desc moe_route_scored_desc;
+int moe_cache_set_scoring(moe_cache *c, int layer, const moe_route_scored_desc *rule);
 int moe_cache_lookup(moe_cache *c, int layer, moe_layer_view *out);
 int moe_cache_trace_open(moe_cache *c, const char *route_path, const char *map_path);
 /* host ids, token-major [n_tok][n_ids] */
@@ -696,14 +704,16 @@ int moe_decode_batch(moe_cache *c, const float *x, const float *bias, float *out
  * lower ids first and with weight 0, only where fewer than K experts are left, so
  * that ids always holds K different experts.  (A group's switched-off experts do
  * not count for its score; w is 0 where the sum is.)  A logit of +inf takes its row's
- * whole softmax, shared by all such logits. */
+ * whole softmax, shared by all such logits.
+ * Without logits they are the router's product W . x, in moe_route's order and
+ * with its limits (H 2048, E a multiple of 64 up to 256, n_tok up to 65535). */
 #define MOE_BLOCK_MAX_TOKENS (1 << 20)
 #define MOE_SCORE_SOFTMAX 0
 #define MOE_SCORE_SIGMOID 1
 #define MOE_ROUTE_SCORED_MAX_E 1024
 #define MOE_ROUTE_SCORED_MAX_K 64
-typedef struct {
-    const void *logits;       /* dev [n_tok][E], MOE_DTYPE_*, rows logits_stride apart */
+struct moe_route_scored_desc {
+    const void *logits;       /* dev [n_tok][E], MOE_DTYPE_*, rows logits_stride apart, or NULL */
     int64_t logits_stride;
     int32_t logits_type;
     int32_t n_tok, E, K;      /* n_tok 0..MOE_BLOCK_MAX_TOKENS, E <= MOE_ROUTE_SCORED_MAX_E,
@@ -721,7 +731,10 @@ typedef struct {
     float *w;                 /* dev out [n_tok][K] */
     int32_t *slots;           /* dev out [n_tok][K] or NULL */
     float *scores;            /* dev out [n_tok][E] s_e, or NULL */
-} moe_route_scored_desc;
+    const float *W, *x;       /* without logits: dev [E][H] and [n_tok][H], f32, 16-byte aligned */
+    int32_t H;
+    void *workspace;          /* without logits: dev, moe_route_workspace_bytes(), 16-byte aligned */
+};
 int moe_route_scored(const moe_route_scored_desc *d, void *stream);
 
 /* The residual stream between two blocks, per token:

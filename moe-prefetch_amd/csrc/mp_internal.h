@@ -65,6 +65,24 @@ struct alignas(256) AheadPost {
     int32_t ids[2][AHEAD_K];
 };
 
+// Operators around the expert products; the fields are those of the descriptors of the same name in
+// moe_prefetch.h, checked by the caller.  Element types there and here: 0 f32, 1 bf16, 2 fp16.
+struct ScoredArgs {
+    const void *logits;
+    int64_t ld;
+    int type, n_tok, E, K, score, renorm, groups, top_groups, group_best;
+    float scale;
+    const float *bias;
+    const int32_t *table;
+    int32_t dummy;
+    int32_t *ids;
+    float *w;
+    int32_t *slots;
+    float *scores;
+    int vec, group_lanes;       // set by the launcher: rows and bias in whole vectors; lanes of a group, or 0
+};
+hipError_t launch_route_scored(const ScoredArgs &a, hipStream_t st);
+
 struct RouteLaunch {
     const float *W;        // [E][H] f32
     const float *x;        // [n_tok][H] f32
@@ -100,6 +118,8 @@ struct RouteLaunch {
     AheadPost *apost;      // the record (mapped host memory, or device memory for a test)
     uint32_t *fresh;       // non-null: read the table at system scope (words may flip in the middle
                            // of the token) and set *fresh when a word carries STREAM_BIT
+    const ScoredArgs *scored; // or null: the experts are chosen by this rule (its buffers are set from the
+                              // ones above) instead of by softmax and top-k; no prior, post or lookahead
 };
 
 struct ExpertArgs {
@@ -309,24 +329,7 @@ hipError_t static_scratch(void **ptr);
 hipError_t launch_swiglu_quant(const float *y2, int P, int I, float *h_out, int n_h, uint16_t *q16, float *dx,
                                uint16_t *bs16, hipStream_t st);
 
-// Operators around the expert products; the fields are those of the descriptors of the same name in
-// moe_prefetch.h, checked by the caller.  Element types there and here: 0 f32, 1 bf16, 2 fp16.
-struct ScoredArgs {
-    const void *logits;
-    int64_t ld;
-    int type, n_tok, E, K, score, renorm, groups, top_groups, group_best;
-    float scale;
-    const float *bias;
-    const int32_t *table;
-    int32_t dummy;
-    int32_t *ids;
-    float *w;
-    int32_t *slots;
-    float *scores;
-    int vec, group_lanes;       // set by the launcher: rows and bias in whole vectors; lanes of a group, or 0
-};
-hipError_t launch_route_scored(const ScoredArgs &a, hipStream_t st);
-
+// the norms around a block, and sampling: as ScoredArgs
 struct NormArgs {
     int n_tok, H, kind, post, x_type, b_type, n_sum, gate_type, gate_act, w_type, y_type;
     const void *x, *branch, *gate, *w, *c, *pw, *pc;

@@ -1670,6 +1670,13 @@ hipError_t launch_route(const RouteLaunch &l, hipStream_t st, hipEvent_t *ev) {
                    dim3(64 * RL_WAVES), st, e0, e1, a);
     }
     if (e != hipSuccess) return e;
+    if (l.scored) {
+        ScoredArgs s = *l.scored;
+        s.logits = l.logits; s.ld = l.E; s.type = 0;
+        s.n_tok = l.n_tok; s.E = l.E; s.K = l.K;
+        s.table = l.table; s.dummy = l.dummy; s.ids = l.ids; s.w = l.w; s.slots = l.slots;
+        return launch_route_scored(s, st);
+    }
     return launch(route_select_kernel, dim3((unsigned)l.n_tok), dim3(256), st, ev ? ev[2] : nullptr,
                   ev ? ev[3] : nullptr, a);
 }

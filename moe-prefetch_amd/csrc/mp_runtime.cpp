@@ -75,6 +75,8 @@ struct Layer {
     const uint8_t *store_dev = nullptr;       // device view of it
     const float *router = nullptr;
     uint8_t *shared = nullptr;                // dev: the always-on shared expert (owned) or null
+    bool scored = false;                      // routed by scores, with this rule
+    mp::ScoredArgs rule{};
     std::vector<int32_t> slot_expert, expert_slot, free_slots, pending;
     std::vector<int32_t> staged;              // [K] expert read from the store at k this token (staged), or -1
     std::vector<uint32_t> use_count;          // heat file: observations per expert (empty: no heat file)
@@ -1866,6 +1868,42 @@ int moe_cache_set_shared(moe_cache *c, int layer, const void *expert, size_t exp
     return MOE_OK;
 }
 
+// a scored routing's rule, apart from its buffers
+static int scored_check(const moe_route_scored_desc *d);
+static mp::ScoredArgs scored_rule(const moe_route_scored_desc *d) {
+    mp::ScoredArgs a{};
+    a.E = d->E; a.K = d->K; a.score = d->score; a.renorm = d->renormalize;
+    a.groups = d->n_groups; a.top_groups = d->top_groups; a.group_best = d->group_best; a.scale = d->scale;
+    a.bias = d->bias;
+    return a;
+}
+
+int moe_cache_set_scoring(moe_cache *c, int layer, const moe_route_scored_desc *rule) {
+    if (!c || layer < 0 || layer >= (int)c->L.size()) return fail(MOE_ERR_ARG, "bad arguments");
+    Layer &ls = c->L[layer];
+    if (!rule) {
+        ls.scored = false;
+        return MOE_OK;
+    }
+    const int r = scored_check(rule);
+    if (r != MOE_OK) return r;
+    if (rule->E != c->E || rule->K != c->K)
+        return fail(MOE_ERR_ARG, "moe_cache_set_scoring: the rule has %d of %d experts, the cache %d of %d", rule->K, rule->E,
+                    c->K, c->E);
+    if ((uintptr_t)rule->bias % 4) return fail(MOE_ERR_ARG, "moe_cache_set_scoring: misaligned bias");
+    if (c->cfg.cache_prior != 0.0f) return fail(MOE_ERR_STATE, "moe_cache_set_scoring: the cache has a prior on softmax routing");
+    ls.rule = scored_rule(rule);
+    ls.scored = true;
+    return MOE_OK;
+}
+
+// the launches of moe_decode_token and moe_decode_layer route by softmax and top-k
+static int softmax_only(const moe_cache *c) {
+    for (const Layer &ls : c->L)
+        if (ls.scored) return fail(MOE_ERR_STATE, "layer %d routes by scores: decode it with moe_decode_batch", ls.il);
+    return MOE_OK;
+}
+
 int moe_cache_lookup(moe_cache *c, int layer, moe_layer_view *out) {
     if (!c || !out || layer < 0 || layer >= (int)c->L.size()) return fail(MOE_ERR_ARG, "bad arguments");
     const Layer &ls = c->L[layer];
@@ -3232,7 +3270,8 @@ int moe_decode_layer(moe_cache *c, int layer, const float *x, const float *bias,
     if (c->st && c->st->live) return fail(MOE_ERR_STATE, "just-in-time streaming decodes whole tokens (moe_decode_token)");
     const hipStream_t st = (hipStream_t)stream;
     const size_t NL = c->L.size();
-    int r = ensure_stage(c);
+    int r = softmax_only(c);
+    if (r == MOE_OK) r = ensure_stage(c);
     if (r == MOE_OK) r = ensure_tev(c);
     if (r != MOE_OK) return r;
     if (c->pl_flags.size() != NL) {
@@ -3328,7 +3367,8 @@ int moe_decode_token(moe_cache *c, const float *x, const float *bias, float *out
     if (c->host_only) return fail(MOE_ERR_STATE, "host-only cache (device < 0) cannot decode");
     hipStream_t st = (hipStream_t)stream;
     const int NL = (int)c->L.size();
-    int er = ensure_tev(c);
+    int er = softmax_only(c);
+    if (er == MOE_OK) er = ensure_tev(c);
     if (er == MOE_OK) er = ensure_stage(c);
     if (er != MOE_OK) return er;
     // layers decoded one by one and not stepped: their kernels finish first,
@@ -3922,6 +3962,7 @@ int moe_decode_batch(moe_cache *c, const float *x, const float *bias, float *out
             xq.xdx = (float *)(ws + w.xdx);
             xq.xbs = (uint16_t *)(ws + w.xbs);
         }
+        if (ls.scored) xq.scored = &ls.rule;
         if ((r = run_route(&rd, st, nullptr, nullptr, nullptr, &xq)) != MOE_OK) return r;
         if (sc) {                       // the routing back to the host for its share
             HIPCHK(hipMemcpyAsync(c->bh_ids + (size_t)l * TK, rd.ids, (size_t)TK * 4, hipMemcpyDeviceToHost, st));
@@ -4003,7 +4044,6 @@ int moe_decode_batch(moe_cache *c, const float *x, const float *bias, float *out
 static bool dtype_ok(int t) { return t == MOE_DTYPE_F32 || t == MOE_DTYPE_BF16 || t == MOE_DTYPE_F16; }
 static bool aligned_to(const void *p, int type) { return (uintptr_t)p % (type == MOE_DTYPE_F32 ? 4 : 2) == 0; }
 
-// a scored routing's rule, apart from its buffers
 static int scored_check(const moe_route_scored_desc *d) {
     if (d->E < 1 || d->E > MOE_ROUTE_SCORED_MAX_E)
         return fail(MOE_ERR_ARG, "moe_route_scored: n_experts %d must be 1..%d", d->E, MOE_ROUTE_SCORED_MAX_E);
@@ -4032,21 +4072,35 @@ int moe_route_scored(const moe_route_scored_desc *d, void *stream) {
         return fail(MOE_ERR_ARG, "moe_route_scored: n_tok %d out of range", d->n_tok);
     if (!dtype_ok(d->logits_type)) return fail(MOE_ERR_ARG, "moe_route_scored: logits_type %d unsupported", d->logits_type);
     if (d->n_tok == 0) return MOE_OK;
-    if (!d->logits || !d->ids || !d->w) return fail(MOE_ERR_ARG, "moe_route_scored: null argument");
-    if (d->logits_stride < d->E)
+    if (!d->ids || !d->w) return fail(MOE_ERR_ARG, "moe_route_scored: null argument");
+    if (d->logits && d->logits_stride < d->E)
         return fail(MOE_ERR_ARG, "moe_route_scored: logits_stride %lld below n_experts", (long long)d->logits_stride);
     if (!aligned_to(d->logits, d->logits_type) ||
         ((uintptr_t)d->bias | (uintptr_t)d->table | (uintptr_t)d->ids | (uintptr_t)d->w | (uintptr_t)d->slots |
          (uintptr_t)d->scores) % 4)
         return fail(MOE_ERR_ARG, "moe_route_scored: misaligned pointer");
-    mp::ScoredArgs a{};
-    a.logits = d->logits; a.ld = d->logits_stride; a.type = d->logits_type;
-    a.n_tok = d->n_tok; a.E = d->E; a.K = d->K; a.score = d->score; a.renorm = d->renormalize;
-    a.groups = d->n_groups; a.top_groups = d->top_groups; a.group_best = d->group_best; a.scale = d->scale;
-    a.bias = d->bias; a.table = d->table; a.dummy = d->dummy;
+    mp::ScoredArgs a = scored_rule(d);
+    a.logits = d->logits; a.ld = d->logits_stride; a.type = d->logits_type; a.n_tok = d->n_tok;
+    a.table = d->table; a.dummy = d->dummy;
     a.ids = d->ids; a.w = d->w; a.slots = d->slots; a.scores = d->scores;
-    HIPCHK(mp::launch_route_scored(a, (hipStream_t)stream));
-    return MOE_OK;
+    if (d->logits) {
+        HIPCHK(mp::launch_route_scored(a, (hipStream_t)stream));
+        return MOE_OK;
+    }
+    // the router's product first
+    if (!d->W || !d->x || !d->workspace) return fail(MOE_ERR_ARG, "moe_route_scored: logits, or W, x and workspace");
+    if (((uintptr_t)d->W | (uintptr_t)d->x | (uintptr_t)d->workspace) % 16)
+        return fail(MOE_ERR_ARG, "moe_route_scored: W, x and workspace must be 16-byte aligned");
+    const int s = check_shape(d->E, d->H, 0, std::min(d->K, 16));
+    if (s != MOE_OK) return s;
+    if (d->n_tok > 65535) return fail(MOE_ERR_ARG, "moe_route_scored: n_tok %d out of range for a product", d->n_tok);
+    moe_route_desc rd{};
+    rd.W = d->W; rd.x = d->x; rd.table = d->table; rd.dummy = d->dummy;
+    rd.E = d->E; rd.H = d->H; rd.K = d->K; rd.n_tok = d->n_tok;
+    rd.ids = d->ids; rd.w = d->w; rd.slots = d->slots; rd.workspace = d->workspace;
+    mp::RouteLaunch l{};
+    l.scored = &a;
+    return run_route(&rd, (hipStream_t)stream, nullptr, nullptr, nullptr, &l);
 }
 
 int moe_block_norm(const moe_block_norm_desc *d, void *stream) {

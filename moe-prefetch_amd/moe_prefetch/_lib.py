@@ -63,7 +63,7 @@ class RouteScoredDesc(ctypes.Structure):
     _fields_ = [("logits", P), ("logits_stride", I64), ("logits_type", I32), ("n_tok", I32), ("E", I32), ("K", I32),
                 ("score", I32), ("renormalize", I32), ("n_groups", I32), ("top_groups", I32), ("group_best", I32),
                 ("scale", F32), ("bias", P), ("table", P), ("dummy", I32), ("ids", P), ("w", P), ("slots", P),
-                ("scores", P)]
+                ("scores", P), ("W", P), ("x", P), ("H", I32), ("workspace", P)]
 
 
 class BlockNormDesc(ctypes.Structure):
@@ -188,6 +188,7 @@ SIGNATURES = {
     "moe_cache_destroy": (ctypes.c_int, [P]),
     "moe_cache_set_host_store": (ctypes.c_int, [P, ctypes.c_int, P, SZ]),
     "moe_cache_set_router": (ctypes.c_int, [P, ctypes.c_int, P]),
+    "moe_cache_set_scoring": (ctypes.c_int, [P, ctypes.c_int, ctypes.POINTER(RouteScoredDesc)]),
     "moe_cache_set_shared": (ctypes.c_int, [P, ctypes.c_int, P, SZ]),
     "moe_cache_lookup": (ctypes.c_int, [P, ctypes.c_int, ctypes.POINTER(LayerView)]),
     "moe_cache_trace_open": (ctypes.c_int, [P, ctypes.c_char_p, ctypes.c_char_p]),

@@ -1,7 +1,8 @@
 """The batched MoE layer (prefill chunks, decode at batch > 1) over the C ABI.
 
     route     moe_route: softmax / top-k / renormalised weights of W.x, or of
-              given logits (build_moe_ffn's router at n_tokens > 1)
+              given logits (build_moe_ffn's router at n_tokens > 1), or
+              moe_route_scored by a ScoredRouter's rule
     dispatch  moe_dispatch: per-expert histogram, exclusive scan and the stable
               permutation of the (token, k) pairs -- the row mapping ggml's
               mul_mat_id builds (patches/0008-fused-cpu-moe-rows.patch:157-167)
@@ -48,10 +49,25 @@ class BatchedMoe:
         ws = lib().moe_grouped_workspace_bytes(n_tok_max, n_expert_used, hidden, intermediate)
         self.ws = torch.empty(ws, dtype=torch.uint8, device=dev)
 
-    def route(self, n_tok, logits=None, W=None, x=None, bias=None, prior=None, table=None, stream=None):
-        """ids/w for n_tok tokens from given logits [n_tok][E], or from W [E][H] . x [n_tok][H] (f32)."""
+    def route(self, n_tok, logits=None, W=None, x=None, bias=None, prior=None, table=None, stream=None, router=None):
+        """ids/w for n_tok tokens from given logits [n_tok][E], or from W [E][H] . x [n_tok][H] (f32).  router (a
+        ScoredRouter): by its rule instead of softmax and top-k (without bias, prior and table)."""
         if n_tok > self.T:
             raise ValueError(f"n_tok {n_tok} > {self.T}")
+        if router is not None:
+            if (router.E, router.K) != (self.E, self.K):
+                raise ValueError(f"the router has {router.K} of {router.E} experts, the layer {self.K} of {self.E}")
+            if bias is not None or prior is not None or table is not None:
+                raise ValueError("a scored routing takes no bias, prior or table here")
+            ids, w = self.ids[:n_tok], self.w[:n_tok]
+            at = 0 if stream is None else stream          # as the calls below: None is the null stream
+            if logits is not None:
+                if logits.shape[0] != n_tok:
+                    raise ValueError(f"logits of {logits.shape[0]} tokens, not {n_tok}")
+                router(logits, ids=ids, w=w, slots=self.slots[:n_tok], stream=at)
+            else:
+                router.from_product(W, x[:n_tok], ids, w, self.slots[:n_tok], self.route_ws, self.H, stream=at)
+            return ids, w
         d = _lib.RouteDesc(_ptr(W), _ptr(x), _ptr(bias), _ptr(prior), _ptr(table), self.E, 0, self.E, self.H,
                            self.K, n_tok, _ptr(self.ids), _ptr(self.w), _ptr(self.slots), None,
                            _ptr(self.q8x) if logits is None else None, _ptr(self.route_ws), _ptr(logits))
@@ -80,10 +96,10 @@ class BatchedMoe:
         return (ms[0], ms[1]) if timing else None
 
     def forward(self, x, out, store, expert_bytes, n_store, down_type, logits=None, W=None, xf32=None, bias=None,
-                stream=None, **kw):
-        """route -> dispatch -> experts for x.shape[0] tokens."""
+                stream=None, router=None, **kw):
+        """route (by router's rule, if given) -> dispatch -> experts for x.shape[0] tokens."""
         n_tok = x.shape[0]
-        self.route(n_tok, logits=logits, W=W, x=xf32, bias=bias, stream=stream)
+        self.route(n_tok, logits=logits, W=W, x=xf32, bias=bias, stream=stream, router=router)
         self.dispatch(n_tok, stream=stream)
         return self.experts(x, out, n_tok, store, expert_bytes, n_store, down_type, stream=stream, **kw)
 

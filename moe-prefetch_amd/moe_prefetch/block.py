@@ -128,8 +128,27 @@ class ScoredRouter:
         if bias is not None:
             _vec(bias, self.E, _F32, bias.get_device(), "bias")
         self._pack, self._fn = _lib.packed(_lib.RouteScoredDesc)[0], _lib.entry("moe_route_scored")
-        none = self._pack(0, 0, 0, 0, *self._rule, 0, 0, 0, 0, 0, 0, 0)     # the rule alone: no tokens
-        check(self._fn(none, None), "moe_route_scored")
+        check(self._fn(self._packed(0, 0, 0, 0), None), "moe_route_scored")     # the rule alone: no tokens
+
+    def _packed(self, logits, ld, kind, T, bias=0, table=0, dummy=0, ids=0, w=0, slots=0, scores=0, W=0, x=0, H=0,
+                workspace=0):
+        return self._pack(logits, ld, kind, T, *self._rule, bias, table, dummy, ids, w, slots, scores, W, x, H, workspace)
+
+    def rule(self):
+        """The rule as a descriptor (MoeCache.set_scoring); its bias stays this object's."""
+        return _lib.RouteScoredDesc.from_buffer_copy(
+            self._packed(0, 0, 0, 0, bias=0 if self.bias is None else self.bias.data_ptr()))
+
+    def from_product(self, W, x, ids, w, slots, workspace, H, stream=None):
+        """The same from W [n_experts][H] and x [tokens][H] (f32), whose product moe_route's kernels make in workspace
+        (BatchedMoe.route: hidden 2048, n_experts a multiple of 64 up to 256)."""
+        T, _, dev = _first(x, H, "x")
+        out = (T, self.K)
+        desc = self._packed(0, 0, 0, T, 0 if self.bias is None else _vec(self.bias, self.E, _F32, dev, "bias"), 0, self.E,
+                            _out(ids, out, _I32, dev, "ids"), _out(w, out, _F32, dev, "w"), _out(slots, out, _I32, dev, "slots"),
+                            0, _out(W, (self.E, H), _F32, dev, "W"), _out(x, (T, H), _F32, dev, "x"), H,
+                            workspace.data_ptr())
+        _call(self._fn, desc, dev, stream, "moe_route_scored")
 
     def __call__(self, logits, ids=None, w=None, table=None, dummy=None, slots=None, scores=None, stream=None):
         """logits [tokens][n_experts] f32, bf16 or fp16 -> ids [tokens][K] int32, w [tokens][K] f32.
@@ -145,12 +164,12 @@ class ScoredRouter:
         if w is None:
             w = _empty(out, _F32, dev, stream)
         bias = self.bias
-        desc = self._pack(logits.data_ptr(), ld, _dtype(logits, "logits"), T, *self._rule,
-                          0 if bias is None else _vec(bias, E, _F32, dev, "bias"),
-                          0 if table is None else _vec(table, E, _I32, dev, "table"), E if dummy is None else dummy,
-                          _out(ids, out, _I32, dev, "ids"), _out(w, out, _F32, dev, "w"),
-                          0 if slots is None else _out(slots, out, _I32, dev, "slots"),
-                          0 if scores is None else _out(scores, (T, E), _F32, dev, "scores"))
+        desc = self._packed(logits.data_ptr(), ld, _dtype(logits, "logits"), T,
+                            0 if bias is None else _vec(bias, E, _F32, dev, "bias"),
+                            0 if table is None else _vec(table, E, _I32, dev, "table"), E if dummy is None else dummy,
+                            _out(ids, out, _I32, dev, "ids"), _out(w, out, _F32, dev, "w"),
+                            0 if slots is None else _out(slots, out, _I32, dev, "slots"),
+                            0 if scores is None else _out(scores, (T, E), _F32, dev, "scores"))
         _call(self._fn, desc, dev, stream, "moe_route_scored")
         return ids, w
 

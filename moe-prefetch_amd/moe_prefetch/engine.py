@@ -79,6 +79,7 @@ class MoeCache:
         self.h = h.value
         self.device = device
         self.cache_prior = cache_prior
+        self._scoring = {}              # layer -> ScoredRouter
         self.prior_space = prior_space
 
     @classmethod
@@ -182,6 +183,13 @@ class MoeCache:
         """Always-on shared expert of `layer` (its [up|gate|down] bytes, host or device); None removes it."""
         check(lib().moe_cache_set_shared(self.h, layer, _ptr(expert), self.expert_bytes(layer) if expert is not None
                                          else 0), "set_shared")
+
+    def set_scoring(self, layer, router):
+        """Route `layer` by a ScoredRouter's rule (read from it now, its bias at every call); None returns to softmax and
+        top-k.  Such a layer decodes through decode_batch, one token too."""
+        rule = None if router is None else router.rule()
+        check(lib().moe_cache_set_scoring(self.h, layer, None if rule is None else ctypes.byref(rule)), "set_scoring")
+        self._scoring[layer] = router     # keeps the bias alive
 
     def lookup(self, layer):
         v = _lib.LayerView()

@@ -27,12 +27,15 @@ def scored(**kw):
     dict(E=0), dict(E=1025), dict(K=0), dict(K=65), dict(E=5, K=6), dict(score=2), dict(n_groups=0), dict(n_groups=65),
     dict(n_groups=5), dict(top_groups=0), dict(top_groups=2), dict(n_groups=16, top_groups=1), dict(group_best=0),
     dict(group_best=3), dict(n_groups=64, top_groups=64, group_best=2), dict(scale=float("inf")),
-    dict(scale=float("nan")), dict(n_tok=-1), dict(n_tok=(1 << 20) + 1), dict(logits_type=3), dict(logits=None), dict(ids=None), dict(w=None),
+    dict(scale=float("nan")), dict(n_tok=-1), dict(n_tok=(1 << 20) + 1), dict(logits_type=3), dict(logits=None), dict(ids=None),
+    dict(logits=None, W=PTR, x=PTR, H=2048), dict(logits=None, W=PTR, x=PTR + 8, H=2048, workspace=PTR),
+    dict(logits=None, W=PTR, x=PTR, H=1024, workspace=PTR), dict(logits=None, W=PTR, x=PTR, H=2048, workspace=PTR, E=72),
+    dict(logits=None, W=PTR, x=PTR, H=2048, workspace=PTR, n_tok=65536), dict(w=None),
     dict(logits_stride=63), dict(logits=PTR + 2), dict(logits_type=1, logits=PTR + 1), dict(ids=PTR + 2),
     dict(bias=PTR + 1), dict(table=PTR + 2), dict(slots=PTR + 3), dict(scores=PTR + 1)])
 def test_scored_refusals(bad):
     assert scored(**bad) == _lib.MOE_ERR_ARG
-    assert b"moe_route_scored" in L.moe_last_error()
+    assert any(w in L.moe_last_error() for w in (b"moe_route_scored", b"hidden size", b"n_experts"))
 
 
 def norm(**kw):
@@ -131,6 +134,36 @@ def test_rules_are_refused_where_they_are_made():
         BlockNorm(64, post_weight=torch.ones(64), post=False)
     with pytest.raises(MoeError, match="vocabulary"):
         Sampler(1 << 21)
+
+
+def test_scoring_of_a_cache():
+    from moe_prefetch import MoeCache
+    c = MoeCache(2, n_experts=128, intermediate=768, n_slots=16, device=-1)
+    try:
+        rule = ScoredRouter(128, 8, score="sigmoid", n_groups=8, top_groups=4, group_best=2, scale=2.5)
+        c.set_scoring(1, rule)
+        c.set_scoring(1, None)
+        with pytest.raises(MoeError, match="the cache 8 of 128"):
+            c.set_scoring(0, ScoredRouter(64, 8))
+        with pytest.raises(MoeError, match="the cache 8 of 128"):
+            c.set_scoring(0, ScoredRouter(128, 6))
+        with pytest.raises(MoeError, match="bad arguments"):
+            c.set_scoring(2, rule)
+        bad = rule.rule()
+        bad.n_groups = 7
+        assert L.moe_cache_set_scoring(c.h, 0, ctypes.byref(bad)) == _lib.MOE_ERR_ARG
+        bad = rule.rule()
+        bad.bias = PTR + 2
+        assert L.moe_cache_set_scoring(c.h, 0, ctypes.byref(bad)) == _lib.MOE_ERR_ARG
+        assert L.moe_cache_set_scoring(None, 0, ctypes.byref(bad)) == _lib.MOE_ERR_ARG
+    finally:
+        c.close()
+    c = MoeCache(1, n_experts=128, intermediate=768, n_slots=16, device=-1, cache_prior=0.01)
+    try:
+        with pytest.raises(MoeError, match="prior"):
+            c.set_scoring(0, rule)
+    finally:
+        c.close()
 
 
 def test_cpu_tensors_are_refused():

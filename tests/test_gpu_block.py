@@ -159,6 +159,37 @@ def test_route_matches_moe_route():
     assert torch.allclose(w, w2, rtol=2e-6, atol=0)
 
 
+def exact_product(g, T, E):
+    """W, x whose product is exact in f32 in any order (small whole numbers, W over 64), and the product."""
+    W = torch.randint(-3, 4, (E, 2048), generator=g, device=DEV).float() / 64.0
+    x = torch.randint(-2, 3, (T, 2048), generator=g, device=DEV).float()
+    return W, x, (x.double() @ W.double().t())
+
+
+@pytest.mark.parametrize("T, E, K", [(1, 64, 6), (3, 256, 8), (37, 128, 8), (300, 256, 10), (1000, 128, 1)])
+def test_route_from_the_routers_product(T, E, K):
+    from moe_prefetch.batched import BatchedMoe
+    g = gen(40 + T)
+    W, x, logits = exact_product(g, T, E)
+    bias = 0.1 * randn(g, E)
+    rule = dict(score="sigmoid", n_groups=8, top_groups=4, group_best=2, scale=2.5)
+    m = BatchedMoe(T + 2, n_experts=E, n_expert_used=K)
+    m.ids.fill_(-3)
+    torch.cuda.synchronize()
+    got = m.route(T, W=W, x=x, router=ScoredRouter(E, K, bias=bias, **rule))
+    torch.cuda.synchronize()
+    check_route(logits, got, K=K, bias=np64(bias), **rule)
+    assert (m.ids[T:] == -3).all()
+    # and from given logits
+    got = m.route(T, logits=logits.float(), router=ScoredRouter(E, K, bias=bias, **rule))
+    torch.cuda.synchronize()
+    check_route(logits, got, K=K, bias=np64(bias), **rule)
+    for bad in (dict(router=ScoredRouter(E, K + 1)), dict(router=ScoredRouter(E, K), table=m.ids),
+                dict(router=ScoredRouter(E, K), logits=logits.float()[:0])):
+        with pytest.raises(ValueError):
+            m.route(T, **{"W": W, "x": x, **bad})
+
+
 # ---- block norm -----------------------------------------------------------------
 def check_norm(dt, x, got, y_dt=None, **kw):
     y, r, e_y, e_r = R.block_norm(np64(x), **{k: np64(v) if torch.is_tensor(v) else v for k, v in kw.items()})
@@ -427,6 +458,110 @@ def test_python_refusals():
         n(x, gate=torch.zeros(64, device=DEV))
     with pytest.raises(_lib.MoeError, match="same memory"):
         n(x, x.clone(), out=x, residual=x)
+
+
+@pytest.mark.parametrize("B", [1, 5, 80])
+@pytest.mark.parametrize("cpu", [False, True])
+def test_decode_batch_of_scored_layers(B, cpu):
+    # a cache with one layer routed by scores and one by softmax: the same bits as the calls it is made of
+    from gpu_rig import Rig
+    from moe_prefetch.batched import BatchedMoe
+    E, K = 128, 8
+    rig = Rig([40, 128], [_lib.TYPE_Q4K, _lib.TYPE_Q6K], T=B, steer=False, admit="window", batch_tables=True)
+    bias = 0.02 * randn(gen(41), E)
+    router = ScoredRouter(E, K, score="sigmoid", bias=bias, n_groups=8, top_groups=4, group_best=2, scale=2.5)
+    st = torch.cuda.current_stream().cuda_stream
+    try:
+        if cpu:
+            rig.cache.set_sidecar(4, (1, 2))
+        rig.cache.set_scoring(0, router)
+        x = rig.x.transpose(0, 1).contiguous()
+        out = torch.empty((2, B, 2048), device=DEV)
+        with pytest.raises(_lib.MoeError, match="moe_decode_batch"):
+            rig.cache.decode_token(x[:, 0].contiguous(), out[:, 0].contiguous(), stream=st)
+        with pytest.raises(_lib.MoeError, match="moe_decode_batch"):
+            rig.cache.decode_layer(1, x[1, 0], out[1, 0], stream=st)
+        for rep in range(3):                          # the slots change between the steps, the outputs do not
+            ids = rig.cache.decode_batch(x, out, stream=st)
+            torch.cuda.synchronize()
+            for l in range(2):
+                m, want = BatchedMoe(B), torch.empty((B, 2048), device=DEV)
+                m.forward(x[l], want, rig.stores[l].dev, rig.eb[l], E, rig.down_types[l], W=rig.W[l], xf32=x[l],
+                          router=router if l == 0 else None, stream=st)
+                torch.cuda.synchronize()
+                assert np.array_equal(ids[l], m.ids[:B].cpu().numpy()), (rep, l)
+                assert torch.equal(out[l], want), (rep, l)
+            bias += 0.01 * randn(gen(42 + rep), E)    # balancing in place reaches the cache's next call
+            torch.cuda.synchronize()
+        rig.cache.set_scoring(0, None)
+        rig.cache.decode_token(x[:, 0].contiguous(), out[:, 0].contiguous(), stream=st)
+    finally:
+        rig.close()
+
+
+def test_a_decode_step_of_all_of_them():
+    # two layers and the next token for a batch: norm, scored routing, expert products, the rows' sum with post-norm,
+    # gate and residual, the next norm, logits, sampling; every step against its definition, then captured and replayed
+    from gpu_rig import Pinned, synth_experts_dev
+    from moe_prefetch.batched import BatchedMoe
+    B, E, K, H, V, eb = 6, 64, 6, 2048, 5003, _lib.lib().moe_expert_bytes(2048, 256, _lib.TYPE_Q4K)
+    g = gen(50)
+    stores = [torch.empty(E * eb, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    for l in range(2):
+        synth_experts_dev(7, l, 0, E, 256, _lib.TYPE_Q4K, stores[l].data_ptr(), eb)
+    torch.cuda.synchronize()
+    wt = lambda: (1.0 + 0.1 * randn(g, H)).to(torch.bfloat16)
+    bf = torch.bfloat16
+    Wr = [0.02 * randn(g, E, H) for _ in range(2)]
+    head = (0.03 * randn(g, V, H)).to(bf)
+    bias = 0.05 * randn(g, E)
+    w_in, w_mid, w_post, w_out = wt(), wt(), wt(), wt()
+    first = BlockNorm(H, weight=w_in)
+    between = [BlockNorm(H, weight=w, post_weight=w_post, scale=0.5, gate_act="sigmoid") for w in (w_mid, w_out)]
+    router = ScoredRouter(E, K, score="sigmoid", bias=bias, n_groups=4, top_groups=2, group_best=2, scale=2.0)
+    sampler = Sampler(V)
+    moe = BatchedMoe(B, n_experts=E, n_expert_used=K, intermediate=256)
+    x = randn(g, B, H).to(bf)
+    gate = randn(g, B)
+    u = torch.rand(B, generator=g, device=DEV)
+    pairs = [torch.empty(B, K, H, device=DEV) for _ in range(2)]
+    scratch = torch.empty(B, H, device=DEV)
+
+    def step(keep=None):
+        r, (y, _) = x, first(x)
+        for l in range(2):
+            st = torch.cuda.current_stream().cuda_stream
+            logits = y.float() @ Wr[l].t()
+            moe.route(B, logits=logits, router=router, stream=st)
+            moe.dispatch(B, stream=st)
+            moe.experts(y, scratch, B, stores[l].data_ptr(), eb, E, _lib.TYPE_Q4K, pair_out=pairs[l], stream=st)
+            was = r
+            y, r = between[l](r, pairs[l], gate)
+            if keep is not None:
+                torch.cuda.synchronize()
+                check_route(logits, (moe.ids, moe.w), K=K, score="sigmoid", bias=np64(bias), n_groups=4, top_groups=2,
+                            group_best=2, scale=2.0)
+                check_norm("bf16", was, (y, r), branch=pairs[l], gate=gate, weight=(w_mid, w_out)[l], post_weight=w_post,
+                           post=True, scale=0.5, gate_act="sigmoid")
+        lm = (y @ head.t()).float()
+        tokens, probs = sampler(lm, u, temperature=0.8, top_k=50, top_p=0.9, min_p=0.02)
+        if keep is not None:
+            check_sample(lm, u, (tokens, probs), temperature=0.8, top_k=50, top_p=0.9, min_p=0.02)
+        return tokens, probs, r
+
+    step(keep=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        x.copy_(randn(g, B, H))
+        u.copy_(torch.rand(B, generator=g, device=DEV))
+        graph.replay()
+        have = [t.clone() for t in got]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(have, want)), i
 
 
 def test_streams_and_two_calls_at_once():
