@@ -398,8 +398,13 @@ struct Row {
             uint64_t in = 0;
             if (vectors) {
                 uint4 q[NV];
+                if (i0 - (int)threadIdx.x * group + NV * step <= V) {             // (uniform) every vector of the workgroup's
 #pragma unroll
-                for (int k = 0; k < NV; ++k) q[k] = vec(i0 + k * step, V);
+                    for (int k = 0; k < NV; ++k) q[k] = *(const uint4 *)(l + i0 + k * step);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < NV; ++k) q[k] = vec(i0 + k * step, V);
+                }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t w = 0;
@@ -555,30 +560,62 @@ struct BinSearch {
     SampleShared &s;
     float vmax, per;
     uint64_t n_all, m_all;
+    // from the histogram in s.cnt and s.mass: each bin's count and mass become those of the bins before it
+    __device__ void prepare() {
+        const int b = SMP_PER * (int)threadIdx.x;
+        uint64_t q[SMP_PER], m = 0;
+        uint32_t k[SMP_PER], c = 0;
+#pragma unroll
+        for (int j = 0; j < SMP_PER; ++j) {
+            c += k[j] = s.cnt[b + j];
+            m += q[j] = s.mass[b + j];
+        }
+        uint64_t cb = block_before(c, s.wc), mb = block_before(m, s.wm);
+        n_all = m_all = 0;
+        for (int w = 0; w < SMP_WAVES; ++w) {
+            n_all += s.wc[w];
+            m_all += s.wm[w];
+        }
+#pragma unroll
+        for (int j = 0; j < SMP_PER; ++j) {
+            s.cnt[b + j] = (uint32_t)cb;
+            s.mass[b + j] = mb;
+            cb += k[j];
+            mb += q[j];
+        }
+        __syncthreads();
+    }
+    __device__ uint64_t cnt_to(int b) const { return b < SMP_BINS ? s.cnt[b] : n_all; }
+    __device__ uint64_t mass_to(int b) const { return b < SMP_BINS ? s.mass[b] : m_all; }
     __device__ void totals(uint64_t &n, uint64_t &m) const { n = n_all; m = m_all; }
     __device__ uint64_t mass_from(uint32_t key) const {
         const int b = bin_of(key_value(key), vmax, per);
         uint64_t sum = 0;
-        for (int i = threadIdx.x; i < b; i += SMP_THREADS) sum += s.mass[i];
-        row.each([&](float v, int) {
-            const uint32_t k = sort_key(v);
-            if (k >= key && bin_of(v, vmax, per) == b) sum += ms.fixed(k);
-        });
-        return block_sum(sum, s);
+        row.among(key_value(key), top_of(b), [&](float v, int) { sum += ms.fixed(sort_key(v)); });
+        return mass_to(b) + block_sum(sum, s);
+    }
+    // a bin's highest value
+    __device__ float top_of(int b) const {
+        const uint32_t kmax = sort_key(vmax);
+        return b == 0 ? vmax : key_value(lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return bin_of(key_value(k), vmax, per) < b; }) - 1);
     }
     __device__ Cut find(bool by_mass, uint64_t target) const {
         __syncthreads();
-        RadixSearch<T>::find_bin(s, by_mass, target, 0, 0);
-        const int b = (int)s.found_bin, n = (int)s.cnt[b];
-        uint64_t nb = s.found_c, mb = s.found_m;
-        if (n > SMP_LIST) return Cut{0, CUT_FULL, 0, 0};
         if (threadIdx.x == 0) s.list.n = 0;
+#pragma unroll
+        for (int j = 0; j < SMP_PER; ++j) {
+            const int b = SMP_PER * (int)threadIdx.x + j;
+            const uint64_t before = by_mass ? mass_to(b) : cnt_to(b), end = by_mass ? mass_to(b + 1) : cnt_to(b + 1);
+            if (before < target && target <= end) s.found_bin = (uint32_t)b;
+        }
         __syncthreads();
+        const int b = (int)s.found_bin, n = (int)(cnt_to(b + 1) - cnt_to(b));
+        uint64_t nb = cnt_to(b), mb = mass_to(b);
+        if (n > SMP_LIST) return Cut{0, CUT_FULL, 0, 0};
         // the bin's values, so that the pass over the row only compares
         const uint32_t kmax = sort_key(vmax);
         const float from = key_value(lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return bin_of(key_value(k), vmax, per) <= b; }));
-        const uint32_t above = b == 0 ? kmax + 1 : lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return bin_of(key_value(k), vmax, per) < b; });
-        row.among(from, key_value(above - 1), [&](float v, int i) { s.list.raw[atomicAdd(&s.list.n, 1u)] = entry(v, (uint32_t)i); });
+        row.among(from, top_of(b), [&](float v, int i) { s.list.raw[atomicAdd(&s.list.n, 1u)] = entry(v, (uint32_t)i); });
         sort_list(s.list, n);
         const int j0 = SMP_PER * (int)threadIdx.x;
         uint64_t q[SMP_PER], m = 0;
@@ -727,17 +764,15 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
         __syncthreads();
         if (!s.last) continue;
         __threadfence();
-        uint64_t c = 0, m = 0;
         for (int i = tid; i < SMP_BINS; i += SMP_THREADS) {
             s.cnt[i] = __hip_atomic_load(&r.cnt[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             s.mass[i] = __hip_atomic_load(&r.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            c += s.cnt[i];
-            m += s.mass[i];
         }
-        c = block_sum(c, s);
-        m = block_sum(m, s);
+        __syncthreads();
         const uint32_t kmax = sort_key(vmax);
-        if (vmax == INFINITY || !sample_row<T>(a, tok, kmax, cut, BinSearch<T>{row, ms, s, vmax, per, c, m}, s))
+        BinSearch<T> bins{row, ms, s, vmax, per, 0, 0};
+        bins.prepare();
+        if (vmax == INFINITY || !sample_row<T>(a, tok, kmax, cut, bins, s))
             sample_row<T>(a, tok, kmax, cut, RadixSearch<T>{row, ms, s}, s);
     }
 }
@@ -855,21 +890,33 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
     auto low = [&](int j) { return !(ms.e(entry_key(s.order[j])) >= (double)cut.min_p); };
     const double top_p = (double)fmaxf(cut.top_p, 0.0f);
     const bool with_p = cut.top_p < 1.0f, with_min = cut.min_p > 0.0f;
-    int kept;                                         // how many of the order stay
-    double total = mass;
-    if (by_k || !open) {
-        const int k = by_k ? min(cut.top_k, n) : n;
-        while (have < k) extend();
-        kept = k;
-        if (!by_k || cut.top_k <= n || !open) {
-            total = s.cum[k - 1];
-            open = false;
-        } else if (with_p) {
-            return false;                             // a share of an unknown mass
+    if (by_k && cut.top_k <= n && cut.top_k <= 64) {  // (about what one round sorts)
+        while (have < cut.top_k) extend();
+        n = have = cut.top_k;
+        sum = s.cum[n - 1];
+        open = false;
+    } else if (by_k && cut.top_k <= n) {              // the top_k candidates alone
+        // at least top_k reach lo, fewer reach hi
+        uint64_t lo = (uint64_t)bound << 32, hi = (uint64_t)(sort_key((float)ms.vmax) + 1) << 32;
+        while (cut.top_k < n && hi - lo > 1) {
+            const uint64_t mid = lo + (hi - lo) / 2;
+            int c = 0;
+#pragma unroll
+            for (int j = 0; j < PICK_PER; ++j) c += __popcll(__ballot(x[j] >= mid));
+            if (c >= cut.top_k) lo = mid;
+            else hi = mid;
+            if (c == cut.top_k) break;
         }
-    } else {
-        // all candidates together may not reach far enough
-        double all = 0.0;
+#pragma unroll
+        for (int j = 0; j < PICK_PER; ++j)
+            if (x[j] < lo) x[j] = 0;
+        n = cut.top_k;
+        open = false;
+    }
+    const bool sure = !by_k || !open;                 // the mass that top-p takes its share of is known
+    double total = mass;
+    if (have < n) {
+        double all = 0.0;                             // of the candidates
         bool low_one = false;
 #pragma unroll
         for (int j = 0; j < PICK_PER; ++j) {
@@ -878,24 +925,29 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
             low_one |= x[j] && !(e >= (double)cut.min_p);
         }
         for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o, 64);
-        const double reach = with_p || with_min ? top_p * total : cut.u * total;
-        if (all * (1.0 + 1e-12) < reach && !(with_min && __ballot(low_one))) return false;
+        const bool any_low = with_min && __ballot(low_one);
+        if (!open) total = all;
+        if (open) {                                   // all candidates together may not reach far enough
+            if (!sure && (with_p || !any_low)) return false;
+            const double reach = with_p || with_min ? top_p * total : cut.u * total;
+            if (all * (1.0 + 1e-12) < reach && !any_low) return false;
+        }
         do extend();
-        while (have < n && !(with_p && sum >= top_p * total) && !(with_min && low(have - 1)) &&
+        while (have < n && !(with_p && sure && sum >= top_p * total) && !(with_min && low(have - 1)) &&
                !(!with_p && !with_min && sum > cut.u * total));
-        kept = have;
     }
-    if (with_p) {
+    int kept = have;                                  // how many of the order stay
+    if (!open && have == n) total = sum;
+    if (with_p && sure) {
         const double want = top_p * total;
         const int f = first_of(kept, [&](int j) { return s.cum[j] >= want; });
-        if (f < kept) { kept = f + 1; open = false; }
+        if (f < kept) { kept = f + 1; open = false; total = s.cum[f]; }
     }
     if (with_min) {
         const int f = first_of(kept, low);
-        if (f < kept) { kept = max(f, 1); open = false; }
+        if (f < kept) { kept = max(f, 1); open = false; total = s.cum[kept - 1]; }
     }
     if (open && (with_p || with_min || by_k)) return false;
-    if (!open) total = s.cum[kept - 1];
     const double t = cut.u * total;
     const int at = first_of(kept, [&](int j) { return s.cum[j] > t; });
     if (at == kept) return false;                     // behind the candidates
