@@ -74,10 +74,16 @@ __device__ inline uint32_t sort_key(float v) {
 }
 __device__ inline float key_value(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 constexpr uint32_t KEY_NONE = 0x007fffffu;            // of -inf
-// an entry of the order: the larger comes first
-__device__ inline uint64_t entry(float v, uint32_t i) { return ((uint64_t)sort_key(v) << 32) | (uint32_t)~i; }
-__device__ inline uint32_t entry_key(uint64_t e) { return (uint32_t)(e >> 32); }
-__device__ inline int32_t entry_token(uint64_t e) { return (int32_t)~(uint32_t)e; }
+// An entry of the order: key and index as the mantissa of a number in [1, 2), so that the larger comes first (the
+// lower index of equal keys) and a comparison is one of f64: four clocks where one of 64-bit integers takes
+// sixteen.  0 is none.
+static_assert(SLICES_MAX * SLICE == 1 << 20, "20 bits of index");
+__device__ inline uint64_t entry_from(uint32_t key) { return (0x3ffull << 52) | ((uint64_t)key << 20); }    // the key's last
+__device__ inline uint64_t entry(float v, uint32_t i) { return entry_from(sort_key(v)) | (i ^ 0xfffffu); }
+__device__ inline uint32_t entry_key(uint64_t e) { return (uint32_t)(e >> 20); }
+__device__ inline int32_t entry_token(uint64_t e) { return (int32_t)(~(uint32_t)e & 0xfffffu); }
+__device__ inline bool gt(uint64_t a, uint64_t b) { return __builtin_bit_cast(double, a) > __builtin_bit_cast(double, b); }
+__device__ inline bool ge(uint64_t a, uint64_t b) { return __builtin_bit_cast(double, a) >= __builtin_bit_cast(double, b); }
 
 struct SampleCuts {
     float temp, top_p, min_p;
@@ -264,30 +270,36 @@ __global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(Sampl
 
 struct SampleList {
     __attribute__((aligned(16))) uint64_t raw[SMP_LIST], sorted[SMP_LIST];
-    uint32_t n;
+    uint32_t n, hits;
 };
-// sorted[0 .. n) = raw[0 .. n) in descending order (the entries differ).  Up to 1,024 entries by each one's rank, four lanes
-// counting (348 entries: 1 us against 9 of the network, whose every step waits for LDS); more by a bitonic network, whose strides below 64 stay within a wave's 128 entries and need no barrier.
+// sorted[0 .. n) = raw[0 .. n) in descending order (the entries differ).  Up to 1,024 entries by each one's rank, four
+// lanes counting for four entries (348 of them: 2 us against 9 of the network, whose every step waits for LDS); more by a
+// bitonic network, whose strides below 64 stay within a wave's 128 entries and need no barrier.
 __device__ inline void sort_list(SampleList &s, int n) {
     const int tid = threadIdx.x;
     __syncthreads();
     if (n <= 1024) {
         for (int i = n + tid; i < (n + 31) / 32 * 32; i += SMP_THREADS) s.raw[i] = 0;
         __syncthreads();
-        for (int i0 = 0; i0 < n; i0 += SMP_THREADS / 4) {
-            const int i = i0 + (tid >> 2);
-            const uint64_t mine = s.raw[min(i, n - 1)];
-            int rank = 0;
+        for (int i0 = 0; i0 < n; i0 += SMP_THREADS) {
+            uint64_t mine[4];
+            int rank[4] = {};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mine[e] = s.raw[min(i0 + (tid >> 2) + e * (SMP_THREADS / 4), n - 1)];
             for (int j = 2 * (tid & 3); j < n; j += 32) {
 #pragma unroll
                 for (int k = 0; k < 32; k += 8) {
                     const ulonglong2 q = *(const ulonglong2 *)&s.raw[j + k];
-                    rank += (q.x > mine) + (q.y > mine);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) rank[e] += gt(q.x, mine[e]) + gt(q.y, mine[e]);
                 }
             }
-            rank += dpp_i<DPP_XOR1>(rank);
-            rank += dpp_i<DPP_XOR2>(rank);
-            if ((tid & 3) == 0 && i < n) s.sorted[rank] = mine;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                rank[e] += dpp_i<DPP_XOR1>(rank[e]);
+                rank[e] += dpp_i<DPP_XOR2>(rank[e]);
+                if ((tid & 3) == e && i0 + (tid >> 2) + e * (SMP_THREADS / 4) < n) s.sorted[rank[e]] = mine[e];
+            }
         }
         __syncthreads();
         return;
@@ -300,7 +312,7 @@ __device__ inline void sort_list(SampleList &s, int n) {
             for (int p = tid; p < m / 2; p += SMP_THREADS) {
                 const int i = 2 * p - (p & (d - 1));  // pairs (i, i + d)
                 const uint64_t x = s.sorted[i], y = s.sorted[i + d];
-                if ((x < y) == ((i & k) == 0)) {
+                if (gt(y, x) == ((i & k) == 0)) {
                     s.sorted[i] = y;
                     s.sorted[i + d] = x;
                 }
@@ -359,91 +371,111 @@ struct Row {
     const raw *l;
     int V;
     __device__ float at(int i) const { return Elem<T>::load(l[i]); }
-    // f(value, index) of every token that is on, of [i0, i1) (i0 a multiple of 8)
-    // (the next vector is on its way while one is worked on)
-    template <class F>
+    // (What follows runs once per row on one CU: its time is that of fetching its instructions as much as of running
+    // them, so the ends of a row go through a short loop of their own instead of tests beside every vector.)
+    // f(value, index) of every token that is on, of [i0, i1) (i0 a multiple of 8); f a vector's elements times in the
+    // code, or once
+    template <bool UNROLL, class F>
     __device__ inline void each(int i0, int i1, F f) const {
         constexpr int VEC = 16 / sizeof(raw);
+        int done = i0;
         if ((uintptr_t)l % 16 == 0) {
+            done = max(i0, i1 / VEC * VEC);
             int i = i0 + (int)threadIdx.x * VEC;
-            uint4 q = vec(i, i1);
-            for (; i < i1; i += SMP_THREADS * VEC) {
-                const uint4 next = vec(i + SMP_THREADS * VEC, i1);
-                raw t[VEC];
-                __builtin_memcpy(t, &q, 16);
+            uint4 next = {};
+            if (i < done) next = *(const uint4 *)(l + i);
+#pragma unroll 1
+            for (; i < done; i += SMP_THREADS * VEC) {
+                uint4 q = next;                       // the next vector is on its way meanwhile
+                if (i + SMP_THREADS * VEC < done) next = *(const uint4 *)(l + i + SMP_THREADS * VEC);
+                if constexpr (UNROLL) {
+                    raw t[VEC];
+                    __builtin_memcpy(t, &q, 16);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float v = Elem<T>::load(t[e]);
-                    if (v > -INFINITY) f(v, i + e);
+                    for (int e = 0; e < VEC; ++e) {
+                        const float v = Elem<T>::load(t[e]);
+                        if (v > -INFINITY) f(v, i + e);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int e = 0; e < VEC; ++e) {
+                        const float v = T == T_F32 ? __uint_as_float(q.x) : Elem<T>::load((raw)q.x);
+                        constexpr int B = 8 * sizeof(raw) % 32;   // the vector moves down by one element
+                        q.x = B ? __builtin_amdgcn_alignbit(q.y, q.x, B) : q.y;
+                        q.y = B ? __builtin_amdgcn_alignbit(q.z, q.y, B) : q.z;
+                        q.z = B ? __builtin_amdgcn_alignbit(q.w, q.z, B) : q.w;
+                        q.w = q.w >> B;
+                        if (v > -INFINITY) f(v, i + e);
+                    }
                 }
-                q = next;
             }
-        } else {
-            for (int i = i0 + (int)threadIdx.x; i < i1; i += SMP_THREADS) {
-                const float v = at(i);
-                if (v > -INFINITY) f(v, i);
-            }
+        }
+#pragma unroll 1
+        for (int i = done + (int)threadIdx.x; i < i1; i += SMP_THREADS) {
+            const float v = at(i);
+            if (v > -INFINITY) f(v, i);
         }
     }
     template <class F>
-    __device__ inline void each(F f) const { each(0, V, f); }
-    // f(value, index) of the few tokens of [from, to]: 64 tokens to a thread at a time become a mask (three
-    // instructions each; a branch for each took 170 clocks), whose values are read again
-    template <class F>
-    __device__ inline void among(float from, float to, F f) const {
-        constexpr int VEC = 16 / sizeof(raw), NV = 64 / VEC;
-        const bool vectors = (uintptr_t)l % 16 == 0;
-        const int step = vectors ? SMP_THREADS * VEC : SMP_THREADS, group = vectors ? VEC : 1;
-        for (int i0 = (int)threadIdx.x * group; i0 < V; i0 += 64 / group * step) {
-            uint64_t in = 0;
-            if (vectors) {
-                uint4 q[NV];
-                if (i0 - (int)threadIdx.x * group + NV * step <= V) {             // (uniform) every vector of the workgroup's
-#pragma unroll
-                    for (int k = 0; k < NV; ++k) q[k] = *(const uint4 *)(l + i0 + k * step);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < NV; ++k) q[k] = vec(i0 + k * step, V);
-                }
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t w = 0;
-#pragma unroll
-                    for (int k = half * NV / 2; k < (half + 1) * NV / 2; ++k) {
-                        raw t[VEC];
-                        __builtin_memcpy(t, &q[k], 16);
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            const float v = Elem<T>::load(t[e]);
-                            w = 2 * w + (__builtin_amdgcn_fmed3f(v, from, to) == v);
-                        }
-                    }
-                    in = (in << 32) | w;
-                }
-            } else {
-                for (int k = 0; k < 64; ++k) {
-                    const int i = i0 + k * step;
-                    const float v = i < V ? at(i) : -INFINITY;
-                    in = 2 * in + (v >= from && v <= to);
-                }
-            }
-            for (; in; in &= ~(0x8000000000000000ull >> __clzll((long long)in))) {
-                const int k = __clzll((long long)in), i = i0 + k / group * step + k % group;
-                f(at(i), i);
-            }
+    __device__ inline void each(F f) const { each<false>(0, V, f); }
+    // The tokens of [from, to], at most SMP_LIST of them, into list.raw.  Values of one sign lie between two bit patterns, so
+    // a token takes a subtraction and a minimum, two 16-bit ones at once; the vectors that hold one are listed first
+    // and read again all at the same time.
+    __device__ inline void among(float from, float to, SampleList &list) const {
+        constexpr int VEC = 16 / sizeof(raw), NV = 16, STEP = SMP_THREADS * VEC;
+        auto take = [&](float v, int i) {
+            if (v >= from && v <= to) list.raw[atomicAdd(&list.n, 1u)] = entry(v, (uint32_t)i);
+        };
+        uint32_t *hit = (uint32_t *)list.sorted;
+        if (threadIdx.x == 0) list.n = list.hits = 0;
+        __syncthreads();
+        const bool same = (__float_as_uint(from) ^ __float_as_uint(to)) >> 31 == 0;
+        if ((uintptr_t)l % 16 != 0 || !same) {
+            each(take);
+            return;
         }
+        const bool neg = __float_as_uint(from) >> 31;
+        const auto x = bits_of(neg ? to : from), y = bits_of(neg ? from : to);  // x <= y as unsigned
+        const int whole = V / VEC * VEC;
+        for (int base = 0; base < whole; base += NV * STEP) {
+            const int i0 = base + (int)threadIdx.x * VEC;
+            uint4 q[NV];
+#pragma unroll
+            for (int k = 0; k < NV; ++k) q[k] = *(const uint4 *)(l + min(i0 + k * STEP, whole - VEC));
+            uint32_t in = 0;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) in = 2 * in + (near(q[k], x, y - x) && i0 + k * STEP < whole);
+            for (; in; in &= in - 1) hit[atomicAdd(&list.hits, 1u)] = (uint32_t)(i0 + (NV - __ffs(in)) * STEP);
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < (int)list.hits; j += SMP_THREADS) {
+            const int i = (int)hit[j];
+            const uint4 q = *(const uint4 *)(l + i);
+            raw t[VEC];
+            __builtin_memcpy(t, &q, 16);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) take(Elem<T>::load(t[e]), i + e);
+        }
+        for (int i = whole + (int)threadIdx.x; i < V; i += SMP_THREADS) take(at(i), i);
     }
 
 private:
-    __device__ inline uint4 vec(int i, int i1) const {            // -inf from i1 on
-        constexpr int VEC = 16 / sizeof(raw);
-        if (i + VEC <= i1) return *(const uint4 *)(l + i);
-        uint4 q;
-        raw t[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) t[e] = i + e < i1 ? l[i + e] : Elem<T>::store(-INFINITY);
-        __builtin_memcpy(&q, t, 16);
-        return q;
+    static __device__ inline auto bits_of(float v) {
+        if constexpr (T == T_F32) return __float_as_uint(v);
+        else return Elem<T>::store(v);
+    }
+    // whether one of the vector's elements e has e - x <= d as unsigned
+    static __device__ inline bool near(uint4 q, uint32_t x, uint32_t d) {
+        if constexpr (T == T_F32) {
+            return min(min(q.x - x, q.y - x), min(q.z - x, q.w - x)) <= d;
+        } else {
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            const u16x2 xx = {(uint16_t)x, (uint16_t)x};
+            auto sub = [&](uint32_t v) { return __builtin_bit_cast(u16x2, v) - xx; };
+            const u16x2 m = __builtin_elementwise_min(__builtin_elementwise_min(sub(q.x), sub(q.y)),
+                                                      __builtin_elementwise_min(sub(q.z), sub(q.w)));
+            return min((uint32_t)m.x, (uint32_t)m.y) <= d;
+        }
     }
 };
 
@@ -591,7 +623,8 @@ struct BinSearch {
     __device__ uint64_t mass_from(uint32_t key) const {
         const int b = bin_of(key_value(key), vmax, per);
         uint64_t sum = 0;
-        row.among(key_value(key), top_of(b), [&](float v, int) { sum += ms.fixed(sort_key(v)); });
+        const float from = key_value(key), to = top_of(b);
+        row.each([&](float v, int) { if (v >= from && v <= to) sum += ms.fixed(sort_key(v)); });
         return mass_to(b) + block_sum(sum, s);
     }
     // a bin's highest value
@@ -601,7 +634,6 @@ struct BinSearch {
     }
     __device__ Cut find(bool by_mass, uint64_t target) const {
         __syncthreads();
-        if (threadIdx.x == 0) s.list.n = 0;
 #pragma unroll
         for (int j = 0; j < SMP_PER; ++j) {
             const int b = SMP_PER * (int)threadIdx.x + j;
@@ -615,7 +647,7 @@ struct BinSearch {
         // the bin's values, so that the pass over the row only compares
         const uint32_t kmax = sort_key(vmax);
         const float from = key_value(lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return bin_of(key_value(k), vmax, per) <= b; }));
-        row.among(from, top_of(b), [&](float v, int i) { s.list.raw[atomicAdd(&s.list.n, 1u)] = entry(v, (uint32_t)i); });
+        row.among(from, top_of(b), s.list);
         sort_list(s.list, n);
         const int j0 = SMP_PER * (int)threadIdx.x;
         uint64_t q[SMP_PER], m = 0;
@@ -746,7 +778,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
         for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { s.cnt[i] = 0; s.mass[i] = 0; }
         __syncthreads();
         if (vmax < INFINITY)
-            row.each(min(part * run, a.V), min((part + 1) * run, a.V), [&](float v, int) {
+            row.template each<true>(min(part * run, a.V), min((part + 1) * run, a.V), [&](float v, int) {
                 const int b = bin_of(v, vmax, per);
                 atomicAdd(&s.cnt[b], 1u);
                 atomicAdd((unsigned long long *)&s.mass[b], (unsigned long long)ms.fixed(sort_key(v)));
@@ -810,11 +842,11 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
 #pragma unroll
         for (int j = 0; j < PICK_PER; ++j) x[j] = 64 * j + lane < n ? s.list[64 * j + lane] : 0;
     } else {                                          // the largest 512 of them
-        uint64_t lo = 0, hi = ~0ull;                  // more than 512 reach lo, at most 512 reach hi
+        uint64_t lo = entry_from(0), hi = entry_from(sort_key((float)ms.vmax) + 1);    // more than 512 reach lo, at most hi
         while (hi - lo > 1) {
             const uint64_t mid = lo + (hi - lo) / 2;
             int c = 0;
-            for (int j = lane; j < n; j += 64) c += s.list[j] >= mid;
+            for (int j = lane; j < n; j += 64) c += ge(s.list[j], mid);
             for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
             if (c > PICK_MAX) lo = mid;
             else hi = mid;
@@ -823,9 +855,9 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
         int c = 0;
         for (int j0 = 0; j0 < n; j0 += 64) {          // moved to the front: never past where they are read
             const uint64_t e = j0 + lane < n ? s.list[j0 + lane] : 0;
-            const uint64_t b = __ballot(e >= hi);
+            const uint64_t b = __ballot(ge(e, hi));
             wave_lds();
-            if (e >= hi) s.list[c + __popcll(b & ((1ull << lane) - 1))] = e;
+            if (ge(e, hi)) s.list[c + __popcll(b & ((1ull << lane) - 1))] = e;
             wave_lds();
             c += __popcll(b);
         }
@@ -842,12 +874,12 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
         uint64_t from = 1;
         if (c > 64) {
             // more than 64 of those left reach lo, at most 64 reach hi
-            uint64_t lo = (uint64_t)bound << 32, hi = min(below, (uint64_t)(sort_key((float)ms.vmax) + 1) << 32);
+            uint64_t lo = entry_from(bound), hi = min(below, entry_from(sort_key((float)ms.vmax) + 1));
             for (;;) {
                 const uint64_t mid = lo + (hi - lo) / 2;
                 c = 0;
 #pragma unroll
-                for (int j = 0; j < PICK_PER; ++j) c += __popcll(__ballot(x[j] >= mid));
+                for (int j = 0; j < PICK_PER; ++j) c += __popcll(__ballot(ge(x[j], mid)));
                 if (c > 64) lo = mid;
                 else hi = mid;
                 if (hi - lo == 1 || (c <= 64 && c >= 40)) break;
@@ -857,7 +889,7 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
         c = 0;
 #pragma unroll
         for (int j = 0; j < PICK_PER; ++j) {
-            const bool in = x[j] >= from;
+            const bool in = ge(x[j], from);
             const uint64_t b = __ballot(in);
             if (in) s.order[have + c + __popcll(b & ((1ull << lane) - 1))] = x[j];
             if (in) x[j] = 0;                         // taken
@@ -867,7 +899,7 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
         const uint64_t mine = lane < c ? s.order[have + lane] : 0;
         int rank = 0;
 #pragma unroll 16
-        for (int l = 0; l < 64; ++l) rank += lane_u64(mine, l) > mine;
+        for (int l = 0; l < 64; ++l) rank += gt(lane_u64(mine, l), mine);
         wave_lds();
         if (lane < c) s.order[have + rank] = mine;
         wave_lds();
@@ -897,19 +929,19 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
         open = false;
     } else if (by_k && cut.top_k <= n) {              // the top_k candidates alone
         // at least top_k reach lo, fewer reach hi
-        uint64_t lo = (uint64_t)bound << 32, hi = (uint64_t)(sort_key((float)ms.vmax) + 1) << 32;
+        uint64_t lo = entry_from(bound), hi = entry_from(sort_key((float)ms.vmax) + 1);
         while (cut.top_k < n && hi - lo > 1) {
             const uint64_t mid = lo + (hi - lo) / 2;
             int c = 0;
 #pragma unroll
-            for (int j = 0; j < PICK_PER; ++j) c += __popcll(__ballot(x[j] >= mid));
+            for (int j = 0; j < PICK_PER; ++j) c += __popcll(__ballot(ge(x[j], mid)));
             if (c >= cut.top_k) lo = mid;
             else hi = mid;
             if (c == cut.top_k) break;
         }
 #pragma unroll
         for (int j = 0; j < PICK_PER; ++j)
-            if (x[j] < lo) x[j] = 0;
+            if (!ge(x[j], lo)) x[j] = 0;
         n = cut.top_k;
         open = false;
     }
