@@ -337,10 +337,8 @@ struct NormArgs {
     int64_t ldx, ldb, ldr, ldy, gate_row;
     int gate_col;
     float scale, offset, eps, post_eps;
-    int vec;                    // set by the launcher: NORM_VEC_*
 };
-constexpr int NORM_VEC_X = 1, NORM_VEC_B = 2, NORM_VEC_G = 4, NORM_VEC_W = 8, NORM_VEC_R = 16, NORM_VEC_Y = 32;
-hipError_t launch_block_norm(NormArgs a, hipStream_t st);
+hipError_t launch_block_norm(const NormArgs &a, hipStream_t st);
 
 struct SampleArgs {
     const void *logits;

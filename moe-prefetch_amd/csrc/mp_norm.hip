@@ -15,53 +15,68 @@
 
 namespace mp {
 
-constexpr int NORM_MAX_WAVES = 16, NORM_ROWS = 8;     // branch rows on their way at once
+constexpr int NORM_MAX_WAVES = 16;
 
-struct alignas(8) Half4 { uint16_t v[4]; };
+template <int N> struct Vals { float v[N]; };         // N elements of a row
 
-// elements i .. i + 3 of a row (those below H; zero from there on); vec: the row may be read in whole vectors
-template <int T>
-__device__ inline float4 load4(const void *row, int64_t o, int i, int H, bool vec) {
-    typedef typename Elem<T>::raw raw;
-    const raw *p = (const raw *)row + o + i;
-    if (vec && i + 4 <= H) {
-        if constexpr (T == T_F32) {
-            return *(const float4 *)p;
-        } else {
-            const Half4 q = *(const Half4 *)p;
-            return make_float4(Elem<T>::load(q.v[0]), Elem<T>::load(q.v[1]), Elem<T>::load(q.v[2]), Elem<T>::load(q.v[3]));
-        }
-    }
-    float f[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = i + e < H ? Elem<T>::load(p[e]) : 0.0f;
-    return make_float4(f[0], f[1], f[2], f[3]);
+// Where a thread's elements lie: with WHOLE, N neighbouring ones at a time, in one vector (every row at whole
+// vectors, H a multiple of N); without, a workgroup's width apart, which keeps the single loads of a wave together.
+template <bool WHOLE, int N>
+__device__ inline int place(int j, int e) {
+    const int tid = (int)threadIdx.x, width = (int)blockDim.x;
+    return WHOLE ? N * (tid + width * j) + e : tid + width * (N * j + e);
 }
-template <int T>
-__device__ inline void store4(void *row, int64_t o, int i, int H, bool vec, float4 v) {
+// the thread's j-th elements of the row at o (0 beyond H)
+template <int T, bool WHOLE, int N>
+__device__ inline Vals<N> load_n(const void *row, int64_t o, int j, int H) {
     typedef typename Elem<T>::raw raw;
-    raw *p = (raw *)row + o + i;
-    if (vec && i + 4 <= H) {
-        if constexpr (T == T_F32) *(float4 *)p = v;
-        else *(Half4 *)p = Half4{{Elem<T>::store(v.x), Elem<T>::store(v.y), Elem<T>::store(v.z), Elem<T>::store(v.w)}};
-        return;
-    }
-    const float f[4] = {v.x, v.y, v.z, v.w};
+    const raw *p = (const raw *)row + o;
+    struct alignas(N * sizeof(raw) < 16 ? N * sizeof(raw) : 16) Vec { raw v[N]; } q;
+    Vals<N> f;
+    if constexpr (WHOLE) {
+        q = *(const Vec *)(p + place<WHOLE, N>(j, 0));
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (i + e < H) p[e] = Elem<T>::store(f[e]);
+        for (int e = 0; e < N; ++e) f.v[e] = Elem<T>::load(q.v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) q.v[e] = p[min(place<WHOLE, N>(j, e), H - 1)];      // (no branch: the loads go out together)
+#pragma unroll
+        for (int e = 0; e < N; ++e) f.v[e] = place<WHOLE, N>(j, e) < H ? Elem<T>::load(q.v[e]) : 0.0f;
+    }
+    return f;
+}
+template <int T, bool WHOLE, int N>
+__device__ inline void store_n(void *row, int64_t o, int j, int H, const Vals<N> &f) {
+    typedef typename Elem<T>::raw raw;
+    raw *p = (raw *)row + o;
+    struct alignas(N * sizeof(raw) < 16 ? N * sizeof(raw) : 16) Vec { raw v[N]; } q;
+    if constexpr (WHOLE) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) q.v[e] = Elem<T>::store(f.v[e]);
+        *(Vec *)(p + place<WHOLE, N>(j, 0)) = q;
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (place<WHOLE, N>(j, e) < H) p[place<WHOLE, N>(j, e)] = Elem<T>::store(f.v[e]);
+    }
 }
 // f32 or T
-template <int T>
-__device__ inline float4 load4_or(int type, const void *row, int64_t o, int i, int H, bool vec) {
-    return type == T_F32 ? load4<T_F32>(row, o, i, H, vec) : load4<T>(row, o, i, H, vec);
+template <int T, bool WHOLE, int N>
+__device__ inline Vals<N> load_or(int type, const void *row, int64_t o, int j, int H) {
+    return type == T_F32 ? load_n<T_F32, WHOLE, N>(row, o, j, H) : load_n<T, WHOLE, N>(row, o, j, H);
 }
 
-template <class F>
-__device__ inline float4 each4(float4 a, F f) { return make_float4(f(a.x), f(a.y), f(a.z), f(a.w)); }
-template <class F>
-__device__ inline float4 each4(float4 a, float4 b, F f) {
-    return make_float4(f(a.x, b.x), f(a.y, b.y), f(a.z, b.z), f(a.w, b.w));
+template <int N, class F>
+__device__ inline Vals<N> each(Vals<N> a, F f) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) a.v[e] = f(a.v[e]);
+    return a;
+}
+template <int N, class F>
+__device__ inline Vals<N> each(Vals<N> a, const Vals<N> &b, F f) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) a.v[e] = f(a.v[e], b.v[e]);
+    return a;
 }
 
 // the sum of v over the workgroup, the same bits on every thread; s: LDS words of this sum alone
@@ -77,92 +92,88 @@ __device__ inline float row_sum(float v, float *s) {
 }
 
 // the mean (layer norms) and 1 / sqrt(mean square about it + eps) of a row held in z, two passes over registers
-template <int NV>
-__device__ inline void moments(const float4 (&z)[NV], int H, int kind, float eps, float (*s)[NORM_MAX_WAVES], float &mu,
+template <bool WHOLE, int N, int NV>
+__device__ inline void moments(const Vals<N> (&z)[NV], int H, int kind, float eps, float (*s)[NORM_MAX_WAVES], float &mu,
                                float &inv) {
     mu = 0.0f;
     if (kind == 1) {
         float t = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int i = 4 * ((int)threadIdx.x + (int)blockDim.x * j);
-            const float d[4] = {z[j].x, z[j].y, z[j].z, z[j].w};
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (i + e < H) t += d[e];
-        }
+            for (int e = 0; e < N; ++e)
+                if (place<WHOLE, N>(j, e) < H) t += z[j].v[e];
         mu = row_sum(t, s[0]) / (float)H;
     }
     float q = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int i = 4 * ((int)threadIdx.x + (int)blockDim.x * j);
-        const float d[4] = {z[j].x - mu, z[j].y - mu, z[j].z - mu, z[j].w - mu};
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (i + e < H) q = fmaf(d[e], d[e], q);
-    }
+        for (int e = 0; e < N; ++e) {
+            const float d = z[j].v[e] - mu;
+            if (place<WHOLE, N>(j, e) < H) q = fmaf(d, d, q);
+        }
     inv = 1.0f / sqrtf(row_sum(q, s[1]) / (float)H + eps);
 }
 
 // B: the branch's type, or -1 without one
-template <int T, int B, int NV>
+template <int T, int B, bool WHOLE, int N, int NV>
 __global__ __launch_bounds__(64 * NORM_MAX_WAVES) void block_norm_kernel(NormArgs a) {
     // weights and gate are read with the row where registers hold them, else where they are used
-    constexpr bool EARLY = NV <= 2;
+    constexpr bool EARLY = NV * N <= (WHOLE ? 8 : 4);
+    constexpr int ROWS = WHOLE && N == 4 ? 8 : 4;     // branch rows on their way at once
     __shared__ float s_sum[4][NORM_MAX_WAVES];
     const int64_t tok = blockIdx.x;
-    int at[NV];
-    float4 z[NV], x[NV], w[NV], c[NV], p[NV], pc[NV], g[NV];
-    auto vec_of = [&](const void *q, int j) { return load4_or<T>(a.w_type, q, 0, at[j], a.H, a.vec & NORM_VEC_W); };
+    Vals<N> z[NV], x[NV], w[NV], c[NV], p[NV], pc[NV], g[NV];
+    auto in = [&](int j) { return place<WHOLE, N>(j, 0) < a.H; };
+    auto vec_of = [&](const void *q, int j) { return load_or<T, WHOLE, N>(a.w_type, q, 0, j, a.H); };
     auto gate_of = [&](int j) {
-        if (a.gate_col) return load4_or<T>(a.gate_type, a.gate, tok * a.gate_row, at[j], a.H, a.vec & NORM_VEC_G);
+        if (a.gate_col) return load_or<T, WHOLE, N>(a.gate_type, a.gate, tok * a.gate_row, j, a.H);
         const float u = a.gate_type == T_F32 ? ((const float *)a.gate)[tok * a.gate_row]
                                              : Elem<T>::load(((const typename Elem<T>::raw *)a.gate)[tok * a.gate_row]);
-        return make_float4(u, u, u, u);
+        Vals<N> v;
+        for (int e = 0; e < N; ++e) v.v[e] = u;
+        return v;
     };
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int i = at[j] = 4 * ((int)threadIdx.x + (int)blockDim.x * j);
-        if (i >= a.H) {
-            x[j] = z[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            continue;
-        }
-        x[j] = load4<T>(a.x, tok * a.ldx, i, a.H, a.vec & NORM_VEC_X);
+        x[j] = z[j] = Vals<N>{};
+        if (!in(j)) continue;
+        x[j] = load_n<T, WHOLE, N>(a.x, tok * a.ldx, j, a.H);
         if (EARLY && a.w) w[j] = vec_of(a.w, j);
         if (EARLY && a.c) c[j] = vec_of(a.c, j);
         if (B < 0) continue;
         if (EARLY && a.pw) p[j] = vec_of(a.pw, j);
         if (EARLY && a.pc) pc[j] = vec_of(a.pc, j);
         if (EARLY && a.gate) g[j] = gate_of(j);
-        int64_t o = tok * a.n_sum * a.ldb;
-        for (int k0 = 0; k0 < a.n_sum; k0 += NORM_ROWS) {
-            float4 b[NORM_ROWS];
+        const int64_t o = tok * a.n_sum * a.ldb;
+        for (int k0 = 0; k0 < a.n_sum; k0 += ROWS) {
+            Vals<N> b[ROWS];
 #pragma unroll
-            for (int k = 0; k < NORM_ROWS; ++k)
-                if (k0 + k < a.n_sum) b[k] = load4<B < 0 ? T : B>(a.branch, o + (k0 + k) * a.ldb, i, a.H, a.vec & NORM_VEC_B);
+            for (int k = 0; k < ROWS; ++k)
+                if (k0 + k < a.n_sum) b[k] = load_n<B < 0 ? T : B, WHOLE, N>(a.branch, o + (k0 + k) * a.ldb, j, a.H);
 #pragma unroll
-            for (int k = 0; k < NORM_ROWS; ++k)
-                if (k0 + k < a.n_sum) z[j] = k0 + k == 0 ? b[0] : each4(z[j], b[k], [](float s, float v) { return s + v; });
+            for (int k = 0; k < ROWS; ++k)
+                if (k0 + k < a.n_sum) z[j] = k0 + k == 0 ? b[0] : each(z[j], b[k], [](float s, float v) { return s + v; });
         }
     }
     float mu, inv;
     if (B >= 0) {
-        if (a.post) moments(z, a.H, a.kind, a.post_eps, s_sum, mu, inv);
+        if (a.post) moments<WHOLE>(z, a.H, a.kind, a.post_eps, s_sum, mu, inv);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            if (at[j] >= a.H) continue;
+            if (!in(j)) continue;
             if (a.post) {
-                z[j] = each4(z[j], [&](float v) { return (v - mu) * inv; });
-                if (a.pw) z[j] = each4(z[j], EARLY ? p[j] : vec_of(a.pw, j), [&](float v, float u) { return v * (u + a.offset); });
-                if (a.pc) z[j] = each4(z[j], EARLY ? pc[j] : vec_of(a.pc, j), [](float v, float u) { return v + u; });
+                z[j] = each(z[j], [&](float v) { return (v - mu) * inv; });
+                if (a.pw) z[j] = each(z[j], EARLY ? p[j] : vec_of(a.pw, j), [&](float v, float u) { return v * (u + a.offset); });
+                if (a.pc) z[j] = each(z[j], EARLY ? pc[j] : vec_of(a.pc, j), [](float v, float u) { return v + u; });
             }
             if (a.gate) {
                 if (!EARLY) g[j] = gate_of(j);
-                if (a.gate_act == 1) g[j] = each4(g[j], [](float u) { return 1.0f / (1.0f + expf(-u)); });
-                z[j] = each4(z[j], g[j], [](float v, float u) { return v * u; });
+                if (a.gate_act == 1) g[j] = each(g[j], [](float u) { return 1.0f / (1.0f + expf(-u)); });
+                z[j] = each(z[j], g[j], [](float v, float u) { return v * u; });
             }
-            z[j] = each4(z[j], x[j], [&](float v, float u) { return fmaf(a.scale, v, u); });
+            z[j] = each(z[j], x[j], [&](float v, float u) { return fmaf(a.scale, v, u); });
         }
     } else {
 #pragma unroll
@@ -171,29 +182,48 @@ __global__ __launch_bounds__(64 * NORM_MAX_WAVES) void block_norm_kernel(NormArg
     if (a.r)
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            if (at[j] < a.H) store4<T>(a.r, tok * a.ldr, at[j], a.H, a.vec & NORM_VEC_R, z[j]);
+            if (in(j)) store_n<T, WHOLE, N>(a.r, tok * a.ldr, j, a.H, z[j]);
     if (!a.y) return;
-    moments(z, a.H, a.kind, a.eps, s_sum + 2, mu, inv);
+    moments<WHOLE>(z, a.H, a.kind, a.eps, s_sum + 2, mu, inv);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        if (at[j] >= a.H) continue;
-        float4 y = each4(z[j], [&](float v) { return (v - mu) * inv; });
-        if (a.w) y = each4(y, EARLY ? w[j] : vec_of(a.w, j), [&](float v, float u) { return v * (u + a.offset); });
-        if (a.c) y = each4(y, EARLY ? c[j] : vec_of(a.c, j), [](float v, float u) { return v + u; });
-        if (a.y_type == T_F32) store4<T_F32>(a.y, tok * a.ldy, at[j], a.H, a.vec & NORM_VEC_Y, y);
-        else store4<T>(a.y, tok * a.ldy, at[j], a.H, a.vec & NORM_VEC_Y, y);
+        if (!in(j)) continue;
+        Vals<N> y = each(z[j], [&](float v) { return (v - mu) * inv; });
+        if (a.w) y = each(y, EARLY ? w[j] : vec_of(a.w, j), [&](float v, float u) { return v * (u + a.offset); });
+        if (a.c) y = each(y, EARLY ? c[j] : vec_of(a.c, j), [](float v, float u) { return v + u; });
+        if (a.y_type == T_F32) store_n<T_F32, WHOLE, N>(a.y, tok * a.ldy, j, a.H, y);
+        else store_n<T, WHOLE, N>(a.y, tok * a.ldy, j, a.H, y);
     }
+}
+
+template <int T, int B, bool WHOLE, int N>
+static hipError_t launch_norm_n(const NormArgs &a, hipStream_t st) {
+    // N elements a thread, up to 1,024 threads; more elements a thread beyond that
+    const int groups = (a.H + N - 1) / N, nv = groups <= 1024 ? 1 : groups <= 2048 ? 2 : 4;
+    const dim3 grid((unsigned)a.n_tok), block((unsigned)(((groups + nv - 1) / nv + 63) / 64 * 64));
+    if (nv == 1) hipLaunchKernelGGL((block_norm_kernel<T, B, WHOLE, N, 1>), grid, block, 0, st, a);
+    else if (nv == 2) hipLaunchKernelGGL((block_norm_kernel<T, B, WHOLE, N, 2>), grid, block, 0, st, a);
+    else if constexpr (N == 4) hipLaunchKernelGGL((block_norm_kernel<T, B, WHOLE, N, 4>), grid, block, 0, st, a);
+    return hipGetLastError();
+}
+
+// whether every row of every tensor begins at whole vectors of n elements (at 16 bytes if those are longer)
+static bool whole_vectors(const NormArgs &a, int n) {
+    auto whole = [n](const void *p, int type, int64_t ld) {
+        const int size = type == T_F32 ? 4 : 2, bytes = size * n < 16 ? size * n : 16;
+        return (uintptr_t)p % bytes == 0 && ld * size % bytes == 0;
+    };
+    return a.H % n == 0 && whole(a.x, a.x_type, a.ldx) && whole(a.branch, a.b_type, a.ldb) &&
+           (!a.gate_col || whole(a.gate, a.gate_type, a.gate_row)) && whole(a.w, a.w_type, 0) && whole(a.c, a.w_type, 0) &&
+           whole(a.pw, a.w_type, 0) && whole(a.pc, a.w_type, 0) && whole(a.r, a.x_type, a.ldr) && whole(a.y, a.y_type, a.ldy);
 }
 
 template <int T, int B>
 static hipError_t launch_norm_b(const NormArgs &a, hipStream_t st) {
-    // a thread four elements, up to 1,024 threads; more elements a thread beyond that
-    const int groups = (a.H + 3) / 4, nv = groups <= 1024 ? 1 : groups <= 2048 ? 2 : 4;
-    const dim3 grid((unsigned)a.n_tok), block((unsigned)(((groups + nv - 1) / nv + 63) / 64 * 64));
-    if (nv == 1) hipLaunchKernelGGL((block_norm_kernel<T, B, 1>), grid, block, 0, st, a);
-    else if (nv == 2) hipLaunchKernelGGL((block_norm_kernel<T, B, 2>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((block_norm_kernel<T, B, 4>), grid, block, 0, st, a);
-    return hipGetLastError();
+    // eight elements a thread where x and the branch are of 16 bits: half the waves, whole 16-byte loads
+    if constexpr (T != T_F32 && B != T_F32)
+        if (whole_vectors(a, 8)) return launch_norm_n<T, B, true, 8>(a, st);
+    return whole_vectors(a, 4) ? launch_norm_n<T, B, true, 4>(a, st) : launch_norm_n<T, B, false, 4>(a, st);
 }
 template <int T>
 static hipError_t launch_norm_t(const NormArgs &a, hipStream_t st) {
@@ -201,17 +231,7 @@ static hipError_t launch_norm_t(const NormArgs &a, hipStream_t st) {
     return a.b_type == T_F32 ? launch_norm_b<T, T_F32>(a, st) : launch_norm_b<T, T>(a, st);
 }
 
-hipError_t launch_block_norm(NormArgs a, hipStream_t st) {
-    // which tensors' rows all begin at whole vectors of four elements
-    auto whole = [](const void *p, int type, int64_t ld) { return (uintptr_t)p % (type == T_F32 ? 16 : 8) == 0 && ld % 4 == 0; };
-    a.vec = 0;
-    if (whole(a.x, a.x_type, a.ldx)) a.vec |= NORM_VEC_X;
-    if (whole(a.branch, a.b_type, a.ldb)) a.vec |= NORM_VEC_B;
-    if (whole(a.gate, a.gate_type, a.gate_row)) a.vec |= NORM_VEC_G;
-    if (whole(a.w, a.w_type, 0) && whole(a.c, a.w_type, 0) && whole(a.pw, a.w_type, 0) && whole(a.pc, a.w_type, 0))
-        a.vec |= NORM_VEC_W;
-    if (whole(a.r, a.x_type, a.ldr)) a.vec |= NORM_VEC_R;
-    if (whole(a.y, a.y_type, a.ldy)) a.vec |= NORM_VEC_Y;
+hipError_t launch_block_norm(const NormArgs &a, hipStream_t st) {
     return a.x_type == T_F32 ? launch_norm_t<T_F32>(a, st)
          : a.x_type == T_BF16 ? launch_norm_t<T_BF16>(a, st) : launch_norm_t<T_F16>(a, st);
 }
