@@ -794,7 +794,7 @@ int moe_block_norm(const moe_block_norm_desc *d, void *stream);
  * +inf share a row's whole mass.)  u of 1 and above counts as the largest number
  * below 1, u below 0 and NaN as 0.  Masses and their sums are computed in 64 bits, in an order that the row
  * alone decides: the same row gives the same token in any batch. */
-#define MOE_SAMPLE_MAX_V (1 << 20)
+#define MOE_SAMPLE_MAX_V 1000000
 #define MOE_SAMPLE_MAX_TOKENS 65535
 typedef struct {
     const void *logits;       /* dev [n_tok][V], MOE_DTYPE_*, rows logits_stride apart */

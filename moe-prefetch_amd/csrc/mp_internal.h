@@ -340,6 +340,7 @@ struct NormArgs {
 };
 hipError_t launch_block_norm(const NormArgs &a, hipStream_t st);
 
+constexpr int MAX_SAMPLE_V = 1000000;
 struct SampleArgs {
     const void *logits;
     int64_t ld;
@@ -350,7 +351,7 @@ struct SampleArgs {
     int top_k_all;
     int32_t *tokens;
     float *probs;
-    int slices, cap, cap_log, keep;     // set by the launcher, and the workspace's parts
+    int slices, cap, cap_log, keep, parts;      // set by the launcher, and the workspace's parts
     void *heads, *lists, *rest;
     uint32_t *n_rest;
 };

@@ -4161,6 +4161,8 @@ size_t moe_sample_workspace_bytes(int n_tok, int V) {
     return n_tok < 1 || V < 1 || V > MOE_SAMPLE_MAX_V ? 0 : mp::sample_ws_bytes(n_tok, V);
 }
 
+static_assert(mp::MAX_SAMPLE_V == MOE_SAMPLE_MAX_V, "header and library disagree");
+
 int moe_sample(const moe_sample_desc *d, void *stream) {
     if (!d) return fail(MOE_ERR_ARG, "moe_sample: null argument");
     if (d->n_tok < 0 || d->n_tok > MOE_SAMPLE_MAX_TOKENS)

@@ -28,7 +28,7 @@ constexpr int SMP_LIST = 2048;                        // tokens that a workgroup
 constexpr int SMP_PER = SMP_LIST / SMP_THREADS;       // of them, or of the bins, to a thread
 static_assert(SMP_BINS == SMP_LIST, "bins and tokens to a thread");
 constexpr int SLICE_WAVES = 4, SLICE_EPT = 64, SLICE = 64 * SLICE_EPT, SLICES_MAX = 256;
-constexpr int REST_PARTS = 16, REST_GRID = 256;
+constexpr int REST_GRID = 256;
 
 // 2^(j / 64), rounded to the nearest
 __constant__ double EXP_TAB[64] = {
@@ -77,7 +77,7 @@ constexpr uint32_t KEY_NONE = 0x007fffffu;            // of -inf
 // An entry of the order: key and index as the mantissa of a number in [1, 2), so that the larger comes first (the
 // lower index of equal keys) and a comparison is one of f64: four clocks where one of 64-bit integers takes
 // sixteen.  0 is none.
-static_assert(SLICES_MAX * SLICE == 1 << 20, "20 bits of index");
+static_assert(SLICES_MAX * SLICE == 1 << 20 && MAX_SAMPLE_V + 7 <= 1 << 20, "20 bits of index");
 __device__ inline uint64_t entry_from(uint32_t key) { return (0x3ffull << 52) | ((uint64_t)key << 20); }    // the key's last
 __device__ inline uint64_t entry(float v, uint32_t i) { return entry_from(sort_key(v)) | (i ^ 0xfffffu); }
 __device__ inline uint32_t entry_key(uint64_t e) { return (uint32_t)(e >> 20); }
@@ -118,6 +118,23 @@ __device__ inline Mass row_mass(const SampleArgs &a, float vmax, float temp, con
     return {(double)vmax, exp64_scale(temp), tab, 62 - (a.V > 1 ? 32 - __clz(a.V - 1) : 0)};
 }
 
+template <int CTRL, int ROWS, int BANKS, class N>
+__device__ inline N scan_step(N v) {                  // v plus the lane's that CTRL names, where it is one
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, BANKS, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, BANKS, false);
+    return v + __builtin_bit_cast(N, ((uint64_t)hi << 32) | lo);
+}
+// the sums of a wave's 64-bit values up to each lane, in a fixed order
+template <class N>
+__device__ inline N wave_scan(N v) {
+    v = scan_step<0x111, 0xf, 0xf>(v);                // row_shr 1, 2, 4, 8, then the rows' last lanes
+    v = scan_step<0x112, 0xf, 0xf>(v);
+    v = scan_step<0x114, 0xf, 0xe>(v);
+    v = scan_step<0x118, 0xf, 0xc>(v);
+    v = scan_step<0x142, 0xa, 0xf>(v);
+    return scan_step<0x143, 0xc, 0xf>(v);
+}
 // ---------------------------------------------------------------------------
 // 1: slices
 
@@ -143,45 +160,38 @@ __global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(Sampl
     const bool live = id < (int64_t)a.n_tok * a.slices;
     const int64_t tok = live ? id / a.slices : 0;
     const int slice = (int)(id - tok * a.slices);
+    // counted from the 16 bytes that the row begins in: element i is token i - m
     const raw *l = (const raw *)a.logits + tok * a.ld;
+    const int m0 = (int)((uintptr_t)l % 16 / sizeof(raw)), end = a.V + m0;
+    l -= m0;
     float v[SLICE_EPT];
     const int i0 = (slice * 64 + lane) * VEC, step = a.slices * 64 * VEC;      // vector j at i0 + j step
-    if (!live) {
+    uint4 q[NV];
+    const bool whole = live && (m0 == 0 || slice > 0) && (NV - 1) * step + (slice + 1) * 64 * VEC <= end;
+    if (whole) {                                      // every vector of the slice lies in the row
 #pragma unroll
-        for (int j = 0; j < SLICE_EPT; ++j) v[j] = -INFINITY;
-    } else if ((uintptr_t)l % 16 == 0) {
-        uint4 q[NV];
-        const bool whole = (NV - 1) * step + (slice + 1) * 64 * VEC <= a.V;    // every vector of the slice
-        if (whole) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) q[j] = *(const uint4 *)(l + i0 + j * step);
-        } else {
+        for (int j = 0; j < NV; ++j) q[j] = *(const uint4 *)(l + i0 + j * step);
+    } else {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int i = i0 + j * step;
-            if (i + VEC <= a.V) {
+            if (live && i >= m0 && i + VEC <= end) {
                 q[j] = *(const uint4 *)(l + i);
             } else {
                 raw t[VEC];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) t[e] = i + e < a.V ? l[i + e] : Elem<T>::store(-INFINITY);
+                for (int e = 0; e < VEC; ++e)
+                    t[e] = live && i + e >= m0 && i + e < end ? l[i + e] : Elem<T>::store(-INFINITY);
                 __builtin_memcpy(&q[j], t, 16);
             }
         }
-        }
+    }
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            raw t[VEC];
-            __builtin_memcpy(t, &q[j], 16);
+    for (int j = 0; j < NV; ++j) {
+        raw t[VEC];
+        __builtin_memcpy(t, &q[j], 16);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[VEC * j + e] = Elem<T>::load(t[e]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < SLICE_EPT; ++j) {
-            const int i = i0 + (j / VEC) * step + j % VEC;
-            v[j] = i < a.V ? Elem<T>::load(l[i]) : -INFINITY;
-        }
+        for (int e = 0; e < VEC; ++e) v[VEC * j + e] = Elem<T>::load(t[e]);
     }
     const SampleCuts cut = load_cuts(a, tok);
     if (threadIdx.x < 64) s_tab[threadIdx.x] = EXP_TAB[threadIdx.x];
@@ -209,7 +219,9 @@ __global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(Sampl
     int keep = greedy ? 1 : a.keep;
     for (;;) {
         uint32_t lo = low, hi = top;                  // at least keep lanes reach lo
-        if (keep > 1) {
+        if (keep > 64) {
+            lo = KEY_NONE;                            // a row short enough to keep whole
+        } else if (keep > 1) {
             for (int it = 0; it < 20 && hi > lo; ++it) {
                 const uint32_t mid = hi - (hi - lo) / 2;
                 const int c = __popcll(__ballot(mk >= mid));
@@ -234,7 +246,7 @@ __global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(Sampl
         for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
         if (greedy) {
             const int j = __clzll((long long)in);
-            uint32_t at = in ? (uint32_t)(i0 + (j / VEC) * step + j % VEC) : 0xffffffffu;
+            uint32_t at = in ? (uint32_t)(i0 + (j / VEC) * step + j % VEC - m0) : 0xffffffffu;
             for (int o = 32; o > 0; o >>= 1) at = min(at, (uint32_t)__shfl_xor(at, o, 64));
             h.at = at;
             break;
@@ -242,25 +254,31 @@ __global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(Sampl
         h.n = (uint32_t)n;
         h.bound = lo > KEY_NONE ? lo : 0;
         if (n <= a.cap) {
-            // few lanes have any: their values are read again rather than picked from 64 registers
-            uint32_t p = 0;
-            for (uint64_t b = __ballot(in != 0); b; b = __ballot(in != 0)) {
-                if (in) {
-                    const int j = __clzll((long long)in);
-                    const uint32_t i = (uint32_t)(i0 + (j / VEC) * step + j % VEC);
-                    list[p + (uint32_t)__popcll(b & ((1ull << lane) - 1))] = entry(Elem<T>::load(l[i]), i);
+            // few lanes have any: their values are read again, four at a time, rather than picked from 64
+            // registers (an unrolled pick spills)
+            uint32_t p = (uint32_t)(wave_scan((uint64_t)__popcll(in)) - __popcll(in));
+            while (__ballot(in != 0)) {
+                raw t[4];
+                uint32_t at[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int j = in ? __clzll((long long)in) : 0;
+                    at[u] = in ? (uint32_t)(i0 + (j / VEC) * step + j % VEC) : 0xffffffffu;
+                    if (in) t[u] = l[at[u]];
                     in &= ~(0x8000000000000000ull >> j);
                 }
-                p += (uint32_t)__popcll(b);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (at[u] != 0xffffffffu) list[p++] = entry(Elem<T>::load(t[u]), at[u] - (uint32_t)m0);
             }
             break;
         }
-        if (keep <= 1) {                              // more equal maxima than that
+        if (keep <= 1) {                              // more equal maxima than cap
             h.n = 0;
             h.bound = 0xffffffffu;
             break;
         }
-        keep = keep / 4;
+        keep = keep / 2;
     }
     if (lane == 0) ((SliceHead *)a.heads)[id] = h;
 }
@@ -323,23 +341,6 @@ __device__ inline void sort_list(SampleList &s, int n) {
     __syncthreads();
 }
 
-template <int CTRL, int ROWS, int BANKS, class N>
-__device__ inline N scan_step(N v) {                  // v plus the lane's that CTRL names, where it is one
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, BANKS, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, BANKS, false);
-    return v + __builtin_bit_cast(N, ((uint64_t)hi << 32) | lo);
-}
-// the sums of a wave's 64-bit values up to each lane, in a fixed order
-template <class N>
-__device__ inline N wave_scan(N v) {
-    v = scan_step<0x111, 0xf, 0xf>(v);                // row_shr 1, 2, 4, 8, then the rows' last lanes
-    v = scan_step<0x112, 0xf, 0xf>(v);
-    v = scan_step<0x114, 0xf, 0xe>(v);
-    v = scan_step<0x118, 0xf, 0xc>(v);
-    v = scan_step<0x142, 0xa, 0xf>(v);
-    return scan_step<0x143, 0xc, 0xf>(v);
-}
 // the sum of v over the threads before this one
 __device__ inline uint64_t block_before(uint64_t v, uint64_t *s_w) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -373,48 +374,53 @@ struct Row {
     __device__ float at(int i) const { return Elem<T>::load(l[i]); }
     // (What follows runs once per row on one CU: its time is that of fetching its instructions as much as of running
     // them, so the ends of a row go through a short loop of their own instead of tests beside every vector.)
-    // f(value, index) of every token that is on, of [i0, i1) (i0 a multiple of 8); f a vector's elements times in the
-    // code, or once
+    // f(value, index) of every token that is on, of [i0, i1); f a vector's elements times in the code, or once
     template <bool UNROLL, class F>
     __device__ inline void each(int i0, int i1, F f) const {
         constexpr int VEC = 16 / sizeof(raw);
-        int done = i0;
-        if ((uintptr_t)l % 16 == 0) {
-            done = max(i0, i1 / VEC * VEC);
-            int i = i0 + (int)threadIdx.x * VEC;
-            uint4 next = {};
-            if (i < done) next = *(const uint4 *)(l + i);
+        int head, tail;
+        vectors(i0, i1, head, tail);
+        int i = head + (int)threadIdx.x * VEC;
+        uint4 next = {};
+        if (i < tail) next = *(const uint4 *)(l + i);
 #pragma unroll 1
-            for (; i < done; i += SMP_THREADS * VEC) {
-                uint4 q = next;                       // the next vector is on its way meanwhile
-                if (i + SMP_THREADS * VEC < done) next = *(const uint4 *)(l + i + SMP_THREADS * VEC);
-                if constexpr (UNROLL) {
-                    raw t[VEC];
-                    __builtin_memcpy(t, &q, 16);
+        for (; i < tail; i += SMP_THREADS * VEC) {
+            uint4 q = next;                           // the next vector is on its way meanwhile
+            if (i + SMP_THREADS * VEC < tail) next = *(const uint4 *)(l + i + SMP_THREADS * VEC);
+            if constexpr (UNROLL) {
+                raw t[VEC];
+                __builtin_memcpy(t, &q, 16);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float v = Elem<T>::load(t[e]);
-                        if (v > -INFINITY) f(v, i + e);
-                    }
-                } else {
+                for (int e = 0; e < VEC; ++e) {
+                    const float v = Elem<T>::load(t[e]);
+                    if (v > -INFINITY) f(v, i + e);
+                }
+            } else {
 #pragma unroll 1
-                    for (int e = 0; e < VEC; ++e) {
-                        const float v = T == T_F32 ? __uint_as_float(q.x) : Elem<T>::load((raw)q.x);
-                        constexpr int B = 8 * sizeof(raw) % 32;   // the vector moves down by one element
-                        q.x = B ? __builtin_amdgcn_alignbit(q.y, q.x, B) : q.y;
-                        q.y = B ? __builtin_amdgcn_alignbit(q.z, q.y, B) : q.z;
-                        q.z = B ? __builtin_amdgcn_alignbit(q.w, q.z, B) : q.w;
-                        q.w = q.w >> B;
-                        if (v > -INFINITY) f(v, i + e);
-                    }
+                for (int e = 0; e < VEC; ++e) {
+                    const float v = T == T_F32 ? __uint_as_float(q.x) : Elem<T>::load((raw)q.x);
+                    constexpr int B = 8 * sizeof(raw) % 32;       // the vector moves down by one element
+                    q.x = B ? __builtin_amdgcn_alignbit(q.y, q.x, B) : q.y;
+                    q.y = B ? __builtin_amdgcn_alignbit(q.z, q.y, B) : q.z;
+                    q.z = B ? __builtin_amdgcn_alignbit(q.w, q.z, B) : q.w;
+                    q.w = q.w >> B;
+                    if (v > -INFINITY) f(v, i + e);
                 }
             }
         }
 #pragma unroll 1
-        for (int i = done + (int)threadIdx.x; i < i1; i += SMP_THREADS) {
-            const float v = at(i);
-            if (v > -INFINITY) f(v, i);
+        for (int k = threadIdx.x; k < head - i0 + i1 - tail; k += SMP_THREADS) {
+            const int j = k < head - i0 ? i0 + k : tail + k - (head - i0);
+            const float v = at(j);
+            if (v > -INFINITY) f(v, j);
         }
+    }
+    // [head, tail): the part of [i0, i1) in whole vectors on 16 bytes
+    __device__ inline void vectors(int i0, int i1, int &head, int &tail) const {
+        constexpr int VEC = 16 / sizeof(raw);
+        const int m = (int)((uintptr_t)(l + i0) % 16 / sizeof(raw));
+        head = min(i1, i0 + (m ? VEC - m : 0));
+        tail = head + (i1 - head) / VEC * VEC;
     }
     template <class F>
     __device__ inline void each(F f) const { each<false>(0, V, f); }
@@ -430,21 +436,22 @@ struct Row {
         if (threadIdx.x == 0) list.n = list.hits = 0;
         __syncthreads();
         const bool same = (__float_as_uint(from) ^ __float_as_uint(to)) >> 31 == 0;
-        if ((uintptr_t)l % 16 != 0 || !same) {
+        if (!same) {
             each(take);
             return;
         }
         const bool neg = __float_as_uint(from) >> 31;
         const auto x = bits_of(neg ? to : from), y = bits_of(neg ? from : to);  // x <= y as unsigned
-        const int whole = V / VEC * VEC;
-        for (int base = 0; base < whole; base += NV * STEP) {
+        int head, tail;
+        vectors(0, V, head, tail);
+        for (int base = head; base < tail; base += NV * STEP) {
             const int i0 = base + (int)threadIdx.x * VEC;
             uint4 q[NV];
 #pragma unroll
-            for (int k = 0; k < NV; ++k) q[k] = *(const uint4 *)(l + min(i0 + k * STEP, whole - VEC));
+            for (int k = 0; k < NV; ++k) q[k] = *(const uint4 *)(l + min(i0 + k * STEP, tail - VEC));
             uint32_t in = 0;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) in = 2 * in + (near(q[k], x, y - x) && i0 + k * STEP < whole);
+            for (int k = 0; k < NV; ++k) in = 2 * in + (near(q[k], x, y - x) && i0 + k * STEP < tail);
             for (; in; in &= in - 1) hit[atomicAdd(&list.hits, 1u)] = (uint32_t)(i0 + (NV - __ffs(in)) * STEP);
         }
         __syncthreads();
@@ -456,7 +463,10 @@ struct Row {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) take(Elem<T>::load(t[e]), i + e);
         }
-        for (int i = whole + (int)threadIdx.x; i < V; i += SMP_THREADS) take(at(i), i);
+        for (int k = threadIdx.x; k < head + V - tail; k += SMP_THREADS) {
+            const int j = k < head ? k : tail + k - head;
+            take(at(j), j);
+        }
     }
 
 private:
@@ -761,19 +771,19 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
     __shared__ SampleShared s;
     __shared__ double s_tab[64];
     const int tid = threadIdx.x;
-    const uint32_t n = *a.n_rest;
-    if (blockIdx.x >= n * REST_PARTS) return;
+    const uint32_t n = *a.n_rest, parts = (uint32_t)a.parts;
+    if (blockIdx.x >= n * parts) return;
     if (tid < 64) s_tab[tid] = EXP_TAB[tid];
-    for (uint32_t task = blockIdx.x; task < n * REST_PARTS; task += gridDim.x) {
-        RestRow &r = ((RestRow *)a.rest)[task / REST_PARTS];
-        const int part = (int)(task % REST_PARTS);
+    for (uint32_t task = blockIdx.x; task < n * parts; task += gridDim.x) {
+        RestRow &r = ((RestRow *)a.rest)[task / parts];
+        const int part = (int)(task % parts);
         const int64_t tok = r.tok;
         const float vmax = r.vmax;
         const SampleCuts cut = load_cuts(a, tok);
         const Row<T> row{(const typename Elem<T>::raw *)a.logits + tok * a.ld, a.V};
         const Mass ms = row_mass(a, vmax, cut.temp, s_tab);
         const float per = bins_per(cut.temp);
-        const int run = ((a.V + REST_PARTS - 1) / REST_PARTS + 7) / 8 * 8;
+        const int run = ((a.V + a.parts - 1) / a.parts + 7) / 8 * 8;
         __syncthreads();
         for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { s.cnt[i] = 0; s.mass[i] = 0; }
         __syncthreads();
@@ -792,7 +802,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
         __threadfence();
         __syncthreads();
         if (tid == 0)
-            s.last = __hip_atomic_fetch_add(&r.parts, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == REST_PARTS - 1;
+            s.last = __hip_atomic_fetch_add(&r.parts, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
         __syncthreads();
         if (!s.last) continue;
         __threadfence();
@@ -812,11 +822,14 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
 // ---------------------------------------------------------------------------
 // 2: one workgroup per row
 
-constexpr int PICK_WAVES = 4, PICK_THREADS = 64 * PICK_WAVES, PICK_PER = 8, PICK_MAX = 64 * PICK_PER;
+constexpr int PICK_WAVES = 4, PICK_THREADS = 64 * PICK_WAVES;
+// PER: candidates a lane holds
+template <int PER>
 struct PickLds {
+    static constexpr int MAX = 64 * PER;
     uint64_t list[SMP_LIST];                          // candidates, in no order
-    uint64_t order[PICK_MAX];                         // the front of the order
-    double cum[PICK_MAX];                             // and its running masses
+    uint64_t order[MAX];                         // the front of the order
+    double cum[MAX];                             // and its running masses
     double tab[64];
     uint32_t n, rest;
 };
@@ -827,11 +840,13 @@ __device__ inline uint64_t lane_u64(uint64_t v, int l) {
 }
 __device__ inline void wave_lds() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }    // a wave's LDS accesses stay in order
 
-// All four waves read the candidates; the first one decides, without a barrier: up to 512 candidates in
+// All four waves read the candidates; the first one decides, without a barrier: up to 512 (or 1,024) candidates in
 // its registers, of which it sorts the next up to 64 at a time (bounded by a bisection) until
 // the cuts and the draw fall within what is sorted.  Returns whether they did.
+template <int PICK_PER>
 __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCuts &cut, const Mass &ms, uint32_t bound,
-                                double mass, PickLds &s) {
+                                double mass, PickLds<PICK_PER> &s) {
+    constexpr int PICK_MAX = PickLds<PICK_PER>::MAX;
     const int lane = threadIdx.x & 63;
     const bool by_k = cut.top_k > 0 && cut.top_k < a.V;
     int n = (int)s.n;
@@ -841,8 +856,8 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
     if (n <= PICK_MAX) {
 #pragma unroll
         for (int j = 0; j < PICK_PER; ++j) x[j] = 64 * j + lane < n ? s.list[64 * j + lane] : 0;
-    } else {                                          // the largest 512 of them
-        uint64_t lo = entry_from(0), hi = entry_from(sort_key((float)ms.vmax) + 1);    // more than 512 reach lo, at most hi
+    } else {                                          // the largest of them that fit
+        uint64_t lo = entry_from(0), hi = entry_from(sort_key((float)ms.vmax) + 1);    // more than fit reach lo, at most hi
         while (hi - lo > 1) {
             const uint64_t mid = lo + (hi - lo) / 2;
             int c = 0;
@@ -991,9 +1006,9 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
     return true;
 }
 
-template <int T>
+template <int PER>
 __global__ __launch_bounds__(PICK_THREADS) void sample_pick_kernel(SampleArgs a) {
-    __shared__ PickLds s;
+    __shared__ PickLds<PER> s;
     const int64_t tok = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63;
     const SliceHead *heads = (const SliceHead *)a.heads + tok * a.slices;
@@ -1093,16 +1108,17 @@ __global__ __launch_bounds__(PICK_THREADS) void sample_pick_kernel(SampleArgs a)
 // ---------------------------------------------------------------------------
 // slices of a row, candidates that a slice has room for, and lanes above its bound
 struct SamplePlan {
-    int slices, cap_log, keep;
+    int slices, cap_log, keep, parts;
 };
 static SamplePlan sample_plan(int V) {
     SamplePlan p;
-    p.slices = (V + SLICE - 1) / SLICE;
+    p.slices = (V + 7 + SLICE - 1) / SLICE;           // (7: a row may begin inside 16 bytes)
     const int want = p.slices >= 64 ? 8 : p.slices >= 25 ? 16 : 400 / p.slices;
     // of 64 maxima over runs of random values, those above the value that `want` of all exceed
-    p.keep = (int)ceil(64.0 * (1.0 - exp(-want / 64.0)));
+    p.keep = V <= 1000 ? 65 : (int)ceil(64.0 * (1.0 - exp(-want / 64.0)));
+    p.parts = V < 16384 ? 1 : V >= 131072 ? 16 : V / 8192;       // workgroups to an undecided row
     p.cap_log = 4;
-    while ((1 << p.cap_log) < want + want / 4) ++p.cap_log;
+    while ((1 << p.cap_log) < want + want / 2 + 8) ++p.cap_log;
     return p;
 }
 
@@ -1127,8 +1143,10 @@ static hipError_t launch_sample_t(const SampleArgs &a, hipStream_t st) {
     const int64_t waves = (int64_t)a.n_tok * a.slices;
     hipLaunchKernelGGL(sample_slice_kernel<T>, dim3((unsigned)((waves + SLICE_WAVES - 1) / SLICE_WAVES)),
                        dim3(64 * SLICE_WAVES), 0, st, a);
-    hipLaunchKernelGGL(sample_pick_kernel<T>, dim3((unsigned)a.n_tok), dim3(PICK_THREADS), 0, st, a);
-    hipLaunchKernelGGL(sample_rest_kernel<T>, dim3((unsigned)min((int64_t)REST_GRID, (int64_t)a.n_tok * REST_PARTS)), dim3(SMP_THREADS), 0, st, a);
+    // short rows have all or most of theirs in one or two lists
+    if (a.slices <= 2) hipLaunchKernelGGL(sample_pick_kernel<16>, dim3((unsigned)a.n_tok), dim3(PICK_THREADS), 0, st, a);
+    else hipLaunchKernelGGL(sample_pick_kernel<8>, dim3((unsigned)a.n_tok), dim3(PICK_THREADS), 0, st, a);
+    hipLaunchKernelGGL(sample_rest_kernel<T>, dim3((unsigned)min((int64_t)REST_GRID, (int64_t)a.n_tok * a.parts)), dim3(SMP_THREADS), 0, st, a);
     return hipGetLastError();
 }
 
@@ -1139,6 +1157,7 @@ hipError_t launch_sample(SampleArgs a, void *ws, hipStream_t st) {
     a.cap_log = p.cap_log;
     a.cap = 1 << p.cap_log;
     a.keep = p.keep;
+    a.parts = p.parts;
     a.lists = (uint8_t *)ws + w.lists;
     a.heads = (uint8_t *)ws + w.heads;
     a.rest = (uint8_t *)ws + w.rest;

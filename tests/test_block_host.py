@@ -69,7 +69,7 @@ def sample(**kw):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(n_tok=-1), dict(n_tok=65536), dict(V=0), dict(V=(1 << 20) + 1), dict(logits_type=-1), dict(logits=None), dict(u=None),
+    dict(n_tok=-1), dict(n_tok=65536), dict(V=0), dict(V=1000001), dict(logits_type=-1), dict(logits=None), dict(u=None),
     dict(tokens=None), dict(logits_stride=99), dict(logits=PTR + 2), dict(logits_type=2, logits=PTR + 1),
     dict(u=PTR + 1), dict(temperature=PTR + 2), dict(top_k=PTR + 2), dict(top_p=PTR + 2), dict(min_p=PTR + 2),
     dict(tokens=PTR + 2), dict(probs=PTR + 2), dict(workspace=None), dict(workspace=PTR + 4)])
