@@ -792,8 +792,9 @@ int moe_block_norm(const moe_block_norm_desc *d, void *stream);
  * them cuts nothing; the first of the order always stays.  Logits of -inf and NaN
  * are switched off; a row with nothing else gives token -1 and prob 0.  (Logits of
  * +inf share a row's whole mass.)  u of 1 and above counts as the largest number
- * below 1, u below 0 and NaN as 0.  Masses and their sums are computed in 64 bits, in an order that the row
- * alone decides: the same row gives the same token in any batch. */
+ * below 1, u below 0 and NaN as 0.  Masses and their sums are computed in 64 bits, in an order that depends on
+ * the row and where in 16 bytes it begins only: the same row gives the same token in any
+ * batch. */
 #define MOE_SAMPLE_MAX_V 1000000
 #define MOE_SAMPLE_MAX_TOKENS 65535
 typedef struct {

@@ -114,8 +114,8 @@ struct Mass {
     }
     __device__ uint64_t fixed(uint32_t key) const { return (uint64_t)(ldexp(e(key), shift) + 0.5); }
 };
-__device__ inline Mass row_mass(const SampleArgs &a, float vmax, float temp, const double *tab) {
-    return {(double)vmax, exp64_scale(temp), tab, 62 - (a.V > 1 ? 32 - __clz(a.V - 1) : 0)};
+__device__ inline Mass row_mass(float vmax, float temp, const double *tab, int shift) {
+    return {(double)vmax, exp64_scale(temp), tab, shift};
 }
 
 template <int CTRL, int ROWS, int BANKS, class N>
@@ -292,7 +292,7 @@ struct SampleList {
 };
 // sorted[0 .. n) = raw[0 .. n) in descending order (the entries differ).  Up to 1,024 entries by each one's rank, four
 // lanes counting for four entries (348 of them: 2 us against 9 of the network, whose every step waits for LDS); more by a
-// bitonic network, whose strides below 64 stay within a wave's 128 entries and need no barrier.
+// bitonic network, whose strides of 64 and below stay within a wave's 128 entries and need no barrier.
 __device__ inline void sort_list(SampleList &s, int n) {
     const int tid = threadIdx.x;
     __syncthreads();
@@ -322,7 +322,7 @@ __device__ inline void sort_list(SampleList &s, int n) {
         __syncthreads();
         return;
     }
-    const int m = 1 << (32 - __clz(n - 1));           // 512, 1024 or 2048
+    constexpr int m = SMP_LIST;
     for (int i = tid; i < m; i += SMP_THREADS) s.sorted[i] = i < n ? s.raw[i] : 0;
     __syncthreads();
     for (int k = 2; k <= m; k <<= 1)
@@ -440,8 +440,13 @@ struct Row {
             each(take);
             return;
         }
+        // the type's own values next to the ends, inside: a vector listed holds a token of the bin, so that the list,
+        // the bin's 2,048 at most, has room for the vectors
         const bool neg = __float_as_uint(from) >> 31;
-        const auto x = bits_of(neg ? to : from), y = bits_of(neg ? from : to);  // x <= y as unsigned
+        auto a = bits_of(from), b = bits_of(to);
+        if (Elem<T>::load(raw_of(a)) < from) a += neg ? -1 : 1;
+        if (Elem<T>::load(raw_of(b)) > to) b += neg ? 1 : -1;
+        const uint32_t x = neg ? b : a, y = neg ? a : b;              // x <= y as unsigned
         int head, tail;
         vectors(0, V, head, tail);
         for (int base = head; base < tail; base += NV * STEP) {
@@ -472,7 +477,11 @@ struct Row {
 private:
     static __device__ inline auto bits_of(float v) {
         if constexpr (T == T_F32) return __float_as_uint(v);
-        else return Elem<T>::store(v);
+        else return (uint32_t)Elem<T>::store(v);
+    }
+    static __device__ inline raw raw_of(uint32_t b) {
+        if constexpr (T == T_F32) return __uint_as_float(b);
+        else return (raw)b;
     }
     // whether one of the vector's elements e has e - x <= d as unsigned
     static __device__ inline bool near(uint4 q, uint32_t x, uint32_t d) {
@@ -640,7 +649,7 @@ struct BinSearch {
     // a bin's highest value
     __device__ float top_of(int b) const {
         const uint32_t kmax = sort_key(vmax);
-        return b == 0 ? vmax : key_value(lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return bin_of(key_value(k), vmax, per) < b; }) - 1);
+        return b == 0 ? vmax + 0.0f : key_value(lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return bin_of(key_value(k), vmax, per) < b; }) - 1);
     }
     __device__ Cut find(bool by_mass, uint64_t target) const {
         __syncthreads();
@@ -761,6 +770,7 @@ struct RestRow {
     uint32_t cnt[SMP_BINS];
     int64_t tok;
     float vmax;
+    int shift;                                        // Mass::shift
     uint32_t parts;                                   // finished
 };
 
@@ -781,7 +791,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
         const float vmax = r.vmax;
         const SampleCuts cut = load_cuts(a, tok);
         const Row<T> row{(const typename Elem<T>::raw *)a.logits + tok * a.ld, a.V};
-        const Mass ms = row_mass(a, vmax, cut.temp, s_tab);
+        const Mass ms = row_mass(vmax, cut.temp, s_tab, r.shift);
         const float per = bins_per(cut.temp);
         const int run = ((a.V + a.parts - 1) / a.parts + 7) / 8 * 8;
         __syncthreads();
@@ -828,9 +838,10 @@ template <int PER>
 struct PickLds {
     static constexpr int MAX = 64 * PER;
     uint64_t list[SMP_LIST];                          // candidates, in no order
-    uint64_t order[MAX];                         // the front of the order
-    double cum[MAX];                             // and its running masses
+    uint64_t order[MAX];                              // the front of the order
+    double cum[MAX];                                  // and its running masses
     double tab[64];
+    double mass, part[PICK_WAVES];
     uint32_t n, rest;
 };
 
@@ -1061,7 +1072,7 @@ __global__ __launch_bounds__(PICK_THREADS) void sample_pick_kernel(SampleArgs a)
         }
         return;
     }
-    const Mass ms = row_mass(a, vmax, cut.temp, s.tab);
+    const Mass ms = row_mass(vmax, cut.temp, s.tab, 0);
     __syncthreads();
     auto take = [&](bool in, uint64_t e) {            // one place in the list for a wave's at a time
         const uint64_t b = __ballot(in);
@@ -1092,13 +1103,36 @@ __global__ __launch_bounds__(PICK_THREADS) void sample_pick_kernel(SampleArgs a)
             for (int o = 1; o < 64; o <<= 1) mass += __shfl_xor(mass, o, 64);
         }
         const bool done = pick_row(a, tok, cut, ms, bound, mass, s);
-        if (lane == 0) s.rest = done ? 0xffffffffu : atomicAdd(a.n_rest, 1u);
+        if (lane == 0) {
+            s.rest = done ? 0xffffffffu : atomicAdd(a.n_rest, 1u);
+            s.mass = mass;
+        }
     }
     __syncthreads();
     if (s.rest == 0xffffffffu) return;
     RestRow &r = ((RestRow *)a.rest)[s.rest];         // undecided: step 3
     for (int i = tid; i < SMP_BINS; i += PICK_THREADS) { r.cnt[i] = 0; r.mass[i] = 0; }
+    // Its masses are integers with as many fractional bits as the row's whole mass leaves of 62: a token far below the
+    // first has its share to 2^-62 of the whole.  Under a top-k that mass is not known, but the candidates' and as much as the
+    // bound's for every token are no less.
+    double whole = s.mass;
+    if (cut.top_k > 0 && cut.top_k < a.V) {
+        double t = 0.0;
+        for (int p = tid; p < places; p += PICK_THREADS) {
+            const uint64_t e = lists[p];
+            if (((uint32_t)p & in_list) < heads[p >> a.cap_log].n && entry_key(e) >= bound) t += ms.e(entry_key(e));
+        }
+        for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
+        if (lane == 0) s.part[tid >> 6] = t;
+        __syncthreads();
+        whole = bound ? (double)a.V * ms.e(min(bound, sort_key(vmax))) : 0.0;
+        for (int w = 0; w < PICK_WAVES; ++w) whole += s.part[w];
+    }
+    if (vmax == INFINITY) whole = a.V;                // every one of them counts 1
     if (tid == 0) {
+        int ex;
+        frexp(whole * (1.0 + 1e-9), &ex);
+        r.shift = 62 - ex;
         r.tok = tok;
         r.vmax = vmax;
         r.parts = 0;
@@ -1125,8 +1159,10 @@ static SamplePlan sample_plan(int V) {
 struct SampleWs {
     size_t lists, heads, rest, n_rest, total;
 };
+constexpr int SMP_ROWS = 4096;                        // of a launch: bounds the workspace
 static SampleWs sample_ws(int n_tok, int V) {
     const SamplePlan p = sample_plan(V);
+    if (n_tok > SMP_ROWS) n_tok = SMP_ROWS;
     SampleWs w;
     size_t o = 0;
     w.lists = o; o += (size_t)n_tok * p.slices << (p.cap_log + 3);
@@ -1162,8 +1198,22 @@ hipError_t launch_sample(SampleArgs a, void *ws, hipStream_t st) {
     a.heads = (uint8_t *)ws + w.heads;
     a.rest = (uint8_t *)ws + w.rest;
     a.n_rest = (uint32_t *)((uint8_t *)ws + w.n_rest);
-    return a.type == T_F32 ? launch_sample_t<T_F32>(a, st)
-         : a.type == T_BF16 ? launch_sample_t<T_BF16>(a, st) : launch_sample_t<T_F16>(a, st);
+    const int all = a.n_tok;
+    for (int t = 0; t < all; t += SMP_ROWS) {         // one after the other in the same workspace
+        a.n_tok = all - t < SMP_ROWS ? all - t : SMP_ROWS;
+        const hipError_t e = a.type == T_F32 ? launch_sample_t<T_F32>(a, st)
+                           : a.type == T_BF16 ? launch_sample_t<T_BF16>(a, st) : launch_sample_t<T_F16>(a, st);
+        if (e != hipSuccess) return e;
+        a.logits = (const uint8_t *)a.logits + (int64_t)SMP_ROWS * a.ld * (a.type == T_F32 ? 4 : 2);
+        a.u += SMP_ROWS;
+        a.tokens += SMP_ROWS;
+        if (a.probs) a.probs += SMP_ROWS;
+        if (a.temp) a.temp += SMP_ROWS;
+        if (a.top_k) a.top_k += SMP_ROWS;
+        if (a.top_p) a.top_p += SMP_ROWS;
+        if (a.min_p) a.min_p += SMP_ROWS;
+    }
+    return hipSuccess;
 }
 
 }  // namespace mp

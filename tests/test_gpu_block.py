@@ -404,6 +404,38 @@ def test_sample_strides_and_rows_left_alone():
             assert (tokens[T:] == -5).all() and (probs[T:] == 9.0).all()
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_sample_of_a_long_tail(dt, sign):
+    # the draw falls among tokens far below the first (the last, open bin of the undecided rows' histogram) beside many
+    # that are switched off; and among equal 16-bit logits next to the bin that is gathered
+    V, g = 100000, gen(60)
+    l = torch.full((6, V), -INF, device=DEV)
+    top = 30.0 if sign > 0 else -1.0
+    for t in range(3):
+        at = torch.randperm(V, generator=g, device=DEV)[:1500]
+        l[t, at] = top - 23.5 - 0.2 * torch.rand(1500, generator=g, device=DEV)
+        l[t, at[0]] = top
+    for t in range(3, 6):                             # thousands of equal logits, the cut among their neighbours
+        l[t] = top - 3.0 - torch.randint(0, 400, (V,), generator=g, device=DEV) / 100.0
+    l = l.to(DT[dt])
+    for s in (1.0 - 2.0 ** -24, 1.0 - 2.0 ** -23, 0.999, 0.5):
+        u = torch.full((6,), s, device=DEV)
+        for cut in (dict(), dict(top_p=0.9), dict(top_k=1400), dict(min_p=1e-12), dict(top_p=0.99999988, min_p=1e-11)):
+            check_sample(l, u, Sampler(V)(l, u, **cut), **cut)
+
+
+def test_sample_more_rows_than_a_launch():
+    V, T = 300, 4096 + 77
+    g = gen(61)
+    logits = 3.0 * randn(g, T, V + 5)[:, 2:V + 2]
+    u = torch.rand(T, generator=g, device=DEV)
+    kw = dict(temperature=0.5 + torch.rand(T, generator=g, device=DEV),
+              top_k=torch.randint(0, 60, (T,), generator=g, device=DEV, dtype=torch.int32),
+              top_p=0.3 + torch.rand(T, generator=g, device=DEV), min_p=0.01 * torch.rand(T, generator=g, device=DEV))
+    check_sample(logits, u, Sampler(V)(logits, u, **kw), **kw)
+
+
 def test_sample_largest_vocabulary():
     V = 1000000
     logits = randn(gen(28), 2, V)
