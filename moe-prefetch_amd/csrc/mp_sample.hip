@@ -974,15 +974,20 @@ __device__ inline bool pick_row(const SampleArgs &a, int64_t tok, const SampleCu
     const bool sure = !by_k || !open;                 // the mass that top-p takes its share of is known
     double total = mass;
     if (have < n) {
-        double all = 0.0;                             // of the candidates
+        // the mass of the candidates, which lie in no certain order: a sum of integers, the 53 bits of e below 1 and the
+        // 53 after them (1,024 of at most 2^53)
+        uint64_t hi = 0, lo = 0;
         bool low_one = false;
 #pragma unroll
         for (int j = 0; j < PICK_PER; ++j) {
-            const double e = x[j] ? ms.e(entry_key(x[j])) : 0.0;
-            all += e;
+            const double e = x[j] ? ms.e(entry_key(x[j])) : 0.0, h = e * 0x1p53, f = floor(h);
+            hi += (uint64_t)f;
+            lo += (uint64_t)((h - f) * 0x1p53);
             low_one |= x[j] && !(e >= (double)cut.min_p);
         }
-        for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o, 64);
+        hi = lane_u64(wave_scan(hi), 63);
+        lo = lane_u64(wave_scan(lo), 63);
+        const double all = (double)hi * 0x1p-53 + (double)lo * 0x1p-106;
         const bool any_low = with_min && __ballot(low_one);
         if (!open) total = all;
         if (open) {                                   // all candidates together may not reach far enough

@@ -290,11 +290,24 @@ def lib():
 
 
 def packed(struct):
-    """(pack, place): pack(*values) gives the bytes of a descriptor, its fields in order; place maps their names."""
+    """(pack, place): pack(*values) gives the bytes of a descriptor, its fields in order (an integer that its field cannot
+    hold is an error); place maps their names."""
     code = {P: "P", I32: "i", I64: "q", U64: "Q", F32: "f"}
     fmt = "@" + "".join(code[t] for _, t in struct._fields_) + "0P"
     assert _struct.calcsize(fmt) == ctypes.sizeof(struct)
-    return _struct.Struct(fmt).pack, {n: i for i, (n, _) in enumerate(struct._fields_)}
+    raw, names = _struct.Struct(fmt).pack, [n for n, _ in struct._fields_]
+
+    def pack(*values):
+        try:
+            return raw(*values)
+        except _struct.error:
+            for name, (_, t), v in zip(names, struct._fields_, values):
+                try:
+                    _struct.pack(code[t], v)
+                except _struct.error:
+                    raise ValueError(f"{struct.__name__}.{name} cannot be {v!r}") from None
+            raise
+    return pack, {n: i for i, n in enumerate(names)}
 
 
 def entry(name):

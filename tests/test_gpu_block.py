@@ -287,15 +287,14 @@ def test_norm_of_zeros_large_values_and_nan():
 def check_sample(logits, u, got, **kw):
     tokens, probs = R.sample(np64(logits), np64(u), **{k: np64(v) if torch.is_tensor(v) else v for k, v in kw.items()})
     np.testing.assert_array_equal(got[0].cpu().numpy(), tokens)
-    # a mass is off by at most half of its last bit, 2^-(63 - ceil(log2 V)), so V of them by V^2 2^-62 beside a total of
-    # at least 1
+    # a mass is off by at most 2^-(63 - ceil(log2 V)), so V of them by V^2 2^-62 beside a total of at least 1
     V = logits.shape[1]
     np.testing.assert_allclose(np64(got[1]), probs, rtol=R.U * 1.000001 + V * V * 2.0 ** -62, atol=2.0 ** -149)
 
 
 CUTS = [dict(), dict(temperature=0.7), dict(top_k=1), dict(top_k=40, temperature=0.8), dict(top_p=0.9),
         dict(min_p=0.05), dict(top_k=50, top_p=0.95, min_p=0.02, temperature=1.1), dict(top_k=1500, top_p=0.999),
-        dict(temperature=3.0, top_p=0.97), dict(temperature=0.0), dict(top_k=5, min_p=0.9)]
+        dict(temperature=3.0, top_p=0.97), dict(temperature=0.0), dict(top_k=5, min_p=0.9), dict(temperature=1e38)]
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
@@ -425,6 +424,43 @@ def test_sample_of_a_long_tail(dt, sign):
             check_sample(l, u, Sampler(V)(l, u, **cut), **cut)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V", [999, 1001, 4088, 4089, 4095, 8184, 8185, 98295, 102400])
+def test_sample_sizes_next_to_the_slices(dt, V):
+    # rows at every alignment of their type, the likely tokens in one run of neighbours or at both ends
+    size = 4 if dt == "f32" else 2
+    for m in range(16 // size):
+        g = gen(70 + m)
+        wide = torch.full((4, V + 16), 50.0, device=DEV).to(DT[dt])
+        rows = wide[:, m:m + V] if (V + 16) * size % 16 == 0 else wide.flatten()[m:m + 4 * V].view(4, V)
+        l = randn(g, 4, V)
+        l[0, V // 3:V // 3 + 700] += 9.0
+        l[1, :8] += 9.0
+        l[1, -8:] += 9.0
+        l[2] *= 0.01
+        l[3] -= 40.0
+        rows.copy_(l)
+        u = torch.rand(4, generator=g, device=DEV)
+        for cut in (dict(), dict(top_k=300), dict(top_p=0.95, temperature=1.5), dict(min_p=0.3), dict(top_k=9, top_p=0.5)):
+            check_sample(rows, u, Sampler(V)(rows, u, **cut), **cut)
+
+
+def test_sample_the_same_bits_each_time():
+    # whatever order workgroups and waves take their turns in
+    V, T, g = 30011, 200, gen(62)
+    logits = (0.3 + 2.0 * torch.rand(T, 1, generator=g, device=DEV)) * randn(g, T, V)
+    u = torch.rand(T, generator=g, device=DEV)
+    for cut in (dict(), dict(top_k=300), dict(top_k=1000, top_p=0.7), dict(top_k=20000, min_p=0.01), dict(top_p=0.9)):
+        want = Sampler(V)(logits, u, **cut)
+        for _ in range(20):
+            got = Sampler(V)(logits, u, **cut)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        for t in (0, 77, 199):
+            one = Sampler(V)(logits[t:t + 1].clone(), u[t:t + 1], **cut)
+            if logits[t].data_ptr() % 16 == 0:
+                assert one[0][0] == want[0][t] and one[1][0] == want[1][t]
+
+
 def test_sample_more_rows_than_a_launch():
     V, T = 300, 4096 + 77
     g = gen(61)
@@ -483,7 +519,8 @@ def test_python_refusals():
                 lambda: n(x, residual=x.half()), lambda: n(x, out=x[:2]), lambda: n(x, out_dtype=torch.float64),
                 lambda: n(x, out=x, out_dtype=torch.float16), lambda: n(x.cpu()),
                 lambda: s(x, u[:3]), lambda: s(x, u.double()), lambda: s(x, u, top_k=u), lambda: s(x, u, top_p=u[:2]),
-                lambda: s(x, u, temperature=u.cpu()), lambda: s(x, u, tokens=u), lambda: s(x[:, ::2], u)):
+                lambda: s(x, u, top_k=1 << 40), lambda: s(x, u, min_p="0"),
+                lambda: r(x, dummy=1 << 31), lambda: s(x, u, temperature=u.cpu()), lambda: s(x, u, tokens=u), lambda: s(x[:, ::2], u)):
         with pytest.raises((ValueError, _lib.MoeError)):
             bad()
     with pytest.raises(_lib.MoeError, match="branch"):
@@ -605,7 +642,7 @@ def test_streams_and_two_calls_at_once():
     want = run()
     torch.cuda.synchronize()
     a, b = torch.cuda.Stream(), torch.cuda.Stream()
-    outs = [run(stream=a), run(stream=b.cuda_stream), run(stream=a), run(stream=b)]
+    outs = [run(stream=a), run(stream=b.cuda_stream), run(stream=a), run(stream=b), run(stream=0)]
     torch.cuda.synchronize()
     for o in outs:
         assert all(torch.equal(p, q) for p, q in zip(o, want))
@@ -632,3 +669,31 @@ def test_graph_replays():
         want = run()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(outs, want)), i
+
+
+def test_two_graphs_of_the_same_objects():
+    g = gen(34)
+    logits, x, voc = randn(g, 9, 128), randn(g, 9, 2048), randn(g, 9, 32003)
+    u = torch.rand(9, generator=g, device=DEV)
+    router, norm, sampler = ScoredRouter(128, 8), BlockNorm(2048), Sampler(32003)
+    runs = [lambda: (*router(logits), *norm(x, x), *sampler(voc, u, top_p=0.95)),
+            lambda: (*router(logits[:5]), *norm(x[:5]), *sampler(voc[:5], u[:5], top_k=500))]
+    graphs, outs = [], []
+    for r in runs:
+        r()
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(r())
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for i in range(4):
+        logits.copy_(randn(g, 9, 128))
+        voc.copy_(randn(g, 9, 32003))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            graphs[0].replay()
+        with torch.cuda.stream(b):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for r, o in zip(runs, outs):
+            assert all(torch.equal(p, q) for p, q in zip(o, r())), i
