@@ -690,7 +690,7 @@ int moe_decode_batch(moe_cache *c, const float *x, const float *bias, float *out
  * graphs are fine as long as their outputs, and moe_sample's workspaces, are apart.
  * Their pointers are of the current device.  Rows may lie apart: a row stride
  * counts elements and is at least the row's length.  No alignment is asked for
- * beyond the element's own; rows of 16-byte aligned vectors run faster. */
+ * beyond the element's own. */
 
 /* The K experts of each token from its router logits:
  *   s_e = sigmoid(l_e)  or  exp(l_e - max) / sum exp(l - max)

@@ -79,7 +79,7 @@ struct ScoredArgs {
     float *w;
     int32_t *slots;
     float *scores;
-    int vec, group_lanes;       // set by the launcher: rows and bias in whole vectors; lanes of a group, or 0
+    int vec, group_lanes;       // set by the launcher: whether rows are whole vectors; lanes of a group, or 0
 };
 hipError_t launch_route_scored(const ScoredArgs &a, hipStream_t st);
 

@@ -3,11 +3,18 @@
 // residual scale and add, and the norm before the next block, in one launch.
 //
 // Every element is read once and stays in registers between the sums over its
-// row: a workgroup has a row, a thread four neighbouring elements of it (up to
-// four times), so that all of a row's loads are on their way at once, those of
-// the weights and the gate too.  Sums are f32: four to sixteen terms a thread, a
-// wave's by DPP, the waves' through LDS, one barrier each.
+// row: a workgroup has a row, a thread N neighbouring elements of it (up to four
+// times), so that all of a row's loads are on their way at once, those of the
+// weights and the gate too.  Sums are f32: one to sixteen terms a thread, a wave's
+// by DPP, the waves' through LDS, one barrier each.  A layer norm's squares are
+// taken about the mean, in a second pass over the registers: sums of squares lose
+// the small variance of a row far from 0.
+// Large calls are bound by memory: 4,096 tokens of eight f32 rows, hidden 2048,
+// bf16, 318 MB in 61 us (5.2 TB/s; a copy of 2 GiB reaches 4.9), 8,191 bf16 rows alone 67 MB in
+// 13.6 (4.9).  Small ones by the launch and two trips to memory: one token 3.2 us.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "mp_device.h"
 #include "mp_elem.h"
@@ -19,51 +26,34 @@ constexpr int NORM_MAX_WAVES = 16;
 
 template <int N> struct Vals { float v[N]; };         // N elements of a row
 
-// Where a thread's elements lie: with WHOLE, N neighbouring ones at a time, in one vector (every row at whole
-// vectors, H a multiple of N); without, a workgroup's width apart, which keeps the single loads of a wave together.
+// A thread's j-th N elements are the row's from N (tid + width j) on.  Where H is no multiple of N (not WHOLE) the last thread's
+// are the row's last N: the ones before its own are another thread's, too, and do not count in its sums.
+template <int N>
+__device__ inline int own(int j) { return N * ((int)threadIdx.x + (int)blockDim.x * j); }
 template <bool WHOLE, int N>
-__device__ inline int place(int j, int e) {
-    const int tid = (int)threadIdx.x, width = (int)blockDim.x;
-    return WHOLE ? N * (tid + width * j) + e : tid + width * (N * j + e);
-}
-// the thread's j-th elements of the row at o (0 beyond H)
-template <int T, bool WHOLE, int N>
-__device__ inline Vals<N> load_n(const void *row, int64_t o, int j, int H) {
-    typedef typename Elem<T>::raw raw;
-    const raw *p = (const raw *)row + o;
-    struct alignas(N * sizeof(raw) < 16 ? N * sizeof(raw) : 16) Vec { raw v[N]; } q;
+__device__ inline int place(int j, int H) { return WHOLE ? own<N>(j) : min(own<N>(j), H - N); }
+// One load or store at the element's own alignment: what a vector off its boundary costs is the line that it spreads into
+// (8,191 rows of 2048 bf16 and a branch, x's rows an odd number of elements apart: 31 us, 29 of whole vectors, 55 of single elements).
+template <int T, int N>
+__device__ inline Vals<N> load_n(const void *row, int64_t o) {
+    typename Elem<T>::raw q[N];
+    __builtin_memcpy(q, (const typename Elem<T>::raw *)row + o, sizeof q);
     Vals<N> f;
-    if constexpr (WHOLE) {
-        q = *(const Vec *)(p + place<WHOLE, N>(j, 0));
 #pragma unroll
-        for (int e = 0; e < N; ++e) f.v[e] = Elem<T>::load(q.v[e]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) q.v[e] = p[min(place<WHOLE, N>(j, e), H - 1)];      // (no branch: the loads go out together)
-#pragma unroll
-        for (int e = 0; e < N; ++e) f.v[e] = place<WHOLE, N>(j, e) < H ? Elem<T>::load(q.v[e]) : 0.0f;
-    }
+    for (int e = 0; e < N; ++e) f.v[e] = Elem<T>::load(q[e]);
     return f;
 }
-template <int T, bool WHOLE, int N>
-__device__ inline void store_n(void *row, int64_t o, int j, int H, const Vals<N> &f) {
-    typedef typename Elem<T>::raw raw;
-    raw *p = (raw *)row + o;
-    struct alignas(N * sizeof(raw) < 16 ? N * sizeof(raw) : 16) Vec { raw v[N]; } q;
-    if constexpr (WHOLE) {
+template <int T, int N>
+__device__ inline void store_n(void *row, int64_t o, const Vals<N> &f) {
+    typename Elem<T>::raw q[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) q.v[e] = Elem<T>::store(f.v[e]);
-        *(Vec *)(p + place<WHOLE, N>(j, 0)) = q;
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (place<WHOLE, N>(j, e) < H) p[place<WHOLE, N>(j, e)] = Elem<T>::store(f.v[e]);
-    }
+    for (int e = 0; e < N; ++e) q[e] = Elem<T>::store(f.v[e]);
+    __builtin_memcpy((typename Elem<T>::raw *)row + o, q, sizeof q);
 }
 // f32 or T
-template <int T, bool WHOLE, int N>
-__device__ inline Vals<N> load_or(int type, const void *row, int64_t o, int j, int H) {
-    return type == T_F32 ? load_n<T_F32, WHOLE, N>(row, o, j, H) : load_n<T, WHOLE, N>(row, o, j, H);
+template <int T, int N>
+__device__ inline Vals<N> load_or(int type, const void *row, int64_t o) {
+    return type == T_F32 ? load_n<T_F32, N>(row, o) : load_n<T, N>(row, o);
 }
 
 template <int N, class F>
@@ -95,6 +85,7 @@ __device__ inline float row_sum(float v, float *s) {
 template <bool WHOLE, int N, int NV>
 __device__ inline void moments(const Vals<N> (&z)[NV], int H, int kind, float eps, float (*s)[NORM_MAX_WAVES], float &mu,
                                float &inv) {
+    auto counts = [H](int j, int e) { return own<N>(j) < H && (WHOLE || place<WHOLE, N>(j, H) + e >= own<N>(j)); };
     mu = 0.0f;
     if (kind == 1) {
         float t = 0.0f;
@@ -102,7 +93,7 @@ __device__ inline void moments(const Vals<N> (&z)[NV], int H, int kind, float ep
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                if (place<WHOLE, N>(j, e) < H) t += z[j].v[e];
+                if (counts(j, e)) t += z[j].v[e];
         mu = row_sum(t, s[0]) / (float)H;
     }
     float q = 0.0f;
@@ -111,7 +102,7 @@ __device__ inline void moments(const Vals<N> (&z)[NV], int H, int kind, float ep
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             const float d = z[j].v[e] - mu;
-            if (place<WHOLE, N>(j, e) < H) q = fmaf(d, d, q);
+            if (counts(j, e)) q = fmaf(d, d, q);
         }
     inv = 1.0f / sqrtf(row_sum(q, s[1]) / (float)H + eps);
 }
@@ -120,15 +111,16 @@ __device__ inline void moments(const Vals<N> (&z)[NV], int H, int kind, float ep
 template <int T, int B, bool WHOLE, int N, int NV>
 __global__ __launch_bounds__(64 * NORM_MAX_WAVES) void block_norm_kernel(NormArgs a) {
     // weights and gate are read with the row where registers hold them, else where they are used
-    constexpr bool EARLY = NV * N <= (WHOLE ? 8 : 4);
-    constexpr int ROWS = WHOLE && N == 4 ? 8 : 4;     // branch rows on their way at once
+    constexpr bool EARLY = NV * N <= 8;
+    constexpr int ROWS = N == 8 ? 4 : 8;                  // branch rows on their way at once
     __shared__ float s_sum[4][NORM_MAX_WAVES];
     const int64_t tok = blockIdx.x;
     Vals<N> z[NV], x[NV], w[NV], c[NV], p[NV], pc[NV], g[NV];
-    auto in = [&](int j) { return place<WHOLE, N>(j, 0) < a.H; };
-    auto vec_of = [&](const void *q, int j) { return load_or<T, WHOLE, N>(a.w_type, q, 0, j, a.H); };
+    auto in = [&](int j) { return own<N>(j) < a.H; };
+    auto at = [&](int j) { return place<WHOLE, N>(j, a.H); };
+    auto vec_of = [&](const void *q, int j) { return load_or<T, N>(a.w_type, q, at(j)); };
     auto gate_of = [&](int j) {
-        if (a.gate_col) return load_or<T, WHOLE, N>(a.gate_type, a.gate, tok * a.gate_row, j, a.H);
+        if (a.gate_col) return load_or<T, N>(a.gate_type, a.gate, tok * a.gate_row + at(j));
         const float u = a.gate_type == T_F32 ? ((const float *)a.gate)[tok * a.gate_row]
                                              : Elem<T>::load(((const typename Elem<T>::raw *)a.gate)[tok * a.gate_row]);
         Vals<N> v;
@@ -139,7 +131,7 @@ __global__ __launch_bounds__(64 * NORM_MAX_WAVES) void block_norm_kernel(NormArg
     for (int j = 0; j < NV; ++j) {
         x[j] = z[j] = Vals<N>{};
         if (!in(j)) continue;
-        x[j] = load_n<T, WHOLE, N>(a.x, tok * a.ldx, j, a.H);
+        x[j] = load_n<T, N>(a.x, tok * a.ldx + at(j));
         if (EARLY && a.w) w[j] = vec_of(a.w, j);
         if (EARLY && a.c) c[j] = vec_of(a.c, j);
         if (B < 0) continue;
@@ -151,7 +143,7 @@ __global__ __launch_bounds__(64 * NORM_MAX_WAVES) void block_norm_kernel(NormArg
             Vals<N> b[ROWS];
 #pragma unroll
             for (int k = 0; k < ROWS; ++k)
-                if (k0 + k < a.n_sum) b[k] = load_n<B < 0 ? T : B, WHOLE, N>(a.branch, o + (k0 + k) * a.ldb, j, a.H);
+                if (k0 + k < a.n_sum) b[k] = load_n<B < 0 ? T : B, N>(a.branch, o + (k0 + k) * a.ldb + at(j));
 #pragma unroll
             for (int k = 0; k < ROWS; ++k)
                 if (k0 + k < a.n_sum) z[j] = k0 + k == 0 ? b[0] : each(z[j], b[k], [](float s, float v) { return s + v; });
@@ -179,10 +171,12 @@ __global__ __launch_bounds__(64 * NORM_MAX_WAVES) void block_norm_kernel(NormArg
 #pragma unroll
         for (int j = 0; j < NV; ++j) z[j] = x[j];
     }
-    if (a.r)
+    if (a.r) {
+        if (!WHOLE) __syncthreads();                  // r may be x, whose last elements two threads read
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            if (in(j)) store_n<T, WHOLE, N>(a.r, tok * a.ldr, j, a.H, z[j]);
+            if (in(j)) store_n<T, N>(a.r, tok * a.ldr + at(j), z[j]);
+    }
     if (!a.y) return;
     moments<WHOLE>(z, a.H, a.kind, a.eps, s_sum + 2, mu, inv);
 #pragma unroll
@@ -191,39 +185,41 @@ __global__ __launch_bounds__(64 * NORM_MAX_WAVES) void block_norm_kernel(NormArg
         Vals<N> y = each(z[j], [&](float v) { return (v - mu) * inv; });
         if (a.w) y = each(y, EARLY ? w[j] : vec_of(a.w, j), [&](float v, float u) { return v * (u + a.offset); });
         if (a.c) y = each(y, EARLY ? c[j] : vec_of(a.c, j), [](float v, float u) { return v + u; });
-        if (a.y_type == T_F32) store_n<T_F32, WHOLE, N>(a.y, tok * a.ldy, j, a.H, y);
-        else store_n<T, WHOLE, N>(a.y, tok * a.ldy, j, a.H, y);
+        if (a.y_type == T_F32) store_n<T_F32, N>(a.y, tok * a.ldy + at(j), y);
+        else store_n<T, N>(a.y, tok * a.ldy + at(j), y);
     }
 }
 
-template <int T, int B, bool WHOLE, int N>
+template <int T, int B, int N>
 static hipError_t launch_norm_n(const NormArgs &a, hipStream_t st) {
     // N elements a thread, up to 1,024 threads; more elements a thread beyond that
     const int groups = (a.H + N - 1) / N, nv = groups <= 1024 ? 1 : groups <= 2048 ? 2 : 4;
     const dim3 grid((unsigned)a.n_tok), block((unsigned)(((groups + nv - 1) / nv + 63) / 64 * 64));
-    if (nv == 1) hipLaunchKernelGGL((block_norm_kernel<T, B, WHOLE, N, 1>), grid, block, 0, st, a);
-    else if (nv == 2) hipLaunchKernelGGL((block_norm_kernel<T, B, WHOLE, N, 2>), grid, block, 0, st, a);
-    else if constexpr (N == 4) hipLaunchKernelGGL((block_norm_kernel<T, B, WHOLE, N, 4>), grid, block, 0, st, a);
-    return hipGetLastError();
-}
-
-// whether every row of every tensor begins at whole vectors of n elements (at 16 bytes if those are longer)
-static bool whole_vectors(const NormArgs &a, int n) {
-    auto whole = [n](const void *p, int type, int64_t ld) {
-        const int size = type == T_F32 ? 4 : 2, bytes = size * n < 16 ? size * n : 16;
-        return (uintptr_t)p % bytes == 0 && ld * size % bytes == 0;
+    auto run = [&](auto whole) {
+        constexpr bool W = decltype(whole)::value;
+        if (nv == 1) hipLaunchKernelGGL((block_norm_kernel<T, B, W, N, 1>), grid, block, 0, st, a);
+        else if constexpr (N > 1) {
+            if (nv == 2) hipLaunchKernelGGL((block_norm_kernel<T, B, W, N, 2>), grid, block, 0, st, a);
+            else if constexpr (N == 4) hipLaunchKernelGGL((block_norm_kernel<T, B, W, N, 4>), grid, block, 0, st, a);
+        }
     };
-    return a.H % n == 0 && whole(a.x, a.x_type, a.ldx) && whole(a.branch, a.b_type, a.ldb) &&
-           (!a.gate_col || whole(a.gate, a.gate_type, a.gate_row)) && whole(a.w, a.w_type, 0) && whole(a.c, a.w_type, 0) &&
-           whole(a.pw, a.w_type, 0) && whole(a.pc, a.w_type, 0) && whole(a.r, a.x_type, a.ldr) && whole(a.y, a.y_type, a.ldy);
+    if constexpr (N == 1) {
+        run(std::true_type());
+    } else {
+        if (a.H % N == 0) run(std::true_type());
+        else run(std::false_type());
+    }
+    return hipGetLastError();
 }
 
 template <int T, int B>
 static hipError_t launch_norm_b(const NormArgs &a, hipStream_t st) {
-    // eight elements a thread where x and the branch are of 16 bits: half the waves, whole 16-byte loads
+    // Eight elements a thread where x and the branch are of 16 bits: half the waves, whole 16-byte loads (8,191 rows of
+    // 2048: 13.6 us alone and 29 with a branch; of four elements 17.6 and 35).  Four beside f32, where eight would hold twice the registers.
+    // Rows shorter than a vector are read by elements.
     if constexpr (T != T_F32 && B != T_F32)
-        if (whole_vectors(a, 8)) return launch_norm_n<T, B, true, 8>(a, st);
-    return whole_vectors(a, 4) ? launch_norm_n<T, B, true, 4>(a, st) : launch_norm_n<T, B, false, 4>(a, st);
+        if (a.H >= 8) return launch_norm_n<T, B, 8>(a, st);
+    return a.H >= 4 ? launch_norm_n<T, B, 4>(a, st) : launch_norm_n<T, B, 1>(a, st);
 }
 template <int T>
 static hipError_t launch_norm_t(const NormArgs &a, hipStream_t st) {

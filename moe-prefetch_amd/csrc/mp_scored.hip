@@ -98,13 +98,13 @@ __global__ __launch_bounds__(64 * SCORED_WAVES) void route_scored_kernel(ScoredA
     bool on[NV];
     float x[NV], bias[NV];
     if (a.vec) {
-        struct alignas(sizeof(raw) * NV > 16 ? 16 : sizeof(raw) * NV) Vec { raw v[NV]; };
-        struct alignas(NV > 4 ? 16 : 4 * NV) Vec4 { float v[NV]; };
         const bool in = NV * lane < a.E;
-        const Vec q = in ? ((const Vec *)l)[lane] : Vec{};
-        const Vec4 b = in && a.bias ? ((const Vec4 *)a.bias)[lane] : Vec4{};
+        raw q[NV] = {};
+        float b[NV] = {};
+        if (in) __builtin_memcpy(q, l + NV * lane, sizeof q);     // (vectors at the element's own alignment)
+        if (in && a.bias) __builtin_memcpy(b, a.bias + NV * lane, sizeof b);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) { x[j] = in ? Elem<T>::load(q.v[j]) : -INFINITY; bias[j] = b.v[j]; }
+        for (int j = 0; j < NV; ++j) { x[j] = in ? Elem<T>::load(q[j]) : -INFINITY; bias[j] = b[j]; }
     } else {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -256,8 +256,7 @@ __global__ __launch_bounds__(64 * SCORED_WAVES) void route_scored_kernel(ScoredA
 
 template <int T, int NV>
 static hipError_t launch_scored_n(ScoredArgs a, hipStream_t st) {
-    const int size = T == T_F32 ? 4 : 2, vec = size * NV < 16 ? size * NV : 16, vecb = 4 * NV < 16 ? 4 * NV : 16;
-    a.vec = a.E % NV == 0 && (uintptr_t)a.logits % vec == 0 && a.ld * size % vec == 0 && (uintptr_t)a.bias % vecb == 0;
+    a.vec = a.E % NV == 0;
     const int n = a.E / a.groups, lanes = n / NV;
     a.group_lanes = n % NV == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
     hipLaunchKernelGGL((route_scored_kernel<T, NV>), dim3((unsigned)((a.n_tok + SCORED_WAVES - 1) / SCORED_WAVES)),

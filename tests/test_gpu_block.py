@@ -252,7 +252,7 @@ def test_norm_without_branch_weights_or_outputs():
     check_norm("bf16", x, BlockNorm(H, post=True)(x, b), branch=b, post=True)
 
 
-@pytest.mark.parametrize("H", [2048, 1537])
+@pytest.mark.parametrize("H", [2048, 1537, 9, 5, 3, 1, 4095, 9001])
 def test_norm_in_place_and_strides(H):
     T, g = 7, gen(14)
     buf = randn(g, T + 2, H + 37).to(torch.bfloat16)
