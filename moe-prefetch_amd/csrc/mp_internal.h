@@ -330,6 +330,7 @@ hipError_t launch_swiglu_quant(const float *y2, int P, int I, float *h_out, int 
                                uint16_t *bs16, hipStream_t st);
 
 // the norms around a block, and sampling: as ScoredArgs
+constexpr int MAX_NORM_H = 16384;
 struct NormArgs {
     int n_tok, H, kind, post, x_type, b_type, n_sum, gate_type, gate_act, w_type, y_type;
     const void *x, *branch, *gate, *w, *c, *pw, *pc;

@@ -3,18 +3,16 @@
 // residual scale and add, and the norm before the next block, in one launch.
 //
 // Every element is read once and stays in registers between the sums over its
-// row: a workgroup has a row, a thread N neighbouring elements of it (up to four
-// times), so that all of a row's loads are on their way at once, those of the
-// weights and the gate too.  Sums are f32: one to sixteen terms a thread, a wave's
+// row: a workgroup has a row, a thread eight neighbouring elements of it (or twice
+// that), so that all of a row's loads are on their way at once, those of the
+// weights and the gate too.  Sums are f32: up to sixteen terms a thread, a wave's
 // by DPP, the waves' through LDS, one barrier each.  A layer norm's squares are
 // taken about the mean, in a second pass over the registers: sums of squares lose
 // the small variance of a row far from 0.
 // Large calls are bound by memory: 4,096 tokens of eight f32 rows, hidden 2048,
 // bf16, 318 MB in 61 us (5.2 TB/s; a copy of 2 GiB reaches 4.9), 8,191 bf16 rows alone 67 MB in
-// 13.6 (4.9).  Small ones by the launch and two trips to memory: one token 3.2 us.
+// 13.6 (4.9).  Small ones by the launch and two trips to memory: one token 3.4 us.
 #include <hip/hip_runtime.h>
-
-#include <type_traits>
 
 #include "mp_device.h"
 #include "mp_elem.h"
@@ -111,8 +109,8 @@ __device__ inline void moments(const Vals<N> (&z)[NV], int H, int kind, float ep
 template <int T, int B, bool WHOLE, int N, int NV>
 __global__ __launch_bounds__(64 * NORM_MAX_WAVES) void block_norm_kernel(NormArgs a) {
     // weights and gate are read with the row where registers hold them, else where they are used
-    constexpr bool EARLY = NV * N <= 8;
-    constexpr int ROWS = N == 8 ? 4 : 8;                  // branch rows on their way at once
+    constexpr bool EARLY = NV == 1;
+    constexpr int ROWS = 4;                               // branch rows on their way at once
     __shared__ float s_sum[4][NORM_MAX_WAVES];
     const int64_t tok = blockIdx.x;
     Vals<N> z[NV], x[NV], w[NV], c[NV], p[NV], pc[NV], g[NV];
@@ -190,36 +188,24 @@ __global__ __launch_bounds__(64 * NORM_MAX_WAVES) void block_norm_kernel(NormArg
     }
 }
 
-template <int T, int B, int N>
+template <int T, int B, bool WHOLE, int N, int NV>
 static hipError_t launch_norm_n(const NormArgs &a, hipStream_t st) {
-    // N elements a thread, up to 1,024 threads; more elements a thread beyond that
-    const int groups = (a.H + N - 1) / N, nv = groups <= 1024 ? 1 : groups <= 2048 ? 2 : 4;
-    const dim3 grid((unsigned)a.n_tok), block((unsigned)(((groups + nv - 1) / nv + 63) / 64 * 64));
-    auto run = [&](auto whole) {
-        constexpr bool W = decltype(whole)::value;
-        if (nv == 1) hipLaunchKernelGGL((block_norm_kernel<T, B, W, N, 1>), grid, block, 0, st, a);
-        else if constexpr (N > 1) {
-            if (nv == 2) hipLaunchKernelGGL((block_norm_kernel<T, B, W, N, 2>), grid, block, 0, st, a);
-            else if constexpr (N == 4) hipLaunchKernelGGL((block_norm_kernel<T, B, W, N, 4>), grid, block, 0, st, a);
-        }
-    };
-    if constexpr (N == 1) {
-        run(std::true_type());
-    } else {
-        if (a.H % N == 0) run(std::true_type());
-        else run(std::false_type());
-    }
+    const int threads = ((a.H + N - 1) / N + NV - 1) / NV;
+    hipLaunchKernelGGL((block_norm_kernel<T, B, WHOLE, N, NV>), dim3((unsigned)a.n_tok), dim3((unsigned)((threads + 63) / 64 * 64)),
+                       0, st, a);
     return hipGetLastError();
 }
-
 template <int T, int B>
 static hipError_t launch_norm_b(const NormArgs &a, hipStream_t st) {
-    // Eight elements a thread where x and the branch are of 16 bits: half the waves, whole 16-byte loads (8,191 rows of
-    // 2048: 13.6 us alone and 29 with a branch; of four elements 17.6 and 35).  Four beside f32, where eight would hold twice the registers.
-    // Rows shorter than a vector are read by elements.
-    if constexpr (T != T_F32 && B != T_F32)
-        if (a.H >= 8) return launch_norm_n<T, B, 8>(a, st);
-    return a.H >= 4 ? launch_norm_n<T, B, 4>(a, st) : launch_norm_n<T, B, 1>(a, st);
+    // Eight elements a thread, up to 1,024 threads, then sixteen.  8,191 rows of 2048 bf16: 13.6 us alone, 29 with a bf16
+    // branch and 33 with an f32 one; of four elements, twice the waves with half the bytes on their way, 20.7, 38 and 37.
+    // A row shorter than eight is read by elements.
+    static_assert(MAX_NORM_H <= 2 * 8 * 64 * NORM_MAX_WAVES, "two vectors a thread");
+    if (a.H < 8) return launch_norm_n<T, B, true, 1, 1>(a, st);
+    const bool whole = a.H % 8 == 0;
+    if (a.H <= 8 * 64 * NORM_MAX_WAVES)
+        return whole ? launch_norm_n<T, B, true, 8, 1>(a, st) : launch_norm_n<T, B, false, 8, 1>(a, st);
+    return whole ? launch_norm_n<T, B, true, 8, 2>(a, st) : launch_norm_n<T, B, false, 8, 2>(a, st);
 }
 template <int T>
 static hipError_t launch_norm_t(const NormArgs &a, hipStream_t st) {

@@ -4161,7 +4161,7 @@ size_t moe_sample_workspace_bytes(int n_tok, int V) {
     return n_tok < 1 || V < 1 || V > MOE_SAMPLE_MAX_V ? 0 : mp::sample_ws_bytes(n_tok, V);
 }
 
-static_assert(mp::MAX_SAMPLE_V == MOE_SAMPLE_MAX_V, "header and library disagree");
+static_assert(mp::MAX_SAMPLE_V == MOE_SAMPLE_MAX_V && mp::MAX_NORM_H == MOE_BLOCK_NORM_MAX_H, "header and library disagree");
 
 int moe_sample(const moe_sample_desc *d, void *stream) {
     if (!d) return fail(MOE_ERR_ARG, "moe_sample: null argument");

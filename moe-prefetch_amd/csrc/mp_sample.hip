@@ -13,7 +13,9 @@
 //   3 rest    rows that step 2 could not decide (a flat distribution: the cut or the
 //             draw lies behind the candidates): a histogram of counts and masses by
 //             several workgroups, the last of which reads the one bin that matters.
-//             Rows of one value or nearly so end in a radix search (locate).
+//             Rows of one value or nearly so end in a radix search.
+// 256 rows of 151,936 bf16 logits (78 MB, 16 us at the rate of a large copy), each with cuts of its own: 36 us + 14 us,
+// and 35 more if a row or a few need step 3 (they go at once); under top-k alone 33 in all; one row 15.
 #include <hip/hip_runtime.h>
 
 #include "mp_device.h"
@@ -149,6 +151,10 @@ struct SliceHead {
 // Chunks of 64 lanes x 16 bytes go to a row's slices in turn, so that neighbouring
 // likely tokens spread over them.  The bound is the value that about `keep` lanes' maxima
 // reach (a bisection; any value would do); should more than `cap` logits lie above it, a higher one.
+// One slice to a wave, 64 logits in its lane's registers: 112 of them, four waves a SIMD, and no barrier behind the first.
+// 256 rows of 151,936 bf16 logits: 27 us where every row is under top-k (2.9 TB/s), 48 where none is: the 39 million
+// exponentials in f64 are some 19 vector operations each, 20 us of every SIMD's time, and a wave's loads come before
+// its own.  (A second slice on its way, or 16-bit logits kept packed, spilled or cost a wave a SIMD, and were slower.)
 template <int T>
 __global__ __launch_bounds__(64 * SLICE_WAVES, 4) void sample_slice_kernel(SampleArgs a) {
     typedef typename Elem<T>::raw raw;
@@ -776,6 +782,9 @@ struct RestRow {
 
 // A fixed number of workgroups take the parts of the undecided rows in turn; the one
 // that finishes a row's last part decides the row.  No workgroup waits for another.
+// A row of 151,936 takes 35 to 40 us however many there are up to 16, all latency: the histogram 4.5 (16 parts), its
+// sums to memory 3 and back 3.6, and a bin's tokens found, gathered and sorted in 12, for the cut and for the draw.
+// (Reading the bins of both in one pass measured 52.5 against 53.8 us for 64 rows and nothing for 256.)
 template <int T>
 __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) {
     __shared__ SampleShared s;
@@ -851,7 +860,8 @@ __device__ inline uint64_t lane_u64(uint64_t v, int l) {
 }
 __device__ inline void wave_lds() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }    // a wave's LDS accesses stay in order
 
-// All four waves read the candidates; the first one decides, without a barrier: up to 512 (or 1,024) candidates in
+// All four waves read the candidates; the first one decides, without a barrier (6 to 7 us for one row, 8 to 14 for 256: a
+// chain of LDS and DPP steps, each waiting for the last): up to 512 (or 1,024) candidates in
 // its registers, of which it sorts the next up to 64 at a time (bounded by a bisection) until
 // the cuts and the draw fall within what is sorted.  Returns whether they did.
 template <int PICK_PER>
@@ -1149,13 +1159,17 @@ __global__ __launch_bounds__(PICK_THREADS) void sample_pick_kernel(SampleArgs a)
 struct SamplePlan {
     int slices, cap_log, keep, parts;
 };
+// `want` candidates of a slice, 300 to 600 of a row: enough for a top-k of 200 and most cuts by mass, and few enough for one
+// wave's registers.  Half as many: 693 us against 80 for 256 rows of 151,936 with cuts of their own (top-k up to 200), whose
+// undecided ones fill step 3; twice as many: 51 against 15 for one row under top-k, whose candidates do not fit.
+// A row of up to 1,000 is kept whole: it needs no step 3.
 static SamplePlan sample_plan(int V) {
     SamplePlan p;
     p.slices = (V + 7 + SLICE - 1) / SLICE;           // (7: a row may begin inside 16 bytes)
     const int want = p.slices >= 64 ? 8 : p.slices >= 25 ? 16 : 400 / p.slices;
     // of 64 maxima over runs of random values, those above the value that `want` of all exceed
     p.keep = V <= 1000 ? 65 : (int)ceil(64.0 * (1.0 - exp(-want / 64.0)));
-    p.parts = V < 16384 ? 1 : V >= 131072 ? 16 : V / 8192;       // workgroups to an undecided row
+    p.parts = V < 16384 ? 1 : V >= 131072 ? 16 : V / 8192;       // workgroups to an undecided row, 8,192 logits to each
     p.cap_log = 4;
     while ((1 << p.cap_log) < want + want / 2 + 8) ++p.cap_log;
     return p;

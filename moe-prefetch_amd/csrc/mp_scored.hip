@@ -7,6 +7,10 @@
 // group's, has to be that of the definition however near they are.  The K best
 // come out in K rounds of a wave maximum over the lanes' best; a round compares the
 // upper words and looks at the lower ones only where two lanes agree in them.
+// One token of 256 experts in 8 groups, 8 chosen: 4.6 us, launch and latency.  8,191
+// of them: 16 us for 8.9 MB (1.8 at the rate of a large copy): the instructions of
+// eight waves a SIMD, of the launch's ~13 us about 5 for the scores in f64, 3 for the groups and 4.5
+// for the rounds (K = 1: 8.2 in all).
 #include <hip/hip_runtime.h>
 
 #include "mp_device.h"
@@ -257,6 +261,7 @@ __global__ __launch_bounds__(64 * SCORED_WAVES) void route_scored_kernel(ScoredA
 template <int T, int NV>
 static hipError_t launch_scored_n(ScoredArgs a, hipStream_t st) {
     a.vec = a.E % NV == 0;
+    // a group of whole lanes is reduced by DPP, others one to a lane out of LDS (8 groups of 32: 16 us for 8,191 tokens; of 25: 17)
     const int n = a.E / a.groups, lanes = n / NV;
     a.group_lanes = n % NV == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
     hipLaunchKernelGGL((route_scored_kernel<T, NV>), dim3((unsigned)((a.n_tok + SCORED_WAVES - 1) / SCORED_WAVES)),
