@@ -617,15 +617,20 @@ struct BinSearch {
     SampleShared &s;
     float vmax, per;
     uint64_t n_all, m_all;
-    // from the histogram in s.cnt and s.mass: each bin's count and mass become those of the bins before it
-    __device__ void prepare() {
+    // the histogram's counts and masses of all parts to s.cnt and s.mass, as those of the bins before each
+    __device__ void prepare(const uint32_t *cnt, const uint64_t *mass) {
         const int b = SMP_PER * (int)threadIdx.x;
         uint64_t q[SMP_PER], m = 0;
         uint32_t k[SMP_PER], c = 0;
 #pragma unroll
         for (int j = 0; j < SMP_PER; ++j) {
-            c += k[j] = s.cnt[b + j];
-            m += q[j] = s.mass[b + j];
+            k[j] = __hip_atomic_load(&cnt[b + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            q[j] = __hip_atomic_load(&mass[b + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+#pragma unroll
+        for (int j = 0; j < SMP_PER; ++j) {
+            c += k[j];
+            m += q[j];
         }
         uint64_t cb = block_before(c, s.wc), mb = block_before(m, s.wm);
         n_all = m_all = 0;
@@ -825,14 +830,9 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
         __syncthreads();
         if (!s.last) continue;
         __threadfence();
-        for (int i = tid; i < SMP_BINS; i += SMP_THREADS) {
-            s.cnt[i] = __hip_atomic_load(&r.cnt[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            s.mass[i] = __hip_atomic_load(&r.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
         const uint32_t kmax = sort_key(vmax);
         BinSearch<T> bins{row, ms, s, vmax, per, 0, 0};
-        bins.prepare();
+        bins.prepare(r.cnt, r.mass);
         if (vmax == INFINITY || !sample_row<T>(a, tok, kmax, cut, bins, s))
             sample_row<T>(a, tok, kmax, cut, RadixSearch<T>{row, ms, s}, s);
     }
