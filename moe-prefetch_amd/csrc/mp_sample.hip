@@ -368,7 +368,7 @@ struct SampleShared {
     uint64_t wm[SMP_WAVES];
     uint64_t wc[SMP_WAVES];
     uint64_t found_m, found_e;
-    uint32_t found_c, found_bin, last;
+    uint32_t found_c, found_bin, last, key[2];
     SampleList list;
 };
 
@@ -653,14 +653,13 @@ struct BinSearch {
     __device__ uint64_t mass_from(uint32_t key) const {
         const int b = bin_of(key_value(key), vmax, per);
         uint64_t sum = 0;
-        const float from = key_value(key), to = top_of(b);
+        const float from = key_value(key), to = b == 0 ? vmax + 0.0f : key_value(lowest_in(b - 1) - 1);
         row.each([&](float v, int) { if (v >= from && v <= to) sum += ms.fixed(sort_key(v)); });
         return mass_to(b) + block_sum(sum, s);
     }
-    // a bin's highest value
-    __device__ float top_of(int b) const {
-        const uint32_t kmax = sort_key(vmax);
-        return b == 0 ? vmax + 0.0f : key_value(lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return bin_of(key_value(k), vmax, per) < b; }) - 1);
+    // the lowest key of bins 0 to b
+    __device__ uint32_t lowest_in(int b) const {
+        return lowest_key(KEY_NONE, sort_key(vmax), [&](uint32_t k) { return bin_of(key_value(k), vmax, per) <= b; });
     }
     __device__ Cut find(bool by_mass, uint64_t target) const {
         __syncthreads();
@@ -674,10 +673,14 @@ struct BinSearch {
         const int b = (int)s.found_bin, n = (int)(cnt_to(b + 1) - cnt_to(b));
         uint64_t nb = cnt_to(b), mb = mass_to(b);
         if (n > SMP_LIST) return Cut{0, CUT_FULL, 0, 0};
-        // the bin's values, so that the pass over the row only compares
-        const uint32_t kmax = sort_key(vmax);
-        const float from = key_value(lowest_key(KEY_NONE, kmax, [&](uint32_t k) { return bin_of(key_value(k), vmax, per) <= b; }));
-        row.among(from, top_of(b), s.list);
+        // the bin's values, so that the pass over the row only compares; a wave to each end
+        const int wave = (int)threadIdx.x >> 6;
+        if (wave < 2 && wave <= b) {
+            const uint32_t k = lowest_in(b - wave);
+            if ((threadIdx.x & 63) == 0) s.key[wave] = k;
+        }
+        __syncthreads();
+        row.among(key_value(s.key[0]), b == 0 ? vmax + 0.0f : key_value(s.key[1] - 1), s.list);
         sort_list(s.list, n);
         const int j0 = SMP_PER * (int)threadIdx.x;
         uint64_t q[SMP_PER], m = 0;
