@@ -610,12 +610,29 @@ __device__ inline uint32_t lowest_key(uint32_t lo, uint32_t hi, F pred) {
     return hi;
 }
 
+// What the slices of a row left: every token of a key from `bound` on
+struct Candidates {
+    const SliceHead *heads;
+    const uint64_t *lists;
+    int slices, cap_log;
+    uint32_t bound;
+    template <class F>
+    __device__ void among(float from, float to, F f) const {
+        for (int p = threadIdx.x; p < slices << cap_log; p += SMP_THREADS) {
+            const uint64_t e = lists[p];              // (what lies behind a list's end is read and left out)
+            const float v = key_value(entry_key(e));
+            if (((uint32_t)p & ((1u << cap_log) - 1)) < heads[p >> cap_log].n && v >= from && v <= to) f(e);
+        }
+    }
+};
+
 template <int T>
 struct BinSearch {
     Row<T> row;
     Mass ms;
     SampleShared &s;
     float vmax, per;
+    Candidates cand;
     uint64_t n_all, m_all;
     // the histogram's counts and masses of all parts to s.cnt and s.mass, as those of the bins before each
     __device__ void prepare(const uint32_t *cnt, const uint64_t *mass) {
@@ -654,7 +671,8 @@ struct BinSearch {
         const int b = bin_of(key_value(key), vmax, per);
         uint64_t sum = 0;
         const float from = key_value(key), to = b == 0 ? vmax + 0.0f : key_value(lowest_in(b - 1) - 1);
-        row.each([&](float v, int) { if (v >= from && v <= to) sum += ms.fixed(sort_key(v)); });
+        if (key >= cand.bound) cand.among(from, to, [&](uint64_t e) { sum += ms.fixed(entry_key(e)); });
+        else row.each([&](float v, int) { if (v >= from && v <= to) sum += ms.fixed(sort_key(v)); });
         return mass_to(b) + block_sum(sum, s);
     }
     // the lowest key of bins 0 to b
@@ -680,7 +698,14 @@ struct BinSearch {
             if ((threadIdx.x & 63) == 0) s.key[wave] = k;
         }
         __syncthreads();
-        row.among(key_value(s.key[0]), b == 0 ? vmax + 0.0f : key_value(s.key[1] - 1), s.list);
+        const float from = key_value(s.key[0]), to = b == 0 ? vmax + 0.0f : key_value(s.key[1] - 1);
+        if (s.key[0] >= cand.bound) {                 // every token of the bin is among the candidates
+            if (threadIdx.x == 0) s.list.n = 0;
+            __syncthreads();
+            cand.among(from, to, [&](uint64_t e) { s.list.raw[atomicAdd(&s.list.n, 1u)] = e; });
+        } else {
+            row.among(from, to, s.list);
+        }
         sort_list(s.list, n);
         const int j0 = SMP_PER * (int)threadIdx.x;
         uint64_t q[SMP_PER], m = 0;
@@ -785,6 +810,7 @@ struct RestRow {
     int64_t tok;
     float vmax;
     int shift;                                        // Mass::shift
+    uint32_t bound;                                   // Candidates::bound
     uint32_t parts;                                   // finished
 };
 
@@ -834,7 +860,9 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) 
         if (!s.last) continue;
         __threadfence();
         const uint32_t kmax = sort_key(vmax);
-        BinSearch<T> bins{row, ms, s, vmax, per, 0, 0};
+        const Candidates cand = {(const SliceHead *)a.heads + tok * a.slices, (const uint64_t *)a.lists + (size_t)(tok * a.slices) * a.cap,
+                                 a.slices, a.cap_log, r.bound};
+        BinSearch<T> bins{row, ms, s, vmax, per, cand, 0, 0};
         bins.prepare(r.cnt, r.mass);
         if (vmax == INFINITY || !sample_row<T>(a, tok, kmax, cut, bins, s))
             sample_row<T>(a, tok, kmax, cut, RadixSearch<T>{row, ms, s}, s);
@@ -1151,6 +1179,7 @@ __global__ __launch_bounds__(PICK_THREADS) void sample_pick_kernel(SampleArgs a)
         int ex;
         frexp(whole * (1.0 + 1e-9), &ex);
         r.shift = 62 - ex;
+        r.bound = bound;
         r.tok = tok;
         r.vmax = vmax;
         r.parts = 0;
