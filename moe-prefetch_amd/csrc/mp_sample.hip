@@ -15,7 +15,7 @@
 //             several workgroups, the last of which reads the one bin that matters.
 //             Rows of one value or nearly so end in a radix search.
 // 256 rows of 151,936 bf16 logits (78 MB, 16 us at the rate of a large copy), each with cuts of its own: 36 us + 14 us,
-// and 35 more if a row or a few need step 3 (they go at once); under top-k alone 33 in all; one row 15.
+// and 30 more if a row or a few need step 3 (they go at once); under top-k alone 33 in all; one row 15.
 #include <hip/hip_runtime.h>
 
 #include "mp_device.h"
@@ -816,9 +816,10 @@ struct RestRow {
 
 // A fixed number of workgroups take the parts of the undecided rows in turn; the one
 // that finishes a row's last part decides the row.  No workgroup waits for another.
-// A row of 151,936 takes 35 to 40 us however many there are up to 16, all latency: the histogram 4.5 (16 parts), its
-// sums to memory 3 and back 3.6, and a bin's tokens found, gathered and sorted in 12, for the cut and for the draw.
-// (Reading the bins of both in one pass measured 52.5 against 53.8 us for 64 rows and nothing for 256.)
+// A row of 151,936 takes 30 to 33 us however many there are up to 16, all latency: the histogram 4.5 (16 parts), its
+// sums to memory 3 and back 3, and a bin's tokens found, gathered and sorted in up to 11, for the cut and for the draw;
+// 6 less where the candidates hold all of the bin, as they do for most draws.  (Reading the bins of both in one
+// pass over the row gained 1 us of 54 and was not kept.)
 template <int T>
 __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) {
     __shared__ SampleShared s;
