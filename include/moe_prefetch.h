@@ -257,8 +257,10 @@ int moe_cache_set_router(moe_cache *c, int layer, const float *W_dev);
 int moe_cache_set_shared(moe_cache *c, int layer, const void *expert, size_t expert_bytes);
 /* Route `layer` by scores (moe_route_scored; of `rule` the score, renormalize,
  * n_groups, top_groups, group_best, scale and bias count, its E and K are the
- * cache's, and the bias is read at every call) instead of by softmax and top-k;
- * NULL returns to that.  Such a layer decodes through moe_decode_batch, one token
+ * cache's) instead of by softmax and top-k; NULL returns to that.  The bias is read
+ * at every call: it lies in memory of the cache's device, or mapped pinned memory,
+ * and stays allocated until the layer has another rule or none, or the cache is
+ * destroyed.  Such a layer decodes through moe_decode_batch, one token
  * too: moe_decode_token and moe_decode_layer, whose launches route by softmax,
  * refuse a cache that has one (MOE_ERR_STATE).  Not with a cache prior. */
 typedef struct moe_route_scored_desc moe_route_scored_desc;

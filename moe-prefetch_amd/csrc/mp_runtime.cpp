@@ -1892,6 +1892,14 @@ int moe_cache_set_scoring(moe_cache *c, int layer, const moe_route_scored_desc *
                     c->K, c->E);
     if ((uintptr_t)rule->bias % 4) return fail(MOE_ERR_ARG, "moe_cache_set_scoring: misaligned bias");
     if (c->cfg.cache_prior != 0.0f) return fail(MOE_ERR_STATE, "moe_cache_set_scoring: the cache has a prior on softmax routing");
+    if (rule->bias && !c->host_only) {                // (a host-only cache never reads it)
+        const int b = check_weight_ptrs("moe_cache_set_scoring", rule->bias, nullptr);
+        if (b != MOE_OK) return b;
+        hipPointerAttribute_t at{};
+        HIPCHK(hipPointerGetAttributes(&at, rule->bias));
+        if (at.type == hipMemoryTypeDevice && at.device != c->cfg.device)
+            return fail(MOE_ERR_ARG, "moe_cache_set_scoring: the bias is on device %d, the cache on %d", at.device, c->cfg.device);
+    }
     ls.rule = scored_rule(rule);
     ls.scored = true;
     return MOE_OK;

@@ -126,7 +126,7 @@ class ScoredRouter:
         self._rule = (self.E, self.K, _lib.SCORE[score], int(bool(renormalize)), int(n_groups), int(top), int(group_best),
                       float(scale))
         if bias is not None:
-            _vec(bias, self.E, _F32, bias.get_device(), "bias")
+            _vec(bias, self.E, _F32, _on_gpu(bias, "bias"), "bias")
         self._pack, self._fn = _lib.packed(_lib.RouteScoredDesc)[0], _lib.entry("moe_route_scored")
         check(self._fn(self._packed(0, 0, 0, 0), None), "moe_route_scored")     # the rule alone: no tokens
 
@@ -135,9 +135,11 @@ class ScoredRouter:
         return self._pack(logits, ld, kind, T, *self._rule, bias, table, dummy, ids, w, slots, scores, W, x, H, workspace)
 
     def rule(self):
-        """The rule as a descriptor (MoeCache.set_scoring); its bias stays this object's."""
+        """The rule as a descriptor (MoeCache.set_scoring), which holds the address of the bias: whoever reads it later keeps
+        that tensor."""
+        bias = self.bias
         return _lib.RouteScoredDesc.from_buffer_copy(
-            self._packed(0, 0, 0, 0, bias=0 if self.bias is None else self.bias.data_ptr()))
+            self._packed(0, 0, 0, 0, bias=0 if bias is None else _vec(bias, self.E, _F32, _on_gpu(bias, "bias"), "bias")))
 
     def from_product(self, W, x, ids, w, slots, workspace, H, stream=None):
         """The same from W [n_experts][H] and x [tokens][H] (f32), whose product moe_route's kernels make in workspace

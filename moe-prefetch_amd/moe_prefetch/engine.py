@@ -79,7 +79,7 @@ class MoeCache:
         self.h = h.value
         self.device = device
         self.cache_prior = cache_prior
-        self._scoring = {}              # layer -> ScoredRouter
+        self._scoring = {}              # layer -> the bias that its scoring rule reads
         self.prior_space = prior_space
 
     @classmethod
@@ -185,11 +185,16 @@ class MoeCache:
                                          else 0), "set_shared")
 
     def set_scoring(self, layer, router):
-        """Route `layer` by a ScoredRouter's rule (read from it now, its bias at every call); None returns to softmax and
-        top-k.  Such a layer decodes through decode_batch, one token too."""
-        rule = None if router is None else router.rule()
+        """Route `layer` by a ScoredRouter's rule, read from it now; None returns to softmax and top-k.  Such a layer decodes
+        through decode_batch, one token too.  The bias that the router has now, a tensor on the cache's GPU, is kept here
+        and read at every call (change it in place; another one takes another set_scoring)."""
+        rule = bias = None
+        if router is not None:
+            rule, bias = router.rule(), router.bias
+            if bias is not None and self.device >= 0 and bias.get_device() != self.device:
+                raise ValueError(f"the router's bias is on {bias.device}, the cache on cuda:{self.device}")
         check(lib().moe_cache_set_scoring(self.h, layer, None if rule is None else ctypes.byref(rule)), "set_scoring")
-        self._scoring[layer] = router     # keeps the bias alive
+        self._scoring[layer] = bias
 
     def lookup(self, layer):
         v = _lib.LayerView()

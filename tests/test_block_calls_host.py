@@ -1,0 +1,82 @@
+"""What ScoredRouter, BlockNorm, Sampler and their callers hand to the library: host code only, no GPU.  OnGpu stands
+for a tensor of a GPU: its address is never read."""
+import pytest
+import torch
+
+from moe_prefetch import MoeCache
+from moe_prefetch.block import ScoredRouter
+
+F32 = torch.float32
+
+
+class OnGpu:
+    """A tensor's shape, strides and dtype, said to be on cuda:<device> at `at`."""
+
+    is_cuda = True
+
+    def __init__(self, *shape, dtype=F32, device=0, at=4096):
+        self._t, self._at, self.device = torch.empty(shape, dtype=dtype, device="meta"), at, torch.device("cuda", device)
+
+    def __getattr__(self, name):
+        return getattr(self._t, name)
+
+    def __getitem__(self, rows):
+        t = OnGpu(dtype=self.dtype, device=self.device.index, at=self._at)
+        t._t = self._t[rows]
+        return t
+
+    def get_device(self):
+        return self.device.index
+
+    def data_ptr(self):
+        return self._at
+
+
+@pytest.fixture
+def cache():
+    c = MoeCache(2, n_experts=128, intermediate=768, n_slots=16, device=-1)
+    yield c
+    c.close()
+
+
+# ---- a cache's scoring rule ---------------------------------------------------------
+def test_a_cpu_bias_is_refused():
+    with pytest.raises(ValueError, match="bias is on cpu, not on a GPU"):
+        ScoredRouter(128, 8, bias=torch.zeros(128))
+
+
+@pytest.mark.parametrize("bias", [torch.zeros(128), OnGpu(127), OnGpu(128, dtype=torch.bfloat16), OnGpu(256)[::2]])
+def test_a_rule_checks_the_bias_that_it_hands_on(cache, bias):
+    # the bias may be exchanged for another tensor after the router was made
+    router = ScoredRouter(128, 8, bias=OnGpu(128))
+    router.bias = bias
+    with pytest.raises(ValueError, match="bias"):
+        router.rule()
+    with pytest.raises(ValueError, match="bias"):
+        cache.set_scoring(0, router)
+
+
+def test_a_cache_takes_a_bias_of_its_own_gpu_alone(cache):
+    cache.device = 1                                  # (the library's part of it has none)
+    with pytest.raises(ValueError, match="bias is on cuda:0"):
+        cache.set_scoring(0, ScoredRouter(128, 8, bias=OnGpu(128)))
+    cache.set_scoring(0, ScoredRouter(128, 8, bias=OnGpu(128, device=1)))
+
+
+def test_a_cache_keeps_the_bias_that_it_reads(cache):
+    import gc
+    import weakref
+    router = ScoredRouter(128, 8, bias=OnGpu(128))
+    given = weakref.ref(router.bias)
+    cache.set_scoring(0, router)
+    router.bias = OnGpu(128, at=8192)                 # of the router's own calls from here on
+    gc.collect()
+    assert given() is not None
+    cache.set_scoring(0, router)
+    gc.collect()
+    assert given() is None
+    given = weakref.ref(router.bias)
+    cache.set_scoring(0, None)
+    del router
+    gc.collect()
+    assert given() is None

@@ -1,0 +1,75 @@
+"""Calls of moe_route_scored, moe_block_norm, moe_sample and of the paths around them that tests/test_gpu_block.py
+does not make."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import block_ref as R
+from moe_prefetch import MoeCache, _lib
+from moe_prefetch.block import ScoredRouter
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(shape, generator=g, device=DEV)
+
+
+def np64(t):
+    return t.double().cpu().numpy()
+
+
+# ---- a cache's scoring rule ---------------------------------------------------------
+def test_a_cache_refuses_a_bias_that_its_gpu_cannot_read():
+    c = MoeCache(1, n_experts=128, intermediate=768, n_slots=16)
+    try:
+        router = ScoredRouter(128, 8, score="sigmoid", bias=torch.zeros(128, device=DEV))
+        c.set_scoring(0, router)
+        on_host = np.zeros(128, np.float32)
+        rule = router.rule()
+        rule.bias = on_host.ctypes.data
+        assert _lib.lib().moe_cache_set_scoring(c.h, 0, ctypes.byref(rule)) == _lib.MOE_ERR_ARG
+        assert b"moe_cache_set_scoring" in _lib.lib().moe_last_error()
+        with pytest.raises(ValueError, match="bias"):
+            router.bias = torch.zeros(128)
+            c.set_scoring(0, router)
+        # the refusal leaves nothing behind for the next launch to report
+        router.bias = torch.zeros(128, device=DEV)
+        logits = randn(gen(1), 5, 128)
+        ids, w = router(logits)
+        want = R.route(np64(logits), 8, score="sigmoid", bias=np.zeros(128))
+        assert np.array_equal(ids.cpu().numpy(), want[0])
+    finally:
+        c.close()
+
+
+def test_a_cache_reads_the_bias_it_was_given():
+    # the router gets another bias, and the first one's memory is offered to others: the cache still reads the first
+    from gpu_rig import Rig
+    from moe_prefetch.batched import BatchedMoe
+    B, E = 5, 128
+    rig = Rig([40], [_lib.TYPE_Q4K], T=B, steer=False, admit="window", batch_tables=True)
+    try:
+        bias = 0.05 * randn(gen(2), E)
+        router = ScoredRouter(E, 8, score="sigmoid", bias=bias.clone())
+        rig.cache.set_scoring(0, router)
+        router.bias = torch.zeros(E, device=DEV)
+        others = [torch.full((E,), 9.0 - i, device=DEV) for i in range(64)]
+        x = rig.x.transpose(0, 1).contiguous()
+        out = torch.empty((1, B, 2048), device=DEV)
+        torch.cuda.synchronize()
+        ids = rig.cache.decode_batch(x, out, stream=torch.cuda.current_stream().cuda_stream)
+        m = BatchedMoe(B)
+        m.route(B, W=rig.W[0], x=x[0], router=ScoredRouter(E, 8, score="sigmoid", bias=bias))
+        torch.cuda.synchronize()
+        assert np.array_equal(ids[0], m.ids.cpu().numpy())
+        del others
+    finally:
+        rig.close()
