@@ -12,12 +12,20 @@ from .engine import MoeCache, parse_slot_profile
 from .predictor import ExpertPredictor
 from .prefetch_engine import ExpertCache
 
-__all__ = ["BlockNorm", "ExpertCache", "ExpertPredictor", "MoeCache", "MoeError", "Sampler", "ScoredRouter",
-           "TYPE_Q4K", "TYPE_Q6K", "lib", "parse_slot_profile"]
+__all__ = ["ExpertCache", "ExpertPredictor", "MoeCache", "MoeError", "TYPE_Q4K", "TYPE_Q6K",
+           "lib", "parse_slot_profile"]
+
+# These need torch, which the rest of the package does not import: they are imported by name, and a star import leaves
+# them out.
+_BLOCK = ("BlockNorm", "Sampler", "ScoredRouter")
 
 
-def __getattr__(name):                # these need torch, which the rest of the package does not import
-    if name in ("BlockNorm", "Sampler", "ScoredRouter"):
+def __getattr__(name):
+    if name in _BLOCK:
         from . import block
         return getattr(block, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted({*globals(), *_BLOCK})
