@@ -143,8 +143,15 @@ class ScoredRouter:
 
     def from_product(self, W, x, ids, w, slots, workspace, H, stream=None):
         """The same from W [n_experts][H] and x [tokens][H] (f32), whose product moe_route's kernels make in workspace
-        (BatchedMoe.route: hidden 2048, n_experts a multiple of 64 up to 256)."""
+        (BatchedMoe.route: hidden 2048, n_experts a multiple of 64 up to 256).  workspace: contiguous, of
+        moe_route_workspace_bytes() at least."""
         T, _, dev = _first(x, H, "x")
+        need = lib().moe_route_workspace_bytes(self.E, T)
+        if workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be contiguous and of {need} bytes at least, not {tuple(workspace.shape)} of "
+                             f"{workspace.dtype}")
+        if workspace.get_device() != dev:
+            _place(workspace, dev, "workspace")
         out = (T, self.K)
         desc = self._packed(0, 0, 0, T, 0 if self.bias is None else _vec(self.bias, self.E, _F32, dev, "bias"), 0, self.E,
                             _out(ids, out, _I32, dev, "ids"), _out(w, out, _F32, dev, "w"), _out(slots, out, _I32, dev, "slots"),

@@ -3,7 +3,7 @@ for a tensor of a GPU: its address is never read."""
 import pytest
 import torch
 
-from moe_prefetch import MoeCache
+from moe_prefetch import MoeCache, block, lib
 from moe_prefetch.block import ScoredRouter
 
 F32 = torch.float32
@@ -80,3 +80,47 @@ def test_a_cache_keeps_the_bias_that_it_reads(cache):
     del router
     gc.collect()
     assert given() is None
+
+
+# ---- what a call hands to the library -------------------------------------------------
+class Calls:
+    """In place of an entry point: notes the descriptor and the stream of each call."""
+
+    def __init__(self):
+        self.seen = []
+
+    def __call__(self, desc, stream):
+        self.seen.append((desc, stream))
+        return 0
+
+
+@pytest.fixture
+def on_device_0(monkeypatch):
+    monkeypatch.setattr(block, "_device", lambda: 0)
+    monkeypatch.setattr(block, "_raw_stream", lambda dev: 77)
+
+
+def noted(obj):
+    obj._fn = Calls()
+    return obj, obj._fn.seen
+
+
+def product(T=5, E=128, K=8, ws=None, **kw):
+    """A call of from_product, as BatchedMoe.route makes it."""
+    router, seen = noted(ScoredRouter(E, K))
+    ws = OnGpu(lib().moe_route_workspace_bytes(E, T), dtype=torch.uint8) if ws is None else ws
+    a = dict(W=OnGpu(E, 2048), x=OnGpu(T, 2048), ids=OnGpu(T, K, dtype=torch.int32), w=OnGpu(T, K),
+             slots=OnGpu(T, K, dtype=torch.int32), workspace=ws, H=2048)
+    router.from_product(**{**a, **kw})
+    return seen
+
+
+def test_the_routers_product_checks_its_workspace(on_device_0):
+    size = lib().moe_route_workspace_bytes(128, 5)
+    assert size > 5 * 128 * 4
+    for ws in (None, OnGpu(size + 256, dtype=torch.uint8), OnGpu(size // 4), OnGpu(2, size // 8)):
+        assert len(product(ws=ws)) == 1
+    for ws in (OnGpu(size - 1, dtype=torch.uint8), OnGpu(size // 4 - 1), OnGpu(0), OnGpu(2 * size, dtype=torch.uint8)[::2],
+               OnGpu(size, dtype=torch.uint8, device=1), torch.zeros(size, dtype=torch.uint8)):
+        with pytest.raises(ValueError, match="workspace"):
+            product(ws=ws)
