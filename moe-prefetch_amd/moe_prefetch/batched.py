@@ -59,6 +59,8 @@ class BatchedMoe:
                 raise ValueError(f"the router has {router.K} of {router.E} experts, the layer {self.K} of {self.E}")
             if bias is not None or prior is not None or table is not None:
                 raise ValueError("a scored routing takes no bias, prior or table here")
+            if not all(hasattr(t, "data_ptr") for t in ((W, x) if logits is None else (logits,))):
+                raise ValueError("a scored routing takes logits, or W and x, as tensors")
             ids, w = self.ids[:n_tok], self.w[:n_tok]
             at = 0 if stream is None else stream          # as the calls below: None is the null stream
             if logits is not None:

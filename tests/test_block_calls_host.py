@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from moe_prefetch import MoeCache, block, lib
+from moe_prefetch.batched import BatchedMoe
 from moe_prefetch.block import ScoredRouter
 
 F32 = torch.float32
@@ -124,3 +125,29 @@ def test_the_routers_product_checks_its_workspace(on_device_0):
                OnGpu(size, dtype=torch.uint8, device=1), torch.zeros(size, dtype=torch.uint8)):
         with pytest.raises(ValueError, match="workspace"):
             product(ws=ws)
+
+
+def layer(T=5, E=128, K=8):
+    """A BatchedMoe without its device memory."""
+    m = BatchedMoe.__new__(BatchedMoe)
+    m.T, m.E, m.K, m.H = T, E, K, 2048
+    m.ids, m.w, m.slots = OnGpu(T, K, dtype=torch.int32), OnGpu(T, K), OnGpu(T, K, dtype=torch.int32)
+    m.route_ws = OnGpu(lib().moe_route_workspace_bytes(E, T), dtype=torch.uint8)
+    return m
+
+
+def test_a_scored_layer_names_the_operand_that_is_missing(on_device_0):
+    m, (router, seen) = layer(), noted(ScoredRouter(128, 8))
+    W, x, logits = OnGpu(128, 2048), OnGpu(5, 2048), OnGpu(5, 128)
+    m.route(5, W=W, x=x, router=router)
+    m.route(3, logits=logits[:3], router=router)
+    assert len(seen) == 2
+    for given in (dict(), dict(W=W), dict(x=x), dict(logits=4096), dict(W=4096, x=x), dict(W=W, x=4096)):
+        with pytest.raises(ValueError, match="takes logits, or W and x, as tensors"):
+            m.route(5, router=router, **given)
+    with pytest.raises(ValueError, match="takes logits, or W and x, as tensors"):
+        m.forward(OnGpu(5, 2048, dtype=torch.bfloat16), None, 0, 0, 0, 12, W=W, router=router)
+    for given in (dict(logits=logits[:3]), dict(W=W, x=x[:3]), dict(W=W[:64], x=x)):
+        with pytest.raises(ValueError):
+            m.route(5, router=router, **given)
+    assert len(seen) == 2
