@@ -57,11 +57,21 @@ def _vec(t, n, dtype, dev, what):
     return t.data_ptr()
 
 
+def _handle(stream, dev):
+    """The raw handle of a given stream: an int as it is, or a torch stream of the call's device."""
+    if isinstance(stream, int):
+        return stream
+    if stream.device.index != dev:
+        raise ValueError(f"the stream is of {stream.device}, the call's tensors on cuda:{dev}")
+    return stream.cuda_stream
+
+
 def _empty(shape, dtype, dev, stream):
     """Memory of the stream that the call runs on: an allocator block is safe to write on the stream it came from."""
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=dev)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, dev) if isinstance(stream, int) else stream):
+    handle = _handle(stream, dev)
+    with torch.cuda.stream(torch.cuda.ExternalStream(handle, dev) if stream is handle else stream):
         return torch.empty(shape, dtype=dtype, device=dev)
 
 
@@ -99,7 +109,7 @@ def _first(t, n, what):
 
 
 def _call(fn, desc, dev, stream, what):
-    raw = _raw_stream(dev) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
+    raw = _raw_stream(dev) if stream is None else _handle(stream, dev)
     if _device() == dev:
         rc = fn(desc, raw)
     else:

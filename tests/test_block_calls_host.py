@@ -5,7 +5,7 @@ import torch
 
 from moe_prefetch import MoeCache, block, lib
 from moe_prefetch.batched import BatchedMoe
-from moe_prefetch.block import ScoredRouter
+from moe_prefetch.block import BlockNorm, Sampler, ScoredRouter
 
 F32 = torch.float32
 
@@ -151,3 +151,36 @@ def test_a_scored_layer_names_the_operand_that_is_missing(on_device_0):
         with pytest.raises(ValueError):
             m.route(5, router=router, **given)
     assert len(seen) == 2
+
+
+class Stream:
+    def __init__(self, device, handle=55):
+        self.device, self.cuda_stream = torch.device("cuda", device), handle
+
+
+def test_a_stream_of_another_device_is_refused(on_device_0, monkeypatch):
+    # (the kernels would run there, on memory and with outputs of this one)
+    monkeypatch.setattr(block, "_empty", lambda shape, dtype, dev, stream: OnGpu(*shape, dtype=dtype))
+    calls = []
+    router, norm, sampler = ScoredRouter(64, 8), BlockNorm(64), Sampler(64)
+    for obj, args in ((router, (OnGpu(3, 64),)), (norm, (OnGpu(3, 64),)), (sampler, (OnGpu(3, 64), OnGpu(3)))):
+        obj, seen = noted(obj)
+        with pytest.raises(ValueError, match="stream is of cuda:1, the call's tensors on cuda:0"):
+            obj(*args, stream=Stream(1))
+        assert not seen
+        obj(*args, stream=Stream(0))
+        obj(*args, stream=66)
+        obj(*args)
+        assert [s for _, s in seen] == [55, 66, 77]
+        calls += seen
+    m, (router, seen) = layer(), noted(ScoredRouter(128, 8))
+    with pytest.raises(ValueError, match="stream is of cuda:1"):
+        m.route(5, W=OnGpu(128, 2048), x=OnGpu(5, 2048), router=router, stream=Stream(1))
+    m.route(5, W=OnGpu(128, 2048), x=OnGpu(5, 2048), router=router)
+    assert [s for _, s in seen] == [0]
+
+
+def test_outputs_are_not_allocated_on_a_refused_stream(on_device_0, monkeypatch):
+    monkeypatch.setattr(block.torch.cuda, "stream", lambda s: pytest.fail("entered"))
+    with pytest.raises(ValueError, match="stream is of cuda:1"):
+        Sampler(64)(OnGpu(3, 64), OnGpu(3), stream=Stream(1))
