@@ -186,6 +186,7 @@ struct moe_cache {
     moe_cache_config cfg{};
     bool host_only = false;            // device < 0: state machine only, no HIP calls
     std::vector<Layer> L;
+    int n_scored = 0;                  // layers that are scored
     int H = 0, I = 0, E = 0, K = 0;
     // tables: device copies and pinned host mirrors, [L][E]
     int32_t *d_tbl = nullptr, *h_tbl = nullptr;
@@ -1882,6 +1883,7 @@ int moe_cache_set_scoring(moe_cache *c, int layer, const moe_route_scored_desc *
     if (!c || layer < 0 || layer >= (int)c->L.size()) return fail(MOE_ERR_ARG, "bad arguments");
     Layer &ls = c->L[layer];
     if (!rule) {
+        c->n_scored -= ls.scored;
         ls.scored = false;
         return MOE_OK;
     }
@@ -1901,12 +1903,14 @@ int moe_cache_set_scoring(moe_cache *c, int layer, const moe_route_scored_desc *
             return fail(MOE_ERR_ARG, "moe_cache_set_scoring: the bias is on device %d, the cache on %d", at.device, c->cfg.device);
     }
     ls.rule = scored_rule(rule);
+    c->n_scored += !ls.scored;
     ls.scored = true;
     return MOE_OK;
 }
 
 // the launches of moe_decode_token and moe_decode_layer route by softmax and top-k
 static int softmax_only(const moe_cache *c) {
+    if (!c->n_scored) return MOE_OK;                  // (once a layer of every token: no walk over the layers)
     for (const Layer &ls : c->L)
         if (ls.scored) return fail(MOE_ERR_STATE, "layer %d routes by scores: decode it with moe_decode_batch", ls.il);
     return MOE_OK;

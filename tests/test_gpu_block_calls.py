@@ -73,3 +73,35 @@ def test_a_cache_reads_the_bias_it_was_given():
         del others
     finally:
         rig.close()
+
+
+def test_the_one_token_paths_come_back_with_the_last_scored_layer():
+    from gpu_rig import Rig
+    rig = Rig([40, 40], [_lib.TYPE_Q4K, _lib.TYPE_Q4K], T=1, steer=False, admit="window")
+    st = torch.cuda.current_stream().cuda_stream
+    x = rig.x.transpose(0, 1)[:, 0].contiguous()
+    out, want = torch.empty_like(x), torch.empty_like(x)
+    router = ScoredRouter(128, 8)
+    try:
+        def decodes():
+            try:
+                rig.cache.decode_token(x, out, stream=st)
+            except _lib.MoeError as e:
+                assert "moe_decode_batch" in str(e)
+                with pytest.raises(_lib.MoeError, match="moe_decode_batch"):
+                    rig.cache.decode_layer(0, x[0], out[0], stream=st)
+                return False
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            return True
+        rig.cache.decode_token(x, want, stream=st)
+        torch.cuda.synchronize()
+        for layer, rule, scored in ((0, None, 0), (0, router, 1), (0, router, 1), (1, router, 2), (0, None, 1), (0, None, 1),
+                                    (1, router, 1), (1, None, 0), (1, None, 0), (1, router, 1), (1, None, 0)):
+            rig.cache.set_scoring(layer, rule)
+            assert decodes() == (scored == 0), (layer, rule is not None)
+        with pytest.raises(_lib.MoeError):
+            rig.cache.set_scoring(0, ScoredRouter(128, 6))            # refused: counts for nothing
+        assert decodes()
+    finally:
+        rig.close()
