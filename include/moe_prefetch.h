@@ -42,7 +42,8 @@
  *                           renormalised or not and scaled (un-vendored upstream)
  *   moe_block_norm          the norm before ffn_gate_inp, the norm after the block, the residual add and its scale
  *                           (un-vendored upstream; the reference's lookahead names that norm, 0010:382-403)
- *   moe_sample              llama.cpp's sampler chain over one row of logits per sequence (un-vendored upstream)
+ *   moe_sample              the choice of the next token from a row of logits (un-vendored upstream, where the order of the
+ *                           cuts is the caller's; here temperature comes before them, see there)
  * No counterpart in the reference: moe_host_alloc/free (the reference pins the model buffer
  * through ggml's CUDA_Host buffer type), moe_synth_* (seeded synthetic weights and inputs).
  */
@@ -782,21 +783,23 @@ typedef struct {
 } moe_block_norm_desc;
 int moe_block_norm(const moe_block_norm_desc *d, void *stream);
 
-/* The next token of each row of logits, from a given uniform number u in [0, 1):
+/* The next token of each row of logits, from a given uniform number u in [0, 1), the temperature applied first:
  *   e_i = exp((l_i - max l) / temperature), the tokens in descending order of l_i, the lower index first on a tie
  *   top_k   the first top_k of them
  *   top_p   of those the shortest run from the front whose mass is at least top_p of theirs
  *   min_p   of those the ones with e_i >= min_p
  *   token   the first of what is left whose running mass exceeds u times the mass of what is left
  *   prob    its share of that mass
+ * (llama.cpp's default chain applies the temperature last: its top-p and min-p look at the probabilities of temperature
+ * 1.  The tokens kept are the same under a temperature of 1, and under any where top_k alone cuts; otherwise they differ.)
  * A temperature that is not above 0 takes the first of the order (prob 1).  top_k
  * outside 1..V-1, top_p not below 1 and min_p not above 0 cut nothing; a NaN among
  * them cuts nothing; the first of the order always stays.  Logits of -inf and NaN
  * are switched off; a row with nothing else gives token -1 and prob 0.  (Logits of
  * +inf share a row's whole mass.)  u of 1 and above counts as the largest number
  * below 1, u below 0 and NaN as 0.  Masses and their sums are computed in 64 bits, in an order that depends on
- * the row and where in 16 bytes it begins only: the same row gives the same token in any
- * batch. */
+ * the row and where in 16 bytes it begins only: the same row at the same place in 16 bytes gives the
+ * same token and the same prob in any batch. */
 #define MOE_SAMPLE_MAX_V 1000000
 #define MOE_SAMPLE_MAX_TOKENS 65535
 typedef struct {

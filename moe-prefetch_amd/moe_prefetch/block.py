@@ -300,7 +300,7 @@ class Sampler:
         [tokens] (the share of the kept mass that the token had).
 
         temperature, top_p, min_p (f32) and top_k (int32): a number for every row, a tensor [tokens], or None
-        (temperature 1, nothing cut).  A temperature of 0 takes the largest logit.
+        (temperature 1, nothing cut).  The temperature comes before the cuts; one of 0 takes the largest logit.
         """
         V = self.V
         T, ld, dev = _first(logits, V, "logits")

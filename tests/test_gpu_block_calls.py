@@ -6,9 +6,10 @@ import numpy as np
 import pytest
 import torch
 
+import block_examples as X
 import block_ref as R
 from moe_prefetch import MoeCache, _lib
-from moe_prefetch.block import ScoredRouter
+from moe_prefetch.block import BlockNorm, Sampler, ScoredRouter
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -24,6 +25,38 @@ def randn(g, *shape):
 
 def np64(t):
     return t.double().cpu().numpy()
+
+
+def f32(v):
+    return None if v is None else torch.tensor(v, dtype=torch.float32, device=DEV)
+
+
+# ---- examples worked by hand ----------------------------------------------------------
+# The logits are logarithms below 2.1 in size, rounded to f32 (2^-24 of that, twice as much at temperature 1/2): a mass is
+# off by 5 x 2^-24 of itself at most, a ratio of two sums of them by 10 x 2^-24, and the result is rounded once.
+@pytest.mark.parametrize("logits, K, rule, ids, w", X.ROUTE)
+def test_route_examples(logits, K, rule, ids, w):
+    got = ScoredRouter(len(logits), K, **{**rule, "bias": f32(rule.get("bias"))})(f32([logits]))
+    assert got[0][0].tolist() == ids
+    np.testing.assert_allclose(np64(got[1][0]), w, rtol=11 * 2.0 ** -24, atol=0)
+
+
+# (at most six roundings on the way from the inputs, which are exact, to r; twelve more to y, whose difference from the
+# mean may be an eighth of r: 8 x 6 + 12)
+@pytest.mark.parametrize("x, rows, gate, rule, y, r", X.NORM)
+def test_norm_examples(x, rows, gate, rule, y, r):
+    weights = {k: f32(rule.get(k)) for k in ("weight", "bias", "post_weight", "post_bias")}
+    got = BlockNorm(len(x), **{**rule, **weights, "eps": 0.0})(f32([x]), None if rows is None else f32([rows]), f32(gate)
+                                                               if rows is not None else None)
+    np.testing.assert_allclose(np64(got[0][0]), y, rtol=60 * 2.0 ** -24, atol=0)
+    np.testing.assert_allclose(np64(got[1][0]), x if r is None else r, rtol=6 * 2.0 ** -24, atol=0)
+
+
+@pytest.mark.parametrize("logits, u, rule, token, prob", X.SAMPLE)
+def test_sample_examples(logits, u, rule, token, prob):
+    got = Sampler(len(logits))(f32([logits]), f32([u]), **rule)
+    assert got[0].item() == token
+    np.testing.assert_allclose(got[1].item(), prob, rtol=11 * 2.0 ** -24, atol=0)
 
 
 # ---- a cache's scoring rule ---------------------------------------------------------
