@@ -138,3 +138,59 @@ def test_the_one_token_paths_come_back_with_the_last_scored_layer():
         assert decodes()
     finally:
         rig.close()
+
+
+# ---- a row and its batch ------------------------------------------------------------
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [30011, 901])
+def test_a_row_gives_the_same_bits_in_any_batch(V, dt):
+    # a row copied to the same place in 16 bytes, alone and among others: odd rows next to each other begin at every place
+    T, g = 64, gen(3)
+    logits = ((0.3 + 2.0 * torch.rand(T, 1, generator=g, device=DEV)) * randn(g, T, V)).to(dt)
+    u = torch.rand(T, generator=g, device=DEV)
+    rows = list(range(0, T, 5)) + [T - 1]
+    where = [logits[t].data_ptr() % 16 // logits.element_size() for t in rows]
+    assert len(set(where)) == 16 // logits.element_size()
+    for cut in (dict(), dict(top_k=300), dict(top_k=1000, top_p=0.7), dict(top_k=20000, min_p=0.01), dict(top_p=0.9),
+                dict(temperature=3.0), dict(temperature=0.0)):
+        want = Sampler(V)(logits, u, **cut)
+        for t, m in zip(rows, where):
+            for n, i in ((1, 0), (7, 3)):
+                ld = (V + 31) // 16 * 16
+                batch = randn(g, n, ld).to(dt)[:, m:m + V]
+                batch[i] = logits[t]
+                assert batch[i].data_ptr() % 16 == logits[t].data_ptr() % 16
+                got = Sampler(V)(batch, u[t:t + 1].expand(n).contiguous(), **cut)
+                assert got[0][i] == want[0][t] and got[1][i] == want[1][t], (cut, t, n)
+
+
+# ---- bounds of the kernels' own arithmetic ----------------------------------------------
+@pytest.mark.parametrize("H", [2048, 2047, 8192, 8191, 16384, 16383])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_norm_within_the_kernels_own_sums(kind, H, monkeypatch):
+    # a sum over a row is a chain of at most 16 terms a thread, six steps of a wave and 16 waves: 38 roundings
+    unit = R._unit
+    monkeypatch.setattr(R, "_unit", lambda *a: unit(*a[:-1], 38))
+    g = gen(4)
+    x, b = 2.0 * randn(g, 3, H) + 0.3, randn(g, 3, 2, H)
+    kw = dict(weight=1.0 + 0.2 * randn(g, H), bias=randn(g, H), post_weight=1.0 + 0.2 * randn(g, H), post_bias=randn(g, H),
+              kind=kind, scale=0.3)
+    got = BlockNorm(H, **kw)(x, b)
+    y, r, e_y, e_r = R.block_norm(np64(x), np64(b), post=True, **{k: np64(v) if torch.is_tensor(v) else v for k, v in kw.items()})
+    for t, want, err in ((got[0], y, e_y), (got[1], r, e_r)):
+        assert (np.abs(np64(t) - want) <= err + R.U * (np.abs(want) + err)).all()
+
+
+@pytest.mark.parametrize("T, V", [(3, 1000000), (5, 151936), (9, 32003), (9, 1000)])
+@pytest.mark.parametrize("spread", [0.3, 2.0])
+def test_sample_probabilities_to_half_a_step(T, V, spread):
+    # a mass is a 64-bit number, or an integer of which the row's whole has 62 bits: half of one a token, V 2^-62 of the
+    # sum (kept tokens are the largest).  Sums in 64 bits, here and in the reference, V 2^-53 each.  The result is rounded once.
+    g = gen(V + T)
+    logits = spread * randn(g, T, V)
+    u = torch.rand(T, generator=g, device=DEV)
+    for cut in (dict(), dict(top_p=0.9), dict(min_p=0.2), dict(temperature=2.0, top_p=0.5), dict(top_k=60)):
+        tokens, probs = R.sample(np64(logits), np64(u), **cut)
+        got = Sampler(V)(logits, u, **cut)
+        np.testing.assert_array_equal(got[0].cpu().numpy(), tokens)
+        np.testing.assert_allclose(np64(got[1]), probs, rtol=R.U * 1.001 + V * (2.0 ** -62 + 2.0 ** -52), atol=0)
