@@ -10,8 +10,10 @@
 // taken about the mean, in a second pass over the registers: sums of squares lose
 // the small variance of a row far from 0.
 // Large calls are bound by memory: 4,096 tokens of eight f32 rows, hidden 2048,
-// bf16, 318 MB in 61 us (5.2 TB/s; a copy of 2 GiB reaches 4.9), 8,191 bf16 rows alone 67 MB in
-// 13.6 (4.9).  Small ones by the launch and two trips to memory: one token 3.4 us.
+// bf16, 319 MB in 60 to 62 us (5.2 TB/s; a copy of 2 GiB reaches 4.9, a read 6.3), 8,191 bf16 rows alone 67 MB in
+// 15.7 (4.3; 13.6 where the same rows are read each time).  Wide rows with both norms and a full gate stay further
+// from it: 4,096 of 4,096, fp16 layer norms, 168 MB in 59 (2.8), of 4,095 in 69 (2.4).  Small ones are bound by the
+// launch and two trips to memory: one token 3.5 us.
 #include <hip/hip_runtime.h>
 
 #include "mp_device.h"
@@ -197,7 +199,7 @@ static hipError_t launch_norm_n(const NormArgs &a, hipStream_t st) {
 }
 template <int T, int B>
 static hipError_t launch_norm_b(const NormArgs &a, hipStream_t st) {
-    // Eight elements a thread, up to 1,024 threads, then sixteen.  8,191 rows of 2048 bf16: 13.6 us alone, 29 with a bf16
+    // Eight elements a thread, up to 1,024 threads, then sixteen.  8,191 rows of 2048 bf16, the same each time: 13.6 us alone, 29 with a bf16
     // branch and 33 with an f32 one; of four elements, twice the waves with half the bytes on their way, 20.7, 38 and 37.
     // A row shorter than eight is read by elements.
     static_assert(MAX_NORM_H <= 2 * 8 * 64 * NORM_MAX_WAVES, "two vectors a thread");

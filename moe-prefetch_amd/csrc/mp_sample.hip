@@ -13,9 +13,13 @@
 //   3 rest    rows that step 2 could not decide (a flat distribution: the cut or the
 //             draw lies behind the candidates): a histogram of counts and masses by
 //             several workgroups, the last of which reads the one bin that matters.
-//             Rows of one value or nearly so end in a radix search.
-// 256 rows of 151,936 bf16 logits (78 MB, 16 us at the rate of a large copy), each with cuts of its own: 36 us + 14 us,
-// and 30 more if a row or a few need step 3 (they go at once); under top-k alone 33 in all; one row 15.
+//             A bin of more than 2,048 tokens (many equal 16-bit logits, or a row nearly flat) ends in a radix search.
+// 256 rows of 151,936 bf16 logits (78 MB, 12 us at the rate of a large read), each with cuts of its own: 36 us + 14 us,
+// and about 30 more if a row or a few need step 3; under top-k alone 33 in all; one row 15.
+// Step 3 is slow where many rows need it, one workgroup ending each: rows under a top-k of 1,000 take 44 us (one row), 79
+// (16), 271 (64) and 1,100 (256) in all, under top-p of 0.9 over normal logits of deviation 1 68, 115, 400 and 1,570.  The
+// radix search more so: under top-p of 0.9 over bf16 logits of mean 20 and deviation 1.5 0.82 ms (one row) and 12.3 (256),
+// of one value only 0.94 and 15, and those under top-k and top-p both 2.5 and 39.
 #include <hip/hip_runtime.h>
 
 #include "mp_device.h"
@@ -816,9 +820,10 @@ struct RestRow {
 
 // A fixed number of workgroups take the parts of the undecided rows in turn; the one
 // that finishes a row's last part decides the row.  No workgroup waits for another.
-// A row of 151,936 takes 30 to 33 us however many there are up to 16, all latency: the histogram 4.5 (16 parts), its
-// sums to memory 3 and back 3, and a bin's tokens found, gathered and sorted in up to 11, for the cut and for the draw;
-// 6 less where the candidates hold all of the bin, as they do for most draws.  (Reading the bins of both in one
+// One row of 151,936 takes 30 us where its bins are small (top-k 1,000 over a peaked row) to 52 (top-p over a broad one), all
+// latency: the histogram 4.5 (16 parts), its sums to memory 3 and back 3, and a bin's tokens found, gathered and
+// sorted in 11 and more, for the cut and for the draw; 6 less where the candidates hold all of the bin, as they do for
+// most draws.  16 rows take twice that, 64 rows 256 us.  (Reading the bins of both in one
 // pass over the row gained 1 us of 54 and was not kept.)
 template <int T>
 __global__ __launch_bounds__(SMP_THREADS) void sample_rest_kernel(SampleArgs a) {
@@ -1195,7 +1200,7 @@ struct SamplePlan {
 // `want` candidates of a slice, 300 to 600 of a row: enough for a top-k of 200 and most cuts by mass, and few enough for one
 // wave's registers.  Half as many: 693 us against 80 for 256 rows of 151,936 with cuts of their own (top-k up to 200), whose
 // undecided ones fill step 3; twice as many: 51 against 15 for one row under top-k, whose candidates do not fit.
-// A row of up to 1,000 is kept whole: it needs no step 3.
+// A row of up to 1,000 is kept whole: it needs no step 3 but for a logit of +inf.
 static SamplePlan sample_plan(int V) {
     SamplePlan p;
     p.slices = (V + 7 + SLICE - 1) / SLICE;           // (7: a row may begin inside 16 bytes)

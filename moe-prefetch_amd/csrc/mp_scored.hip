@@ -7,10 +7,11 @@
 // group's, has to be that of the definition however near they are.  The K best
 // come out in K rounds of a wave maximum over the lanes' best; a round compares the
 // upper words and looks at the lower ones only where two lanes agree in them.
-// One token of 256 experts in 8 groups, 8 chosen: 4.6 us, launch and latency.  8,191
-// of them: 16 us for 8.9 MB (1.8 at the rate of a large copy): the instructions of
-// eight waves a SIMD, of the launch's ~13 us about 5 for the scores in f64, 3 for the groups and 4.5
-// for the rounds (K = 1: 8.2 in all).
+// One token of 256 experts in 8 groups, 8 chosen: 4.7 us, launch and latency.  8,191
+// of them: 15 us a call among others for 8.9 MB (1.4 at the rate of a large read), of which the instructions of
+// eight waves a SIMD are 13.3: about 5 for the scores in f64, 3 for the groups and 4.5
+// for the rounds (K = 1: 8.2 us a call).  512 experts: 7.9 us one token, 33 for 8,191; 1,024, whose lanes order sixteen
+// values each, 28 and 137.
 #include <hip/hip_runtime.h>
 
 #include "mp_device.h"
@@ -49,7 +50,9 @@ __device__ inline double exp_d(double x) {
     const double m = fma(x, 1.4426950408889634074, MAGIC);
     const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, m);
     const double f = m - MAGIC;
-    const double r = fma(f, -1.9082149292705877e-10, fma(f, -0.693147180369123816490, x));   // ln 2 in two parts
+    // ln 2 in two parts, the first so short that its product with f is exact (Cody and Waite, Software Manual for the
+    // Elementary Functions, 1980)
+    const double r = fma(f, -1.9082149292705877e-10, fma(f, -0.693147180369123816490, x));
     double p = 1.0 / 6227020800.0;
     p = fma(p, r, 1.0 / 479001600.0);
     p = fma(p, r, 1.0 / 39916800.0);
@@ -261,7 +264,7 @@ __global__ __launch_bounds__(64 * SCORED_WAVES) void route_scored_kernel(ScoredA
 template <int T, int NV>
 static hipError_t launch_scored_n(ScoredArgs a, hipStream_t st) {
     a.vec = a.E % NV == 0;
-    // a group of whole lanes is reduced by DPP, others one to a lane out of LDS (8 groups of 32: 16 us for 8,191 tokens; of 25: 17)
+    // a group of whole lanes is reduced by DPP, others one to a lane out of LDS (8 groups of 32: 15 us a call for 8,191 tokens; of 25: 17)
     const int n = a.E / a.groups, lanes = n / NV;
     a.group_lanes = n % NV == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
     hipLaunchKernelGGL((route_scored_kernel<T, NV>), dim3((unsigned)((a.n_tok + SCORED_WAVES - 1) / SCORED_WAVES)),
