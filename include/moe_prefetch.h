@@ -791,7 +791,7 @@ int moe_block_norm(const moe_block_norm_desc *d, void *stream);
  *   token   the first of what is left whose running mass exceeds u times the mass of what is left
  *   prob    its share of that mass
  * (llama.cpp's default chain applies the temperature last: its top-p and min-p look at the probabilities of temperature
- * 1.  The tokens kept are the same under a temperature of 1, and under any where top_k alone cuts; otherwise they differ.)
+ * 1.  The tokens kept are the same under a temperature of 1, and under any where top_k alone cuts; otherwise they may differ.)
  * A temperature that is not above 0 takes the first of the order (prob 1).  top_k
  * outside 1..V-1, top_p not below 1 and min_p not above 0 cut nothing; a NaN among
  * them cuts nothing; the first of the order always stays.  Logits of -inf and NaN

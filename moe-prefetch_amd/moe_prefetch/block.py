@@ -157,7 +157,7 @@ class ScoredRouter:
         moe_route_workspace_bytes() at least."""
         T, _, dev = _first(x, H, "x")
         need = lib().moe_route_workspace_bytes(self.E, T)
-        if workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
+        if workspace.nbytes < need or not workspace.is_contiguous():
             raise ValueError(f"workspace must be contiguous and of {need} bytes at least, not {tuple(workspace.shape)} of "
                              f"{workspace.dtype}")
         if workspace.get_device() != dev:
