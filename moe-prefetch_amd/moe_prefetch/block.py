@@ -197,7 +197,8 @@ class BlockNorm:
     """r = x + scale * gate * post_norm(sum of the branch rows);  y = norm(r).
 
     weight, bias: of the norm before the next block; post_weight, post_bias: of the norm after this block, which
-    is there if post (by default: if one of them is given).  All [hidden], of one dtype: f32 or x's.  kind "rms" or "layer";
+    is there if post (by default: if one of them is given).  All [hidden], of one dtype: f32 or x's; read at each call from
+    the memory that they have now (a parameter whose data is exchanged takes another BlockNorm).  kind "rms" or "layer";
     weight_offset is added to the given weights (1 for weights stored as their distance from 1).
     """
 
@@ -211,7 +212,8 @@ class BlockNorm:
         self.post = int((post_weight is not None or post_bias is not None) if post is None else bool(post))
         if not self.post and (post_weight is not None or post_bias is not None):
             raise ValueError("post-norm weights without a post-norm")
-        self.weights = (weight, bias, post_weight, post_bias)
+        # aliases: they keep the memory whose addresses the calls hand on, also if a parameter's data is exchanged
+        self.weights = tuple(None if t is None else t.detach() for t in (weight, bias, post_weight, post_bias))
         given = [t for t in self.weights if t is not None]
         if len({t.dtype for t in given}) > 1:
             raise ValueError("the weights must be of one dtype")

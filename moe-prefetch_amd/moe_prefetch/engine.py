@@ -194,7 +194,7 @@ class MoeCache:
             if bias is not None and self.device >= 0 and bias.get_device() != self.device:
                 raise ValueError(f"the router's bias is on {bias.device}, the cache on cuda:{self.device}")
         check(lib().moe_cache_set_scoring(self.h, layer, None if rule is None else ctypes.byref(rule)), "set_scoring")
-        self._scoring[layer] = bias
+        self._scoring[layer] = None if bias is None else bias.detach()    # an alias: keeps the memory at that address
 
     def lookup(self, layer):
         v = _lib.LayerView()

@@ -10,21 +10,29 @@ from moe_prefetch.block import BlockNorm, Sampler, ScoredRouter
 F32 = torch.float32
 
 
+class Memory:
+    """What a tensor's address points to."""
+
+
 class OnGpu:
-    """A tensor's shape, strides and dtype, said to be on cuda:<device> at `at`."""
+    """A tensor's shape, strides and dtype, said to be on cuda:<device> at `at`, in memory that its aliases share."""
 
     is_cuda = True
 
     def __init__(self, *shape, dtype=F32, device=0, at=4096):
         self._t, self._at, self.device = torch.empty(shape, dtype=dtype, device="meta"), at, torch.device("cuda", device)
+        self.memory = Memory()
 
     def __getattr__(self, name):
         return getattr(self._t, name)
 
     def __getitem__(self, rows):
         t = OnGpu(dtype=self.dtype, device=self.device.index, at=self._at)
-        t._t = self._t[rows]
+        t._t, t.memory = self._t[rows], self.memory
         return t
+
+    def detach(self):
+        return self[...]
 
     def get_device(self):
         return self.device.index
@@ -68,15 +76,16 @@ def test_a_cache_keeps_the_bias_that_it_reads(cache):
     import gc
     import weakref
     router = ScoredRouter(128, 8, bias=OnGpu(128))
-    given = weakref.ref(router.bias)
+    given = weakref.ref(router.bias.memory)
     cache.set_scoring(0, router)
+    router.bias.memory = Memory()                     # as an assignment to a tensor's data
     router.bias = OnGpu(128, at=8192)                 # of the router's own calls from here on
     gc.collect()
     assert given() is not None
     cache.set_scoring(0, router)
     gc.collect()
     assert given() is None
-    given = weakref.ref(router.bias)
+    given = weakref.ref(router.bias.memory)
     cache.set_scoring(0, None)
     del router
     gc.collect()
@@ -184,3 +193,19 @@ def test_outputs_are_not_allocated_on_a_refused_stream(on_device_0, monkeypatch)
     monkeypatch.setattr(block.torch.cuda, "stream", lambda s: pytest.fail("entered"))
     with pytest.raises(ValueError, match="stream is of cuda:1"):
         Sampler(64)(OnGpu(3, 64), OnGpu(3), stream=Stream(1))
+
+
+def test_a_norm_keeps_the_memory_of_its_weights():
+    import gc
+    import weakref
+    given = [OnGpu(64) for _ in range(4)]
+    norm = BlockNorm(64, *given)
+    held = [weakref.ref(t.memory) for t in given]
+    for t in given:
+        t.memory = Memory()                           # as an assignment to a parameter's data: the address stays the norm's
+    del given, t
+    gc.collect()
+    assert all(h() is not None for h in held)
+    del norm
+    gc.collect()
+    assert all(h() is None for h in held)

@@ -194,3 +194,18 @@ def test_sample_probabilities_to_half_a_step(T, V, spread):
         got = Sampler(V)(logits, u, **cut)
         np.testing.assert_array_equal(got[0].cpu().numpy(), tokens)
         np.testing.assert_allclose(np64(got[1]), probs, rtol=R.U * 1.001 + V * (2.0 ** -62 + 2.0 ** -52), atol=0)
+
+
+def test_a_norm_reads_the_memory_it_was_given():
+    # a parameter's data is exchanged and its first memory offered to others: the norm still reads that
+    H, g = 2048, gen(5)
+    first = 1.0 + 0.2 * randn(g, H)
+    p = torch.nn.Parameter(first.clone())
+    norm = BlockNorm(H, weight=p)
+    p.data = torch.zeros(H, device=DEV)
+    others = [torch.full((H,), 9.0 - i, device=DEV) for i in range(64)]
+    x = randn(g, 7, H)
+    assert torch.equal(norm(x)[0], BlockNorm(H, weight=first)(x)[0])
+    norm.weights[0].zero_()                           # a change in place reaches it
+    assert (norm(x)[0] == 0).all()
+    del others
