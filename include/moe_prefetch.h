@@ -44,6 +44,8 @@
  *                           (un-vendored upstream; the reference's lookahead names that norm, 0010:382-403)
  *   moe_sample              the choice of the next token from a row of logits (un-vendored upstream, where the order of the
  *                           cuts is the caller's; here temperature comes before them, see there)
+ *   moe_fp8_layer           build_moe_ffn over experts of e4m3 weights with a scale for each block of 128 x 128 (no
+ *                           ggml type has them); moe_fp8_product and moe_fp8_quantize are its parts
  * No counterpart in the reference: moe_host_alloc/free (the reference pins the model buffer
  * through ggml's CUDA_Host buffer type), moe_synth_* (seeded synthetic weights and inputs).
  */
@@ -821,6 +823,90 @@ typedef struct {
 } moe_sample_desc;
 size_t moe_sample_workspace_bytes(int n_tok, int V);
 int moe_sample(const moe_sample_desc *d, void *stream);
+
+/* ---- e4m3 weights with a scale for each block ----------------------------------
+ * Weights of 8-bit floating-point numbers (e4m3: four exponent bits, three of
+ * mantissa, no infinities, NaN 0x7f and 0xff) with one f32 scale for each block of
+ * 128 x 128, resident in HBM: a quantizer, products, and a layer of experts
+ * beside moe_grouped_experts'.  Rows of K values fall into ceil(K / 128) blocks,
+ * the last one as short as it comes out; likewise the rows of a weight.
+ * The calls launch on `stream`, allocate nothing and keep nothing between calls:
+ * calls on several streams or threads at once and calls captured into HIP graphs
+ * are fine as long as their outputs and workspaces are apart.  Pointers are of the
+ * current device.  Strides count elements and are at least the row's length; no
+ * alignment is asked for beyond the element's own, but codes whose rows begin on 16
+ * bytes are read faster.  Inputs and outputs do not overlap.  Inference only. */
+#define MOE_DTYPE_E4M3 3           /* of the x of moe_fp8_product only */
+#define MOE_FP8_BLOCK 128
+#define MOE_FP8_MAX_DIM (1 << 18)
+
+/* q = e4m3(x / s), to the nearest, ties to even, for blocks of 128 columns and
+ * `rows` rows; s = 2^e with e the least integer, from -126 on, such that the
+ * largest finite |x| of the block is at most 448 s.  NaN and infinities become NaN. */
+typedef struct {
+    const void *x;             /* dev [n_tok][K], MOE_DTYPE_F32, BF16 or F16, rows x_stride apart */
+    int64_t x_stride;
+    int32_t x_type;
+    int32_t rows;              /* 1 (activations) or 128 (weights) */
+    int32_t n_tok, K;          /* n_tok 0..MOE_BLOCK_MAX_TOKENS, K 1..MOE_FP8_MAX_DIM */
+    uint8_t *q;                /* dev out [n_tok][K] */
+    int64_t q_stride;
+    float *scale;              /* dev out [ceil(n_tok / rows)][ceil(K / 128)] */
+    int64_t scale_stride;
+} moe_fp8_quantize_desc;
+int moe_fp8_quantize(const moe_fp8_quantize_desc *d, void *stream);
+
+typedef struct {               /* [E][N][K] codes (E: of a layer's experts) */
+    const uint8_t *q;
+    int64_t stride, expert_stride;
+    const float *scale;        /* [E][ceil(N / 128)][ceil(K / 128)] */
+    int64_t scale_stride, scale_expert_stride;
+} moe_fp8_weight;
+
+/* y[m][n] = sum over the blocks b of K of xs[m][b] * ws[n / 128][b] * (xq[m] . wq[n] over the block),
+ * a block's dot and the sum over the blocks in f32, one rounding to y's type.  xq and xs are x and x_scale if x is
+ * e4m3, else x quantized as moe_fp8_quantize does (rows 1). */
+typedef struct {
+    const void *x;             /* dev [n_tok][K], MOE_DTYPE_*, rows x_stride apart */
+    int64_t x_stride;
+    const float *x_scale;      /* dev [n_tok][ceil(K / 128)], for e4m3 x */
+    int64_t x_scale_stride;
+    int32_t x_type;
+    int32_t n_tok, N, K;       /* n_tok 0..MOE_BLOCK_MAX_TOKENS, N and K 1..MOE_FP8_MAX_DIM */
+    moe_fp8_weight weight;     /* (no expert strides) */
+    void *y;                   /* dev out [n_tok][N], rows y_stride apart */
+    int64_t y_stride;
+    int32_t y_type;            /* MOE_DTYPE_F32, BF16 or F16 */
+    void *workspace;           /* dev, moe_fp8_product_workspace_bytes(), 16-byte aligned; NULL if that is 0 */
+} moe_fp8_product_desc;
+size_t moe_fp8_product_workspace_bytes(int n_tok, int N, int K, int x_type);
+int moe_fp8_product(const moe_fp8_product_desc *d, void *stream);
+
+/* A layer of E experts, K for each token:
+ *   ids, w   moe_route_scored's of route.logits, or given
+ *   h        silu(gate_e . x) * (up_e . x), products as moe_fp8_product's, silu(g) = g / (1 + exp(-g))
+ *   out[t]   sum over k, in order, of w[t][k] * (down_e . h), e = ids[t][k]
+ * with h f32 until it is quantized for the product with down.  A pair whose id is outside [0, E) adds nothing;
+ * an id may stand twice for one token.  n_tok * K <= 65535. */
+#define MOE_FP8_MAX_E 256
+typedef struct {
+    const void *x;             /* dev [n_tok][H], MOE_DTYPE_F32, BF16 or F16, rows x_stride apart */
+    int64_t x_stride;
+    int32_t x_type;
+    int32_t n_tok, E, K, H, I; /* E 1..MOE_FP8_MAX_E, K 1..MOE_ROUTE_SCORED_MAX_K, H and I 1..MOE_FP8_MAX_DIM */
+    moe_fp8_weight gate, up;   /* dev [E][I][H] */
+    moe_fp8_weight down;       /* dev [E][H][I] */
+    int32_t *ids;              /* dev [n_tok][K]: out with route.logits, else in */
+    float *w;                  /* dev [n_tok][K]: as ids */
+    void *out;                 /* dev out [n_tok][H], rows out_stride apart */
+    int64_t out_stride;
+    int32_t out_type;          /* MOE_DTYPE_F32, BF16 or F16 */
+    void *workspace;           /* dev, moe_fp8_layer_workspace_bytes(), 16-byte aligned */
+    moe_route_scored_desc route;   /* the rule, and logits [n_tok][E] or NULL; E, K and n_tok are the layer's, ids, w, W and x
+                                      not read */
+} moe_fp8_layer_desc;
+size_t moe_fp8_layer_workspace_bytes(int n_tok, int E, int K, int H, int I);
+int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream);
 
 /* ---- slab pool behind the Python ExpertCache ------------------------------- */
 typedef struct moe_pool moe_pool;

@@ -359,6 +359,51 @@ struct SampleArgs {
 size_t sample_ws_bytes(int n_tok, int V);
 hipError_t launch_sample(SampleArgs a, void *ws, hipStream_t st);
 
+// e4m3 weights with block scales (mp_fp8.hip); strides of codes count bytes, those of scales elements
+constexpr int FP8_BLOCK = 128;
+struct Fp8QuantArgs {
+    const void *x;
+    int64_t ldx;
+    int x_type, rows, n_tok, K;   // rows of a block: 1 or FP8_BLOCK
+    uint8_t *q;
+    int64_t ldq;
+    float *s;
+    int64_t lds;
+};
+hipError_t launch_fp8_quant(const Fp8QuantArgs &a, hipStream_t st);
+struct Fp8Mat {                   // [E][N][K] codes, [E][N / 128][K / 128] scales
+    const uint8_t *w;
+    int64_t ld, ex;
+    const float *s;
+    int64_t sld, sex;
+};
+struct Fp8Args {
+    Fp8Mat m[2];                  // the weight, or gate and up
+    int gated;                    // y = up * silu(gate)
+    const uint8_t *x;             // [rows][K] codes
+    int64_t ldx;
+    const float *xs;              // [rows][K / 128]
+    int64_t ldxs;
+    const int32_t *offsets;       // [E + 1] and
+    const int32_t *perm;          // [pairs] from the dispatch, or null: one expert, rows 0 .. M - 1
+    int top;                      // the row of x of pair i is i / top; 0: its place in the dispatch
+    int M, N, K, E;               // M: rows without a dispatch, else the most pairs that there may be
+    const float *pair_w;          // weights of the pairs: y is in the order of pairs and scaled, or null: in that of the dispatch
+    void *y;
+    int64_t ldy;
+    int y_type;
+};
+hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st);
+struct Fp8CombineArgs {
+    const float *rows;            // [n_tok * K][H]
+    const int32_t *ids;
+    int n_tok, K, E, H;
+    void *out;
+    int64_t ldo;
+    int out_type;
+};
+hipError_t launch_fp8_combine(const Fp8CombineArgs &a, hipStream_t st);
+
 // ev (optional): [logits start, logits end, select start, select end]
 hipError_t launch_route(const RouteLaunch &l, hipStream_t st, hipEvent_t *ev = nullptr);
 hipError_t launch_experts(const ExpertArgs &a, hipStream_t st);

@@ -4199,6 +4199,175 @@ int moe_sample(const moe_sample_desc *d, void *stream) {
     return MOE_OK;
 }
 
+// ---- e4m3 weights with block scales ---------------------------------------------
+static int64_t fp8_blocks(int64_t n) { return (n + mp::FP8_BLOCK - 1) / mp::FP8_BLOCK; }
+static bool fp8_dim(int n) { return n >= 1 && n <= MOE_FP8_MAX_DIM; }
+// a piece of a workspace, 256-byte aligned
+static size_t take(size_t &at, size_t bytes) {
+    const size_t o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+}
+static_assert(MOE_FP8_BLOCK == mp::FP8_BLOCK && MOE_FP8_MAX_E == mp::MAX_E, "header and library disagree");
+
+int moe_fp8_quantize(const moe_fp8_quantize_desc *d, void *stream) {
+    if (!d) return fail(MOE_ERR_ARG, "moe_fp8_quantize: null argument");
+    if (d->n_tok < 0 || d->n_tok > MOE_BLOCK_MAX_TOKENS)
+        return fail(MOE_ERR_ARG, "moe_fp8_quantize: n_tok %d out of range", d->n_tok);
+    if (!fp8_dim(d->K)) return fail(MOE_ERR_ARG, "moe_fp8_quantize: K %d must be 1..%d", d->K, MOE_FP8_MAX_DIM);
+    if (!dtype_ok(d->x_type)) return fail(MOE_ERR_ARG, "moe_fp8_quantize: x_type %d unsupported", d->x_type);
+    if (d->rows != 1 && d->rows != MOE_FP8_BLOCK)
+        return fail(MOE_ERR_ARG, "moe_fp8_quantize: blocks of %d rows: 1 or %d", d->rows, MOE_FP8_BLOCK);
+    if (d->n_tok == 0) return MOE_OK;
+    if (!d->x || !d->q || !d->scale) return fail(MOE_ERR_ARG, "moe_fp8_quantize: null argument");
+    if (d->x_stride < d->K || d->q_stride < d->K || d->scale_stride < fp8_blocks(d->K))
+        return fail(MOE_ERR_ARG, "moe_fp8_quantize: a row stride below the row's length");
+    if (!aligned_to(d->x, d->x_type) || (uintptr_t)d->scale % 4) return fail(MOE_ERR_ARG, "moe_fp8_quantize: misaligned pointer");
+    const mp::Fp8QuantArgs a{d->x, d->x_stride, d->x_type, d->rows, d->n_tok, d->K, d->q, d->q_stride, d->scale, d->scale_stride};
+    HIPCHK(mp::launch_fp8_quant(a, (hipStream_t)stream));
+    return MOE_OK;
+}
+
+static int fp8_weight_check(const char *call, const char *what, const moe_fp8_weight &m, int E, int N, int K) {
+    if (!m.q || !m.scale) return fail(MOE_ERR_ARG, "%s: null argument (%s)", call, what);
+    if ((N > 1 && m.stride < K) || (fp8_blocks(N) > 1 && m.scale_stride < fp8_blocks(K)) || m.stride < 0 || m.scale_stride < 0)
+        return fail(MOE_ERR_ARG, "%s: a row stride of %s below the row's length", call, what);
+    if (E > 1 && (m.expert_stride < 0 || m.scale_expert_stride < 0))
+        return fail(MOE_ERR_ARG, "%s: an expert stride of %s below 0", call, what);
+    if ((uintptr_t)m.scale % 4) return fail(MOE_ERR_ARG, "%s: misaligned pointer (%s)", call, what);
+    return MOE_OK;
+}
+static mp::Fp8Mat fp8_mat(const moe_fp8_weight &m) {
+    return {m.q, m.stride, m.expert_stride, m.scale, m.scale_stride, m.scale_expert_stride};
+}
+
+struct Fp8Rows {                                       // quantized rows in a workspace
+    int64_t ld, nb;
+    size_t q, s;
+};
+static Fp8Rows fp8_rows(size_t &at, int64_t rows, int K) {
+    Fp8Rows r{(K + 15) / 16 * 16, fp8_blocks(K), 0, 0};
+    r.q = take(at, (size_t)(rows * r.ld));
+    r.s = take(at, (size_t)(rows * r.nb) * 4);
+    return r;
+}
+
+size_t moe_fp8_product_workspace_bytes(int n_tok, int N, int K, int x_type) {
+    if (n_tok < 1 || n_tok > MOE_BLOCK_MAX_TOKENS || !fp8_dim(N) || !fp8_dim(K) || x_type == MOE_DTYPE_E4M3) return 0;
+    size_t at = 0;
+    fp8_rows(at, n_tok, K);
+    return at;
+}
+
+int moe_fp8_product(const moe_fp8_product_desc *d, void *stream) {
+    if (!d) return fail(MOE_ERR_ARG, "moe_fp8_product: null argument");
+    if (d->n_tok < 0 || d->n_tok > MOE_BLOCK_MAX_TOKENS)
+        return fail(MOE_ERR_ARG, "moe_fp8_product: n_tok %d out of range", d->n_tok);
+    if (!fp8_dim(d->N) || !fp8_dim(d->K))
+        return fail(MOE_ERR_ARG, "moe_fp8_product: a weight of %d x %d: each must be 1..%d", d->N, d->K, MOE_FP8_MAX_DIM);
+    const bool e4m3 = d->x_type == MOE_DTYPE_E4M3;
+    if (!e4m3 && !dtype_ok(d->x_type)) return fail(MOE_ERR_ARG, "moe_fp8_product: x_type %d unsupported", d->x_type);
+    if (!dtype_ok(d->y_type)) return fail(MOE_ERR_ARG, "moe_fp8_product: y_type %d unsupported", d->y_type);
+    const int r = fp8_weight_check("moe_fp8_product", "weight", d->weight, 1, d->N, d->K);
+    if (r != MOE_OK) return r;
+    if (d->n_tok == 0) return MOE_OK;
+    if (!d->x || !d->y || (e4m3 && !d->x_scale)) return fail(MOE_ERR_ARG, "moe_fp8_product: null argument");
+    if (d->x_stride < d->K || d->y_stride < d->N || (e4m3 && d->x_scale_stride < fp8_blocks(d->K)))
+        return fail(MOE_ERR_ARG, "moe_fp8_product: a row stride below the row's length");
+    if ((!e4m3 && !aligned_to(d->x, d->x_type)) || (e4m3 && (uintptr_t)d->x_scale % 4) || !aligned_to(d->y, d->y_type))
+        return fail(MOE_ERR_ARG, "moe_fp8_product: misaligned pointer");
+    if (!e4m3 && (!d->workspace || (uintptr_t)d->workspace % 16))
+        return fail(MOE_ERR_ARG, "moe_fp8_product: workspace must be given and 16-byte aligned");
+    mp::Fp8Args a{};
+    a.m[0] = fp8_mat(d->weight);
+    a.x = (const uint8_t *)d->x; a.ldx = d->x_stride; a.xs = d->x_scale; a.ldxs = d->x_scale_stride;
+    a.M = d->n_tok; a.N = d->N; a.K = d->K; a.E = 1;
+    a.y = d->y; a.ldy = d->y_stride; a.y_type = d->y_type;
+    if (!e4m3) {
+        size_t at = 0;
+        const Fp8Rows q = fp8_rows(at, d->n_tok, d->K);
+        uint8_t *ws = (uint8_t *)d->workspace;
+        const mp::Fp8QuantArgs qa{d->x, d->x_stride, d->x_type, 1, d->n_tok, d->K, ws + q.q, q.ld, (float *)(ws + q.s), q.nb};
+        HIPCHK(mp::launch_fp8_quant(qa, (hipStream_t)stream));
+        a.x = ws + q.q; a.ldx = q.ld; a.xs = (const float *)(ws + q.s); a.ldxs = q.nb;
+    }
+    HIPCHK(mp::launch_fp8_product(a, (hipStream_t)stream));
+    return MOE_OK;
+}
+
+struct Fp8LayerWs {
+    Fp8Rows x, h;
+    size_t counts, offsets, perm, act, rows, total;
+};
+static Fp8LayerWs fp8_layer_ws(int64_t n_tok, int E, int K, int H, int I) {
+    Fp8LayerWs w{};
+    const int64_t P = n_tok * K;
+    w.x = fp8_rows(w.total, n_tok, H);
+    w.h = fp8_rows(w.total, P, I);
+    w.counts = take(w.total, (size_t)E * 4);
+    w.offsets = take(w.total, (size_t)(E + 1) * 4);
+    w.perm = take(w.total, (size_t)P * 4);
+    w.act = take(w.total, (size_t)(P * I) * 4);
+    w.rows = take(w.total, (size_t)(P * H) * 4);
+    return w;
+}
+static bool fp8_layer_shape(int n_tok, int E, int K, int H, int I) {
+    return n_tok >= 0 && E >= 1 && E <= MOE_FP8_MAX_E && K >= 1 && K <= MOE_ROUTE_SCORED_MAX_K && (int64_t)n_tok * K <= 65535 &&
+           fp8_dim(H) && fp8_dim(I);
+}
+size_t moe_fp8_layer_workspace_bytes(int n_tok, int E, int K, int H, int I) {
+    return n_tok < 1 || !fp8_layer_shape(n_tok, E, K, H, I) ? 0 : fp8_layer_ws(n_tok, E, K, H, I).total;
+}
+
+int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream) {
+    if (!d) return fail(MOE_ERR_ARG, "moe_fp8_layer: null argument");
+    if (!fp8_layer_shape(d->n_tok, d->E, d->K, d->H, d->I))
+        return fail(MOE_ERR_ARG, "moe_fp8_layer: %d tokens of %d of %d experts, %d x %d: at most %d experts, %d a token, 65535 pairs and "
+                    "%d wide", d->n_tok, d->K, d->E, d->I, d->H, MOE_FP8_MAX_E, MOE_ROUTE_SCORED_MAX_K, MOE_FP8_MAX_DIM);
+    if (!dtype_ok(d->x_type)) return fail(MOE_ERR_ARG, "moe_fp8_layer: x_type %d unsupported", d->x_type);
+    if (!dtype_ok(d->out_type)) return fail(MOE_ERR_ARG, "moe_fp8_layer: out_type %d unsupported", d->out_type);
+    int r;
+    if ((r = fp8_weight_check("moe_fp8_layer", "gate", d->gate, d->E, d->I, d->H)) != MOE_OK ||
+        (r = fp8_weight_check("moe_fp8_layer", "up", d->up, d->E, d->I, d->H)) != MOE_OK ||
+        (r = fp8_weight_check("moe_fp8_layer", "down", d->down, d->E, d->H, d->I)) != MOE_OK)
+        return r;
+    moe_route_scored_desc rt = d->route;
+    rt.E = d->E; rt.K = d->K; rt.n_tok = d->n_tok;
+    rt.ids = d->ids; rt.w = d->w;
+    if (rt.logits && (r = scored_check(&rt)) != MOE_OK) return r;
+    if (d->n_tok == 0) return MOE_OK;
+    if (!d->x || !d->ids || !d->w || !d->out || !d->workspace) return fail(MOE_ERR_ARG, "moe_fp8_layer: null argument");
+    if (d->x_stride < d->H || d->out_stride < d->H)
+        return fail(MOE_ERR_ARG, "moe_fp8_layer: a row stride below the row's length");
+    if (!aligned_to(d->x, d->x_type) || !aligned_to(d->out, d->out_type) || ((uintptr_t)d->ids | (uintptr_t)d->w) % 4 ||
+        (uintptr_t)d->workspace % 16)
+        return fail(MOE_ERR_ARG, "moe_fp8_layer: misaligned pointer");
+    if (rt.logits && (r = moe_route_scored(&rt, stream)) != MOE_OK) return r;
+    hipStream_t st = (hipStream_t)stream;
+    const Fp8LayerWs l = fp8_layer_ws(d->n_tok, d->E, d->K, d->H, d->I);
+    uint8_t *ws = (uint8_t *)d->workspace;
+    const int P = d->n_tok * d->K;
+    int32_t *offsets = (int32_t *)(ws + l.offsets), *perm = (int32_t *)(ws + l.perm);
+    HIPCHK(mp::launch_dispatch(d->ids, P, d->E, (int32_t *)(ws + l.counts), offsets, perm, st));
+    HIPCHK(mp::launch_fp8_quant({d->x, d->x_stride, d->x_type, 1, d->n_tok, d->H, ws + l.x.q, l.x.ld, (float *)(ws + l.x.s), l.x.nb}, st));
+    mp::Fp8Args a{};
+    a.m[0] = fp8_mat(d->gate); a.m[1] = fp8_mat(d->up); a.gated = 1;
+    a.x = ws + l.x.q; a.ldx = l.x.ld; a.xs = (const float *)(ws + l.x.s); a.ldxs = l.x.nb;
+    a.offsets = offsets; a.perm = perm; a.top = d->K;
+    a.M = P; a.N = d->I; a.K = d->H; a.E = d->E;
+    a.y = ws + l.act; a.ldy = d->I; a.y_type = MOE_DTYPE_F32;
+    HIPCHK(mp::launch_fp8_product(a, st));
+    HIPCHK(mp::launch_fp8_quant({ws + l.act, d->I, MOE_DTYPE_F32, 1, P, d->I, ws + l.h.q, l.h.ld, (float *)(ws + l.h.s), l.h.nb}, st));
+    a.m[0] = fp8_mat(d->down); a.gated = 0;
+    a.x = ws + l.h.q; a.ldx = l.h.ld; a.xs = (const float *)(ws + l.h.s); a.ldxs = l.h.nb;
+    a.top = 0; a.N = d->H; a.K = d->I;
+    a.pair_w = d->w;
+    a.y = ws + l.rows; a.ldy = d->H;
+    HIPCHK(mp::launch_fp8_product(a, st));
+    HIPCHK(mp::launch_fp8_combine({(const float *)(ws + l.rows), d->ids, d->n_tok, d->K, d->E, d->H, d->out, d->out_stride, d->out_type}, st));
+    return MOE_OK;
+}
+
 // ---- slab pool --------------------------------------------------------------
 int moe_pool_create(int n_layers, int capacity, size_t bytes_per_expert, int device, moe_pool **out) {
     if (!out || n_layers <= 0 || capacity <= 0 || bytes_per_expert == 0) return fail(MOE_ERR_ARG, "bad arguments");

@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "libmoeprefetch.so")
 MOE_OK = 0
 MOE_ERR_ARG, MOE_ERR_HIP, MOE_ERR_NOMEM, MOE_ERR_STATE = -1, -2, -3, -4
 TYPE_Q4K, TYPE_Q6K = 12, 14
-DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_E4M3 = 0, 1, 2, 3
 SCORE = {"softmax": 0, "sigmoid": 1}
 NORM = {"rms": 0, "layer": 1}
 GATE_ACT = {None: 0, "sigmoid": 1}
@@ -79,6 +79,33 @@ class SampleDesc(ctypes.Structure):
     _fields_ = [("logits", P), ("logits_stride", I64), ("logits_type", I32), ("n_tok", I32), ("V", I32), ("u", P),
                 ("temperature", P), ("top_k", P), ("top_p", P), ("min_p", P), ("temperature_all", F32),
                 ("top_k_all", I32), ("top_p_all", F32), ("min_p_all", F32), ("tokens", P), ("probs", P), ("workspace", P)]
+
+
+class Fp8QuantizeDesc(ctypes.Structure):
+    _fields_ = [("x", P), ("x_stride", I64), ("x_type", I32), ("rows", I32), ("n_tok", I32), ("K", I32), ("q", P),
+                ("q_stride", I64), ("scale", P), ("scale_stride", I64)]
+
+
+def _fp8_weight(name):
+    """moe_fp8_weight's fields"""
+    return [(name, P), (name + "_stride", I64), (name + "_expert", I64), (name + "_scale", P),
+            (name + "_scale_stride", I64), (name + "_scale_expert", I64)]
+
+
+class Fp8ProductDesc(ctypes.Structure):
+    _fields_ = [("x", P), ("x_stride", I64), ("x_scale", P), ("x_scale_stride", I64), ("x_type", I32), ("n_tok", I32),
+                ("N", I32), ("K", I32), *_fp8_weight("weight"), ("y", P), ("y_stride", I64), ("y_type", I32), ("workspace", P)]
+
+
+class Fp8LayerHead(ctypes.Structure):
+    """moe_fp8_layer_desc up to its routing rule"""
+    _fields_ = [("x", P), ("x_stride", I64), ("x_type", I32), ("n_tok", I32), ("E", I32), ("K", I32), ("H", I32), ("I", I32),
+                *_fp8_weight("gate"), *_fp8_weight("up"), *_fp8_weight("down"), ("ids", P), ("w", P), ("out", P),
+                ("out_stride", I64), ("out_type", I32), ("workspace", P)]
+
+
+class Fp8LayerDesc(ctypes.Structure):
+    _fields_ = [*Fp8LayerHead._fields_, ("route", RouteScoredDesc)]
 
 
 class CacheConfig(ctypes.Structure):
@@ -261,6 +288,11 @@ SIGNATURES = {
     "moe_block_norm": (ctypes.c_int, [ctypes.POINTER(BlockNormDesc), P]),
     "moe_sample_workspace_bytes": (SZ, [ctypes.c_int, ctypes.c_int]),
     "moe_sample": (ctypes.c_int, [ctypes.POINTER(SampleDesc), P]),
+    "moe_fp8_quantize": (ctypes.c_int, [ctypes.POINTER(Fp8QuantizeDesc), P]),
+    "moe_fp8_product_workspace_bytes": (SZ, [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "moe_fp8_product": (ctypes.c_int, [ctypes.POINTER(Fp8ProductDesc), P]),
+    "moe_fp8_layer_workspace_bytes": (SZ, [ctypes.c_int] * 5),
+    "moe_fp8_layer": (ctypes.c_int, [ctypes.POINTER(Fp8LayerDesc), P]),
     "moe_combine": (ctypes.c_int, [P, ctypes.c_int, ctypes.c_int, ctypes.c_int, P, ctypes.c_int, P]),
     "moe_pool_create": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, SZ, ctypes.c_int, ctypes.POINTER(P)]),
     "moe_pool_destroy": (ctypes.c_int, [P]),

@@ -151,6 +151,12 @@ class ScoredRouter:
         return _lib.RouteScoredDesc.from_buffer_copy(
             self._packed(0, 0, 0, 0, bias=0 if bias is None else _vec(bias, self.E, _F32, _on_gpu(bias, "bias"), "bias")))
 
+    def head(self, logits, ld, dev):
+        """The rule and a call's logits as a part of another descriptor (Fp8Moe), whose call writes ids and w."""
+        bias = self.bias
+        return self._packed(logits.data_ptr(), ld, _dtype(logits, "logits"), logits.shape[0],
+                            0 if bias is None else _vec(bias, self.E, _F32, dev, "bias"), 0, self.E)
+
     def from_product(self, W, x, ids, w, slots, workspace, H, stream=None):
         """The same from W [n_experts][H] and x [tokens][H] (f32), whose product moe_route's kernels make in workspace
         (BatchedMoe.route: hidden 2048, n_experts a multiple of 64 up to 256).  workspace: contiguous, of

@@ -1,0 +1,121 @@
+"""e4m3 quantization, products with block scales and a layer of experts from their definitions, in 64 bits (numpy), with the
+rounding bounds of the kernels' 32-bit parts.
+
+U is half a step of f32 at 1.  A block's dot adds 128 exact products in f32 in an order of the matrix core's own; each of its
+additions is taken as off by a whole step (2 U) of the sum of the products' magnitudes, so that truncation is covered.  Then a
+scale is the rounded product of two (U), an fma a block adds to the running sum (U of it each), and the partial sums of a
+workgroup's waves are added (at most 8 more).  With A = sum over the blocks of |scale| * sum |products|, all of it is within
+    (2 * 128 + 1) U A + (blocks + 8) U A.
+"""
+import numpy as np
+
+U = 2.0 ** -24
+B = 128
+HALF = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}           # half a step, relative
+TINY = {"f32": 2.0 ** -149, "bf16": 2.0 ** -134, "f16": 2.0 ** -25}        # half a step (f32: one) below the normal numbers
+
+VALUES = np.empty(256)
+for _c in range(256):
+    _e, _m = (_c >> 3) & 15, _c & 7
+    _v = _m / 8.0 * 2.0 ** -6 if _e == 0 else (1.0 + _m / 8.0) * 2.0 ** (_e - 7)
+    VALUES[_c] = np.nan if _e == 15 and _m == 7 else -_v if _c & 128 else _v
+
+
+def blocks(n):
+    return -(-n // B)
+
+
+def e4m3(v):
+    """To the nearest e4m3 value, ties to even; |v| <= 448 or NaN."""
+    v = np.asarray(v, np.float64)
+    step = np.exp2(np.maximum(np.frexp(np.where(np.isfinite(v), v, 0.0))[1] - 1, -6) - 3.0)
+    return np.rint(v / step) * step
+
+
+def scale_of(amax):
+    """The least power of two s >= 2^-126 with amax <= 448 s."""
+    m, e = np.frexp(np.asarray(amax, np.float64))                # amax = m 2^e, m in [1/2, 1);  448 = 7/8 * 2^9
+    e = np.where(np.asarray(amax) > 0, np.where(m > 0.875, e - 8, e - 9), -126)
+    return np.exp2(np.maximum(e, -126).astype(np.float64))
+
+
+def spread(s, rows, n, k):
+    """Block scales as factors of the [..][n][k] values."""
+    return np.repeat(np.repeat(s, rows, axis=-2)[..., :n, :], B, axis=-1)[..., :k]
+
+
+def block_max(x, rows):
+    n, k = x.shape
+    p = np.zeros((-(-n // rows) * rows, blocks(k) * B))
+    p[:n, :k] = np.where(np.isfinite(x), np.abs(x), 0.0)
+    return p.reshape(-1, rows, blocks(k), B).max(axis=(1, 3))
+
+
+def quantize(x, rows=1):
+    """(values of the codes, scales) of x [n][k]"""
+    x = np.asarray(x, np.float64)
+    s = scale_of(block_max(x, rows))
+    x = np.where(np.isfinite(x), x, np.nan)
+    return e4m3(x / spread(s, rows, *x.shape)), s
+
+
+def dequant(q, s, rows):
+    return q * spread(s, rows, *q.shape[-2:])
+
+
+def product(xq, xs, wq, ws):
+    """(y, a bound of the error of its f32 arithmetic)"""
+    x, w = dequant(xq, xs, 1), dequant(wq, ws, B)
+    y = x @ w.T
+    a = np.abs(x) @ np.abs(w).T
+    nb = blocks(xq.shape[1])
+    # (scales below the normal numbers of f32 lose bits of their own)
+    return y, ((2 * B + 1) + nb + 8) * U * a + nb * B * 2.0 ** -149 * 448.0 ** 2
+
+
+def out_bound(y, err, dt):
+    """The bound of a result within err of y, rounded to dt."""
+    return err + (np.abs(y) + err) * HALF[dt] * 1.001 + TINY[dt]
+
+
+def silu(g):
+    with np.errstate(over="ignore"):
+        return g / (1.0 + np.exp(-g))
+
+
+def layer(x, ids, w, gate, up, down):
+    """(out, bound) of a layer; gate, up and down: (values [E][n][k], scales).  The activation h is known within a bound only, and a
+    code of it, or its block's scale, may be either of two where a border lies within that bound: the difference counts."""
+    T, K = ids.shape
+    E, H = gate[0].shape[0], x.shape[1]
+    xq, xs = quantize(x)
+    out, err = np.zeros((T, H)), np.zeros((T, H))
+    sums = np.zeros((T, H))
+    for e in range(E):
+        tok, k = np.nonzero(ids == e)
+        if not len(tok):
+            continue
+        g, e_g = product(xq[tok], xs[tok], gate[0][e], gate[1][e])
+        u, e_u = product(xq[tok], xs[tok], up[0][e], up[1][e])
+        h = u * silu(g)
+        # |silu'| <= 1.1; exp, the sum, the division and two products are taken as 16 half steps
+        e_h = np.abs(silu(g)) * e_u + 1.1 * e_g * (np.abs(u) + e_u) + 16 * U * np.abs(h) + 2.0 ** -126
+        hq, hs = quantize(h)
+        ref = dequant(hq, hs, 1)
+        off = np.zeros_like(h)
+        # the block's largest within the bounds of all of them
+        m = np.abs(h)
+        lo, hi = block_max(np.maximum(m - e_h, 0.0), 1), block_max(m + e_h, 1)
+        for s in (scale_of(lo), scale_of(hi)):
+            f = spread(s, 1, *h.shape)
+            for d in (-1.0, 1.0):
+                v = np.clip((h + d * e_h) / f, -448.0, 448.0)
+                off = np.maximum(off, np.abs(e4m3(v) * f - ref))
+        wd = dequant(down[0][e], down[1][e], B)
+        y, e_y = product(hq, hs, down[0][e], down[1][e])
+        e_y = e_y * (1.0 + 2.0 ** -3) + off @ np.abs(wd).T
+        wt = np.asarray(w, np.float64)[tok, k][:, None]
+        np.add.at(out, tok, wt * y)
+        np.add.at(err, tok, np.abs(wt) * e_y)
+        np.add.at(sums, tok, np.abs(wt) * (np.abs(y) + e_y))
+    return out, err + (K + 2) * U * sums
