@@ -12,6 +12,8 @@
 // have 1e-8.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "mp_device.h"
 #include "mp_elem.h"
 #include "mp_internal.h"
@@ -230,7 +232,312 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
     }
 }
 
+// ---- products of many rows: tiles through LDS --------------------------------------
+// A workgroup computes BN rows of the weight (GATED: BN / 2 of gate and as many of up) for BM rows of x, a wave TN x TM tiles of
+// 16 x 16 of it.  A block of K (128 bytes a row) of both operands is one stage of LDS; the next stage's loads, which go to LDS
+// without registers, are on their way while this one is multiplied.
+// The eight 16-byte chunks of a row lie in LDS at chunk ^ (row & 7): the lanes that read one chunk of eight rows then touch
+// all banks once.
+__device__ inline float4_v mfma_e4m3(int8_v w, int8_v x) {
+    const float4_v z = {0.0f, 0.0f, 0.0f, 0.0f};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, z, 0, 0, 0, 0, 0, 0);
+}
+
+// expert and first row (in the dispatch's order) of a workgroup's rows of x, the slot-th run of BM; false: there is none
+__device__ inline bool find_run(const int32_t *offsets, int E, int bm, int slot, int &e, int &p0, int &end, int *s_run) {
+    if (threadIdx.x < 64) {
+        const int lane = threadIdx.x;
+        int tiles[4], o[5], sum = 0;
+#pragma unroll
+        for (int j = 0; j < 5; ++j) o[j] = offsets[min(4 * lane + j, E)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            tiles[j] = (o[j + 1] - o[j] + bm - 1) / bm;
+            sum += tiles[j];
+        }
+        int incl = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int t = __shfl_up(incl, d, 64);
+            if (lane >= d) incl += t;
+        }
+        if (lane == 63) s_run[3] = slot < incl;
+        int at = incl - sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (slot >= at && slot < at + tiles[j]) {
+                s_run[0] = 4 * lane + j;
+                s_run[1] = o[j] + (slot - at) * bm;
+                s_run[2] = o[j + 1];
+            }
+            at += tiles[j];
+        }
+    }
+    __syncthreads();
+    e = __builtin_amdgcn_readfirstlane(s_run[0]);
+    p0 = __builtin_amdgcn_readfirstlane(s_run[1]);
+    end = __builtin_amdgcn_readfirstlane(s_run[2]);
+    return s_run[3] != 0;
+}
+
+template <bool GATED, bool EXACT, bool ALIGNED, int WN, int WM, int TN, int TM>
+__global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n_tiles) {
+    constexpr int THREADS = 64 * WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, CH = (BN + BM) * 8 / THREADS;
+    static_assert((BN + BM) * 8 % THREADS == 0 && BN % 8 == 0, "whole loads");
+    __shared__ uint4 s_0[(BN + BM) * 8], s_1[(BN + BM) * 8];
+    __shared__ int s_run[4];
+    __shared__ float s_max[WN][BM];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int wn = wave % WN, wm = wave / WN;
+    const int total = gridDim.x, per = total / 8;
+    // neighbouring tiles on one XCD (workgroups go round the eight), where they share what they read
+    const int id = blockIdx.x < per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+    int e = 0, p0, end = a.M;
+    int n_tile;
+    if (a.offsets) {
+        n_tile = id % n_tiles;
+        if (!find_run(a.offsets, a.E, BM, id / n_tiles, e, p0, end, s_run)) return;
+    } else {
+        const int m_tiles = total / n_tiles;
+        n_tile = id / m_tiles;
+        p0 = id % m_tiles * BM;
+    }
+    constexpr int ROWS = GATED ? BN / 2 : BN;           // rows of y's columns
+    const int n0 = n_tile * ROWS;
+
+    // the row that chunk q of a stage is of
+    auto row_of = [&](int q) -> const uint8_t * {
+        const int r = q >> 3;
+        if (r < BN) {
+            // a wave's rows: TN / 2 tiles of gate and as many of up
+            const int w = r / (16 * TN), t = r % (16 * TN);
+            const bool up = GATED && t >= 8 * TN;
+            const int row = n0 + (GATED ? w * 8 * TN + t % (8 * TN) : r);
+            const Fp8Mat &m = a.m[up];
+            return m.w + e * m.ex + (int64_t)min(row, a.N - 1) * m.ld;
+        }
+        const int p = min(p0 + r - BN, end - 1);
+        return a.x + (int64_t)(a.top ? a.perm[p] / a.top : p) * a.ldx;
+    };
+    auto chunk_of = [](int q) { return (q & 7) ^ (q >> 3 & 7); };
+    const uint8_t *src[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int q = i * THREADS + threadIdx.x;
+        src[i] = row_of(q) + 16 * chunk_of(q);
+    }
+    // a whole block's loads; rows off 16 bytes go through registers (landed)
+    uint4 held[ALIGNED ? 1 : CH];
+    auto stage = [&](uint4 *s, int b) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const uint8_t *from = src[i] + (int64_t)b * FB;
+            if (ALIGNED)
+                __builtin_amdgcn_global_load_lds((const void *)from, (__attribute__((address_space(3))) void *)(s + i * THREADS + 64 * wave), 16, 0, 0);
+            else
+                held[i] = load16(from, 16);
+        }
+    };
+    auto landed = [&](uint4 *s) {
+        if (!ALIGNED)
+#pragma unroll
+            for (int i = 0; i < CH; ++i) s[i * THREADS + threadIdx.x] = held[i];
+        __syncthreads();                                // this stage is there, and the one before free
+    };
+    // the scales of a block: of the weight's rows (gate's and up's), and of a lane's row of x in each tile
+    const float *sw0, *sw1 = nullptr, *sx[TM];
+    {
+        const int nblk = (n0 + (GATED ? wn * 8 * TN : wn * 16 * TN)) / FB;
+        const int last = (a.N - 1) / FB;
+        sw0 = a.m[0].s + e * a.m[0].sex + (int64_t)min(nblk, last) * a.m[0].sld;
+        if (GATED) sw1 = a.m[1].s + e * a.m[1].sex + (int64_t)min(nblk, last) * a.m[1].sld;
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            const int p = min(p0 + (wm * TM + j) * 16 + c, end - 1);
+            sx[j] = a.xs + (int64_t)(a.top ? a.perm[p] / a.top : p) * a.ldxs;
+        }
+    }
+    float4_v acc[TN][TM] = {};
+    float fx[TM], f0, f1 = 0.0f;
+    auto scales = [&](int b) {
+        f0 = sw0[b];
+        if (GATED) f1 = sw1[b];
+#pragma unroll
+        for (int j = 0; j < TM; ++j) fx[j] = sx[j][b];
+    };
+    auto frag = [&](const uint4 *s, int r) {
+        const uint4 u = s[r * 8 + (g ^ (r & 7))], v = s[r * 8 + ((4 + g) ^ (r & 7))];
+        return int8_v{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w};
+    };
+    auto multiply = [&](const uint4 *s, float c0, float c1, const float (&cx)[TM]) {
+        int8_v xf[TM];
+        half8_v xh[TM][4];
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            xf[j] = frag(s, BN + (wm * TM + j) * 16 + c);
+            if (EXACT)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) xh[j][k] = halves(xf[j][2 * k], xf[j][2 * k + 1]);
+        }
+        // a row of tiles' products while the row before is scaled and added (EXACT: products take four times as long, and
+        // their operands the registers of that), and the row after is read
+        constexpr int LAG = EXACT ? 0 : 1;
+        int8_v wf = frag(s, wn * TN * 16 + c);
+        float4_v d[LAG + 1][TM];
+#pragma unroll
+        for (int i = 0; i < TN + LAG; ++i) {
+            int8_v wnext;
+            if (i + 1 < TN) wnext = frag(s, (wn * TN + i + 1) * 16 + c);
+            if (i < TN) {
+                half8_v wh[4];
+                if (EXACT)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) wh[k] = halves(wf[2 * k], wf[2 * k + 1]);
+#pragma unroll
+                for (int j = 0; j < TM; ++j) {
+                    if (EXACT) {
+                        float4_v t = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[k], xh[j][k], t, 0, 0, 0);
+                        d[0][j] = t;
+                    } else {
+                        d[i & LAG][j] = mfma_e4m3(wf, xf[j]);
+                    }
+                }
+            }
+            const int l = i - LAG;
+            if (l >= 0) {
+                const float sw = GATED && l >= TN / 2 ? c1 : c0;
+#pragma unroll
+                for (int j = 0; j < TM; ++j) {
+                    const float f = cx[j] * sw;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[l][j][k] = fmaf(d[l & LAG][j][k], f, acc[l][j][k]);
+                }
+            }
+            wf = wnext;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // this stage multiplied while the next one's loads are on their way
+    auto step = [&](const uint4 *s, uint4 *next, int b) {
+        float c0 = f0, c1 = f1, cx[TM];
+#pragma unroll
+        for (int j = 0; j < TM; ++j) cx[j] = fx[j];
+        stage(next, b + 1);
+        scales(b + 1);
+        multiply(s, c0, c1, cx);
+        landed(next);
+    };
+    const int whole = a.K / FB;
+    if (whole) {
+        stage(s_0, 0);
+        scales(0);
+        landed(s_0);
+        int b = 0;
+        for (; b + 2 < whole; b += 2) {
+            step(s_0, s_1, b);
+            step(s_1, s_0, b + 1);
+        }
+        if (b + 1 < whole) step(s_0, s_1, b);
+        multiply(b + 1 < whole ? s_1 : s_0, f0, f1, fx);
+    }
+    if (a.K % FB) {                                     // the last block
+        __syncthreads();
+#pragma unroll 1
+        for (int q = threadIdx.x; q < (BN + BM) * 8; q += THREADS) {
+            const int k = whole * FB + 16 * chunk_of(q);
+            s_0[q] = load16(row_of(q) + k, a.K - k);
+        }
+        scales(whole);
+        __syncthreads();
+        multiply(s_0, f0, f1, fx);
+    }
+
+    if (GATED) {
+        // h, and its codes: a workgroup has whole blocks of 128 of I
+        static_assert(!GATED || ROWS == FB, "a block");
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < TN / 2; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int n = n0 + wn * 8 * TN + 16 * i + 4 * g + k;
+                    const float h = n < a.N ? finite_or_nan(silu_times(acc[i][j][k], acc[i + TN / 2][j][k])) : 0.0f;
+                    acc[i][j][k] = h;
+                    m = fmaxf(m, fabsf(h));
+                }
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            if (g == 0) s_max[wn][(wm * TM + j) * 16 + c] = m;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            const int col = (wm * TM + j) * 16 + c;
+            const int64_t p = p0 + col;
+            float m = s_max[0][col];
+#pragma unroll
+            for (int w = 1; w < WN; ++w) m = fmaxf(m, s_max[w][col]);
+            const int ex = scale_exp(m);
+            const float inv = pow2(-ex);
+            if (p >= end) continue;
+            if (wn == 0 && g == 0) a.hs[p * a.ldhs + n_tile] = pow2(ex);
+#pragma unroll
+            for (int i = 0; i < TN / 2; ++i) {
+                const int n = n0 + wn * 8 * TN + 16 * i + 4 * g;
+                int q = __builtin_amdgcn_cvt_pk_fp8_f32(acc[i][j][0] * inv, acc[i][j][1] * inv, 0, false);
+                q = __builtin_amdgcn_cvt_pk_fp8_f32(acc[i][j][2] * inv, acc[i][j][3] * inv, q, true);
+                // (ldh is a multiple of 16: four codes stay inside the row)
+                if (n < a.N) *(int *)(a.hq + p * a.ldh + n) = q;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+        int64_t p = p0 + (wm * TM + j) * 16 + c;
+        if (p >= end) continue;
+        float w = 1.0f;
+        if (a.pair_w) {
+            p = a.perm[p];
+            w = a.pair_w[p];
+        }
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            const int n = n0 + (wn * TN + i) * 16 + 4 * g;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (n + k < a.N) store_elem(a.y, p * a.ldy + n + k, a.y_type, a.pair_w ? w * acc[i][j][k] : acc[i][j][k]);
+        }
+    }
+}
+
+template <bool GATED, bool EXACT, bool ALIGNED, int WN, int WM, int TN, int TM>
+static hipError_t launch_tile_n(const Fp8Args &a, hipStream_t st) {
+    constexpr int ROWS = 16 * TN * WN / (GATED ? 2 : 1), BM = 16 * TM * WM;
+    const int64_t n_tiles = (a.N + ROWS - 1) / ROWS;
+    // with a dispatch: whole runs, and one a used expert that is not whole
+    const int64_t runs = a.offsets ? a.M / BM + std::min(a.E, a.M) : (a.M + BM - 1) / BM;
+    hipLaunchKernelGGL((fp8_tile_kernel<GATED, EXACT, ALIGNED, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM), 0,
+                       st, a, (int)n_tiles);
+    return hipGetLastError();
+}
+template <bool GATED, bool EXACT>
+static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
+    auto whole = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0; };
+    const bool al = whole(a.m[0]) && (!GATED || whole(a.m[1])) && ((uintptr_t)a.x | a.ldx) % 16 == 0;
+    if (al) return launch_tile_n<GATED, EXACT, true, 4, 2, 4, 4>(a, st);
+    return launch_tile_n<GATED, EXACT, false, 4, 2, 4, 4>(a, st);
+}
+
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
+    if (a.M >= FP8_TILE_ROWS * a.E) {
+        if (a.gated) return a.exact ? launch_tile<true, true>(a, st) : launch_tile<true, false>(a, st);
+        return a.exact ? launch_tile<false, true>(a, st) : launch_tile<false, false>(a, st);
+    }
     const int64_t chunks = a.offsets ? 4 : (a.M + 15) / 16;
     const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)a.E, (unsigned)(chunks < 1024 ? chunks : 1024));
     if (a.gated) hipLaunchKernelGGL((fp8_stream_kernel<true>), grid, dim3(256), 0, st, a);

@@ -392,7 +392,14 @@ struct Fp8Args {
     void *y;
     int64_t ldy;
     int y_type;
+    int exact;                    // sums of products in f32 throughout (see mp_fp8.hip)
+    uint8_t *hq;                  // gated, many rows: y's codes and scales instead of y
+    int64_t ldh;
+    float *hs;
+    int64_t ldhs;
 };
+// rows of x for each expert from which products run on tiles
+constexpr int FP8_TILE_ROWS = 48;
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st);
 struct Fp8CombineArgs {
     const float *rows;            // [n_tok * K][H]

@@ -4282,6 +4282,7 @@ int moe_fp8_product(const moe_fp8_product_desc *d, void *stream) {
     a.m[0] = fp8_mat(d->weight);
     a.x = (const uint8_t *)d->x; a.ldx = d->x_stride; a.xs = d->x_scale; a.ldxs = d->x_scale_stride;
     a.M = d->n_tok; a.N = d->N; a.K = d->K; a.E = 1;
+    a.exact = d->y_type == MOE_DTYPE_F32;
     a.y = d->y; a.ldy = d->y_stride; a.y_type = d->y_type;
     if (!e4m3) {
         size_t at = 0;
@@ -4356,11 +4357,15 @@ int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream) {
     a.offsets = offsets; a.perm = perm; a.top = d->K;
     a.M = P; a.N = d->I; a.K = d->H; a.E = d->E;
     a.y = ws + l.act; a.ldy = d->I; a.y_type = MOE_DTYPE_F32;
+    a.exact = d->out_type != MOE_DTYPE_BF16;
+    a.hq = ws + l.h.q; a.ldh = l.h.ld; a.hs = (float *)(ws + l.h.s); a.ldhs = l.h.nb;
     HIPCHK(mp::launch_fp8_product(a, st));
+    if (P < mp::FP8_TILE_ROWS * d->E)
     HIPCHK(mp::launch_fp8_quant({ws + l.act, d->I, MOE_DTYPE_F32, 1, P, d->I, ws + l.h.q, l.h.ld, (float *)(ws + l.h.s), l.h.nb}, st));
     a.m[0] = fp8_mat(d->down); a.gated = 0;
     a.x = ws + l.h.q; a.ldx = l.h.ld; a.xs = (const float *)(ws + l.h.s); a.ldxs = l.h.nb;
     a.top = 0; a.N = d->H; a.K = d->I;
+    a.exact = d->out_type == MOE_DTYPE_F32;
     a.pair_w = d->w;
     a.y = ws + l.rows; a.ldy = d->H;
     HIPCHK(mp::launch_fp8_product(a, st));
