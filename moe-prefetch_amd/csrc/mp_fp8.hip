@@ -58,15 +58,18 @@ __device__ inline float max16(float v) {
     return fmaxf(v, dpp_f<DPP_MIRROR>(v));
 }
 
-// n of eight elements of a row
+// n of eight elements of a row, the rest zeros
 template <int T>
 __device__ inline void load8(const typename Elem<T>::raw *p, int n, float *v) {
-    typename Elem<T>::raw q[8] = {};
-    if (n >= 8) __builtin_memcpy(q, p, sizeof q);
-    else
-        for (int i = 0; i < n; ++i) q[i] = p[i];
+    if (n >= 8) {
+        typename Elem<T>::raw q[8];
+        __builtin_memcpy(q, p, sizeof q);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = finite_or_nan(Elem<T>::load(q[i]));
+        for (int i = 0; i < 8; ++i) v[i] = Elem<T>::load(q[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? Elem<T>::load(p[i]) : 0.0f;
+    }
 }
 __device__ inline void store8(uint8_t *p, int n, uint2 c) {
     if (n >= 8) __builtin_memcpy(p, &c, 8);
@@ -78,21 +81,39 @@ __device__ inline float amax8(const float *v, float m) {
     for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));        // passes over a NaN
     return m;
 }
+// the largest finite magnitude of a lane's values, if m, the largest of any lane's it is compared with, is infinite
+__device__ inline float without_inf(float *v, float m) {
+    if (!(m == INFINITY)) return m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = finite_or_nan(v[i]);
+    return amax8(v, 0.0f);
+}
 
-// sixteen lanes a block of one row, eight neighbouring elements each
-template <int T>
-__global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a) {
-    const uint32_t nb = (uint32_t)((a.K + FB - 1) / FB);
-    const uint64_t g = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16;
-    if (g >= (uint64_t)a.n_tok * nb) return;
-    const int64_t row = (int64_t)(g / nb);
-    const int b = (int)(g % nb), l = threadIdx.x % 16;
-    const int k = b * FB + 8 * l, n = a.K - k;
-    float v[8] = {};
-    if (n > 0) load8<T>((const typename Elem<T>::raw *)a.x + row * a.ldx + k, n, v);
-    const int e = scale_exp(max16(amax8(v, 0.0f)));
-    if (n > 0) store8(a.q + row * a.ldq + k, n, codes8(v, pow2(-e)));
-    if (l == 0) a.s[row * a.lds + b] = pow2(e);
+// Sixteen lanes a block of one row, eight neighbouring elements each in one load; NB blocks a lane, sixteen apart, whose loads are on their
+// way together.  magic, shift: the division by the blocks of a row.
+template <int T, int NB>
+__global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a, uint32_t nb, uint32_t total, uint32_t magic, int shift) {
+    const uint32_t g0 = blockIdx.x * (16 * NB) + threadIdx.x / 16;
+    const int l = threadIdx.x % 16;
+    float v[NB][8];
+    uint32_t row[NB], b[NB];
+    int n[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const uint32_t g = g0 + 16 * i;
+        row[i] = (uint32_t)((uint64_t)g * magic >> shift);
+        b[i] = g - row[i] * nb;
+        n[i] = g < total ? a.K - (int)(b[i] * FB) - 8 * l : 0;
+        load8<T>((const typename Elem<T>::raw *)a.x + row[i] * a.ldx + b[i] * FB + 8 * l, n[i], v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        float m = max16(amax8(v[i], 0.0f));
+        if (__any(m == INFINITY)) m = max16(without_inf(v[i], m));
+        const int e = scale_exp(m);
+        if (n[i] > 0) store8(a.q + row[i] * a.ldq + b[i] * FB + 8 * l, n[i], codes8(v[i], pow2(-e)));
+        if (l == 0 && n[i] > 0) a.s[row[i] * a.lds + b[i]] = pow2(e);
+    }
 }
 
 // a workgroup a block of 128 rows
@@ -101,18 +122,28 @@ __global__ __launch_bounds__(256) void fp8_quant_block_kernel(Fp8QuantArgs a) {
     __shared__ float s_max[4];
     const int64_t r0 = (int64_t)blockIdx.y * FB;
     const int b = blockIdx.x, l = threadIdx.x % 16, k = b * FB + 8 * l, n = a.K - k;
-    float v[8][8] = {};
+    float v[8][8];
     float m = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int64_t row = r0 + threadIdx.x / 16 + 16 * i;
-        if (n > 0 && row < a.n_tok) load8<T>((const typename Elem<T>::raw *)a.x + row * a.ldx + k, n, v[i]);
+        load8<T>((const typename Elem<T>::raw *)a.x + row * a.ldx + k, row < a.n_tok ? n : 0, v[i]);
         m = amax8(v[i], m);
     }
-    m = wave_max(m);
-    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    auto largest = [&](float m) {
+        m = wave_max(m);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
+        __syncthreads();
+        return fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    };
+    m = largest(m);
+    if (m == INFINITY) {                                  // (the same on every thread)
+        m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, without_inf(v[i], INFINITY));
+        m = largest(m);
+    }
     const int e = scale_exp(m);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -124,11 +155,22 @@ __global__ __launch_bounds__(256) void fp8_quant_block_kernel(Fp8QuantArgs a) {
 
 template <int T>
 static hipError_t launch_quant_t(const Fp8QuantArgs &a, hipStream_t st) {
-    const int64_t nb = (a.K + FB - 1) / FB;
-    if (a.rows == 1)
-        hipLaunchKernelGGL((fp8_quant_rows_kernel<T>), dim3((unsigned)((a.n_tok * nb + 15) / 16)), dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((fp8_quant_block_kernel<T>), dim3((unsigned)nb, (unsigned)((a.n_tok + FB - 1) / FB)), dim3(256), 0, st, a);
+    const uint32_t nb = (uint32_t)((a.K + FB - 1) / FB);
+    if (a.rows == 1) {
+        const uint32_t total = (uint32_t)a.n_tok * nb;                // at most 2^31
+        // g / nb = g * magic >> shift for every g below 2^31 + 2^12 (Granlund and Montgomery, Division by Invariant Integers, 1994)
+        int bits = 0;
+        while ((1u << bits) < nb) ++bits;
+        const int shift = 31 + bits;
+        const uint32_t magic = (uint32_t)(((1ull << shift) + nb - 1) / nb);
+        // four blocks a lane where that leaves every compute unit four workgroups
+        if (total >= 256 * 4 * 64)
+            hipLaunchKernelGGL((fp8_quant_rows_kernel<T, 4>), dim3((total + 63) / 64), dim3(256), 0, st, a, nb, total, magic, shift);
+        else
+            hipLaunchKernelGGL((fp8_quant_rows_kernel<T, 1>), dim3((total + 15) / 16), dim3(256), 0, st, a, nb, total, magic, shift);
+    } else {
+        hipLaunchKernelGGL((fp8_quant_block_kernel<T>), dim3(nb, (unsigned)((a.n_tok + FB - 1) / FB)), dim3(256), 0, st, a);
+    }
     return hipGetLastError();
 }
 hipError_t launch_fp8_quant(const Fp8QuantArgs &a, hipStream_t st) {
@@ -529,6 +571,7 @@ template <bool GATED, bool EXACT>
 static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
     auto whole = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0; };
     const bool al = whole(a.m[0]) && (!GATED || whole(a.m[1])) && ((uintptr_t)a.x | a.ldx) % 16 == 0;
+    if (al && !GATED && !EXACT && a.M >= 2048) return launch_tile_n<GATED, EXACT, true, 2, 4, 8, 4>(a, st);
     if (al) return launch_tile_n<GATED, EXACT, true, 4, 2, 4, 4>(a, st);
     return launch_tile_n<GATED, EXACT, false, 4, 2, 4, 4>(a, st);
 }
