@@ -20,6 +20,8 @@
 
 namespace mp {
 
+typedef int int4_v __attribute__((ext_vector_type(4)));
+typedef int int4_u __attribute__((ext_vector_type(4), aligned(1)));       // wherever it begins
 typedef int int8_v __attribute__((ext_vector_type(8)));
 typedef float float4_v __attribute__((ext_vector_type(4)));
 typedef _Float16 half2_v __attribute__((ext_vector_type(2)));
@@ -194,18 +196,16 @@ __device__ inline float4_v mfma_block(int8_v w, int8_v x) {
 
 // A lane's 32 of the 128 codes of a row's block: bytes 16 g .. and 64 + 16 g .., g = lane / 16 (which codes meet which is the same
 // for both operands).  n: bytes of the row from here on; codes past it are zeros.
-__device__ inline uint4 load16(const uint8_t *p, int n) {
-    uint64_t v[2] = {0, 0};
-    if (n >= 16) __builtin_memcpy(v, p, 16);
-    else {
-        for (int i = min(n, 8) - 1; i >= 0; --i) v[0] = v[0] << 8 | p[i];
-        for (int i = n - 1; i >= 8; --i) v[1] = v[1] << 8 | p[i];
-    }
-    return make_uint4((uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32));
+__device__ inline int4_v load16(const uint8_t *p, int n) {
+    if (n >= 16) return *(const int4_u *)p;
+    uint64_t lo = 0, hi = 0;
+    for (int i = min(n, 8) - 1; i >= 0; --i) lo = lo << 8 | p[i];
+    for (int i = n - 1; i >= 8; --i) hi = hi << 8 | p[i];
+    return int4_v{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 }
 __device__ inline int8_v load_frag(const uint8_t *row, int k, int K, int g) {
-    const uint4 a = load16(row + k + 16 * g, K - k - 16 * g), b = load16(row + k + 64 + 16 * g, K - k - 64 - 16 * g);
-    return int8_v{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+    return __builtin_shufflevector(load16(row + k + 16 * g, K - k - 16 * g), load16(row + k + 64 + 16 * g, K - k - 64 - 16 * g), 0, 1, 2, 3, 4,
+                                   5, 6, 7);
 }
 
 __device__ inline void store_elem(void *p, int64_t i, int type, float v) {
@@ -322,44 +322,49 @@ __device__ inline bool find_run(const int32_t *offsets, int E, int bm, int slot,
     return s_run[3] != 0;
 }
 
-template <bool GATED, bool EXACT, bool ALIGNED, int WN, int WM, int TN, int TM>
-__global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n_tiles) {
+// a barrier that leaves loads from memory on their way
+__device__ inline void barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <bool GATED, bool EXACT, int WN, int WM, int TN, int TM>
+__global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n_tiles, int m_tiles) {
     constexpr int THREADS = 64 * WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, CH = (BN + BM) * 8 / THREADS;
-    static_assert((BN + BM) * 8 % THREADS == 0 && BN % 8 == 0, "whole loads");
-    __shared__ uint4 s_0[(BN + BM) * 8], s_1[(BN + BM) * 8];
+    static_assert((BN + BM) * 8 % THREADS == 0, "whole loads");
+    __shared__ int4_v s_0[(BN + BM) * 8], s_1[(BN + BM) * 8];
     __shared__ int s_run[4];
     __shared__ float s_max[WN][BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     const int wn = wave % WN, wm = wave / WN;
-    const int total = gridDim.x, per = total / 8;
-    // neighbouring tiles on one XCD (workgroups go round the eight), where they share what they read
-    const int id = blockIdx.x < per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
     int e = 0, p0, end = a.M;
     int n_tile;
     if (a.offsets) {
-        n_tile = id % n_tiles;
-        if (!find_run(a.offsets, a.E, BM, id / n_tiles, e, p0, end, s_run)) return;
+        n_tile = blockIdx.x % n_tiles;
+        if (!find_run(a.offsets, a.E, BM, blockIdx.x / n_tiles, e, p0, end, s_run)) return;
     } else {
-        const int m_tiles = total / n_tiles;
-        n_tile = id / m_tiles;
-        p0 = id % m_tiles * BM;
+        // workgroups go round the eight XCDs: each has a run of tiles, in strips of eight tiles of x, so that those at work
+        // at once share what they read in its L2
+        const int total = n_tiles * m_tiles, per = total / 8;
+        const int id = blockIdx.x < per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+        const int strip = id / (8 * n_tiles), wide = min(8, m_tiles - 8 * strip), in = id - strip * 8 * n_tiles;
+        n_tile = in / wide;
+        p0 = (8 * strip + in % wide) * BM;
     }
     constexpr int ROWS = GATED ? BN / 2 : BN;           // rows of y's columns
     const int n0 = n_tile * ROWS;
 
-    // the row that chunk q of a stage is of
+    // the row that chunk q of a stage is of, and which of its chunks
     auto row_of = [&](int q) -> const uint8_t * {
         const int r = q >> 3;
-        if (r < BN) {
-            // a wave's rows: TN / 2 tiles of gate and as many of up
-            const int w = r / (16 * TN), t = r % (16 * TN);
-            const bool up = GATED && t >= 8 * TN;
-            const int row = n0 + (GATED ? w * 8 * TN + t % (8 * TN) : r);
-            const Fp8Mat &m = a.m[up];
-            return m.w + e * m.ex + (int64_t)min(row, a.N - 1) * m.ld;
+        if (r >= BN) {
+            const int p = min(p0 + r - BN, end - 1);
+            return a.x + (int64_t)(a.top ? a.perm[p] / a.top : p) * a.ldx;
         }
-        const int p = min(p0 + r - BN, end - 1);
-        return a.x + (int64_t)(a.top ? a.perm[p] / a.top : p) * a.ldx;
+        const int w = r / (16 * TN), t = r % (16 * TN);  // a wave's rows: TN / 2 tiles of gate and as many of up
+        const Fp8Mat &m = a.m[GATED && t >= 8 * TN];
+        return m.w + e * m.ex + (int64_t)min(n0 + (GATED ? w * 8 * TN + t % (8 * TN) : r), a.N - 1) * m.ld;
     };
     auto chunk_of = [](int q) { return (q & 7) ^ (q >> 3 & 7); };
     const uint8_t *src[CH];
@@ -368,23 +373,13 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
         const int q = i * THREADS + threadIdx.x;
         src[i] = row_of(q) + 16 * chunk_of(q);
     }
-    // a whole block's loads; rows off 16 bytes go through registers (landed)
-    uint4 held[ALIGNED ? 1 : CH];
-    auto stage = [&](uint4 *s, int b) {
+    auto load = [&](int4_v (&h)[CH], int b) {           // a thread's chunks of a stage
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const uint8_t *from = src[i] + (int64_t)b * FB;
-            if (ALIGNED)
-                __builtin_amdgcn_global_load_lds((const void *)from, (__attribute__((address_space(3))) void *)(s + i * THREADS + 64 * wave), 16, 0, 0);
-            else
-                held[i] = load16(from, 16);
-        }
+        for (int i = 0; i < CH; ++i) h[i] = *(const int4_u *)(src[i] + (int64_t)b * FB);
     };
-    auto landed = [&](uint4 *s) {
-        if (!ALIGNED)
+    auto store = [&](const int4_v (&h)[CH], int4_v *s) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) s[i * THREADS + threadIdx.x] = held[i];
-        __syncthreads();                                // this stage is there, and the one before free
+        for (int i = 0; i < CH; ++i) s[i * THREADS + threadIdx.x] = h[i];
     };
     // the scales of a block: of the weight's rows (gate's and up's), and of a lane's row of x in each tile
     const float *sw0, *sw1 = nullptr, *sx[TM];
@@ -407,11 +402,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
 #pragma unroll
         for (int j = 0; j < TM; ++j) fx[j] = sx[j][b];
     };
-    auto frag = [&](const uint4 *s, int r) {
-        const uint4 u = s[r * 8 + (g ^ (r & 7))], v = s[r * 8 + ((4 + g) ^ (r & 7))];
-        return int8_v{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w};
+    auto frag = [&](const int4_v *s, int r) {
+        return __builtin_shufflevector(s[r * 8 + (g ^ (r & 7))], s[r * 8 + ((4 + g) ^ (r & 7))], 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    auto multiply = [&](const uint4 *s, float c0, float c1, const float (&cx)[TM]) {
+    auto multiply = [&](const int4_v *s, float c0, float c1, const float (&cx)[TM]) {
         int8_v xf[TM];
         half8_v xh[TM][4];
 #pragma unroll
@@ -461,28 +455,43 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // this stage multiplied while the next one's loads are on their way
-    auto step = [&](const uint4 *s, uint4 *next, int b) {
+    // A stage is multiplied while the loads of the next two (EXACT, whose operands take the registers: of the next) are on their way,
+    // and the next is then stored.  Its place was read before the last barrier.
+    constexpr int AHEAD = EXACT ? 1 : 2;
+    const int whole = a.K / FB;
+    int4_v h0[CH], h1[CH];
+    auto step = [&](const int4_v *s, int4_v *next, int4_v (&held)[CH], int4_v (&after)[CH], int b, bool more) {
         float c0 = f0, c1 = f1, cx[TM];
 #pragma unroll
         for (int j = 0; j < TM; ++j) cx[j] = fx[j];
-        stage(next, b + 1);
+        if (AHEAD == 1) load(held, b + 1);
+        else if (more) load(after, b + 2);
         scales(b + 1);
         multiply(s, c0, c1, cx);
-        landed(next);
+        store(held, next);
+        barrier();
     };
-    const int whole = a.K / FB;
     if (whole) {
-        stage(s_0, 0);
+        load(h0, 0);
         scales(0);
-        landed(s_0);
+        if (AHEAD == 2 && whole > 1) load(h1, 1);
+        store(h0, s_0);
+        barrier();
         int b = 0;
-        for (; b + 2 < whole; b += 2) {
-            step(s_0, s_1, b);
-            step(s_1, s_0, b + 1);
+        for (; b + 3 < whole; b += 2) {
+            step(s_0, s_1, h1, h0, b, true);
+            step(s_1, s_0, h0, h1, b + 1, true);
         }
-        if (b + 1 < whole) step(s_0, s_1, b);
-        multiply(b + 1 < whole ? s_1 : s_0, f0, f1, fx);
+        if (b + 2 < whole) {                            // three are left, or two, or one
+            step(s_0, s_1, h1, h0, b, true);
+            step(s_1, s_0, h0, h1, b + 1, false);
+            multiply(s_0, f0, f1, fx);
+        } else if (b + 1 < whole) {
+            step(s_0, s_1, h1, h0, b, false);
+            multiply(s_1, f0, f1, fx);
+        } else {
+            multiply(s_0, f0, f1, fx);
+        }
     }
     if (a.K % FB) {                                     // the last block
         __syncthreads();
@@ -557,23 +566,19 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
     }
 }
 
-template <bool GATED, bool EXACT, bool ALIGNED, int WN, int WM, int TN, int TM>
+template <bool GATED, bool EXACT, int WN, int WM, int TN, int TM>
 static hipError_t launch_tile_n(const Fp8Args &a, hipStream_t st) {
     constexpr int ROWS = 16 * TN * WN / (GATED ? 2 : 1), BM = 16 * TM * WM;
     const int64_t n_tiles = (a.N + ROWS - 1) / ROWS;
-    // with a dispatch: whole runs, and one a used expert that is not whole
+    // (a dispatch: whole runs, and one for each used expert that is not whole)
     const int64_t runs = a.offsets ? a.M / BM + std::min(a.E, a.M) : (a.M + BM - 1) / BM;
-    hipLaunchKernelGGL((fp8_tile_kernel<GATED, EXACT, ALIGNED, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM), 0,
-                       st, a, (int)n_tiles);
+    hipLaunchKernelGGL((fp8_tile_kernel<GATED, EXACT, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM), 0,
+                       st, a, (int)n_tiles, (int)runs);
     return hipGetLastError();
 }
 template <bool GATED, bool EXACT>
 static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
-    auto whole = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0; };
-    const bool al = whole(a.m[0]) && (!GATED || whole(a.m[1])) && ((uintptr_t)a.x | a.ldx) % 16 == 0;
-    if (al && !GATED && !EXACT && a.M >= 2048) return launch_tile_n<GATED, EXACT, true, 2, 4, 8, 4>(a, st);
-    if (al) return launch_tile_n<GATED, EXACT, true, 4, 2, 4, 4>(a, st);
-    return launch_tile_n<GATED, EXACT, false, 4, 2, 4, 4>(a, st);
+    return launch_tile_n<GATED, EXACT, 4, 2, 4, 4>(a, st);
 }
 
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
