@@ -214,6 +214,24 @@ __device__ inline void store_elem(void *p, int64_t i, int type, float v) {
     else ((uint16_t *)p)[i] = Elem<T_F16>::store(v);
 }
 
+// n of four neighbouring elements
+__device__ inline void store4(void *p, int64_t i, int type, float4_v v, int n) {
+    if (n >= 4) {
+        if (type == T_F32) {
+            __builtin_memcpy((float *)p + i, &v, 16);
+        } else {
+            uint16_t q[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) q[k] = type == T_BF16 ? Elem<T_BF16>::store(v[k]) : Elem<T_F16>::store(v[k]);
+            __builtin_memcpy((uint16_t *)p + i, q, 8);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (k < n) store_elem(p, i + k, type, v[k]);
+    }
+}
+
 __device__ inline float silu_times(float g, float u) { return u * (g / (1.0f + expf(-g))); }
 
 // Sixteen rows of a weight (of gate and up: GATED), sixteen rows of x at a time; four waves, every fourth block of K each, whose sums
@@ -331,11 +349,11 @@ __device__ inline void barrier() {
 
 template <bool GATED, bool EXACT, int WN, int WM, int TN, int TM>
 __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n_tiles, int m_tiles) {
-    constexpr int THREADS = 64 * WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, CH = (BN + BM) * 8 / THREADS;
-    static_assert((BN + BM) * 8 % THREADS == 0, "whole loads");
+    constexpr int THREADS = 64 * WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, CH = (BN + BM) * 8 / THREADS, SB = 32;
+    static_assert((BN + BM) * 8 % THREADS == 0 && THREADS % BM == 0 && SB % (THREADS / BM) == 0 && SB * 2 * WN <= THREADS, "whole loads");
     __shared__ int4_v s_0[(BN + BM) * 8], s_1[(BN + BM) * 8];
     __shared__ int s_run[4];
-    __shared__ float s_max[WN][BM];
+    __shared__ float s_max[WN][BM], s_sx[SB][BM], s_sw[SB][2 * WN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     const int wn = wave % WN, wm = wave / WN;
     int e = 0, p0, end = a.M;
@@ -353,7 +371,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
         p0 = (8 * strip + in % wide) * BM;
     }
     constexpr int ROWS = GATED ? BN / 2 : BN;           // rows of y's columns
-    const int n0 = n_tile * ROWS;
+    const int n0 = n_tile * ROWS, nb = (a.K + FB - 1) / FB;
 
     // the row that chunk q of a stage is of, and which of its chunks
     auto row_of = [&](int q) -> const uint8_t * {
@@ -381,31 +399,34 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
 #pragma unroll
         for (int i = 0; i < CH; ++i) s[i * THREADS + threadIdx.x] = h[i];
     };
-    // the scales of a block: of the weight's rows (gate's and up's), and of a lane's row of x in each tile
-    const float *sw0, *sw1 = nullptr, *sx[TM];
-    {
-        const int nblk = (n0 + (GATED ? wn * 8 * TN : wn * 16 * TN)) / FB;
-        const int last = (a.N - 1) / FB;
-        sw0 = a.m[0].s + e * a.m[0].sex + (int64_t)min(nblk, last) * a.m[0].sld;
-        if (GATED) sw1 = a.m[1].s + e * a.m[1].sex + (int64_t)min(nblk, last) * a.m[1].sld;
+    // The scales of SB blocks, by block: of the rows of x, and of each wave's rows of the weight (of gate and up).  Read one block at a
+    // time, each row's would be a line of its own for every block.
+    auto load_scales = [&](int b0) {
+        constexpr int PER = THREADS / BM, EACH = SB / PER;
+        const int col = threadIdx.x % BM, first = threadIdx.x / BM * EACH;
+        const int p = min(p0 + col, end - 1);
+        const float *sx = a.xs + (int64_t)(a.top ? a.perm[p] / a.top : p) * a.ldxs;
+        float v[EACH];
 #pragma unroll
-        for (int j = 0; j < TM; ++j) {
-            const int p = min(p0 + (wm * TM + j) * 16 + c, end - 1);
-            sx[j] = a.xs + (int64_t)(a.top ? a.perm[p] / a.top : p) * a.ldxs;
+        for (int i = 0; i < EACH; ++i) v[i] = b0 + first + i < nb ? sx[b0 + first + i] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) s_sx[first + i][col] = v[i];
+        if (threadIdx.x < SB * 2 * WN) {
+            const int i = threadIdx.x / (2 * WN), w = threadIdx.x % (2 * WN) / 2, up = GATED && threadIdx.x % 2;
+            const Fp8Mat &m = a.m[up];
+            const int block = min((n0 + w * (GATED ? 8 : 16) * TN) / FB, (a.N - 1) / FB);
+            s_sw[i][threadIdx.x % (2 * WN)] = b0 + i < nb ? m.s[e * m.sex + block * m.sld + b0 + i] : 0.0f;
         }
-    }
-    float4_v acc[TN][TM] = {};
-    float fx[TM], f0, f1 = 0.0f;
-    auto scales = [&](int b) {
-        f0 = sw0[b];
-        if (GATED) f1 = sw1[b];
-#pragma unroll
-        for (int j = 0; j < TM; ++j) fx[j] = sx[j][b];
     };
+    float4_v acc[TN][TM] = {};
     auto frag = [&](const int4_v *s, int r) {
         return __builtin_shufflevector(s[r * 8 + (g ^ (r & 7))], s[r * 8 + ((4 + g) ^ (r & 7))], 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    auto multiply = [&](const int4_v *s, float c0, float c1, const float (&cx)[TM]) {
+    auto multiply = [&](const int4_v *s, int b) {
+        const float c0 = s_sw[b % SB][2 * wn], c1 = GATED ? s_sw[b % SB][2 * wn + 1] : 0.0f;
+        float cx[TM];
+#pragma unroll
+        for (int j = 0; j < TM; ++j) cx[j] = s_sx[b % SB][(wm * TM + j) * 16 + c];
         int8_v xf[TM];
         half8_v xh[TM][4];
 #pragma unroll
@@ -461,19 +482,23 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
     const int whole = a.K / FB;
     int4_v h0[CH], h1[CH];
     auto step = [&](const int4_v *s, int4_v *next, int4_v (&held)[CH], int4_v (&after)[CH], int b, bool more) {
-        float c0 = f0, c1 = f1, cx[TM];
-#pragma unroll
-        for (int j = 0; j < TM; ++j) cx[j] = fx[j];
         if (AHEAD == 1) load(held, b + 1);
         else if (more) load(after, b + 2);
-        scales(b + 1);
-        multiply(s, c0, c1, cx);
+        multiply(s, b);
+#pragma unroll
+        for (int i = 0; i < TN; ++i)                    // the sums are done here, not after the barrier
+#pragma unroll
+            for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(acc[i][j]));
         store(held, next);
+        if ((b + 1) % SB == 0) {
+            barrier();
+            load_scales(b + 1);
+        }
         barrier();
     };
+    load_scales(0);
     if (whole) {
         load(h0, 0);
-        scales(0);
         if (AHEAD == 2 && whole > 1) load(h1, 1);
         store(h0, s_0);
         barrier();
@@ -485,12 +510,12 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
         if (b + 2 < whole) {                            // three are left, or two, or one
             step(s_0, s_1, h1, h0, b, true);
             step(s_1, s_0, h0, h1, b + 1, false);
-            multiply(s_0, f0, f1, fx);
+            multiply(s_0, b + 2);
         } else if (b + 1 < whole) {
             step(s_0, s_1, h1, h0, b, false);
-            multiply(s_1, f0, f1, fx);
+            multiply(s_1, b + 1);
         } else {
-            multiply(s_0, f0, f1, fx);
+            multiply(s_0, b);
         }
     }
     if (a.K % FB) {                                     // the last block
@@ -500,9 +525,9 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
             const int k = whole * FB + 16 * chunk_of(q);
             s_0[q] = load16(row_of(q) + k, a.K - k);
         }
-        scales(whole);
+        if (whole % SB == 0 && whole) load_scales(whole);
         __syncthreads();
-        multiply(s_0, f0, f1, fx);
+        multiply(s_0, whole);
     }
 
     if (GATED) {
@@ -559,9 +584,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
 #pragma unroll
         for (int i = 0; i < TN; ++i) {
             const int n = n0 + (wn * TN + i) * 16 + 4 * g;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (n + k < a.N) store_elem(a.y, p * a.ldy + n + k, a.y_type, a.pair_w ? w * acc[i][j][k] : acc[i][j][k]);
+            store4(a.y, p * a.ldy + n, a.y_type, a.pair_w ? acc[i][j] * w : acc[i][j], a.N - n);
         }
     }
 }
