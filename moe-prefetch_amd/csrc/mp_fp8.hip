@@ -340,6 +340,9 @@ __device__ inline bool find_run(const int32_t *offsets, int E, int bm, int slot,
     return s_run[3] != 0;
 }
 
+// every load of the wave's but the last N is done
+template <int N>
+__device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // a barrier that leaves loads from memory on their way
 __device__ inline void barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -347,13 +350,14 @@ __device__ inline void barrier() {
     asm volatile("" ::: "memory");
 }
 
-template <bool GATED, bool EXACT, int WN, int WM, int TN, int TM>
+// ALIGNED: rows begin on 16 bytes
+template <bool GATED, bool EXACT, bool ALIGNED, int WN, int WM, int TN, int TM>
 __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n_tiles, int m_tiles) {
-    constexpr int THREADS = 64 * WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, CH = (BN + BM) * 8 / THREADS, SB = 32;
-    static_assert((BN + BM) * 8 % THREADS == 0 && THREADS % BM == 0 && SB % (THREADS / BM) == 0 && SB * 2 * WN <= THREADS, "whole loads");
-    __shared__ int4_v s_0[(BN + BM) * 8], s_1[(BN + BM) * 8];
+    constexpr int THREADS = 64 * WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, CH = (BN + BM) * 8 / THREADS, SB = 6;
+    static_assert((BN + BM) * 8 % THREADS == 0 && THREADS % BM == 0 && SB * 2 * WN <= THREADS, "whole loads");
+    __shared__ int4_v s_0[(BN + BM) * 8], s_1[ALIGNED ? (BN + BM) * 8 : 1], s_2[ALIGNED ? (BN + BM) * 8 : 1];
     __shared__ int s_run[4];
-    __shared__ float s_max[WN][BM], s_sx[SB][BM], s_sw[SB][2 * WN];
+    __shared__ float s_max[WN][BM], s_sx[2][SB][BM], s_sw[2][SB][2 * WN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     const int wn = wave % WN, wm = wave / WN;
     int e = 0, p0, end = a.M;
@@ -374,7 +378,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
     const int n0 = n_tile * ROWS, nb = (a.K + FB - 1) / FB;
 
     // the row that chunk q of a stage is of, and which of its chunks
-    auto row_of = [&](int q) -> const uint8_t * {
+    auto row_of = [&](int q) __attribute__((always_inline)) -> const uint8_t * {
         const int r = q >> 3;
         if (r >= BN) {
             const int p = min(p0 + r - BN, end - 1);
@@ -391,60 +395,70 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
         const int q = i * THREADS + threadIdx.x;
         src[i] = row_of(q) + 16 * chunk_of(q);
     }
-    auto load = [&](int4_v (&h)[CH], int b) {           // a thread's chunks of a stage
+    // a whole block's loads, to LDS without registers
+    auto stage = [&](int4_v *s, int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) h[i] = *(const int4_u *)(src[i] + (int64_t)b * FB);
-    };
-    auto store = [&](const int4_v (&h)[CH], int4_v *s) {
-#pragma unroll
-        for (int i = 0; i < CH; ++i) s[i * THREADS + threadIdx.x] = h[i];
+        for (int i = 0; i < CH; ++i)
+            __builtin_amdgcn_global_load_lds((const void *)(src[i] + (int64_t)b * FB),
+                                             (__attribute__((address_space(3))) void *)(s + i * THREADS + 64 * wave), 16, 0, 0);
     };
     // The scales of SB blocks, by block: of the rows of x, and of each wave's rows of the weight (of gate and up).  Read one block at a
     // time, each row's would be a line of its own for every block.
-    auto load_scales = [&](int b0) {
-        constexpr int PER = THREADS / BM, EACH = SB / PER;
-        const int col = threadIdx.x % BM, first = threadIdx.x / BM * EACH;
-        const int p = min(p0 + col, end - 1);
-        const float *sx = a.xs + (int64_t)(a.top ? a.perm[p] / a.top : p) * a.ldxs;
-        float v[EACH];
+    constexpr int PER = THREADS / BM, EACH = (SB + PER - 1) / PER;
+    const float *from_x, *from_w;
+    {
+        const int p = min(p0 + (int)threadIdx.x % BM, end - 1);
+        from_x = a.xs + (int64_t)(a.top ? a.perm[p] / a.top : p) * a.ldxs;
+        const int w = threadIdx.x % (2 * WN) / 2;
+        const Fp8Mat &m = a.m[GATED && threadIdx.x % 2];
+        from_w = m.s + e * m.sex + (int64_t)min((n0 + w * (GATED ? 8 : 16) * TN) / FB, (a.N - 1) / FB) * m.sld;
+    }
+    float held_x[EACH], held_w = 0.0f;
+    auto fetch_scales = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) v[i] = b0 + first + i < nb ? sx[b0 + first + i] : 0.0f;
+        for (int i = 0; i < EACH; ++i) held_x[i] = from_x[min(b + (int)threadIdx.x / BM + PER * i, nb - 1)];
+        if (threadIdx.x < SB * 2 * WN) held_w = from_w[min(b + (int)threadIdx.x / (2 * WN), nb - 1)];
+    };
+    auto put_scales = [&](int par) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) s_sx[first + i][col] = v[i];
-        if (threadIdx.x < SB * 2 * WN) {
-            const int i = threadIdx.x / (2 * WN), w = threadIdx.x % (2 * WN) / 2, up = GATED && threadIdx.x % 2;
-            const Fp8Mat &m = a.m[up];
-            const int block = min((n0 + w * (GATED ? 8 : 16) * TN) / FB, (a.N - 1) / FB);
-            s_sw[i][threadIdx.x % (2 * WN)] = b0 + i < nb ? m.s[e * m.sex + block * m.sld + b0 + i] : 0.0f;
-        }
+        for (int i = 0; i < EACH; ++i)
+            if (SB % PER == 0 || threadIdx.x / BM + PER * i < SB) s_sx[par][threadIdx.x / BM + PER * i][threadIdx.x % BM] = held_x[i];
+        if (threadIdx.x < SB * 2 * WN) s_sw[par][threadIdx.x / (2 * WN)][threadIdx.x % (2 * WN)] = held_w;
     };
     float4_v acc[TN][TM] = {};
-    auto frag = [&](const int4_v *s, int r) {
+    auto frag = [&](const int4_v *s, int r) __attribute__((always_inline)) {
         return __builtin_shufflevector(s[r * 8 + (g ^ (r & 7))], s[r * 8 + ((4 + g) ^ (r & 7))], 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    auto multiply = [&](const int4_v *s, int b) {
-        const float c0 = s_sw[b % SB][2 * wn], c1 = GATED ? s_sw[b % SB][2 * wn + 1] : 0.0f;
-        float cx[TM];
+    struct Operands {                                   // what a wave's first row of tiles of a stage needs
+        int8_v x[TM], w;
+        float f0, f1, fx[TM];
+    };
+    auto fetch = [&](Operands &o, const int4_v *s, int par, int u) __attribute__((always_inline)) {
+        o.w = frag(s, wn * TN * 16 + c);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) cx[j] = s_sx[b % SB][(wm * TM + j) * 16 + c];
-        int8_v xf[TM];
+        for (int j = 0; j < TM; ++j) o.x[j] = frag(s, BN + (wm * TM + j) * 16 + c);
+        o.f0 = s_sw[par][u][2 * wn];
+        o.f1 = GATED ? s_sw[par][u][2 * wn + 1] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < TM; ++j) o.fx[j] = s_sx[par][u][(wm * TM + j) * 16 + c];
+    };
+    // A stage's products, a row of tiles' while the row before is scaled and added (EXACT: products take four times as long, and their
+    // operands the registers of that) and the row after is read; before the last row, when every read of the stage is done, then().
+    auto multiply = [&](const int4_v *s, const Operands &o, auto then) __attribute__((always_inline)) {
         half8_v xh[TM][4];
+        if (EXACT)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) {
-            xf[j] = frag(s, BN + (wm * TM + j) * 16 + c);
-            if (EXACT)
+            for (int j = 0; j < TM; ++j)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) xh[j][k] = halves(xf[j][2 * k], xf[j][2 * k + 1]);
-        }
-        // a row of tiles' products while the row before is scaled and added (EXACT: products take four times as long, and
-        // their operands the registers of that), and the row after is read
+                for (int k = 0; k < 4; ++k) xh[j][k] = halves(o.x[j][2 * k], o.x[j][2 * k + 1]);
         constexpr int LAG = EXACT ? 0 : 1;
-        int8_v wf = frag(s, wn * TN * 16 + c);
+        int8_v wf = o.w;
         float4_v d[LAG + 1][TM];
 #pragma unroll
         for (int i = 0; i < TN + LAG; ++i) {
             int8_v wnext;
             if (i + 1 < TN) wnext = frag(s, (wn * TN + i + 1) * 16 + c);
+            if (i == TN - 1) then();
             if (i < TN) {
                 half8_v wh[4];
                 if (EXACT)
@@ -458,64 +472,85 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
                         for (int k = 0; k < 4; ++k) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[k], xh[j][k], t, 0, 0, 0);
                         d[0][j] = t;
                     } else {
-                        d[i & LAG][j] = mfma_e4m3(wf, xf[j]);
+                        d[i & LAG][j] = mfma_e4m3(wf, o.x[j]);
                     }
                 }
             }
+            if (LAG) __builtin_amdgcn_sched_barrier(0);     // first the products
             const int l = i - LAG;
             if (l >= 0) {
-                const float sw = GATED && l >= TN / 2 ? c1 : c0;
+                const float sw = GATED && l >= TN / 2 ? o.f1 : o.f0;
 #pragma unroll
                 for (int j = 0; j < TM; ++j) {
-                    const float f = cx[j] * sw;
+                    const float f = o.fx[j] * sw;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) acc[l][j][k] = fmaf(d[l & LAG][j][k], f, acc[l][j][k]);
+                    asm volatile("" : "+v"(acc[l][j]));     // here, not further on, where every product would wait in registers
                 }
             }
             wf = wnext;
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // A stage is multiplied while the loads of the next two (EXACT, whose operands take the registers: of the next) are on their way,
-    // and the next is then stored.  Its place was read before the last barrier.
-    constexpr int AHEAD = EXACT ? 1 : 2;
+    auto nothing = []() {};
     const int whole = a.K / FB;
-    int4_v h0[CH], h1[CH];
-    auto step = [&](const int4_v *s, int4_v *next, int4_v (&held)[CH], int4_v (&after)[CH], int b, bool more) {
-        if (AHEAD == 1) load(held, b + 1);
-        else if (more) load(after, b + 2);
-        multiply(s, b);
-#pragma unroll
-        for (int i = 0; i < TN; ++i)                    // the sums are done here, not after the barrier
-#pragma unroll
-            for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(acc[i][j]));
-        store(held, next);
-        if ((b + 1) % SB == 0) {
-            barrier();
-            load_scales(b + 1);
-        }
+    int b = 0, par = 0;
+    Operands o0, o1;
+    if (ALIGNED && whole) {
+        // Three stages: one is multiplied while the loads of the two after it are on their way.  Before its last row of tiles, when
+        // every wave has read all of it, its place is loaded anew and the next stage's first operands are read.  At the end of K the
+        // loads are of its last block again, so that every step is alike.  Steps stand in the code one by one, each with its own places in
+        // LDS, so that reads wait for the loads to their own place alone; at the loop's head they wait for all.
+        auto step = [&](int4_v *s, const int4_v *next, const Operands &o, Operands &on, int u) __attribute__((always_inline)) {
+            multiply(s, o, [&]() __attribute__((always_inline)) {
+                if (u == SB - 1) put_scales(par ^= 1);
+                wait_loads<CH>();                       // the next stage is there
+                barrier();                              // and every wave's part of it
+                stage(s, min(b + u + 3, whole - 1));
+                fetch(on, next, par, (u + 1) % SB);
+            });
+        };
+        auto steps = [&](int n) __attribute__((always_inline)) {
+            step(s_0, s_1, o0, o1, 0);
+            if (n > 1) step(s_1, s_2, o1, o0, 1);
+            if (n > 2) step(s_2, s_0, o0, o1, 2);
+            if (n > 3) step(s_0, s_1, o1, o0, 3);
+            if (n > 4) step(s_1, s_2, o0, o1, 4);
+            if (n > 5) step(s_2, s_0, o1, o0, 5);
+        };
+        fetch_scales(0);
+        stage(s_0, 0);
+        stage(s_1, min(1, whole - 1));
+        stage(s_2, min(2, whole - 1));
+        put_scales(0);
+        wait_loads<2 * CH>();
         barrier();
-    };
-    load_scales(0);
-    if (whole) {
-        load(h0, 0);
-        if (AHEAD == 2 && whole > 1) load(h1, 1);
-        store(h0, s_0);
-        barrier();
-        int b = 0;
-        for (; b + 3 < whole; b += 2) {
-            step(s_0, s_1, h1, h0, b, true);
-            step(s_1, s_0, h0, h1, b + 1, true);
+        fetch(o0, s_0, 0, 0);
+        for (; b + SB <= whole; b += SB) {
+            fetch_scales(b + SB);
+            steps(SB);
         }
-        if (b + 2 < whole) {                            // three are left, or two, or one
-            step(s_0, s_1, h1, h0, b, true);
-            step(s_1, s_0, h0, h1, b + 1, false);
-            multiply(s_0, b + 2);
-        } else if (b + 1 < whole) {
-            step(s_0, s_1, h1, h0, b, false);
-            multiply(s_1, b + 1);
-        } else {
-            multiply(s_0, b);
+        if (b < whole) steps(whole - b);
+        wait_loads<0>();
+    } else {
+        fetch_scales(0);
+        put_scales(0);
+        for (; b < whole; b += SB) {
+#pragma unroll 1
+            for (int u = 0; u < SB && b + u < whole; ++u) {
+                int4_v held[CH];
+#pragma unroll
+                for (int i = 0; i < CH; ++i) held[i] = *(const int4_u *)(src[i] + (int64_t)(b + u) * FB);
+                __syncthreads();                        // the stage is free
+#pragma unroll
+                for (int i = 0; i < CH; ++i) s_0[i * THREADS + threadIdx.x] = held[i];
+                __syncthreads();
+                fetch(o0, s_0, par, u);
+                multiply(s_0, o0, nothing);
+            }
+            if (b + SB > whole) break;
+            fetch_scales(b + SB);
+            put_scales(par ^= 1);
         }
     }
     if (a.K % FB) {                                     // the last block
@@ -525,9 +560,9 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
             const int k = whole * FB + 16 * chunk_of(q);
             s_0[q] = load16(row_of(q) + k, a.K - k);
         }
-        if (whole % SB == 0 && whole) load_scales(whole);
         __syncthreads();
-        multiply(s_0, whole);
+        fetch(o0, s_0, par, whole - b);
+        multiply(s_0, o0, nothing);
     }
 
     if (GATED) {
@@ -589,19 +624,22 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
     }
 }
 
-template <bool GATED, bool EXACT, int WN, int WM, int TN, int TM>
+template <bool GATED, bool EXACT, bool ALIGNED, int WN, int WM, int TN, int TM>
 static hipError_t launch_tile_n(const Fp8Args &a, hipStream_t st) {
     constexpr int ROWS = 16 * TN * WN / (GATED ? 2 : 1), BM = 16 * TM * WM;
     const int64_t n_tiles = (a.N + ROWS - 1) / ROWS;
     // (a dispatch: whole runs, and one for each used expert that is not whole)
     const int64_t runs = a.offsets ? a.M / BM + std::min(a.E, a.M) : (a.M + BM - 1) / BM;
-    hipLaunchKernelGGL((fp8_tile_kernel<GATED, EXACT, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM), 0,
+    hipLaunchKernelGGL((fp8_tile_kernel<GATED, EXACT, ALIGNED, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM), 0,
                        st, a, (int)n_tiles, (int)runs);
     return hipGetLastError();
 }
 template <bool GATED, bool EXACT>
 static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
-    return launch_tile_n<GATED, EXACT, 4, 2, 4, 4>(a, st);
+    auto whole = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0; };
+    const bool aligned = whole(a.m[0]) && (!GATED || whole(a.m[1])) && ((uintptr_t)a.x | a.ldx) % 16 == 0;
+    if (!aligned) return launch_tile_n<GATED, EXACT, false, 4, 2, 4, 4>(a, st);
+    return launch_tile_n<GATED, EXACT, true, 4, 2, 4, 4>(a, st);
 }
 
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
