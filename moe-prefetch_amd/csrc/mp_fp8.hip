@@ -350,12 +350,12 @@ __device__ inline void barrier() {
     asm volatile("" ::: "memory");
 }
 
-// ALIGNED: rows begin on 16 bytes
-template <bool GATED, bool EXACT, bool ALIGNED, int WN, int WM, int TN, int TM>
+// NS stages; 1: rows of any alignment, through registers
+template <bool GATED, bool EXACT, int NS, int WN, int WM, int TN, int TM>
 __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n_tiles, int m_tiles) {
     constexpr int THREADS = 64 * WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, CH = (BN + BM) * 8 / THREADS, SB = 6;
-    static_assert((BN + BM) * 8 % THREADS == 0 && THREADS % BM == 0 && SB * 2 * WN <= THREADS, "whole loads");
-    __shared__ int4_v s_0[(BN + BM) * 8], s_1[ALIGNED ? (BN + BM) * 8 : 1], s_2[ALIGNED ? (BN + BM) * 8 : 1];
+    static_assert((BN + BM) * 8 % THREADS == 0 && BN * 8 % THREADS == 0 && THREADS % BM == 0 && SB * 2 * WN <= THREADS, "whole loads");
+    __shared__ int4_v s_0[(BN + BM) * 8], s_1[NS > 1 ? (BN + BM) * 8 : 1], s_2[NS > 2 ? (BN + BM) * 8 : 1];
     __shared__ int s_run[4];
     __shared__ float s_max[WN][BM], s_sx[2][SB][BM], s_sw[2][SB][2 * WN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
@@ -377,30 +377,43 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
     constexpr int ROWS = GATED ? BN / 2 : BN;           // rows of y's columns
     const int n0 = n_tile * ROWS, nb = (a.K + FB - 1) / FB;
 
-    // the row that chunk q of a stage is of, and which of its chunks
-    auto row_of = [&](int q) __attribute__((always_inline)) -> const uint8_t * {
+    // The row of chunk q of a stage: of a weight, from n0 on (a wave's rows: TN / 2 tiles of gate and as many of up), or of x; and which of its
+    // chunks it is
+    auto weight_row = [&](int q) __attribute__((always_inline)) {
         const int r = q >> 3;
-        if (r >= BN) {
-            const int p = min(p0 + r - BN, end - 1);
-            return a.x + (int64_t)(a.top ? a.perm[p] / a.top : p) * a.ldx;
-        }
-        const int w = r / (16 * TN), t = r % (16 * TN);  // a wave's rows: TN / 2 tiles of gate and as many of up
-        const Fp8Mat &m = a.m[GATED && t >= 8 * TN];
-        return m.w + e * m.ex + (int64_t)min(n0 + (GATED ? w * 8 * TN + t % (8 * TN) : r), a.N - 1) * m.ld;
+        return min(GATED ? r / (16 * TN) * 8 * TN + r % (8 * TN) : r, a.N - 1 - n0);
     };
-    auto chunk_of = [](int q) { return (q & 7) ^ (q >> 3 & 7); };
+    auto is_up = [](int q) __attribute__((always_inline)) { return GATED && (q >> 3) % (16 * TN) >= 8 * TN; };
+    auto x_row = [&](int q) __attribute__((always_inline)) -> int64_t {
+        const int p = min(p0 + (q >> 3) - BN, end - 1);
+        return a.top ? a.perm[p] / a.top : p;
+    };
+    auto chunk_of = [](int q) __attribute__((always_inline)) { return (q & 7) ^ (q >> 3 & 7); };
+    const uint8_t *const w0 = a.m[0].w + e * a.m[0].ex + n0 * a.m[0].ld, *const w1 = GATED ? a.m[1].w + e * a.m[1].ex + n0 * a.m[1].ld : w0;
+    auto row_of = [&](int q) __attribute__((always_inline)) -> const uint8_t * {
+        if (q >= BN * 8) return a.x + x_row(q) * a.ldx;
+        return is_up(q) ? w1 + weight_row(q) * a.m[1].ld : w0 + weight_row(q) * a.m[0].ld;
+    };
+    // a whole block's loads, to LDS without registers: a place that is the same for all lanes, and a lane's 32 bits from there
+    const uint8_t *const x0 = a.top ? a.x : a.x + p0 * a.ldx;
+    uint32_t from[CH];
     const uint8_t *src[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int q = i * THREADS + threadIdx.x;
-        src[i] = row_of(q) + 16 * chunk_of(q);
+        if (NS == 1) src[i] = row_of(q) + 16 * chunk_of(q);
+        else if (i * THREADS < BN * 8) from[i] = (uint32_t)(weight_row(q) * (is_up(q) ? a.m[1].ld : a.m[0].ld)) + 16 * chunk_of(q);
+        else from[i] = (uint32_t)((x_row(q) - (a.top ? 0 : p0)) * a.ldx) + 16 * chunk_of(q);
     }
-    // a whole block's loads, to LDS without registers
     auto stage = [&](int4_v *s, int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i)
-            __builtin_amdgcn_global_load_lds((const void *)(src[i] + (int64_t)b * FB),
-                                             (__attribute__((address_space(3))) void *)(s + i * THREADS + 64 * wave), 16, 0, 0);
+        for (int i = 0; i < CH; ++i) {
+            // (a wave's 64 chunks are eight rows, all of gate, of up or of x)
+            const uint8_t *base = (i * THREADS >= BN * 8 ? x0 : is_up(i * THREADS + 64 * wave) ? w1 : w0) + (int64_t)b * FB;
+            uint32_t o = from[i];
+            asm volatile("" : "+v"(o));                 // (not a pointer kept for every chunk)
+            __builtin_amdgcn_global_load_lds((const void *)(base + o), (__attribute__((address_space(3))) void *)(s + i * THREADS + 64 * wave), 16, 0, 0);
+        }
     };
     // The scales of SB blocks, by block: of the rows of x, and of each wave's rows of the weight (of gate and up).  Read one block at a
     // time, each row's would be a line of its own for every block.
@@ -451,7 +464,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
             for (int j = 0; j < TM; ++j)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) xh[j][k] = halves(o.x[j][2 * k], o.x[j][2 * k + 1]);
-        constexpr int LAG = EXACT ? 0 : 1;
+        constexpr int LAG = EXACT || TN * TM > 16 ? 0 : 1;
         int8_v wf = o.w;
         float4_v d[LAG + 1][TM];
 #pragma unroll
@@ -496,36 +509,59 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
     const int whole = a.K / FB;
     int b = 0, par = 0;
     Operands o0, o1;
-    if (ALIGNED && whole) {
-        // Three stages: one is multiplied while the loads of the two after it are on their way.  Before its last row of tiles, when
-        // every wave has read all of it, its place is loaded anew and the next stage's first operands are read.  At the end of K the
-        // loads are of its last block again, so that every step is alike.  Steps stand in the code one by one, each with its own places in
-        // LDS, so that reads wait for the loads to their own place alone; at the loop's head they wait for all.
-        auto step = [&](int4_v *s, const int4_v *next, const Operands &o, Operands &on, int u) __attribute__((always_inline)) {
-            multiply(s, o, [&]() __attribute__((always_inline)) {
+    if (NS > 1 && whole) {
+        // Steps stand in the code one by one, each with its own places in LDS, so that reads wait for the loads to their own place alone; at
+        // the loop's head they wait for all.  At the end of K the loads are of its last block again, so that every step is alike.
+        // Three stages: one is multiplied while the loads of the two after it are on their way.  Before its last row of tiles, when every
+        // wave has read all of it, its place is loaded anew and the next stage's first operands are read.
+        // Two: one is multiplied while the other is loaded.
+        auto step = [&](int4_v *s, int4_v *next, Operands &o, Operands &on, int u) __attribute__((always_inline)) {
+            if (NS == 3) {
+                multiply(s, o, [&]() __attribute__((always_inline)) {
+                    if (u == SB - 1) put_scales(par ^= 1);
+                    wait_loads<CH>();                   // the next stage is there
+                    barrier();                          // and every wave's part of it
+                    stage(s, min(b + u + 3, whole - 1));
+                    fetch(on, next, par, (u + 1) % SB);
+                });
+            } else {
+                wait_loads<0>();
+                barrier();                              // this stage is there, and the other free
+                stage(next, min(b + u + 1, whole - 1));
+                fetch(o0, s, par, u);
+                multiply(s, o0, nothing);
                 if (u == SB - 1) put_scales(par ^= 1);
-                wait_loads<CH>();                       // the next stage is there
-                barrier();                              // and every wave's part of it
-                stage(s, min(b + u + 3, whole - 1));
-                fetch(on, next, par, (u + 1) % SB);
-            });
+            }
         };
         auto steps = [&](int n) __attribute__((always_inline)) {
-            step(s_0, s_1, o0, o1, 0);
-            if (n > 1) step(s_1, s_2, o1, o0, 1);
-            if (n > 2) step(s_2, s_0, o0, o1, 2);
-            if (n > 3) step(s_0, s_1, o1, o0, 3);
-            if (n > 4) step(s_1, s_2, o0, o1, 4);
-            if (n > 5) step(s_2, s_0, o1, o0, 5);
+            if (NS == 3) {
+                step(s_0, s_1, o0, o1, 0);
+                if (n > 1) step(s_1, s_2, o1, o0, 1);
+                if (n > 2) step(s_2, s_0, o0, o1, 2);
+                if (n > 3) step(s_0, s_1, o1, o0, 3);
+                if (n > 4) step(s_1, s_2, o0, o1, 4);
+                if (n > 5) step(s_2, s_0, o1, o0, 5);
+            } else {
+                step(s_0, s_1, o0, o1, 0);
+                if (n > 1) step(s_1, s_0, o0, o1, 1);
+                if (n > 2) step(s_0, s_1, o0, o1, 2);
+                if (n > 3) step(s_1, s_0, o0, o1, 3);
+                if (n > 4) step(s_0, s_1, o0, o1, 4);
+                if (n > 5) step(s_1, s_0, o0, o1, 5);
+            }
         };
         fetch_scales(0);
         stage(s_0, 0);
-        stage(s_1, min(1, whole - 1));
-        stage(s_2, min(2, whole - 1));
+        if (NS == 3) {
+            stage(s_1, min(1, whole - 1));
+            stage(s_2, min(2, whole - 1));
+        }
         put_scales(0);
-        wait_loads<2 * CH>();
-        barrier();
-        fetch(o0, s_0, 0, 0);
+        if (NS == 3) {
+            wait_loads<2 * CH>();
+            barrier();
+            fetch(o0, s_0, 0, 0);
+        }
         for (; b + SB <= whole; b += SB) {
             fetch_scales(b + SB);
             steps(SB);
@@ -624,22 +660,25 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
     }
 }
 
-template <bool GATED, bool EXACT, bool ALIGNED, int WN, int WM, int TN, int TM>
+template <bool GATED, bool EXACT, int NS, int WN, int WM, int TN, int TM>
 static hipError_t launch_tile_n(const Fp8Args &a, hipStream_t st) {
     constexpr int ROWS = 16 * TN * WN / (GATED ? 2 : 1), BM = 16 * TM * WM;
     const int64_t n_tiles = (a.N + ROWS - 1) / ROWS;
     // (a dispatch: whole runs, and one for each used expert that is not whole)
     const int64_t runs = a.offsets ? a.M / BM + std::min(a.E, a.M) : (a.M + BM - 1) / BM;
-    hipLaunchKernelGGL((fp8_tile_kernel<GATED, EXACT, ALIGNED, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM), 0,
+    hipLaunchKernelGGL((fp8_tile_kernel<GATED, EXACT, NS, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM), 0,
                        st, a, (int)n_tiles, (int)runs);
     return hipGetLastError();
 }
 template <bool GATED, bool EXACT>
 static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
-    auto whole = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0; };
-    const bool aligned = whole(a.m[0]) && (!GATED || whole(a.m[1])) && ((uintptr_t)a.x | a.ldx) % 16 == 0;
-    if (!aligned) return launch_tile_n<GATED, EXACT, false, 4, 2, 4, 4>(a, st);
-    return launch_tile_n<GATED, EXACT, true, 4, 2, 4, 4>(a, st);
+    // rows on 16 bytes, and a workgroup's within 4 GiB (those of x from a dispatch: all)
+    auto near = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0 && 256 * m.ld < 1ll << 32; };
+    const int64_t rows = a.top ? (a.M + a.top - 1) / a.top : 256;
+    if (!near(a.m[0]) || (GATED && !near(a.m[1])) || ((uintptr_t)a.x | a.ldx) % 16 || a.ldx * rows >= 1ll << 32)
+        return launch_tile_n<GATED, EXACT, 1, 4, 2, 4, 4>(a, st);
+    if (!GATED && !EXACT && !a.offsets && a.M >= 4096) return launch_tile_n<GATED, EXACT, 2, 2, 4, 8, 4>(a, st);
+    return launch_tile_n<GATED, EXACT, 3, 4, 2, 4, 4>(a, st);
 }
 
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
