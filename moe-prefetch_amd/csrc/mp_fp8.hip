@@ -405,9 +405,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
         else if (i * THREADS < BN * 8) from[i] = (uint32_t)(weight_row(q) * (is_up(q) ? a.m[1].ld : a.m[0].ld)) + 16 * chunk_of(q);
         else from[i] = (uint32_t)((x_row(q) - (a.top ? 0 : p0)) * a.ldx) + 16 * chunk_of(q);
     }
-    auto stage = [&](int4_v *s, int b) __attribute__((always_inline)) {
+    auto stage = [&](int4_v *s, int b, int first, int n) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
+            if (i < first || i >= first + n) continue;
             // (a wave's 64 chunks are eight rows, all of gate, of up or of x)
             const uint8_t *base = (i * THREADS >= BN * 8 ? x0 : is_up(i * THREADS + 64 * wave) ? w1 : w0) + (int64_t)b * FB;
             uint32_t o = from[i];
@@ -456,8 +457,9 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
         for (int j = 0; j < TM; ++j) o.fx[j] = s_sx[par][u][(wm * TM + j) * 16 + c];
     };
     // A stage's products, a row of tiles' while the row before is scaled and added (EXACT: products take four times as long, and their
-    // operands the registers of that) and the row after is read; before the last row, when every read of the stage is done, then().
-    auto multiply = [&](const int4_v *s, const Operands &o, auto then) __attribute__((always_inline)) {
+    // operands the registers of that) and the row after is read; before the last row, when every read of the stage is done, then(); in each
+    // row, after its products, along(row).
+    auto multiply = [&](const int4_v *s, const Operands &o, auto then, auto along) __attribute__((always_inline)) {
         half8_v xh[TM][4];
         if (EXACT)
 #pragma unroll
@@ -490,6 +492,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
                 }
             }
             if (LAG) __builtin_amdgcn_sched_barrier(0);     // first the products
+            if (i < TN) along(i);
             const int l = i - LAG;
             if (l >= 0) {
                 const float sw = GATED && l >= TN / 2 ? o.f1 : o.f0;
@@ -513,52 +516,52 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
         // Steps stand in the code one by one, each with its own places in LDS, so that reads wait for the loads to their own place alone; at
         // the loop's head they wait for all.  At the end of K the loads are of its last block again, so that every step is alike.
         // Three stages: one is multiplied while the loads of the two after it are on their way.  Before its last row of tiles, when every
-        // wave has read all of it, its place is loaded anew and the next stage's first operands are read.
-        // Two: one is multiplied while the other is loaded.
-        auto step = [&](int4_v *s, int4_v *next, Operands &o, Operands &on, int u) __attribute__((always_inline)) {
+        // wave has read all of it, the next stage's first operands are read.  Two stages: one is multiplied while the other is loaded.
+        // The loads stand between the rows of tiles: all at once they would hold up the reads and products behind them.
+        constexpr int SPREAD = NS == 3 ? TN - 1 : TN / 2, EACH_ROW = (CH + SPREAD - 1) / SPREAD;
+        auto step = [&](int4_v *s, int4_v *next, int4_v *after, Operands &o, Operands &on, int u) __attribute__((always_inline)) {
             if (NS == 3) {
                 multiply(s, o, [&]() __attribute__((always_inline)) {
                     if (u == SB - 1) put_scales(par ^= 1);
                     wait_loads<CH>();                   // the next stage is there
-                    barrier();                          // and every wave's part of it
-                    stage(s, min(b + u + 3, whole - 1));
+                    barrier();                          // and every wave's part of it; and all have read this one
                     fetch(on, next, par, (u + 1) % SB);
+                }, [&](int i) __attribute__((always_inline)) {
+                    if (i < SPREAD) stage(after, min(b + u + 2, whole - 1), i * EACH_ROW, EACH_ROW);
                 });
             } else {
                 wait_loads<0>();
                 barrier();                              // this stage is there, and the other free
-                stage(next, min(b + u + 1, whole - 1));
                 fetch(o0, s, par, u);
-                multiply(s, o0, nothing);
+                multiply(s, o0, nothing, [&](int i) __attribute__((always_inline)) {
+                    if (i < SPREAD) stage(next, min(b + u + 1, whole - 1), i * EACH_ROW, EACH_ROW);
+                });
                 if (u == SB - 1) put_scales(par ^= 1);
             }
         };
         auto steps = [&](int n) __attribute__((always_inline)) {
             if (NS == 3) {
-                step(s_0, s_1, o0, o1, 0);
-                if (n > 1) step(s_1, s_2, o1, o0, 1);
-                if (n > 2) step(s_2, s_0, o0, o1, 2);
-                if (n > 3) step(s_0, s_1, o1, o0, 3);
-                if (n > 4) step(s_1, s_2, o0, o1, 4);
-                if (n > 5) step(s_2, s_0, o1, o0, 5);
+                step(s_0, s_1, s_2, o0, o1, 0);
+                if (n > 1) step(s_1, s_2, s_0, o1, o0, 1);
+                if (n > 2) step(s_2, s_0, s_1, o0, o1, 2);
+                if (n > 3) step(s_0, s_1, s_2, o1, o0, 3);
+                if (n > 4) step(s_1, s_2, s_0, o0, o1, 4);
+                if (n > 5) step(s_2, s_0, s_1, o1, o0, 5);
             } else {
-                step(s_0, s_1, o0, o1, 0);
-                if (n > 1) step(s_1, s_0, o0, o1, 1);
-                if (n > 2) step(s_0, s_1, o0, o1, 2);
-                if (n > 3) step(s_1, s_0, o0, o1, 3);
-                if (n > 4) step(s_0, s_1, o0, o1, 4);
-                if (n > 5) step(s_1, s_0, o0, o1, 5);
+                step(s_0, s_1, s_1, o0, o1, 0);
+                if (n > 1) step(s_1, s_0, s_0, o0, o1, 1);
+                if (n > 2) step(s_0, s_1, s_1, o0, o1, 2);
+                if (n > 3) step(s_1, s_0, s_0, o0, o1, 3);
+                if (n > 4) step(s_0, s_1, s_1, o0, o1, 4);
+                if (n > 5) step(s_1, s_0, s_0, o0, o1, 5);
             }
         };
         fetch_scales(0);
-        stage(s_0, 0);
-        if (NS == 3) {
-            stage(s_1, min(1, whole - 1));
-            stage(s_2, min(2, whole - 1));
-        }
+        stage(s_0, 0, 0, CH);
+        if (NS == 3) stage(s_1, min(1, whole - 1), 0, CH);
         put_scales(0);
         if (NS == 3) {
-            wait_loads<2 * CH>();
+            wait_loads<CH>();
             barrier();
             fetch(o0, s_0, 0, 0);
         }
@@ -582,7 +585,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
                 for (int i = 0; i < CH; ++i) s_0[i * THREADS + threadIdx.x] = held[i];
                 __syncthreads();
                 fetch(o0, s_0, par, u);
-                multiply(s_0, o0, nothing);
+                multiply(s_0, o0, nothing, [](int) {});
             }
             if (b + SB > whole) break;
             fetch_scales(b + SB);
@@ -598,7 +601,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
         }
         __syncthreads();
         fetch(o0, s_0, par, whole - b);
-        multiply(s_0, o0, nothing);
+        multiply(s_0, o0, nothing, [](int) {});
     }
 
     if (GATED) {
