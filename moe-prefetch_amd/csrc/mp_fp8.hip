@@ -28,6 +28,7 @@ typedef _Float16 half2_v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_v __attribute__((ext_vector_type(8)));
 
 constexpr int FB = FP8_BLOCK;
+#define FP8_INLINE __attribute__((always_inline))
 
 // ---- the quantizer ---------------------------------------------------------------
 // The scale of a block whose largest finite magnitude is amax: the least power of two s, from 2^-126 on, with amax <= 448 s.
@@ -187,7 +188,14 @@ __device__ inline half8_v halves(uint32_t lo, uint32_t hi) {
     const half2_v c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
     return half8_v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+// A block's dot from the cores' own e4m3 products.
+__device__ inline float4_v mfma_e4m3(int8_v w, int8_v x) {
+    const float4_v z = {0.0f, 0.0f, 0.0f, 0.0f};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, z, 0, 0, 0, 0, 0, 0);
+}
+template <bool EXACT>
 __device__ inline float4_v mfma_block(int8_v w, int8_v x) {
+    if (!EXACT) return mfma_e4m3(w, x);
     float4_v d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 8; i += 2) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(w[i], w[i + 1]), halves(x[i], x[i + 1]), d, 0, 0, 0);
@@ -204,10 +212,11 @@ __device__ inline int4_v load16(const uint8_t *p, int n) {
     return int4_v{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 }
 __device__ inline int8_v load_frag(const uint8_t *row, int k, int K, int g) {
+    if (k + FB <= K)                                    // (the same for all lanes)
+        return __builtin_shufflevector(*(const int4_u *)(row + k + 16 * g), *(const int4_u *)(row + k + 64 + 16 * g), 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_shufflevector(load16(row + k + 16 * g, K - k - 16 * g), load16(row + k + 64 + 16 * g, K - k - 64 - 16 * g), 0, 1, 2, 3, 4,
                                    5, 6, 7);
 }
-
 __device__ inline void store_elem(void *p, int64_t i, int type, float v) {
     if (type == T_F32) ((float *)p)[i] = v;
     else if (type == T_BF16) ((uint16_t *)p)[i] = Elem<T_BF16>::store(v);
@@ -234,62 +243,366 @@ __device__ inline void store4(void *p, int64_t i, int type, float4_v v, int n) {
 
 __device__ inline float silu_times(float g, float u) { return u * (g / (1.0f + expf(-g))); }
 
-// Sixteen rows of a weight (of gate and up: GATED), sixteen rows of x at a time; four waves, every fourth block of K each, whose sums
-// are added in their order.
-template <bool GATED>
+// ---- products of few rows ----------------------------------------------------------
+// Where a product's rows of x come from, and go to.
+constexpr int OF_ALL = 0;         // rows 0 .. M - 1
+constexpr int OF_DISPATCH = 1;    // an expert's pairs from a dispatch
+
+// Sixteen rows of a weight (of gate and up: GATED) for 16 NT rows of codes at a time.  Four waves share K, a block each in turn, and their sums are
+// added in their order.  A wave's loads of DEEP blocks of the weight are on their way together: every weight is read once, and
+// memory bounds the call.
+template <int FROM, bool GATED, bool EXACT, int NT>
 __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
-    __shared__ float s_acc[2][4][16][17];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int e = blockIdx.y, n0 = blockIdx.x * 16;
-    const int begin = a.offsets ? a.offsets[e] : 0, end = a.offsets ? a.offsets[e + 1] : a.M;
-    const int nb = (a.K + FB - 1) / FB;
+    constexpr int WAVES = 4, DEEP = GATED ? 2 : 4, MATS = GATED ? 2 : 1;
+    __shared__ float s_acc[MATS][WAVES][16 * NT][17];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int n0 = blockIdx.x * 16, nb = (a.K + FB - 1) / FB;
+    const int e = FROM == OF_ALL ? 0 : (int)blockIdx.y;
+    const int begin = FROM == OF_ALL ? 0 : a.offsets[e], end = FROM == OF_ALL ? a.M : a.offsets[e + 1];
     const int64_t wrow = min(n0 + c, a.N - 1);
-    const uint8_t *w0 = a.m[0].w + e * a.m[0].ex + wrow * a.m[0].ld;
-    const float *s0 = a.m[0].s + e * a.m[0].sex + (int64_t)(n0 / FB) * a.m[0].sld;
-    const uint8_t *w1 = nullptr;
-    const float *s1 = nullptr;
-    if (GATED) {
-        w1 = a.m[1].w + e * a.m[1].ex + wrow * a.m[1].ld;
-        s1 = a.m[1].s + e * a.m[1].sex + (int64_t)(n0 / FB) * a.m[1].sld;
-    }
-    for (int64_t p0 = begin + 16ll * blockIdx.z; p0 < end; p0 += 16ll * gridDim.z) {
-        const int64_t p = p0 + c < end ? p0 + c : end - 1;
-        const int64_t xrow = a.top ? a.perm[p] / a.top : p;
-        const uint8_t *x = a.x + xrow * a.ldx;
-        const float *xs = a.xs + xrow * a.ldxs;
-        float4_v t0 = {}, t1 = {};
-        for (int b = wave; b < nb; b += 4) {
-            const int8_v xf = load_frag(x, b * FB, a.K, g);
-            const float s = xs[b];
-            const float4_v d0 = mfma_block(load_frag(w0, b * FB, a.K, g), xf);
-            for (int i = 0; i < 4; ++i) t0[i] = fmaf(d0[i], s * s0[b], t0[i]);
-            if (GATED) {
-                const float4_v d1 = mfma_block(load_frag(w1, b * FB, a.K, g), xf);
-                for (int i = 0; i < 4; ++i) t1[i] = fmaf(d1[i], s * s1[b], t1[i]);
+    const uint8_t *w[2] = {a.m[0].w + e * a.m[0].ex + wrow * a.m[0].ld, GATED ? a.m[1].w + e * a.m[1].ex + wrow * a.m[1].ld : nullptr};
+    const float *ws[2] = {a.m[0].s + e * a.m[0].sex + (int64_t)(n0 / FB) * a.m[0].sld,
+                          GATED ? a.m[1].s + e * a.m[1].sex + (int64_t)(n0 / FB) * a.m[1].sld : nullptr};
+    for (int64_t p0 = begin + 16ll * NT * blockIdx.z; p0 < end; p0 += 16ll * NT * gridDim.z) {
+        int64_t xrow[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int64_t p = min(p0 + 16 * t + c, (int64_t)end - 1);
+            xrow[t] = FROM == OF_DISPATCH && a.top ? a.perm[p] / a.top : p;
+        }
+        float4_v acc[2][NT] = {};
+        for (int b0 = wave; b0 < nb; b0 += WAVES * DEEP) {
+            int8_v wf[DEEP][2];
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i)
+                if (b0 + i * WAVES < nb)
+#pragma unroll
+                    for (int m = 0; m < MATS; ++m) wf[i][m] = load_frag(w[m], (b0 + i * WAVES) * FB, a.K, g);
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) {
+                const int b = b0 + i * WAVES;
+                if (b >= nb) break;
+                const float f0 = ws[0][b], f1 = GATED ? ws[1][b] : 0.0f;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if (t > 0 && p0 + 16 * t >= end) break;
+                    const int8_v xf = load_frag(a.x + xrow[t] * a.ldx, b * FB, a.K, g);
+                    const float s = a.xs[xrow[t] * a.ldxs + b];
+#pragma unroll
+                    for (int m = 0; m < MATS; ++m) {
+                        const float4_v d = mfma_block<EXACT>(wf[i][m], xf);
+                        const float f = s * (m ? f1 : f0);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) acc[m][t][k] = fmaf(d[k], f, acc[m][t][k]);
+                    }
+                }
             }
         }
         __syncthreads();
-        for (int i = 0; i < 4; ++i) {
-            s_acc[0][wave][c][4 * g + i] = t0[i];
-            if (GATED) s_acc[1][wave][c][4 * g + i] = t1[i];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s_acc[m][wave][16 * t + c][4 * g + k] = acc[m][t][k];
+        __syncthreads();
+        const int r = threadIdx.x & 15;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int col = 16 * t + (threadIdx.x >> 4);
+            if (n0 + r >= a.N || p0 + col >= end) continue;
+            float y[2];
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) {
+                y[m] = s_acc[m][0][col][r];
+#pragma unroll
+                for (int i = 1; i < WAVES; ++i) y[m] += s_acc[m][i][col][r];
+            }
+            int64_t out = p0 + col;
+            float v = GATED ? silu_times(y[0], y[1]) : y[0];
+            if (FROM == OF_DISPATCH && a.pair_w) {
+                out = a.perm[out];
+                v *= a.pair_w[out];
+            }
+            store_elem(a.y, out * a.ldy + n0 + r, a.y_type, v);
         }
+    }
+}
+
+// Rows quantized into LDS by a workgroup of THREADS, sixteen lanes a block: row i of n (from(i) gives its elements) at q + i * stride with nothing
+// behind its K elements but zeros up to a whole block, its scales at s + i * blocks.
+template <int T, int THREADS, class F>
+__device__ inline void quant_to_lds(int n, int K, F from, uint8_t *q, int stride, float *s) {
+    constexpr int NB = 4;
+    const int nb = (K + FB - 1) / FB, l = threadIdx.x % 16;
+    for (int g0 = threadIdx.x / 16; g0 < n * nb; g0 += THREADS / 16 * NB) {
+        float v[NB][8];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int g = g0 + THREADS / 16 * i, row = g / nb, k = (g - row * nb) * FB + 8 * l;
+            if (g < n * nb) load8<T>(from(row) + k, K - k, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int g = g0 + THREADS / 16 * i, row = g / nb, k = (g - row * nb) * FB + 8 * l;
+            if (g >= n * nb) break;                     // (the same for the sixteen lanes)
+            float m = max16(amax8(v[i], 0.0f));
+            if (m == INFINITY) m = max16(without_inf(v[i], m));
+            const int e = scale_exp(m);
+            *(uint2 *)(q + row * stride + k) = codes8(v[i], pow2(-e));
+            if (l == 0) s[row * nb + (g - row * nb)] = pow2(e);
+        }
+    }
+}
+// a row's stride there: sixteen rows' chunks in banks of their own
+__host__ __device__ inline int lds_stride(int K) { return (K + FB - 1) / FB * FB + 16; }
+__device__ inline int8_v lds_frag(const uint8_t *q, int b, int g) {
+    const int4_v *p = (const int4_v *)(q + b * FB + 16 * g);
+    return __builtin_shufflevector(p[0], p[4], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// The places of the set bits of m, by one wave: list[i] of the i-th
+__device__ inline void list_bits(uint64_t m, uint8_t *list) {
+    const int lane = threadIdx.x & 63;
+    if (m >> lane & 1) list[__popcll(m & ((1ull << lane) - 1))] = (uint8_t)lane;
+}
+
+// Sixteen rows of a weight (of gate and up: GATED) for few rows of x, which are quantized into LDS while the weight is on its way: one
+// launch, and nothing between.  Four waves share K.
+// GATED: workgroup y has the expert of pair y, where that is the expert's first pair, and all of its pairs among the ids
+// (at most 64); h goes out in f32 in the order of pairs.  Else rows 0 .. M - 1 of x.
+template <int T, bool GATED, bool EXACT>
+__global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
+    constexpr int WAVES = 4, DEEP = 4, MATS = GATED ? 2 : 1;
+    extern __shared__ __align__(16) uint8_t s_q[];      // [16][stride] codes, [16][nb] scales
+    __shared__ float s_acc[MATS][WAVES][16][17];
+    __shared__ uint8_t s_list[64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int n0 = blockIdx.x * 16, nb = (a.K + FB - 1) / FB, stride = lds_stride(a.K);
+    float *s_s = (float *)(s_q + a.cols * stride);
+    int e = 0, n = a.M;
+    if (GATED) {
+        const int mine = lane < a.M ? a.ids[lane] : -1;
+        e = __builtin_amdgcn_readlane(mine, blockIdx.y);
+        const uint64_t m = __ballot(mine == e);
+        if ((uint32_t)e >= (uint32_t)a.E || __ffsll((unsigned long long)m) - 1 != (int)blockIdx.y) return;
+        n = __popcll(m);
+        if (wave == 0) list_bits(m, s_list);
+    }
+    const int64_t wrow = min(n0 + c, a.N - 1);
+    const uint8_t *w[2] = {a.m[0].w + e * a.m[0].ex + wrow * a.m[0].ld, GATED ? a.m[1].w + e * a.m[1].ex + wrow * a.m[1].ld : nullptr};
+    const float *ws[2] = {a.m[0].s + e * a.m[0].sex + (int64_t)(n0 / FB) * a.m[0].sld,
+                          GATED ? a.m[1].s + e * a.m[1].sex + (int64_t)(n0 / FB) * a.m[1].sld : nullptr};
+    int8_v wf[DEEP][2];
+    float f[DEEP][2];
+    auto load_w = [&](int b0) FP8_INLINE {
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i)
+            if (b0 + i * WAVES < nb)
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) {
+                    wf[i][m] = load_frag(w[m], (b0 + i * WAVES) * FB, a.K, g);
+                    f[i][m] = ws[m][b0 + i * WAVES];
+                }
+    };
+    load_w(wave);
+    bool loaded = true;
+    if (GATED) __syncthreads();
+    for (int p0 = 0; p0 < n; p0 += a.cols) {
+        const int cols = min(n - p0, a.cols);
+        quant_to_lds<T, 256>(cols, a.K, [&](int i) {
+            return (const typename Elem<T>::raw *)a.x + (int64_t)(GATED ? s_list[p0 + i] / a.top : p0 + i) * a.ldx;
+        }, s_q, stride, s_s);
+        __syncthreads();
+        const uint8_t *q = s_q + min(c, cols - 1) * stride;
+        const float *s = s_s + min(c, cols - 1) * nb;
+        float4_v acc[2] = {};
+        for (int b0 = wave; b0 < nb; b0 += WAVES * DEEP) {
+            if (!loaded) load_w(b0);
+            loaded = false;
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) {
+                const int b = b0 + i * WAVES;
+                if (b >= nb) break;
+                const int8_v xf = lds_frag(q, b, g);
+                const float sx = s[b];
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) {
+                    const float4_v d = mfma_block<EXACT>(wf[i][m], xf);
+                    const float v = sx * f[i][m];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[m][k] = fmaf(d[k], v, acc[m][k]);
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s_acc[m][wave][c][4 * g + k] = acc[m][k];
         __syncthreads();
         const int r = threadIdx.x & 15, col = threadIdx.x >> 4;
-        if (n0 + r >= a.N || p0 + col >= end) continue;
-        float y = s_acc[0][0][col][r];
-        for (int i = 1; i < 4; ++i) y += s_acc[0][i][col][r];
-        if (GATED) {
-            float u = s_acc[1][0][col][r];
-            for (int i = 1; i < 4; ++i) u += s_acc[1][i][col][r];
-            y = silu_times(y, u);
+        if (n0 + r < a.N && col < cols) {
+            float y[2];
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) {
+                y[m] = s_acc[m][0][col][r];
+#pragma unroll
+                for (int i = 1; i < WAVES; ++i) y[m] += s_acc[m][i][col][r];
+            }
+            const int64_t out = GATED ? s_list[p0 + col] : p0 + col;
+            store_elem(a.y, out * a.ldy + n0 + r, a.y_type, GATED ? silu_times(y[0], y[1]) : y[0]);
         }
-        int64_t out = p0 + col;
-        if (a.pair_w) {
-            out = a.perm[out];
-            y *= a.pair_w[out];
-        }
-        store_elem(a.y, out * a.ldy + n0 + r, a.y_type, y);
     }
+}
+
+// The down product of a few tokens' layer and the sum over their experts: sixteen columns of out for all tokens.  h of all pairs is quantized into
+// LDS while the first weights are on their way; eight waves share the experts in use (where these are fewer, also K), the next
+// one's weights on their way while one is multiplied.  The pairs' rows meet in LDS, where each token's are added in order.
+template <bool EXACT>
+__global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
+    constexpr int WAVES = 8, DEEP = 6;
+    extern __shared__ __align__(16) uint8_t s_q[];      // [P][stride] codes, [P][nb] scales, [parts][P][17] rows
+    __shared__ uint8_t s_col[WAVES][64];
+    __shared__ float s_w[64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int n0 = blockIdx.x * 16, nb = (a.I + FB - 1) / FB, P = a.n_tok * a.K, stride = lds_stride(a.I);
+    float *s_s = (float *)(s_q + P * stride), *s_rows = s_s + P * nb;
+    const int per = WAVES / a.parts, part = wave / per;
+    const int64_t wrow = min(n0 + c, a.H - 1);
+    const int mine = lane < P ? a.ids[lane] : -1;
+    const bool is = (uint32_t)mine < (uint32_t)a.E;
+    if (wave == 0 && lane < P) s_w[lane] = is ? a.w[lane] : 0.0f;
+    const uint64_t used = __ballot(is);
+    uint64_t same = used;                               // the pairs of a lane's expert, found bit by bit of the id
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const bool bit = mine >> b & 1;
+        const uint64_t m = __ballot(bit);
+        same &= bit ? m : ~m;
+    }
+    const uint64_t firsts = __ballot(is && __ffsll((unsigned long long)same) - 1 == lane);      // the experts' first pairs
+    int8_v wf[2][DEEP];
+    float f[2][DEEP];
+    auto weight = [&](int j, int b, float &s) FP8_INLINE {
+        const int64_t e = __builtin_amdgcn_readlane(mine, j);
+        s = (a.down.s + e * a.down.sex + (int64_t)(n0 / FB) * a.down.sld)[b];
+        return load_frag(a.down.w + e * a.down.ex + wrow * a.down.ld, b * FB, a.I, g);
+    };
+    auto load_w = [&](int8_v (&wd)[DEEP], float (&fd)[DEEP], int j) FP8_INLINE {
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i)
+            if (part + i * a.parts < nb) wd[i] = weight(j, part + i * a.parts, fd[i]);
+    };
+    // this wave's experts: every per-th of those in use
+    uint64_t todo = firsts;
+    auto next = [&](int skip) FP8_INLINE {
+        for (; skip > 0 && todo; --skip) todo &= todo - 1;
+        return todo ? __ffsll((unsigned long long)todo) - 1 : -1;
+    };
+    int j = next(wave % per);
+    if (j >= 0) load_w(wf[0], f[0], j);
+    quant_to_lds<T_F32, 512>(P, a.I, [&](int i) { return a.h + (int64_t)i * a.I; }, s_q, stride, s_s);
+    __syncthreads();
+    auto expert = [&](int j, const int8_v (&wd)[DEEP], const float (&fd)[DEEP]) FP8_INLINE {
+        const uint64_t m = __ballot(mine == __builtin_amdgcn_readlane(mine, j));
+        const int n = __popcll(m);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        list_bits(m, s_col[wave]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int p0 = 0; p0 < n; p0 += 16) {
+            const int pair = s_col[wave][min(p0 + c, n - 1)];
+            const uint8_t *q = s_q + pair * stride;
+            float4_v acc = {};
+            auto add = [&](int8_v w, int b, float sw) FP8_INLINE {
+                const float4_v d = mfma_block<EXACT>(w, lds_frag(q, b, g));
+                const float v = s_s[pair * nb + b] * sw;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = fmaf(d[k], v, acc[k]);
+            };
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i)
+                if (part + i * a.parts < nb) add(wd[i], part + i * a.parts, fd[i]);
+            for (int b = part + DEEP * a.parts; b < nb; b += a.parts) {
+                float sw;
+                const int8_v w = weight(j, b, sw);
+                add(w, b, sw);
+            }
+            if (p0 + c < n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s_rows[(part * P + pair) * 17 + 4 * g + k] = acc[k];
+        }
+    };
+    while (j >= 0) {
+        const int j1 = next(per);
+        if (j1 >= 0) load_w(wf[1], f[1], j1);
+        expert(j, wf[0], f[0]);
+        if (j1 < 0) break;
+        j = next(per);
+        if (j >= 0) load_w(wf[0], f[0], j);
+        expert(j1, wf[1], f[1]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.n_tok * 16; i += 64 * WAVES) {
+        const int t = i >> 4, r = i & 15;
+        if (n0 + r >= a.H) continue;
+        float sum = 0.0f;
+        for (int k = 0; k < a.K; ++k) {
+            const int pair = t * a.K + k;
+            if (!(used >> pair & 1)) continue;          // of no expert: nothing stands there
+            float v = s_rows[pair * 17 + r];
+            for (int q = 1; q < a.parts; ++q) v += s_rows[(q * P + pair) * 17 + r];
+            sum += s_w[pair] * v;
+        }
+        store_elem(a.out, (int64_t)t * a.ldo + n0 + r, a.out_type, sum);
+    }
+}
+
+constexpr int FEW_LDS = 60 * 1024;
+// Which layers and products take these kernels: as many pairs as a wave has lanes, and rows that LDS holds.
+bool fp8_few_layer(int n_tok, int K, int H, int I) {
+    const int64_t P = (int64_t)n_tok * K;
+    return P <= 64 && std::min(P, (int64_t)16) * (lds_stride(H) + 4 * ((H + FB - 1) / FB)) <= FEW_LDS - 10000 &&
+           P * (lds_stride(I) + 4 * ((I + FB - 1) / FB)) + std::max(P, (int64_t)8) * 17 * 4 <= FEW_LDS;
+}
+bool fp8_few_product(int M, int K) { return M <= 16 && (int64_t)M * (lds_stride(K) + 4 * ((K + FB - 1) / FB)) <= FEW_LDS - 6000; }
+
+template <int T, bool GATED>
+static hipError_t launch_few_t(Fp8Args a, hipStream_t st) {
+    a.cols = std::min(a.M, 16);
+    const dim3 grid((unsigned)((a.N + 15) / 16), GATED ? (unsigned)a.M : 1);
+    const size_t lds = (size_t)a.cols * (lds_stride(a.K) + 4 * ((a.K + FB - 1) / FB));
+    if (a.exact) hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED, true>), grid, dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED, false>), grid, dim3(256), lds, st, a);
+    return hipGetLastError();
+}
+hipError_t launch_fp8_few_up(const Fp8Args &a, int x_type, hipStream_t st) {
+    if (a.gated) return x_type == T_F32 ? launch_few_t<T_F32, true>(a, st) : x_type == T_BF16 ? launch_few_t<T_BF16, true>(a, st) : launch_few_t<T_F16, true>(a, st);
+    return x_type == T_F32 ? launch_few_t<T_F32, false>(a, st) : x_type == T_BF16 ? launch_few_t<T_BF16, false>(a, st) : launch_few_t<T_F16, false>(a, st);
+}
+hipError_t launch_fp8_few_down(Fp8FewArgs a, hipStream_t st) {
+    const int P = a.n_tok * a.K, nb = (a.I + FB - 1) / FB;
+    a.parts = 1;
+    while (2 * a.parts * P <= 8 && 2 * a.parts <= nb) a.parts *= 2;
+    const dim3 grid((unsigned)((a.H + 15) / 16));
+    const size_t lds = (size_t)P * (lds_stride(a.I) + 4 * nb) + (size_t)a.parts * P * 17 * 4;
+    if (a.exact) hipLaunchKernelGGL((fp8_few_down_kernel<true>), grid, dim3(512), lds, st, a);
+    else hipLaunchKernelGGL((fp8_few_down_kernel<false>), grid, dim3(512), lds, st, a);
+    return hipGetLastError();
+}
+
+template <int FROM, bool GATED, int NT>
+static hipError_t launch_stream_n(const Fp8Args &a, hipStream_t st) {
+    const int64_t groups = (a.M + 16 * NT - 1) / (16 * NT);
+    const dim3 grid((unsigned)((a.N + 15) / 16), FROM == OF_ALL ? 1 : (unsigned)a.E, FROM == OF_ALL ? (unsigned)std::min(groups, (int64_t)4096) : 1);
+    if (a.exact) hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, true, NT>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, false, NT>), grid, dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+template <int FROM, bool GATED>
+static hipError_t launch_stream(const Fp8Args &a, hipStream_t st) {
+    const int rows = a.M / a.E;                         // of an expert, about
+    return rows <= 16 ? launch_stream_n<FROM, GATED, 1>(a, st) : rows <= 32 ? launch_stream_n<FROM, GATED, 2>(a, st)
+                                                               : launch_stream_n<FROM, GATED, 4>(a, st);
 }
 
 // ---- products of many rows: tiles through LDS --------------------------------------
@@ -298,11 +611,6 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
 // without registers, are on their way while this one is multiplied.
 // The eight 16-byte chunks of a row lie in LDS at chunk ^ (row & 7): the lanes that read one chunk of eight rows then touch
 // all banks once.
-__device__ inline float4_v mfma_e4m3(int8_v w, int8_v x) {
-    const float4_v z = {0.0f, 0.0f, 0.0f, 0.0f};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, z, 0, 0, 0, 0, 0, 0);
-}
-
 // expert and first row (in the dispatch's order) of a workgroup's rows of x, the slot-th run of BM; false: there is none
 __device__ inline bool find_run(const int32_t *offsets, int E, int bm, int slot, int &e, int &p0, int &end, int *s_run) {
     if (threadIdx.x < 64) {
@@ -350,12 +658,12 @@ __device__ inline void barrier() {
     asm volatile("" ::: "memory");
 }
 
-// NS stages; 1: rows of any alignment, through registers
-template <bool GATED, bool EXACT, int NS, int WN, int WM, int TN, int TM>
+// DIRECT: loads to LDS without registers (rows on 16 bytes, near one another)
+template <bool GATED, bool EXACT, bool DIRECT, int WN, int WM, int TN, int TM>
 __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n_tiles, int m_tiles) {
     constexpr int THREADS = 64 * WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, CH = (BN + BM) * 8 / THREADS, SB = 6;
     static_assert((BN + BM) * 8 % THREADS == 0 && BN * 8 % THREADS == 0 && THREADS % BM == 0 && SB * 2 * WN <= THREADS, "whole loads");
-    __shared__ int4_v s_0[(BN + BM) * 8], s_1[NS > 1 ? (BN + BM) * 8 : 1], s_2[NS > 2 ? (BN + BM) * 8 : 1];
+    __shared__ int4_v s_0[(BN + BM) * 8], s_1[DIRECT ? (BN + BM) * 8 : 1], s_2[DIRECT ? (BN + BM) * 8 : 1];
     __shared__ int s_run[4];
     __shared__ float s_max[WN][BM], s_sx[2][SB][BM], s_sw[2][SB][2 * WN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
@@ -379,18 +687,18 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
 
     // The row of chunk q of a stage: of a weight, from n0 on (a wave's rows: TN / 2 tiles of gate and as many of up), or of x; and which of its
     // chunks it is
-    auto weight_row = [&](int q) __attribute__((always_inline)) {
+    auto weight_row = [&](int q) FP8_INLINE {
         const int r = q >> 3;
         return min(GATED ? r / (16 * TN) * 8 * TN + r % (8 * TN) : r, a.N - 1 - n0);
     };
-    auto is_up = [](int q) __attribute__((always_inline)) { return GATED && (q >> 3) % (16 * TN) >= 8 * TN; };
-    auto x_row = [&](int q) __attribute__((always_inline)) -> int64_t {
+    auto is_up = [](int q) FP8_INLINE { return GATED && (q >> 3) % (16 * TN) >= 8 * TN; };
+    auto x_row = [&](int q) FP8_INLINE -> int64_t {
         const int p = min(p0 + (q >> 3) - BN, end - 1);
         return a.top ? a.perm[p] / a.top : p;
     };
-    auto chunk_of = [](int q) __attribute__((always_inline)) { return (q & 7) ^ (q >> 3 & 7); };
+    auto chunk_of = [](int q) FP8_INLINE { return (q & 7) ^ (q >> 3 & 7); };
     const uint8_t *const w0 = a.m[0].w + e * a.m[0].ex + n0 * a.m[0].ld, *const w1 = GATED ? a.m[1].w + e * a.m[1].ex + n0 * a.m[1].ld : w0;
-    auto row_of = [&](int q) __attribute__((always_inline)) -> const uint8_t * {
+    auto row_of = [&](int q) FP8_INLINE -> const uint8_t * {
         if (q >= BN * 8) return a.x + x_row(q) * a.ldx;
         return is_up(q) ? w1 + weight_row(q) * a.m[1].ld : w0 + weight_row(q) * a.m[0].ld;
     };
@@ -401,11 +709,11 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int q = i * THREADS + threadIdx.x;
-        if (NS == 1) src[i] = row_of(q) + 16 * chunk_of(q);
+        if (!DIRECT) src[i] = row_of(q) + 16 * chunk_of(q);
         else if (i * THREADS < BN * 8) from[i] = (uint32_t)(weight_row(q) * (is_up(q) ? a.m[1].ld : a.m[0].ld)) + 16 * chunk_of(q);
         else from[i] = (uint32_t)((x_row(q) - (a.top ? 0 : p0)) * a.ldx) + 16 * chunk_of(q);
     }
-    auto stage = [&](int4_v *s, int b, int first, int n) __attribute__((always_inline)) {
+    auto stage = [&](int4_v *s, int b, int first, int n) FP8_INLINE {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             if (i < first || i >= first + n) continue;
@@ -428,26 +736,26 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
         from_w = m.s + e * m.sex + (int64_t)min((n0 + w * (GATED ? 8 : 16) * TN) / FB, (a.N - 1) / FB) * m.sld;
     }
     float held_x[EACH], held_w = 0.0f;
-    auto fetch_scales = [&](int b) __attribute__((always_inline)) {
+    auto fetch_scales = [&](int b) FP8_INLINE {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) held_x[i] = from_x[min(b + (int)threadIdx.x / BM + PER * i, nb - 1)];
         if (threadIdx.x < SB * 2 * WN) held_w = from_w[min(b + (int)threadIdx.x / (2 * WN), nb - 1)];
     };
-    auto put_scales = [&](int par) __attribute__((always_inline)) {
+    auto put_scales = [&](int par) FP8_INLINE {
 #pragma unroll
         for (int i = 0; i < EACH; ++i)
             if (SB % PER == 0 || threadIdx.x / BM + PER * i < SB) s_sx[par][threadIdx.x / BM + PER * i][threadIdx.x % BM] = held_x[i];
         if (threadIdx.x < SB * 2 * WN) s_sw[par][threadIdx.x / (2 * WN)][threadIdx.x % (2 * WN)] = held_w;
     };
     float4_v acc[TN][TM] = {};
-    auto frag = [&](const int4_v *s, int r) __attribute__((always_inline)) {
+    auto frag = [&](const int4_v *s, int r) FP8_INLINE {
         return __builtin_shufflevector(s[r * 8 + (g ^ (r & 7))], s[r * 8 + ((4 + g) ^ (r & 7))], 0, 1, 2, 3, 4, 5, 6, 7);
     };
     struct Operands {                                   // what a wave's first row of tiles of a stage needs
         int8_v x[TM], w;
         float f0, f1, fx[TM];
     };
-    auto fetch = [&](Operands &o, const int4_v *s, int par, int u) __attribute__((always_inline)) {
+    auto fetch = [&](Operands &o, const int4_v *s, int par, int u) FP8_INLINE {
         o.w = frag(s, wn * TN * 16 + c);
 #pragma unroll
         for (int j = 0; j < TM; ++j) o.x[j] = frag(s, BN + (wm * TM + j) * 16 + c);
@@ -459,14 +767,14 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
     // A stage's products, a row of tiles' while the row before is scaled and added (EXACT: products take four times as long, and their
     // operands the registers of that) and the row after is read; before the last row, when every read of the stage is done, then(); in each
     // row, after its products, along(row).
-    auto multiply = [&](const int4_v *s, const Operands &o, auto then, auto along) __attribute__((always_inline)) {
+    auto multiply = [&](const int4_v *s, const Operands &o, auto then, auto along) FP8_INLINE {
         half8_v xh[TM][4];
         if (EXACT)
 #pragma unroll
             for (int j = 0; j < TM; ++j)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) xh[j][k] = halves(o.x[j][2 * k], o.x[j][2 * k + 1]);
-        constexpr int LAG = EXACT || TN * TM > 16 ? 0 : 1;
+        constexpr int LAG = EXACT ? 0 : 1;
         int8_v wf = o.w;
         float4_v d[LAG + 1][TM];
 #pragma unroll
@@ -512,59 +820,38 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
     const int whole = a.K / FB;
     int b = 0, par = 0;
     Operands o0, o1;
-    if (NS > 1 && whole) {
+    if (DIRECT && whole) {
         // Steps stand in the code one by one, each with its own places in LDS, so that reads wait for the loads to their own place alone; at
         // the loop's head they wait for all.  At the end of K the loads are of its last block again, so that every step is alike.
         // Three stages: one is multiplied while the loads of the two after it are on their way.  Before its last row of tiles, when every
-        // wave has read all of it, the next stage's first operands are read.  Two stages: one is multiplied while the other is loaded.
-        // The loads stand between the rows of tiles: all at once they would hold up the reads and products behind them.
-        constexpr int SPREAD = NS == 3 ? TN - 1 : TN / 2, EACH_ROW = (CH + SPREAD - 1) / SPREAD;
-        auto step = [&](int4_v *s, int4_v *next, int4_v *after, Operands &o, Operands &on, int u) __attribute__((always_inline)) {
-            if (NS == 3) {
-                multiply(s, o, [&]() __attribute__((always_inline)) {
-                    if (u == SB - 1) put_scales(par ^= 1);
-                    wait_loads<CH>();                   // the next stage is there
-                    barrier();                          // and every wave's part of it; and all have read this one
-                    fetch(on, next, par, (u + 1) % SB);
-                }, [&](int i) __attribute__((always_inline)) {
-                    if (i < SPREAD) stage(after, min(b + u + 2, whole - 1), i * EACH_ROW, EACH_ROW);
-                });
-            } else {
-                wait_loads<0>();
-                barrier();                              // this stage is there, and the other free
-                fetch(o0, s, par, u);
-                multiply(s, o0, nothing, [&](int i) __attribute__((always_inline)) {
-                    if (i < SPREAD) stage(next, min(b + u + 1, whole - 1), i * EACH_ROW, EACH_ROW);
-                });
+        // wave has read all of it, the next stage's first operands are read.  The loads stand between the rows of tiles: all at once
+        // they would hold up the reads and products behind them (4096^3: 96 us, 79 so).
+        constexpr int EACH_ROW = (CH + TN - 2) / (TN - 1);
+        auto step = [&](int4_v *s, int4_v *next, int4_v *after, Operands &o, Operands &on, int u) FP8_INLINE {
+            multiply(s, o, [&]() FP8_INLINE {
                 if (u == SB - 1) put_scales(par ^= 1);
-            }
+                wait_loads<CH>();                       // the next stage is there
+                barrier();                              // and every wave's part of it; and all have read this one
+                fetch(on, next, par, (u + 1) % SB);
+            }, [&](int i) FP8_INLINE {
+                if (i < TN - 1) stage(after, min(b + u + 2, whole - 1), i * EACH_ROW, EACH_ROW);
+            });
         };
-        auto steps = [&](int n) __attribute__((always_inline)) {
-            if (NS == 3) {
-                step(s_0, s_1, s_2, o0, o1, 0);
-                if (n > 1) step(s_1, s_2, s_0, o1, o0, 1);
-                if (n > 2) step(s_2, s_0, s_1, o0, o1, 2);
-                if (n > 3) step(s_0, s_1, s_2, o1, o0, 3);
-                if (n > 4) step(s_1, s_2, s_0, o0, o1, 4);
-                if (n > 5) step(s_2, s_0, s_1, o1, o0, 5);
-            } else {
-                step(s_0, s_1, s_1, o0, o1, 0);
-                if (n > 1) step(s_1, s_0, s_0, o0, o1, 1);
-                if (n > 2) step(s_0, s_1, s_1, o0, o1, 2);
-                if (n > 3) step(s_1, s_0, s_0, o0, o1, 3);
-                if (n > 4) step(s_0, s_1, s_1, o0, o1, 4);
-                if (n > 5) step(s_1, s_0, s_0, o0, o1, 5);
-            }
+        auto steps = [&](int n) FP8_INLINE {
+            step(s_0, s_1, s_2, o0, o1, 0);
+            if (n > 1) step(s_1, s_2, s_0, o1, o0, 1);
+            if (n > 2) step(s_2, s_0, s_1, o0, o1, 2);
+            if (n > 3) step(s_0, s_1, s_2, o1, o0, 3);
+            if (n > 4) step(s_1, s_2, s_0, o0, o1, 4);
+            if (n > 5) step(s_2, s_0, s_1, o1, o0, 5);
         };
         fetch_scales(0);
         stage(s_0, 0, 0, CH);
-        if (NS == 3) stage(s_1, min(1, whole - 1), 0, CH);
+        stage(s_1, min(1, whole - 1), 0, CH);
         put_scales(0);
-        if (NS == 3) {
-            wait_loads<CH>();
-            barrier();
-            fetch(o0, s_0, 0, 0);
-        }
+        wait_loads<CH>();
+        barrier();
+        fetch(o0, s_0, 0, 0);
         for (; b + SB <= whole; b += SB) {
             fetch_scales(b + SB);
             steps(SB);
@@ -663,13 +950,13 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
     }
 }
 
-template <bool GATED, bool EXACT, int NS, int WN, int WM, int TN, int TM>
+template <bool GATED, bool EXACT, bool DIRECT, int WN, int WM, int TN, int TM>
 static hipError_t launch_tile_n(const Fp8Args &a, hipStream_t st) {
     constexpr int ROWS = 16 * TN * WN / (GATED ? 2 : 1), BM = 16 * TM * WM;
     const int64_t n_tiles = (a.N + ROWS - 1) / ROWS;
     // (a dispatch: whole runs, and one for each used expert that is not whole)
     const int64_t runs = a.offsets ? a.M / BM + std::min(a.E, a.M) : (a.M + BM - 1) / BM;
-    hipLaunchKernelGGL((fp8_tile_kernel<GATED, EXACT, NS, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM), 0,
+    hipLaunchKernelGGL((fp8_tile_kernel<GATED, EXACT, DIRECT, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM), 0,
                        st, a, (int)n_tiles, (int)runs);
     return hipGetLastError();
 }
@@ -679,9 +966,8 @@ static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
     auto near = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0 && 256 * m.ld < 1ll << 32; };
     const int64_t rows = a.top ? (a.M + a.top - 1) / a.top : 256;
     if (!near(a.m[0]) || (GATED && !near(a.m[1])) || ((uintptr_t)a.x | a.ldx) % 16 || a.ldx * rows >= 1ll << 32)
-        return launch_tile_n<GATED, EXACT, 1, 4, 2, 4, 4>(a, st);
-    if (!GATED && !EXACT && !a.offsets && a.M >= 4096) return launch_tile_n<GATED, EXACT, 2, 2, 4, 8, 4>(a, st);
-    return launch_tile_n<GATED, EXACT, 3, 4, 2, 4, 4>(a, st);
+        return launch_tile_n<GATED, EXACT, false, 4, 2, 4, 4>(a, st);
+    return launch_tile_n<GATED, EXACT, true, 4, 2, 4, 4>(a, st);
 }
 
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
@@ -689,11 +975,8 @@ hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
         if (a.gated) return a.exact ? launch_tile<true, true>(a, st) : launch_tile<true, false>(a, st);
         return a.exact ? launch_tile<false, true>(a, st) : launch_tile<false, false>(a, st);
     }
-    const int64_t chunks = a.offsets ? 4 : (a.M + 15) / 16;
-    const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)a.E, (unsigned)(chunks < 1024 ? chunks : 1024));
-    if (a.gated) hipLaunchKernelGGL((fp8_stream_kernel<true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((fp8_stream_kernel<false>), grid, dim3(256), 0, st, a);
-    return hipGetLastError();
+    if (!a.offsets) return launch_stream<OF_ALL, false>(a, st);
+    return a.gated ? launch_stream<OF_DISPATCH, true>(a, st) : launch_stream<OF_DISPATCH, false>(a, st);
 }
 
 // out[t] = the sum over k, in order, of the rows of t's pairs; a pair whose id is no expert's has none

@@ -397,7 +397,26 @@ struct Fp8Args {
     int64_t ldh;
     float *hs;
     int64_t ldhs;
+    const int32_t *ids;           // few tokens: their experts [M], in place of a dispatch
+    int cols;                     // set by the launcher
 };
+// A layer of few tokens: gate and up from ids (a.x: rows of x_type, quantized on the way, ldx in elements; y: h f32 in the order of
+// pairs), then down and the sum over a token's experts.  A product of few rows likewise, without gate.
+struct Fp8FewArgs {
+    Fp8Mat down;
+    const float *h;               // [n_tok * K][I]
+    const int32_t *ids;
+    const float *w;
+    int n_tok, E, K, H, I, exact;
+    void *out;
+    int64_t ldo;
+    int out_type;
+    int parts;                    // set by the launcher
+};
+bool fp8_few_layer(int n_tok, int K, int H, int I);
+bool fp8_few_product(int M, int K);
+hipError_t launch_fp8_few_up(const Fp8Args &a, int x_type, hipStream_t st);
+hipError_t launch_fp8_few_down(Fp8FewArgs a, hipStream_t st);
 // rows of x for each expert from which products run on tiles
 constexpr int FP8_TILE_ROWS = 48;
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st);

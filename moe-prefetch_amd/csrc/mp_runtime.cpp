@@ -4284,6 +4284,10 @@ int moe_fp8_product(const moe_fp8_product_desc *d, void *stream) {
     a.M = d->n_tok; a.N = d->N; a.K = d->K; a.E = 1;
     a.exact = d->y_type == MOE_DTYPE_F32;
     a.y = d->y; a.ldy = d->y_stride; a.y_type = d->y_type;
+    if (!e4m3 && mp::fp8_few_product(d->n_tok, d->K)) {
+        HIPCHK(mp::launch_fp8_few_up(a, d->x_type, (hipStream_t)stream));
+        return MOE_OK;
+    }
     if (!e4m3) {
         size_t at = 0;
         const Fp8Rows q = fp8_rows(at, d->n_tok, d->K);
@@ -4349,15 +4353,24 @@ int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream) {
     uint8_t *ws = (uint8_t *)d->workspace;
     const int P = d->n_tok * d->K;
     int32_t *offsets = (int32_t *)(ws + l.offsets), *perm = (int32_t *)(ws + l.perm);
-    HIPCHK(mp::launch_dispatch(d->ids, P, d->E, (int32_t *)(ws + l.counts), offsets, perm, st));
-    HIPCHK(mp::launch_fp8_quant({d->x, d->x_stride, d->x_type, 1, d->n_tok, d->H, ws + l.x.q, l.x.ld, (float *)(ws + l.x.s), l.x.nb}, st));
     mp::Fp8Args a{};
     a.m[0] = fp8_mat(d->gate); a.m[1] = fp8_mat(d->up); a.gated = 1;
-    a.x = ws + l.x.q; a.ldx = l.x.ld; a.xs = (const float *)(ws + l.x.s); a.ldxs = l.x.nb;
-    a.offsets = offsets; a.perm = perm; a.top = d->K;
+    a.top = d->K;
     a.M = P; a.N = d->I; a.K = d->H; a.E = d->E;
     a.y = ws + l.act; a.ldy = d->I; a.y_type = MOE_DTYPE_F32;
     a.exact = d->out_type != MOE_DTYPE_BF16;
+    if (mp::fp8_few_layer(d->n_tok, d->K, d->H, d->I)) {
+        a.x = (const uint8_t *)d->x; a.ldx = d->x_stride;
+        a.ids = d->ids;
+        HIPCHK(mp::launch_fp8_few_up(a, d->x_type, st));
+        HIPCHK(mp::launch_fp8_few_down({fp8_mat(d->down), (const float *)(ws + l.act), d->ids, d->w, d->n_tok, d->E, d->K, d->H, d->I,
+                                        d->out_type == MOE_DTYPE_F32, d->out, d->out_stride, d->out_type}, st));
+        return MOE_OK;
+    }
+    HIPCHK(mp::launch_dispatch(d->ids, P, d->E, (int32_t *)(ws + l.counts), offsets, perm, st));
+    HIPCHK(mp::launch_fp8_quant({d->x, d->x_stride, d->x_type, 1, d->n_tok, d->H, ws + l.x.q, l.x.ld, (float *)(ws + l.x.s), l.x.nb}, st));
+    a.x = ws + l.x.q; a.ldx = l.x.ld; a.xs = (const float *)(ws + l.x.s); a.ldxs = l.x.nb;
+    a.offsets = offsets; a.perm = perm;
     a.hq = ws + l.h.q; a.ldh = l.h.ld; a.hs = (float *)(ws + l.h.s); a.ldhs = l.h.nb;
     HIPCHK(mp::launch_fp8_product(a, st));
     if (P < mp::FP8_TILE_ROWS * d->E)
