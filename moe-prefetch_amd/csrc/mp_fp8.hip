@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mp_device.h"
 #include "mp_elem.h"
@@ -202,6 +203,16 @@ __device__ inline float4_v mfma_block(int8_v w, int8_v x) {
     return d;
 }
 
+// acc += s * (w . x over a block).  The sum is done here: without the empty statement the compiler moves it behind a branch that follows, and there
+// it reads the product too early (it waits after the first of the four reads).
+template <bool EXACT>
+__device__ inline void add_block(float4_v &acc, int8_v w, int8_v x, float s) {
+    const float4_v d = mfma_block<EXACT>(w, x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = fmaf(d[k], s, acc[k]);
+    asm volatile("" : "+v"(acc));
+}
+
 // A lane's 32 of the 128 codes of a row's block: bytes 16 g .. and 64 + 16 g .., g = lane / 16 (which codes meet which is the same
 // for both operands).  n: bytes of the row from here on; codes past it are zeros.
 __device__ inline int4_v load16(const uint8_t *p, int n) {
@@ -211,12 +222,16 @@ __device__ inline int4_v load16(const uint8_t *p, int n) {
     for (int i = n - 1; i >= 8; --i) hi = hi << 8 | p[i];
     return int4_v{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 }
-__device__ inline int8_v load_frag(const uint8_t *row, int k, int K, int g) {
-    if (k + FB <= K)                                    // (the same for all lanes)
-        return __builtin_shufflevector(*(const int4_u *)(row + k + 16 * g), *(const int4_u *)(row + k + 64 + 16 * g), 0, 1, 2, 3, 4, 5, 6, 7);
+__device__ inline int8_v load_frag(const uint8_t *row, int b, int g) {              // of a whole block
+    const uint8_t *p = row + b * FB + 16 * g;
+    return __builtin_shufflevector(*(const int4_u *)p, *(const int4_u *)(p + 64), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ inline int8_v load_last(const uint8_t *row, int K, int g) {              // of the last one of K codes, which is not whole
+    const int k = K / FB * FB;
     return __builtin_shufflevector(load16(row + k + 16 * g, K - k - 16 * g), load16(row + k + 64 + 16 * g, K - k - 64 - 16 * g), 0, 1, 2, 3, 4,
                                    5, 6, 7);
 }
+
 __device__ inline void store_elem(void *p, int64_t i, int type, float v) {
     if (type == T_F32) ((float *)p)[i] = v;
     else if (type == T_BF16) ((uint16_t *)p)[i] = Elem<T_BF16>::store(v);
@@ -248,17 +263,19 @@ __device__ inline float silu_times(float g, float u) { return u * (g / (1.0f + e
 constexpr int OF_ALL = 0;         // rows 0 .. M - 1
 constexpr int OF_DISPATCH = 1;    // an expert's pairs from a dispatch
 
-// Sixteen rows of a weight (of gate and up: GATED) for 16 NT rows of codes at a time.  Four waves share K, a block each in turn, and their sums are
-// added in their order.  A wave's loads of DEEP blocks of the weight are on their way together: every weight is read once, and
-// memory bounds the call.
-template <int FROM, bool GATED, bool EXACT, int NT>
+// Sixteen rows of a weight (of gate and up: GATED) for 16 NT rows of codes at a time: every weight is read once, and memory bounds the call.
+// KS waves share K, a block each in turn, and their sums are added in their order; with KS 1 each of the workgroup's four has
+// sixteen rows of its own.  A wave's loads of DEEP blocks of the weight are on their way together.
+template <int FROM, bool GATED, bool EXACT, int NT, int KS>
 __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
-    constexpr int WAVES = 4, DEEP = GATED ? 2 : 4, MATS = GATED ? 2 : 1;
-    __shared__ float s_acc[MATS][WAVES][16 * NT][17];
+    // (two blocks of gate and up, three of down: 64 tokens of 128 experts 141 us; one and two 145, four and six 147: waves count, too)
+    constexpr int DEEP = NT > 1 ? (GATED ? 1 : 2) : GATED ? 2 : 3, MATS = GATED ? 2 : 1;
+    __shared__ float s_acc[KS > 1 ? MATS : 1][KS][KS > 1 ? 16 * NT : 1][17];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
-    const int n0 = blockIdx.x * 16, nb = (a.K + FB - 1) / FB;
+    const int n0 = (KS > 1 ? blockIdx.x : blockIdx.x * 4 + wave) * 16, whole = a.K / FB, first = KS > 1 ? wave : 0;
     const int e = FROM == OF_ALL ? 0 : (int)blockIdx.y;
     const int begin = FROM == OF_ALL ? 0 : a.offsets[e], end = FROM == OF_ALL ? a.M : a.offsets[e + 1];
+    if (KS == 1 && n0 >= a.N) return;
     const int64_t wrow = min(n0 + c, a.N - 1);
     const uint8_t *w[2] = {a.m[0].w + e * a.m[0].ex + wrow * a.m[0].ld, GATED ? a.m[1].w + e * a.m[1].ex + wrow * a.m[1].ld : nullptr};
     const float *ws[2] = {a.m[0].s + e * a.m[0].sex + (int64_t)(n0 / FB) * a.m[0].sld,
@@ -271,32 +288,71 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
             xrow[t] = FROM == OF_DISPATCH && a.top ? a.perm[p] / a.top : p;
         }
         float4_v acc[2][NT] = {};
-        for (int b0 = wave; b0 < nb; b0 += WAVES * DEEP) {
-            int8_v wf[DEEP][2];
-#pragma unroll
-            for (int i = 0; i < DEEP; ++i)
-                if (b0 + i * WAVES < nb)
-#pragma unroll
-                    for (int m = 0; m < MATS; ++m) wf[i][m] = load_frag(w[m], (b0 + i * WAVES) * FB, a.K, g);
+        for (int b0 = first; b0 < whole; b0 += KS * DEEP) {
+            int8_v wf[DEEP][2], xf[DEEP];               // (those of the other rows of x come one by one)
+            float f[DEEP][2], s[DEEP];
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) {
-                const int b = b0 + i * WAVES;
-                if (b >= nb) break;
-                const float f0 = ws[0][b], f1 = GATED ? ws[1][b] : 0.0f;
+                const int b = b0 + i * KS;
+                if (b >= whole) break;
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) {
+                    wf[i][m] = load_frag(w[m], b, g);
+                    f[i][m] = ws[m][b];
+                }
+                xf[i] = load_frag(a.x + xrow[0] * a.ldx, b, g);
+                s[i] = a.xs[xrow[0] * a.ldxs + b];
+            }
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) {
+                const int b = b0 + i * KS;
+                if (b >= whole) break;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     if (t > 0 && p0 + 16 * t >= end) break;
-                    const int8_v xf = load_frag(a.x + xrow[t] * a.ldx, b * FB, a.K, g);
-                    const float s = a.xs[xrow[t] * a.ldxs + b];
+                    const int8_v xt = t ? load_frag(a.x + xrow[t] * a.ldx, b, g) : xf[i];
+                    const float st = t ? a.xs[xrow[t] * a.ldxs + b] : s[i];
 #pragma unroll
-                    for (int m = 0; m < MATS; ++m) {
-                        const float4_v d = mfma_block<EXACT>(wf[i][m], xf);
-                        const float f = s * (m ? f1 : f0);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) acc[m][t][k] = fmaf(d[k], f, acc[m][t][k]);
-                    }
+                    for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m][t], wf[i][m], xt, st * f[i][m]);
                 }
             }
+        }
+        if (a.K % FB && whole % KS == first) {          // the last block
+            int8_v wf[MATS];
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) wf[m] = load_last(w[m], a.K, g);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int8_v xt = load_last(a.x + xrow[t] * a.ldx, a.K, g);
+                const float st = a.xs[xrow[t] * a.ldxs + whole];
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m][t], wf[m], xt, st * ws[m][whole]);
+            }
+        }
+        // (y, or h, of row p0 + col) -> where it goes, and its weight
+        auto out_of = [&](int col, float &weight) FP8_INLINE {
+            int64_t out = p0 + col;
+            weight = 1.0f;
+            if (FROM == OF_DISPATCH && a.pair_w) {
+                out = a.perm[out];
+                weight = a.pair_w[out];
+            }
+            return out;
+        };
+        if (KS == 1) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int col = 16 * t + c, n = n0 + 4 * g;
+                if (p0 + col >= end) continue;
+                float weight;
+                const int64_t out = out_of(col, weight);
+                float4_v y = acc[0][t];
+                if (GATED)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[k] = silu_times(y[k], acc[1][t][k]);
+                store4(a.y, out * a.ldy + n, a.y_type, FROM == OF_DISPATCH && a.pair_w ? y * weight : y, a.N - n);
+            }
+            continue;
         }
         __syncthreads();
 #pragma unroll
@@ -304,7 +360,7 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s_acc[m][wave][16 * t + c][4 * g + k] = acc[m][t][k];
+                for (int k = 0; k < 4; ++k) s_acc[m][first][16 * t + c][4 * g + k] = acc[m][t][k];
         __syncthreads();
         const int r = threadIdx.x & 15;
 #pragma unroll
@@ -316,15 +372,12 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
             for (int m = 0; m < MATS; ++m) {
                 y[m] = s_acc[m][0][col][r];
 #pragma unroll
-                for (int i = 1; i < WAVES; ++i) y[m] += s_acc[m][i][col][r];
+                for (int i = 1; i < KS; ++i) y[m] += s_acc[m][i][col][r];
             }
-            int64_t out = p0 + col;
-            float v = GATED ? silu_times(y[0], y[1]) : y[0];
-            if (FROM == OF_DISPATCH && a.pair_w) {
-                out = a.perm[out];
-                v *= a.pair_w[out];
-            }
-            store_elem(a.y, out * a.ldy + n0 + r, a.y_type, v);
+            float weight;
+            const int64_t out = out_of(col, weight);
+            const float v = GATED ? silu_times(y[0], y[1]) : y[0];
+            store_elem(a.y, out * a.ldy + n0 + r, a.y_type, FROM == OF_DISPATCH && a.pair_w ? v * weight : v);
         }
     }
 }
@@ -378,7 +431,7 @@ __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
     __shared__ float s_acc[MATS][WAVES][16][17];
     __shared__ uint8_t s_list[64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
-    const int n0 = blockIdx.x * 16, nb = (a.K + FB - 1) / FB, stride = lds_stride(a.K);
+    const int n0 = blockIdx.x * 16, nb = (a.K + FB - 1) / FB, whole = a.K / FB, stride = lds_stride(a.K);
     float *s_s = (float *)(s_q + a.cols * stride);
     int e = 0, n = a.M;
     if (GATED) {
@@ -398,10 +451,10 @@ __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
     auto load_w = [&](int b0) FP8_INLINE {
 #pragma unroll
         for (int i = 0; i < DEEP; ++i)
-            if (b0 + i * WAVES < nb)
+            if (b0 + i * WAVES < whole)
 #pragma unroll
                 for (int m = 0; m < MATS; ++m) {
-                    wf[i][m] = load_frag(w[m], (b0 + i * WAVES) * FB, a.K, g);
+                    wf[i][m] = load_frag(w[m], b0 + i * WAVES, g);
                     f[i][m] = ws[m][b0 + i * WAVES];
                 }
     };
@@ -417,24 +470,20 @@ __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
         const uint8_t *q = s_q + min(c, cols - 1) * stride;
         const float *s = s_s + min(c, cols - 1) * nb;
         float4_v acc[2] = {};
-        for (int b0 = wave; b0 < nb; b0 += WAVES * DEEP) {
+        auto add = [&](int8_v w, float f, int b, int m) FP8_INLINE { add_block<EXACT>(acc[m], w, lds_frag(q, b, g), s[b] * f); };
+        for (int b0 = wave; b0 < whole; b0 += WAVES * DEEP) {
             if (!loaded) load_w(b0);
             loaded = false;
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) {
-                const int b = b0 + i * WAVES;
-                if (b >= nb) break;
-                const int8_v xf = lds_frag(q, b, g);
-                const float sx = s[b];
+                if (b0 + i * WAVES >= whole) break;
 #pragma unroll
-                for (int m = 0; m < MATS; ++m) {
-                    const float4_v d = mfma_block<EXACT>(wf[i][m], xf);
-                    const float v = sx * f[i][m];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[m][k] = fmaf(d[k], v, acc[m][k]);
-                }
+                for (int m = 0; m < MATS; ++m) add(wf[i][m], f[i][m], b0 + i * WAVES, m);
             }
         }
+        if (whole < nb && whole % WAVES == wave)        // the last block
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) add(load_last(w[m], a.K, g), ws[m][whole], whole, m);
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
 #pragma unroll
@@ -460,12 +509,12 @@ __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
 // one's weights on their way while one is multiplied.  The pairs' rows meet in LDS, where each token's are added in order.
 template <bool EXACT>
 __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
-    constexpr int WAVES = 8, DEEP = 6;
+    constexpr int WAVES = 8, DEEP = EXACT ? 4 : 6;
     extern __shared__ __align__(16) uint8_t s_q[];      // [P][stride] codes, [P][nb] scales, [parts][P][17] rows
     __shared__ uint8_t s_col[WAVES][64];
     __shared__ float s_w[64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
-    const int n0 = blockIdx.x * 16, nb = (a.I + FB - 1) / FB, P = a.n_tok * a.K, stride = lds_stride(a.I);
+    const int n0 = blockIdx.x * 16, nb = (a.I + FB - 1) / FB, whole = a.I / FB, P = a.n_tok * a.K, stride = lds_stride(a.I);
     float *s_s = (float *)(s_q + P * stride), *s_rows = s_s + P * nb;
     const int per = WAVES / a.parts, part = wave / per;
     const int64_t wrow = min(n0 + c, a.H - 1);
@@ -483,15 +532,19 @@ __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
     const uint64_t firsts = __ballot(is && __ffsll((unsigned long long)same) - 1 == lane);      // the experts' first pairs
     int8_v wf[2][DEEP];
     float f[2][DEEP];
-    auto weight = [&](int j, int b, float &s) FP8_INLINE {
-        const int64_t e = __builtin_amdgcn_readlane(mine, j);
-        s = (a.down.s + e * a.down.sex + (int64_t)(n0 / FB) * a.down.sld)[b];
-        return load_frag(a.down.w + e * a.down.ex + wrow * a.down.ld, b * FB, a.I, g);
+    auto row = [&](int j) FP8_INLINE {
+        return a.down.w + __builtin_amdgcn_readlane(mine, j) * a.down.ex + wrow * a.down.ld;
+    };
+    auto scale = [&](int j, int b) FP8_INLINE {
+        return (a.down.s + __builtin_amdgcn_readlane(mine, j) * a.down.sex + (int64_t)(n0 / FB) * a.down.sld)[b];
     };
     auto load_w = [&](int8_v (&wd)[DEEP], float (&fd)[DEEP], int j) FP8_INLINE {
 #pragma unroll
         for (int i = 0; i < DEEP; ++i)
-            if (part + i * a.parts < nb) wd[i] = weight(j, part + i * a.parts, fd[i]);
+            if (part + i * a.parts < whole) {
+                wd[i] = load_frag(row(j), part + i * a.parts, g);
+                fd[i] = scale(j, part + i * a.parts);
+            }
     };
     // this wave's experts: every per-th of those in use
     uint64_t todo = firsts;
@@ -513,20 +566,12 @@ __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
             const int pair = s_col[wave][min(p0 + c, n - 1)];
             const uint8_t *q = s_q + pair * stride;
             float4_v acc = {};
-            auto add = [&](int8_v w, int b, float sw) FP8_INLINE {
-                const float4_v d = mfma_block<EXACT>(w, lds_frag(q, b, g));
-                const float v = s_s[pair * nb + b] * sw;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] = fmaf(d[k], v, acc[k]);
-            };
+            auto add = [&](int8_v w, int b, float sw) FP8_INLINE { add_block<EXACT>(acc, w, lds_frag(q, b, g), s_s[pair * nb + b] * sw); };
 #pragma unroll
             for (int i = 0; i < DEEP; ++i)
-                if (part + i * a.parts < nb) add(wd[i], part + i * a.parts, fd[i]);
-            for (int b = part + DEEP * a.parts; b < nb; b += a.parts) {
-                float sw;
-                const int8_v w = weight(j, b, sw);
-                add(w, b, sw);
-            }
+                if (part + i * a.parts < whole) add(wd[i], part + i * a.parts, fd[i]);
+            for (int b = part + DEEP * a.parts; b < whole; b += a.parts) add(load_frag(row(j), b, g), b, scale(j, b));
+            if (whole < nb && whole % a.parts == part) add(load_last(row(j), a.I, g), whole, scale(j, whole));
             if (p0 + c < n)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) s_rows[(part * P + pair) * 17 + 4 * g + k] = acc[k];
@@ -590,19 +635,20 @@ hipError_t launch_fp8_few_down(Fp8FewArgs a, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <int FROM, bool GATED, int NT>
+template <int FROM, bool GATED, int NT, int KS>
 static hipError_t launch_stream_n(const Fp8Args &a, hipStream_t st) {
     const int64_t groups = (a.M + 16 * NT - 1) / (16 * NT);
-    const dim3 grid((unsigned)((a.N + 15) / 16), FROM == OF_ALL ? 1 : (unsigned)a.E, FROM == OF_ALL ? (unsigned)std::min(groups, (int64_t)4096) : 1);
-    if (a.exact) hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, true, NT>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, false, NT>), grid, dim3(256), 0, st, a);
+    const int rows = KS > 1 ? 16 : 64;
+    const dim3 grid((unsigned)((a.N + rows - 1) / rows), FROM == OF_ALL ? 1 : (unsigned)a.E, FROM == OF_ALL ? (unsigned)std::min(groups, (int64_t)4096) : 1);
+    if (a.exact) hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, true, NT, KS>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, false, NT, KS>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
-template <int FROM, bool GATED>
+template <bool GATED>
 static hipError_t launch_stream(const Fp8Args &a, hipStream_t st) {
     const int rows = a.M / a.E;                         // of an expert, about
-    return rows <= 16 ? launch_stream_n<FROM, GATED, 1>(a, st) : rows <= 32 ? launch_stream_n<FROM, GATED, 2>(a, st)
-                                                               : launch_stream_n<FROM, GATED, 4>(a, st);
+    return rows <= 16 ? launch_stream_n<OF_DISPATCH, GATED, 1, 1>(a, st) : rows <= 32 ? launch_stream_n<OF_DISPATCH, GATED, 2, 1>(a, st)
+                                                                           : launch_stream_n<OF_DISPATCH, GATED, 4, 1>(a, st);
 }
 
 // ---- products of many rows: tiles through LDS --------------------------------------
@@ -827,37 +873,51 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Args a, int n
         // wave has read all of it, the next stage's first operands are read.  The loads stand between the rows of tiles: all at once
         // they would hold up the reads and products behind them (4096^3: 96 us, 79 so).
         constexpr int EACH_ROW = (CH + TN - 2) / (TN - 1);
-        auto step = [&](int4_v *s, int4_v *next, int4_v *after, Operands &o, Operands &on, int u) FP8_INLINE {
-            multiply(s, o, [&]() FP8_INLINE {
-                if (u == SB - 1) put_scales(par ^= 1);
-                wait_loads<CH>();                       // the next stage is there
-                barrier();                              // and every wave's part of it; and all have read this one
-                fetch(on, next, par, (u + 1) % SB);
-            }, [&](int i) FP8_INLINE {
-                if (i < TN - 1) stage(after, min(b + u + 2, whole - 1), i * EACH_ROW, EACH_ROW);
-            });
+        auto run = [&](auto live) FP8_INLINE {
+            constexpr bool LIVE = decltype(live)::value;
+            auto step = [&](int4_v *s, int4_v *next, int4_v *after, Operands &o, Operands &on, int u) FP8_INLINE {
+                auto along = [&](int i) FP8_INLINE {
+                    if (i < TN - 1) stage(after, min(b + u + 2, whole - 1), i * EACH_ROW, EACH_ROW);
+                };
+                auto then = [&]() FP8_INLINE {
+                    if (u == SB - 1) put_scales(par ^= 1);
+                    wait_loads<CH>();                   // the next stage is there
+                    barrier();                          // and every wave's part of it; and all have read this one
+                    if (LIVE) fetch(on, next, par, (u + 1) % SB);
+                };
+                if (LIVE) {
+                    multiply(s, o, then, along);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < TN - 1; ++i) along(i);
+                    then();
+                }
+            };
+            auto steps = [&](int n) FP8_INLINE {
+                step(s_0, s_1, s_2, o0, o1, 0);
+                if (n > 1) step(s_1, s_2, s_0, o1, o0, 1);
+                if (n > 2) step(s_2, s_0, s_1, o0, o1, 2);
+                if (n > 3) step(s_0, s_1, s_2, o1, o0, 3);
+                if (n > 4) step(s_1, s_2, s_0, o0, o1, 4);
+                if (n > 5) step(s_2, s_0, s_1, o1, o0, 5);
+            };
+            fetch_scales(0);
+            stage(s_0, 0, 0, CH);
+            stage(s_1, min(1, whole - 1), 0, CH);
+            put_scales(0);
+            wait_loads<CH>();
+            barrier();
+            if (LIVE) fetch(o0, s_0, 0, 0);
+            for (; b + SB <= whole; b += SB) {
+                fetch_scales(b + SB);
+                steps(SB);
+            }
+            if (b < whole) steps(whole - b);
+            wait_loads<0>();
         };
-        auto steps = [&](int n) FP8_INLINE {
-            step(s_0, s_1, s_2, o0, o1, 0);
-            if (n > 1) step(s_1, s_2, s_0, o1, o0, 1);
-            if (n > 2) step(s_2, s_0, s_1, o0, o1, 2);
-            if (n > 3) step(s_0, s_1, s_2, o1, o0, 3);
-            if (n > 4) step(s_1, s_2, s_0, o0, o1, 4);
-            if (n > 5) step(s_2, s_0, s_1, o1, o0, 5);
-        };
-        fetch_scales(0);
-        stage(s_0, 0, 0, CH);
-        stage(s_1, min(1, whole - 1), 0, CH);
-        put_scales(0);
-        wait_loads<CH>();
-        barrier();
-        fetch(o0, s_0, 0, 0);
-        for (; b + SB <= whole; b += SB) {
-            fetch_scales(b + SB);
-            steps(SB);
-        }
-        if (b < whole) steps(whole - b);
-        wait_loads<0>();
+        // a wave none of whose rows of x are there only loads
+        if (p0 + 16 * TM * wm < end) run(std::true_type{});
+        else run(std::false_type{});
     } else {
         fetch_scales(0);
         put_scales(0);
@@ -960,40 +1020,61 @@ static hipError_t launch_tile_n(const Fp8Args &a, hipStream_t st) {
                        st, a, (int)n_tiles, (int)runs);
     return hipGetLastError();
 }
-template <bool GATED, bool EXACT>
-static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
+template <bool GATED, bool EXACT, int WN, int WM, int TN, int TM>
+static hipError_t launch_tile_d(const Fp8Args &a, hipStream_t st) {
     // rows on 16 bytes, and a workgroup's within 4 GiB (those of x from a dispatch: all)
     auto near = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0 && 256 * m.ld < 1ll << 32; };
     const int64_t rows = a.top ? (a.M + a.top - 1) / a.top : 256;
     if (!near(a.m[0]) || (GATED && !near(a.m[1])) || ((uintptr_t)a.x | a.ldx) % 16 || a.ldx * rows >= 1ll << 32)
-        return launch_tile_n<GATED, EXACT, false, 4, 2, 4, 4>(a, st);
-    return launch_tile_n<GATED, EXACT, true, 4, 2, 4, 4>(a, st);
+        return launch_tile_n<GATED, EXACT, false, WN, WM, TN, TM>(a, st);
+    return launch_tile_n<GATED, EXACT, true, WN, WM, TN, TM>(a, st);
+}
+template <bool GATED>
+static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
+    return a.exact ? launch_tile_d<GATED, true, 4, 2, 4, 4>(a, st) : launch_tile_d<GATED, false, 4, 2, 4, 4>(a, st);
 }
 
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
-    if (a.M >= FP8_TILE_ROWS * a.E) {
-        if (a.gated) return a.exact ? launch_tile<true, true>(a, st) : launch_tile<true, false>(a, st);
-        return a.exact ? launch_tile<false, true>(a, st) : launch_tile<false, false>(a, st);
+    if (!a.offsets) {
+        if (a.M <= 16) return launch_stream_n<OF_ALL, false, 1, 4>(a, st);
+        // 256 x 128 tiles where they are many enough for every compute unit, else 64 x 64
+        if ((int64_t)((a.N + 255) / 256) * ((a.M + 127) / 128) >= 200) return launch_tile<false>(a, st);
+        return a.exact ? launch_tile_d<false, true, 2, 2, 2, 2>(a, st) : launch_tile_d<false, false, 2, 2, 2, 2>(a, st);
     }
-    if (!a.offsets) return launch_stream<OF_ALL, false>(a, st);
-    return a.gated ? launch_stream<OF_DISPATCH, true>(a, st) : launch_stream<OF_DISPATCH, false>(a, st);
+    if (a.M >= FP8_TILE_ROWS * a.E) return a.gated ? launch_tile<true>(a, st) : launch_tile<false>(a, st);
+    return a.gated ? launch_stream<true>(a, st) : launch_stream<false>(a, st);
 }
 
-// out[t] = the sum over k, in order, of the rows of t's pairs; a pair whose id is no expert's has none
+// out[t] = the sum over k, in order, of the rows of t's pairs; a pair whose id is no expert's has none.  Four columns a thread, four rows on
+// their way at once.
 __global__ __launch_bounds__(256) void fp8_combine_kernel(Fp8CombineArgs a) {
-    const int h = blockIdx.x * 256 + threadIdx.x;
+    const int h = 4 * (blockIdx.x * 256 + threadIdx.x), n = a.H - h;
     const int64_t t = blockIdx.y + (int64_t)gridDim.y * blockIdx.z;
-    if (h >= a.H || t >= a.n_tok) return;
-    float s = 0.0f;
-    for (int k = 0; k < a.K; ++k) {
-        const int64_t i = t * a.K + k;
-        if ((uint32_t)a.ids[i] < (uint32_t)a.E) s += a.rows[i * a.H + h];
+    if (n <= 0 || t >= a.n_tok) return;
+    const int32_t *ids = a.ids + t * a.K;
+    const float *rows = a.rows + t * a.K * a.H + h;
+    float4_v s = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = 0; k0 < a.K; k0 += 4) {
+        float4_v v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = float4_v{0.0f, 0.0f, 0.0f, 0.0f};
+            if (k0 + k >= a.K || (uint32_t)ids[k0 + k] >= (uint32_t)a.E) continue;
+            const float *p = rows + (int64_t)(k0 + k) * a.H;
+            if (n >= 4) __builtin_memcpy(&v[k], p, 16);
+            else
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    if (i < n) v[k][i] = p[i];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s += v[k];
     }
-    store_elem(a.out, t * a.ldo + h, a.out_type, s);
+    store4(a.out, t * a.ldo + h, a.out_type, s, n);
 }
 hipError_t launch_fp8_combine(const Fp8CombineArgs &a, hipStream_t st) {
     const unsigned y = (unsigned)(a.n_tok < 32768 ? a.n_tok : 32768);
-    hipLaunchKernelGGL(fp8_combine_kernel, dim3((unsigned)((a.H + 255) / 256), y, (unsigned)((a.n_tok + y - 1) / y)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(fp8_combine_kernel, dim3((unsigned)((a.H + 1023) / 1024), y, (unsigned)((a.n_tok + y - 1) / y)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
