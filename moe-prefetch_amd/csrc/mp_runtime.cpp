@@ -4253,7 +4253,9 @@ static Fp8Rows fp8_rows(size_t &at, int64_t rows, int K) {
 }
 
 size_t moe_fp8_product_workspace_bytes(int n_tok, int N, int K, int x_type) {
-    if (n_tok < 1 || n_tok > MOE_BLOCK_MAX_TOKENS || !fp8_dim(N) || !fp8_dim(K) || x_type == MOE_DTYPE_E4M3) return 0;
+    if (n_tok < 1 || n_tok > MOE_BLOCK_MAX_TOKENS || !fp8_dim(N) || !fp8_dim(K) || x_type == MOE_DTYPE_E4M3 ||
+        mp::fp8_few_product(n_tok, K))
+        return 0;
     size_t at = 0;
     fp8_rows(at, n_tok, K);
     return at;
@@ -4276,7 +4278,8 @@ int moe_fp8_product(const moe_fp8_product_desc *d, void *stream) {
         return fail(MOE_ERR_ARG, "moe_fp8_product: a row stride below the row's length");
     if ((!e4m3 && !aligned_to(d->x, d->x_type)) || (e4m3 && (uintptr_t)d->x_scale % 4) || !aligned_to(d->y, d->y_type))
         return fail(MOE_ERR_ARG, "moe_fp8_product: misaligned pointer");
-    if (!e4m3 && (!d->workspace || (uintptr_t)d->workspace % 16))
+    const bool few = !e4m3 && mp::fp8_few_product(d->n_tok, d->K);
+    if (!e4m3 && !few && (!d->workspace || (uintptr_t)d->workspace % 16))
         return fail(MOE_ERR_ARG, "moe_fp8_product: workspace must be given and 16-byte aligned");
     mp::Fp8Args a{};
     a.m[0] = fp8_mat(d->weight);
@@ -4284,7 +4287,7 @@ int moe_fp8_product(const moe_fp8_product_desc *d, void *stream) {
     a.M = d->n_tok; a.N = d->N; a.K = d->K; a.E = 1;
     a.exact = d->y_type == MOE_DTYPE_F32;
     a.y = d->y; a.ldy = d->y_stride; a.y_type = d->y_type;
-    if (!e4m3 && mp::fp8_few_product(d->n_tok, d->K)) {
+    if (few) {
         HIPCHK(mp::launch_fp8_few_up(a, d->x_type, (hipStream_t)stream));
         return MOE_OK;
     }

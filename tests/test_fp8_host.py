@@ -40,7 +40,7 @@ def weight(name, n, k, **kw):
 
 
 def product(**kw):
-    d = dict(x=PTR, x_stride=300, x_type=1, n_tok=2, N=200, K=300, y=PTR, y_stride=200, y_type=1, workspace=PTR)
+    d = dict(x=PTR, x_stride=300, x_type=1, n_tok=20, N=200, K=300, y=PTR, y_stride=200, y_type=1, workspace=PTR)
     d.update(weight("weight", 200, 300))
     d.update(kw)
     return L.moe_fp8_product(ctypes.byref(_lib.Fp8ProductDesc(**d)), None)
@@ -113,6 +113,7 @@ def test_workspaces():
     assert L.moe_fp8_product_workspace_bytes(4, 100, 300, 3) == 0
     assert L.moe_fp8_product_workspace_bytes(0, 100, 300, 1) == 0
     assert L.moe_fp8_product_workspace_bytes(4, 0, 300, 1) == 0
+    assert L.moe_fp8_product_workspace_bytes(16, 100, 300, 1) == 0 < L.moe_fp8_product_workspace_bytes(16, 100, 1 << 18, 1)
     assert L.moe_fp8_product_workspace_bytes(1000, 100, 300, 1) >= 1000 * (300 + 12)
     assert L.moe_fp8_layer_workspace_bytes(0, 8, 2, 256, 128) == 0
     assert L.moe_fp8_layer_workspace_bytes(32768, 8, 2, 256, 128) == 0
@@ -179,9 +180,9 @@ def test_quantize_hands_on(monkeypatch):
 def test_linear_hands_on():
     lin = Fp8Linear(OnGpu(200, 320, dtype=F8, at=99)[:, :300], OnGpu(2, 5)[:, :3])
     seen, lin._fn = given(lin, _lib.Fp8ProductDesc)
-    y = lin(OnGpu(4, 300, dtype=BF16))
+    y = lin(OnGpu(40, 300, dtype=BF16))
     d, stream = seen[0]
-    assert (d.weight, d.weight_stride, d.weight_scale_stride, d.N, d.K, d.n_tok) == (99, 320, 5, 200, 300, 4)
+    assert (d.weight, d.weight_stride, d.weight_scale_stride, d.N, d.K, d.n_tok) == (99, 320, 5, 200, 300, 40)
     assert (d.x_type, d.y_type, d.y_stride, d.workspace, stream, y.dtype) == (1, 1, 200, 1 << 20, 77, BF16)
     y = lin(OnGpu(4, 300, dtype=F8), OnGpu(4, 3, at=555))
     d = seen[1][0]
