@@ -504,87 +504,157 @@ __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
     }
 }
 
-// The down product of a few tokens' layer and the sum over their experts: sixteen columns of out for all tokens.  h of all pairs is quantized into
-// LDS while the first weights are on their way; eight waves share the experts in use (where these are fewer, also K), the next
-// one's weights on their way while one is multiplied.  The pairs' rows meet in LDS, where each token's are added in order.
+constexpr int MID_PAIRS = 512;
+// The same for up to MID_PAIRS pairs: workgroup y has expert y (where experts are more than pairs: the expert of pair y, if that is its first one),
+// whose pairs every wave finds among the ids, and each of its four waves sixteen rows of the weights.  The expert's rows of x (GATED; else of h: in f32 and in the order of pairs, as GATED leaves them) are quantized into LDS
+// by the workgroup, a wave's weights of DEEP blocks on their way while those before are multiplied.
+template <int T, bool GATED, bool EXACT>
+__global__ __launch_bounds__(256) void fp8_mid_kernel(Fp8Args a) {
+    constexpr int DEEP = GATED ? 1 : 2, MATS = GATED ? 2 : 1;
+    extern __shared__ __align__(16) uint8_t s_q[];      // [cols][stride] codes, [cols][nb] scales
+    __shared__ uint16_t s_list[MID_PAIRS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int n0 = (blockIdx.x * 4 + wave) * 16, nb = (a.K + FB - 1) / FB, whole = a.K / FB, stride = lds_stride(a.K);
+    const int e = a.E > a.M ? a.ids[blockIdx.y] : blockIdx.y;
+    float *s_s = (float *)(s_q + a.cols * stride);
+    int ids[MID_PAIRS / 64], n = 0, first = -1;
+#pragma unroll
+    for (int j = 0; j < MID_PAIRS / 64; ++j) ids[j] = 64 * j + lane < a.M ? a.ids[64 * j + lane] : -1;
+#pragma unroll
+    for (int j = 0; j < MID_PAIRS / 64; ++j) {
+        const uint64_t m = __ballot(ids[j] == e);
+        if (wave == 0 && ids[j] == e) s_list[n + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)(64 * j + lane);
+        if (n == 0 && m) first = 64 * j + __ffsll((unsigned long long)m) - 1;
+        n += __popcll(m);
+    }
+    if (n == 0 || (uint32_t)e >= (uint32_t)a.E || (a.E > a.M && first != (int)blockIdx.y)) return;
+    const int64_t wrow = min(n0 + c, a.N - 1), srow = min(n0, a.N - 1) / FB;
+    const uint8_t *w[2] = {a.m[0].w + e * a.m[0].ex + wrow * a.m[0].ld, GATED ? a.m[1].w + e * a.m[1].ex + wrow * a.m[1].ld : nullptr};
+    const float *ws[2] = {a.m[0].s + e * a.m[0].sex + srow * a.m[0].sld, GATED ? a.m[1].s + e * a.m[1].sex + srow * a.m[1].sld : nullptr};
+    struct Weights {
+        int8_v w[DEEP][MATS];
+        float s[DEEP][MATS];
+    };
+    Weights w0, w1;
+    auto load_w = [&](Weights &t, int b0) FP8_INLINE {
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i)
+            if (b0 + i < whole)
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) {
+                    t.w[i][m] = load_frag(w[m], b0 + i, g);
+                    t.s[i][m] = ws[m][b0 + i];
+                }
+    };
+    load_w(w0, 0);
+    __syncthreads();                                    // the list
+    for (int p0 = 0; p0 < n; p0 += a.cols) {
+        const int cols = min(n - p0, a.cols);
+        if (p0) {
+            load_w(w0, 0);
+            __syncthreads();                            // the rows before are read
+        }
+        quant_to_lds<T, 256>(cols, a.K, [&](int i) {
+            return (const typename Elem<T>::raw *)a.x + (int64_t)(GATED ? s_list[p0 + i] / a.top : s_list[p0 + i]) * a.ldx;
+        }, s_q, stride, s_s);
+        __syncthreads();
+        const uint8_t *q = s_q + min(c, cols - 1) * stride;
+        const float *s = s_s + min(c, cols - 1) * nb;
+        float4_v acc[2] = {};
+        auto add = [&](const Weights &t, int b0) FP8_INLINE {
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i)
+                if (b0 + i < whole)
+#pragma unroll
+                    for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m], t.w[i][m], lds_frag(q, b0 + i, g), s[b0 + i] * t.s[i][m]);
+        };
+        for (int b0 = 0; b0 < whole; b0 += 2 * DEEP) {
+            load_w(w1, b0 + DEEP);
+            add(w0, b0);
+            load_w(w0, b0 + 2 * DEEP);
+            add(w1, b0 + DEEP);
+        }
+        if (whole < nb)                                 // the last block
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m], load_last(w[m], a.K, g), lds_frag(q, whole, g), s[whole] * ws[m][whole]);
+        const int n1 = n0 + 4 * g;
+        if (c < cols && n1 < a.N) {
+            const int pair = s_list[p0 + c];
+            float4_v y = acc[0];
+            if (GATED)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[k] = silu_times(y[k], acc[1][k]);
+            else y *= a.pair_w[pair];
+            store4(a.y, (int64_t)pair * a.ldy + n1, T_F32, y, a.N - n1);
+        }
+    }
+}
+
+// The down product of DOWN_PAIRS pairs at most and the sum over a token's experts: sixteen columns of out for all tokens.  h of all pairs is
+// quantized into LDS while the weights are on their way; eight waves share the experts in use, and K.  The pairs' rows meet in LDS,
+// where each token's are added in order.
+constexpr int DOWN_PAIRS = 4;
 template <bool EXACT>
 __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
-    constexpr int WAVES = 8, DEEP = EXACT ? 4 : 6;
+    constexpr int WAVES = 8, DEEP = 6;
     extern __shared__ __align__(16) uint8_t s_q[];      // [P][stride] codes, [P][nb] scales, [parts][P][17] rows
-    __shared__ uint8_t s_col[WAVES][64];
-    __shared__ float s_w[64];
+    __shared__ float s_w[DOWN_PAIRS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     const int n0 = blockIdx.x * 16, nb = (a.I + FB - 1) / FB, whole = a.I / FB, P = a.n_tok * a.K, stride = lds_stride(a.I);
     float *s_s = (float *)(s_q + P * stride), *s_rows = s_s + P * nb;
-    const int per = WAVES / a.parts, part = wave / per;
+    // this wave's expert: the one of pair `mine`, if that is its first, and which of the parts of K
+    const int per = WAVES / a.parts, part = wave / per, mine = wave % per;
     const int64_t wrow = min(n0 + c, a.H - 1);
-    const int mine = lane < P ? a.ids[lane] : -1;
-    const bool is = (uint32_t)mine < (uint32_t)a.E;
-    if (wave == 0 && lane < P) s_w[lane] = is ? a.w[lane] : 0.0f;
-    const uint64_t used = __ballot(is);
-    uint64_t same = used;                               // the pairs of a lane's expert, found bit by bit of the id
+    int ids[DOWN_PAIRS], e = -1, n = 0, pair = 0;       // pair: of this lane's column, the c-th of e's
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
-        const bool bit = mine >> b & 1;
-        const uint64_t m = __ballot(bit);
-        same &= bit ? m : ~m;
+    for (int j = 0; j < DOWN_PAIRS; ++j) {
+        ids[j] = j < P ? a.ids[j] : -1;
+        if (j == mine) e = ids[j];
     }
-    const uint64_t firsts = __ballot(is && __ffsll((unsigned long long)same) - 1 == lane);      // the experts' first pairs
-    int8_v wf[2][DEEP];
-    float f[2][DEEP];
-    auto row = [&](int j) FP8_INLINE {
-        return a.down.w + __builtin_amdgcn_readlane(mine, j) * a.down.ex + wrow * a.down.ld;
-    };
-    auto scale = [&](int j, int b) FP8_INLINE {
-        return (a.down.s + __builtin_amdgcn_readlane(mine, j) * a.down.sex + (int64_t)(n0 / FB) * a.down.sld)[b];
-    };
-    auto load_w = [&](int8_v (&wd)[DEEP], float (&fd)[DEEP], int j) FP8_INLINE {
+    bool live = (uint32_t)e < (uint32_t)a.E;
+#pragma unroll
+    for (int j = 0; j < DOWN_PAIRS; ++j) {
+        if (j >= P || ids[j] != e) continue;
+        if (j < mine) live = false;                     // another wave's
+        if (n <= c) pair = j;
+        ++n;
+    }
+    if (threadIdx.x < P) s_w[threadIdx.x] = a.w[threadIdx.x];
+    const uint8_t *w = a.down.w + (live ? e : 0) * a.down.ex + wrow * a.down.ld;
+    const float *ws = a.down.s + (live ? e : 0) * a.down.sex + (int64_t)(n0 / FB) * a.down.sld;
+    int8_v wf[DEEP];
+    float f[DEEP];
+    if (live)
 #pragma unroll
         for (int i = 0; i < DEEP; ++i)
             if (part + i * a.parts < whole) {
-                wd[i] = load_frag(row(j), part + i * a.parts, g);
-                fd[i] = scale(j, part + i * a.parts);
+                wf[i] = load_frag(w, part + i * a.parts, g);
+                f[i] = ws[part + i * a.parts];
             }
-    };
-    // this wave's experts: every per-th of those in use
-    uint64_t todo = firsts;
-    auto next = [&](int skip) FP8_INLINE {
-        for (; skip > 0 && todo; --skip) todo &= todo - 1;
-        return todo ? __ffsll((unsigned long long)todo) - 1 : -1;
-    };
-    int j = next(wave % per);
-    if (j >= 0) load_w(wf[0], f[0], j);
     quant_to_lds<T_F32, 512>(P, a.I, [&](int i) { return a.h + (int64_t)i * a.I; }, s_q, stride, s_s);
     __syncthreads();
-    auto expert = [&](int j, const int8_v (&wd)[DEEP], const float (&fd)[DEEP]) FP8_INLINE {
-        const uint64_t m = __ballot(mine == __builtin_amdgcn_readlane(mine, j));
-        const int n = __popcll(m);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        list_bits(m, s_col[wave]);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        for (int p0 = 0; p0 < n; p0 += 16) {
-            const int pair = s_col[wave][min(p0 + c, n - 1)];
-            const uint8_t *q = s_q + pair * stride;
-            float4_v acc = {};
-            auto add = [&](int8_v w, int b, float sw) FP8_INLINE { add_block<EXACT>(acc, w, lds_frag(q, b, g), s_s[pair * nb + b] * sw); };
+    if (live) {
+        const uint8_t *q = s_q + pair * stride;
+        float4_v acc = {};
+        auto add = [&](int8_v w, int b, float sw) FP8_INLINE { add_block<EXACT>(acc, w, lds_frag(q, b, g), s_s[pair * nb + b] * sw); };
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i)
+            if (part + i * a.parts < whole) add(wf[i], part + i * a.parts, f[i]);
+        for (int b0 = part + DEEP * a.parts; b0 < whole; b0 += DEEP * a.parts) {
 #pragma unroll
             for (int i = 0; i < DEEP; ++i)
-                if (part + i * a.parts < whole) add(wd[i], part + i * a.parts, fd[i]);
-            for (int b = part + DEEP * a.parts; b < whole; b += a.parts) add(load_frag(row(j), b, g), b, scale(j, b));
-            if (whole < nb && whole % a.parts == part) add(load_last(row(j), a.I, g), whole, scale(j, whole));
-            if (p0 + c < n)
+                if (b0 + i * a.parts < whole) {
+                    wf[i] = load_frag(w, b0 + i * a.parts, g);
+                    f[i] = ws[b0 + i * a.parts];
+                }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s_rows[(part * P + pair) * 17 + 4 * g + k] = acc[k];
+            for (int i = 0; i < DEEP; ++i)
+                if (b0 + i * a.parts < whole) add(wf[i], b0 + i * a.parts, f[i]);
         }
-    };
-    while (j >= 0) {
-        const int j1 = next(per);
-        if (j1 >= 0) load_w(wf[1], f[1], j1);
-        expert(j, wf[0], f[0]);
-        if (j1 < 0) break;
-        j = next(per);
-        if (j >= 0) load_w(wf[0], f[0], j);
-        expert(j1, wf[1], f[1]);
+        if (whole < nb && whole % a.parts == part) add(load_last(w, a.I, g), whole, ws[whole]);
+        if (c < n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s_rows[(part * P + pair) * 17 + 4 * g + k] = acc[k];
     }
     __syncthreads();
     for (int i = threadIdx.x; i < a.n_tok * 16; i += 64 * WAVES) {
@@ -593,7 +663,7 @@ __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
         float sum = 0.0f;
         for (int k = 0; k < a.K; ++k) {
             const int pair = t * a.K + k;
-            if (!(used >> pair & 1)) continue;          // of no expert: nothing stands there
+            if ((uint32_t)a.ids[pair] >= (uint32_t)a.E) continue;      // of no expert: nothing stands there
             float v = s_rows[pair * 17 + r];
             for (int q = 1; q < a.parts; ++q) v += s_rows[(q * P + pair) * 17 + r];
             sum += s_w[pair] * v;
@@ -602,29 +672,30 @@ __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
     }
 }
 
-constexpr int FEW_LDS = 60 * 1024;
-// Which layers and products take these kernels: as many pairs as a wave has lanes, and rows that LDS holds.
-bool fp8_few_layer(int n_tok, int K, int H, int I) {
-    const int64_t P = (int64_t)n_tok * K;
-    return P <= 64 && std::min(P, (int64_t)16) * (lds_stride(H) + 4 * ((H + FB - 1) / FB)) <= FEW_LDS - 10000 &&
-           P * (lds_stride(I) + 4 * ((I + FB - 1) / FB)) + std::max(P, (int64_t)8) * 17 * 4 <= FEW_LDS;
+// Rows of K codes in LDS, at most sixteen, beside a kernel's own 9 KiB
+static int lds_rows(int K) { return std::min(16, 54 * 1024 / (lds_stride(K) + 4 * ((K + FB - 1) / FB))); }
+bool fp8_few_product(int M, int K) { return M <= lds_rows(K); }
+// Which layers take these kernels: few pairs, an expert's about one tile of them; and rows that LDS holds, all or not too few at once.
+bool fp8_few_layer(int64_t P, int E, int H, int I) {
+    return P <= MID_PAIRS && P <= std::max(64, 16 * E) && std::min(P, (int64_t)2) <= lds_rows(std::max(H, I));
 }
-bool fp8_few_product(int M, int K) { return M <= 16 && (int64_t)M * (lds_stride(K) + 4 * ((K + FB - 1) / FB)) <= FEW_LDS - 6000; }
 
 template <int T, bool GATED>
 static hipError_t launch_few_t(Fp8Args a, hipStream_t st) {
-    a.cols = std::min(a.M, 16);
+    a.cols = std::min(a.M, lds_rows(a.K));
     const dim3 grid((unsigned)((a.N + 15) / 16), GATED ? (unsigned)a.M : 1);
     const size_t lds = (size_t)a.cols * (lds_stride(a.K) + 4 * ((a.K + FB - 1) / FB));
     if (a.exact) hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED, true>), grid, dim3(256), lds, st, a);
     else hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED, false>), grid, dim3(256), lds, st, a);
     return hipGetLastError();
 }
-hipError_t launch_fp8_few_up(const Fp8Args &a, int x_type, hipStream_t st) {
-    if (a.gated) return x_type == T_F32 ? launch_few_t<T_F32, true>(a, st) : x_type == T_BF16 ? launch_few_t<T_BF16, true>(a, st) : launch_few_t<T_F16, true>(a, st);
-    return x_type == T_F32 ? launch_few_t<T_F32, false>(a, st) : x_type == T_BF16 ? launch_few_t<T_BF16, false>(a, st) : launch_few_t<T_F16, false>(a, st);
+template <bool GATED>
+static hipError_t launch_few(const Fp8Args &a, int x_type, hipStream_t st) {
+    return x_type == T_F32 ? launch_few_t<T_F32, GATED>(a, st) : x_type == T_BF16 ? launch_few_t<T_BF16, GATED>(a, st) : launch_few_t<T_F16, GATED>(a, st);
 }
-hipError_t launch_fp8_few_down(Fp8FewArgs a, hipStream_t st) {
+hipError_t launch_fp8_few_product(const Fp8Args &a, int x_type, hipStream_t st) { return launch_few<false>(a, x_type, st); }
+
+static hipError_t launch_few_down(Fp8FewArgs a, hipStream_t st) {
     const int P = a.n_tok * a.K, nb = (a.I + FB - 1) / FB;
     a.parts = 1;
     while (2 * a.parts * P <= 8 && 2 * a.parts <= nb) a.parts *= 2;
@@ -633,6 +704,38 @@ hipError_t launch_fp8_few_down(Fp8FewArgs a, hipStream_t st) {
     if (a.exact) hipLaunchKernelGGL((fp8_few_down_kernel<true>), grid, dim3(512), lds, st, a);
     else hipLaunchKernelGGL((fp8_few_down_kernel<false>), grid, dim3(512), lds, st, a);
     return hipGetLastError();
+}
+
+template <int T, bool GATED>
+static hipError_t launch_mid_t(Fp8Args a, hipStream_t st) {
+    a.cols = std::min(a.M, lds_rows(a.K));
+    const dim3 grid((unsigned)((a.N + 63) / 64), (unsigned)std::min(a.E, a.M));
+    const size_t lds = (size_t)a.cols * (lds_stride(a.K) + 4 * ((a.K + FB - 1) / FB));
+    if (a.exact) hipLaunchKernelGGL((fp8_mid_kernel<T, GATED, true>), grid, dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((fp8_mid_kernel<T, GATED, false>), grid, dim3(256), lds, st, a);
+    return hipGetLastError();
+}
+// Gate and up: as many pairs as a wave has lanes by one kernel, more by the other (64 pairs of 256 experts, 512 of 2,048: 26 us and 30).
+static hipError_t launch_few_gated(const Fp8Args &a, int x_type, hipStream_t st) {
+    if (a.M <= 64) return launch_few<true>(a, x_type, st);
+    return x_type == T_F32 ? launch_mid_t<T_F32, true>(a, st) : x_type == T_BF16 ? launch_mid_t<T_BF16, true>(a, st) : launch_mid_t<T_F16, true>(a, st);
+}
+// Down with the sum over a token's experts where pairs are DOWN_PAIRS at most (a layer of one token, two experts of 2,048 of 1,024: 14.0 us,
+// through pair rows 18.0; one of 8,192 of 5,120: 40.6 and 50.7; but eight of 768 of 2,048: 21.0 and 21.4, sixteen 30.3 and 27.7), else into
+// pair rows.
+hipError_t launch_fp8_few_layer(Fp8Args a, int x_type, Fp8FewArgs f, float *rows, hipStream_t st) {
+    hipError_t err = launch_few_gated(a, x_type, st);
+    if (err != hipSuccess) return err;
+    if (a.M <= DOWN_PAIRS && a.M <= lds_rows(f.I)) return launch_few_down(f, st);
+    a.m[0] = f.down; a.gated = 0;
+    a.x = (const uint8_t *)f.h; a.ldx = f.I;
+    a.N = f.H; a.K = f.I;
+    a.exact = f.exact;
+    a.pair_w = f.w;
+    a.y = rows; a.ldy = f.H;
+    err = launch_mid_t<T_F32, false>(a, st);
+    if (err != hipSuccess) return err;
+    return launch_fp8_combine({rows, f.ids, f.n_tok, f.K, f.E, f.H, f.out, f.ldo, f.out_type}, st);
 }
 
 template <int FROM, bool GATED, int NT, int KS>
@@ -711,10 +814,9 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
     constexpr int THREADS = 64 * WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, CH = (BN + BM) * 8 / THREADS, SB = 6;
     static_assert(KG == 1 || (NS > 1 && !GATED && (KG - 1) * THREADS * TN * TM <= KG * (BN + BM) * 8), "sums fit a stage");
     static_assert((BN + BM) * 8 % THREADS == 0 && BN * 8 % THREADS == 0 && THREADS % BM == 0 && SB * 2 * WN <= THREADS, "whole loads");
-    static_assert(NS == 1 || SB % NS == 0, "each step its own places");
+    static_assert(NS == 1 || (NS == 3 && SB % NS == 0), "each step its own places");
     constexpr int CHUNKS = (BN + BM) * 8 * KG;
-    __shared__ int4_v s_0[CHUNKS], s_1[NS > 1 ? CHUNKS : 1], s_2[NS > 2 ? CHUNKS : 1], s_3[NS > 3 ? CHUNKS : 1], s_4[NS > 4 ? CHUNKS : 1],
-        s_5[NS > 5 ? CHUNKS : 1];
+    __shared__ int4_v s_0[CHUNKS], s_1[NS > 1 ? CHUNKS : 1], s_2[NS > 1 ? CHUNKS : 1];
     __shared__ int s_run[4];
     __shared__ float s_max[WN][BM], s_sx[KG][2][SB][BM], s_sw[KG][2][SB][2 * WN];
     const int lane = threadIdx.x & 63, tid = threadIdx.x % THREADS, kg = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
@@ -886,7 +988,7 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
             constexpr bool LIVE = decltype(live)::value;
             auto place = [&](int u) FP8_INLINE {
                 u %= NS;
-                return (u == 0 ? s_0 : u == 1 ? s_1 : u == 2 ? s_2 : u == 3 ? s_3 : u == 4 ? s_4 : s_5) + kg * (CHUNKS / KG);
+                return (u == 0 ? s_0 : u == 1 ? s_1 : s_2) + kg * (CHUNKS / KG);
             };
             auto step = [&](Operands &o, Operands &on, int u) FP8_INLINE {
                 auto along = [&](int i) FP8_INLINE {

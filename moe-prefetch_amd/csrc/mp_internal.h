@@ -413,10 +413,10 @@ struct Fp8FewArgs {
     int out_type;
     int parts;                    // set by the launcher
 };
-bool fp8_few_layer(int n_tok, int K, int H, int I);
+bool fp8_few_layer(int64_t P, int E, int H, int I);
 bool fp8_few_product(int M, int K);
-hipError_t launch_fp8_few_up(const Fp8Args &a, int x_type, hipStream_t st);
-hipError_t launch_fp8_few_down(Fp8FewArgs a, hipStream_t st);
+hipError_t launch_fp8_few_layer(Fp8Args a, int x_type, Fp8FewArgs f, float *rows, hipStream_t st);      // rows: [n_tok * K][H]
+hipError_t launch_fp8_few_product(const Fp8Args &a, int x_type, hipStream_t st);
 // rows of x for each expert from which products run on tiles
 constexpr int FP8_TILE_ROWS = 48;
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st);

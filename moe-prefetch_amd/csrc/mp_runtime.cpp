@@ -4288,7 +4288,7 @@ int moe_fp8_product(const moe_fp8_product_desc *d, void *stream) {
     a.exact = d->y_type == MOE_DTYPE_F32;
     a.y = d->y; a.ldy = d->y_stride; a.y_type = d->y_type;
     if (few) {
-        HIPCHK(mp::launch_fp8_few_up(a, d->x_type, (hipStream_t)stream));
+        HIPCHK(mp::launch_fp8_few_product(a, d->x_type, (hipStream_t)stream));
         return MOE_OK;
     }
     if (!e4m3) {
@@ -4362,12 +4362,12 @@ int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream) {
     a.M = P; a.N = d->I; a.K = d->H; a.E = d->E;
     a.y = ws + l.act; a.ldy = d->I; a.y_type = MOE_DTYPE_F32;
     a.exact = d->out_type != MOE_DTYPE_BF16;
-    if (mp::fp8_few_layer(d->n_tok, d->K, d->H, d->I)) {
+    if (mp::fp8_few_layer(P, d->E, d->H, d->I)) {
         a.x = (const uint8_t *)d->x; a.ldx = d->x_stride;
         a.ids = d->ids;
-        HIPCHK(mp::launch_fp8_few_up(a, d->x_type, st));
-        HIPCHK(mp::launch_fp8_few_down({fp8_mat(d->down), (const float *)(ws + l.act), d->ids, d->w, d->n_tok, d->E, d->K, d->H, d->I,
-                                        d->out_type == MOE_DTYPE_F32, d->out, d->out_stride, d->out_type}, st));
+        HIPCHK(mp::launch_fp8_few_layer(a, d->x_type, {fp8_mat(d->down), (const float *)(ws + l.act), d->ids, d->w, d->n_tok, d->E, d->K, d->H,
+                                                       d->I, d->out_type == MOE_DTYPE_F32, d->out, d->out_stride, d->out_type},
+                                        (float *)(ws + l.rows), st));
         return MOE_OK;
     }
     HIPCHK(mp::launch_dispatch(d->ids, P, d->E, (int32_t *)(ws + l.counts), offsets, perm, st));
@@ -4376,8 +4376,8 @@ int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream) {
     a.offsets = offsets; a.perm = perm;
     a.hq = ws + l.h.q; a.ldh = l.h.ld; a.hs = (float *)(ws + l.h.s); a.ldhs = l.h.nb;
     HIPCHK(mp::launch_fp8_product(a, st));
-    if (P < mp::FP8_TILE_ROWS * d->E)
-    HIPCHK(mp::launch_fp8_quant({ws + l.act, d->I, MOE_DTYPE_F32, 1, P, d->I, ws + l.h.q, l.h.ld, (float *)(ws + l.h.s), l.h.nb}, st));
+    if (P < mp::FP8_TILE_ROWS * d->E)                   // (the tiles quantize h themselves)
+        HIPCHK(mp::launch_fp8_quant({ws + l.act, d->I, MOE_DTYPE_F32, 1, P, d->I, ws + l.h.q, l.h.ld, (float *)(ws + l.h.s), l.h.nb}, st));
     a.m[0] = fp8_mat(d->down); a.gated = 0;
     a.x = ws + l.h.q; a.ldx = l.h.ld; a.xs = (const float *)(ws + l.h.s); a.ldxs = l.h.nb;
     a.top = 0; a.N = d->H; a.K = d->I;
