@@ -760,8 +760,11 @@ static hipError_t launch_stream(const Fp8Args &a, hipStream_t st) {
 // without registers, are on their way while this one is multiplied.
 // The eight 16-byte chunks of a row lie in LDS at chunk ^ (row & 7): the lanes that read one chunk of eight rows then touch
 // all banks once.
-// expert and first row (in the dispatch's order) of a workgroup's rows of x, the slot-th run of BM; false: there is none
-__device__ inline bool find_run(const int32_t *offsets, int E, int bm, int slot, int &e, int &p0, int &end, int *s_run) {
+// Workgroups go round the eight XCDs: each has a run of the tiles, so that those at work at once share what they read in its L2.
+__device__ inline int xcd_tile(int id, int total) { return id < total / 8 * 8 ? (id % 8) * (total / 8) + id / 8 : id; }
+// A workgroup's tile of a dispatch's products: its expert and first row (in the dispatch's order) of a run of bm, and its place among the
+// run's n_tiles, which follow one another (2,048 tokens of 128 experts: gate and up XXX us, YYY round the XCDs); false: there is none
+__device__ inline bool find_run(const int32_t *offsets, int E, int bm, int n_tiles, int &n_tile, int &e, int &p0, int &end, int *s_run) {
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x;
         int tiles[4], o[5], sum = 0;
@@ -778,7 +781,12 @@ __device__ inline bool find_run(const int32_t *offsets, int E, int bm, int slot,
             const int t = __shfl_up(incl, d, 64);
             if (lane >= d) incl += t;
         }
-        if (lane == 63) s_run[3] = slot < incl;
+        const int total = __builtin_amdgcn_readlane(incl, 63) * n_tiles;
+        const int id = xcd_tile(blockIdx.x, total), slot = id / n_tiles;
+        if (lane == 0) {
+            s_run[3] = (int)blockIdx.x < total;
+            s_run[4] = id - slot * n_tiles;
+        }
         int at = incl - sum;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -794,6 +802,7 @@ __device__ inline bool find_run(const int32_t *offsets, int E, int bm, int slot,
     e = __builtin_amdgcn_readfirstlane(s_run[0]);
     p0 = __builtin_amdgcn_readfirstlane(s_run[1]);
     end = __builtin_amdgcn_readfirstlane(s_run[2]);
+    n_tile = __builtin_amdgcn_readfirstlane(s_run[4]);
     return s_run[3] != 0;
 }
 
@@ -817,7 +826,7 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
     static_assert(NS == 1 || (NS == 3 && SB % NS == 0), "each step its own places");
     constexpr int CHUNKS = (BN + BM) * 8 * KG;
     __shared__ int4_v s_0[CHUNKS], s_1[NS > 1 ? CHUNKS : 1], s_2[NS > 1 ? CHUNKS : 1];
-    __shared__ int s_run[4];
+    __shared__ int s_run[5];
     __shared__ float s_max[WN][BM], s_sx[KG][2][SB][BM], s_sw[KG][2][SB][2 * WN];
     const int lane = threadIdx.x & 63, tid = threadIdx.x % THREADS, kg = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
@@ -825,13 +834,10 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
     int e = 0, p0, end = a.M;
     int n_tile;
     if (a.offsets) {
-        n_tile = blockIdx.x % n_tiles;
-        if (!find_run(a.offsets, a.E, BM, blockIdx.x / n_tiles, e, p0, end, s_run)) return;
+        if (!find_run(a.offsets, a.E, BM, n_tiles, n_tile, e, p0, end, s_run)) return;
     } else {
-        // workgroups go round the eight XCDs: each has a run of tiles, in strips of eight tiles of x, so that those at work
-        // at once share what they read in its L2
-        const int total = n_tiles * m_tiles, per = total / 8;
-        const int id = blockIdx.x < per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+        // (in strips of eight tiles of x)
+        const int id = xcd_tile(blockIdx.x, n_tiles * m_tiles);
         const int strip = id / (8 * n_tiles), wide = min(8, m_tiles - 8 * strip), in = id - strip * 8 * n_tiles;
         n_tile = in / wide;
         p0 = (8 * strip + in % wide) * BM;
