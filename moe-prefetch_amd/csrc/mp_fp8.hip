@@ -263,14 +263,14 @@ __device__ inline float silu_times(float g, float u) { return u * (g / (1.0f + e
 constexpr int OF_ALL = 0;         // rows 0 .. M - 1
 constexpr int OF_DISPATCH = 1;    // an expert's pairs from a dispatch
 
-// Sixteen rows of a weight (of gate and up: GATED) for 16 NT rows of codes at a time: every weight is read once, and memory bounds the call.
-// KS waves share K, a block each in turn, and their sums are added in their order; with KS 1 each of the workgroup's four has
-// sixteen rows of its own.  A wave's loads of DEEP blocks of the weight are on their way together.
-template <int FROM, bool GATED, bool EXACT, int NT, int KS>
+// Sixteen rows of a weight (of gate and up: GATED) for sixteen rows of codes at a time: every weight is read once for them, and memory bounds the
+// call.  KS waves share K, a block each in turn, and their sums are added in their order; with KS 1 each of the workgroup's four has
+// sixteen rows of its own.  A wave's loads of DEEP blocks are on their way together.
+template <int FROM, bool GATED, bool EXACT, int KS>
 __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
     // (two blocks of gate and up, three of down: 64 tokens of 128 experts 141 us; one and two 145, four and six 147: waves count, too)
-    constexpr int DEEP = NT > 1 ? (GATED ? 1 : 2) : GATED ? 2 : 3, MATS = GATED ? 2 : 1;
-    __shared__ float s_acc[KS > 1 ? MATS : 1][KS][KS > 1 ? 16 * NT : 1][17];
+    constexpr int DEEP = GATED ? 2 : 3, MATS = GATED ? 2 : 1;
+    __shared__ float s_acc[KS > 1 ? MATS : 1][KS][KS > 1 ? 16 : 1][17];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     const int n0 = (KS > 1 ? blockIdx.x : blockIdx.x * 4 + wave) * 16, whole = a.K / FB, first = KS > 1 ? wave : 0;
     const int e = FROM == OF_ALL ? 0 : (int)blockIdx.y;
@@ -280,16 +280,14 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
     const uint8_t *w[2] = {a.m[0].w + e * a.m[0].ex + wrow * a.m[0].ld, GATED ? a.m[1].w + e * a.m[1].ex + wrow * a.m[1].ld : nullptr};
     const float *ws[2] = {a.m[0].s + e * a.m[0].sex + (int64_t)(n0 / FB) * a.m[0].sld,
                           GATED ? a.m[1].s + e * a.m[1].sex + (int64_t)(n0 / FB) * a.m[1].sld : nullptr};
-    for (int64_t p0 = begin + 16ll * NT * blockIdx.z; p0 < end; p0 += 16ll * NT * gridDim.z) {
-        int64_t xrow[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int64_t p = min(p0 + 16 * t + c, (int64_t)end - 1);
-            xrow[t] = FROM == OF_DISPATCH && a.top ? a.perm[p] / a.top : p;
-        }
-        float4_v acc[2][NT] = {};
+    for (int p0 = begin; p0 < end; p0 += 16) {
+        const int p = min(p0 + c, end - 1);
+        const int64_t xrow = FROM == OF_DISPATCH && a.top ? a.perm[p] / a.top : p;
+        const uint8_t *x = a.x + xrow * a.ldx;
+        const float *xs = a.xs + xrow * a.ldxs;
+        float4_v acc[2] = {};
         for (int b0 = first; b0 < whole; b0 += KS * DEEP) {
-            int8_v wf[DEEP][2], xf[DEEP];               // (those of the other rows of x come one by one)
+            int8_v wf[DEEP][2], xf[DEEP];
             float f[DEEP][2], s[DEEP];
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) {
@@ -300,34 +298,20 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
                     wf[i][m] = load_frag(w[m], b, g);
                     f[i][m] = ws[m][b];
                 }
-                xf[i] = load_frag(a.x + xrow[0] * a.ldx, b, g);
-                s[i] = a.xs[xrow[0] * a.ldxs + b];
+                xf[i] = load_frag(x, b, g);
+                s[i] = xs[b];
             }
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) {
-                const int b = b0 + i * KS;
-                if (b >= whole) break;
+                if (b0 + i * KS >= whole) break;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    if (t > 0 && p0 + 16 * t >= end) break;
-                    const int8_v xt = t ? load_frag(a.x + xrow[t] * a.ldx, b, g) : xf[i];
-                    const float st = t ? a.xs[xrow[t] * a.ldxs + b] : s[i];
-#pragma unroll
-                    for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m][t], wf[i][m], xt, st * f[i][m]);
-                }
+                for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m], wf[i][m], xf[i], s[i] * f[i][m]);
             }
         }
         if (a.K % FB && whole % KS == first) {          // the last block
-            int8_v wf[MATS];
+            const int8_v xt = load_last(x, a.K, g);
 #pragma unroll
-            for (int m = 0; m < MATS; ++m) wf[m] = load_last(w[m], a.K, g);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int8_v xt = load_last(a.x + xrow[t] * a.ldx, a.K, g);
-                const float st = a.xs[xrow[t] * a.ldxs + whole];
-#pragma unroll
-                for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m][t], wf[m], xt, st * ws[m][whole]);
-            }
+            for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m], load_last(w[m], a.K, g), xt, xs[whole] * ws[m][whole]);
         }
         // (y, or h, of row p0 + col) -> where it goes, and its weight
         auto out_of = [&](int col, float &weight) FP8_INLINE {
@@ -340,45 +324,36 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
             return out;
         };
         if (KS == 1) {
+            const int n = n0 + 4 * g;
+            if (p0 + c >= end) continue;
+            float weight;
+            const int64_t out = out_of(c, weight);
+            float4_v y = acc[0];
+            if (GATED)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int col = 16 * t + c, n = n0 + 4 * g;
-                if (p0 + col >= end) continue;
-                float weight;
-                const int64_t out = out_of(col, weight);
-                float4_v y = acc[0][t];
-                if (GATED)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) y[k] = silu_times(y[k], acc[1][t][k]);
-                store4(a.y, out * a.ldy + n, a.y_type, FROM == OF_DISPATCH && a.pair_w ? y * weight : y, a.N - n);
-            }
+                for (int k = 0; k < 4; ++k) y[k] = silu_times(y[k], acc[1][k]);
+            store4(a.y, out * a.ldy + n, a.y_type, FROM == OF_DISPATCH && a.pair_w ? y * weight : y, a.N - n);
             continue;
         }
         __syncthreads();
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s_acc[m][first][16 * t + c][4 * g + k] = acc[m][t][k];
+            for (int k = 0; k < 4; ++k) s_acc[m][first][c][4 * g + k] = acc[m][k];
         __syncthreads();
-        const int r = threadIdx.x & 15;
+        const int r = threadIdx.x & 15, col = threadIdx.x >> 4;
+        if (n0 + r >= a.N || p0 + col >= end) continue;
+        float y[2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int col = 16 * t + (threadIdx.x >> 4);
-            if (n0 + r >= a.N || p0 + col >= end) continue;
-            float y[2];
+        for (int m = 0; m < MATS; ++m) {
+            y[m] = s_acc[m][0][col][r];
 #pragma unroll
-            for (int m = 0; m < MATS; ++m) {
-                y[m] = s_acc[m][0][col][r];
-#pragma unroll
-                for (int i = 1; i < KS; ++i) y[m] += s_acc[m][i][col][r];
-            }
-            float weight;
-            const int64_t out = out_of(col, weight);
-            const float v = GATED ? silu_times(y[0], y[1]) : y[0];
-            store_elem(a.y, out * a.ldy + n0 + r, a.y_type, FROM == OF_DISPATCH && a.pair_w ? v * weight : v);
+            for (int i = 1; i < KS; ++i) y[m] += s_acc[m][i][col][r];
         }
+        float weight;
+        const int64_t out = out_of(col, weight);
+        const float v = GATED ? silu_times(y[0], y[1]) : y[0];
+        store_elem(a.y, out * a.ldy + n0 + r, a.y_type, FROM == OF_DISPATCH && a.pair_w ? v * weight : v);
     }
 }
 
@@ -675,9 +650,19 @@ __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
 // Rows of K codes in LDS, at most sixteen, beside a kernel's own 9 KiB
 static int lds_rows(int K) { return std::min(16, 54 * 1024 / (lds_stride(K) + 4 * ((K + FB - 1) / FB))); }
 bool fp8_few_product(int M, int K) { return M <= lds_rows(K); }
-// Which layers take these kernels: few pairs, an expert's about one tile of them; and rows that LDS holds, all or not too few at once.
-bool fp8_few_layer(int64_t P, int E, int H, int I) {
-    return P <= MID_PAIRS && P <= std::max(64, 16 * E) && std::min(P, (int64_t)2) <= lds_rows(std::max(H, I));
+// From how many rows an expert (on average) a layer's products run on tiles.  Weights on 16 bytes: 8 (128 experts of 768 of 2,048, 1,024 pairs:
+// 161 us for the layer, from codes sixteen rows at a time 164; 640: 159 and 145; 1,536: 166 and 192).  Others: 16 (60 of 200 of 1,000, 1,920
+// pairs: 63 and 67; 600: 58 and 43).
+int fp8_tile_rows(const Fp8Mat &gate, const Fp8Mat &up, const Fp8Mat &down) {
+    auto on16 = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0; };
+    return on16(gate) && on16(up) && on16(down) ? 8 : 16;
+}
+// Which layers take the kernels above: few pairs, fewer than tiles have, and of an expert as many as LDS holds, for else its weights are read
+// again (80 pairs of 8 experts of 2,048 of 1,024: 35 us, tiles 43; 256 of 32 of 768 of 2,048: 78 and 64; 128 of 8 of 14,336 of 4,096: 870 and
+// 368).
+bool fp8_few_layer(int64_t P, int E, int H, int I, int tile_rows) {
+    const int64_t fit = lds_rows(std::max(H, I));
+    return P <= MID_PAIRS && (P <= 128 || P < (int64_t)tile_rows * E) && P <= fit * E && std::min(P, (int64_t)2) <= fit;
 }
 
 template <int T, bool GATED>
@@ -738,20 +723,13 @@ hipError_t launch_fp8_few_layer(Fp8Args a, int x_type, Fp8FewArgs f, float *rows
     return launch_fp8_combine({rows, f.ids, f.n_tok, f.K, f.E, f.H, f.out, f.ldo, f.out_type}, st);
 }
 
-template <int FROM, bool GATED, int NT, int KS>
-static hipError_t launch_stream_n(const Fp8Args &a, hipStream_t st) {
-    const int64_t groups = (a.M + 16 * NT - 1) / (16 * NT);
-    const int rows = KS > 1 ? 16 : 64;
-    const dim3 grid((unsigned)((a.N + rows - 1) / rows), FROM == OF_ALL ? 1 : (unsigned)a.E, FROM == OF_ALL ? (unsigned)std::min(groups, (int64_t)4096) : 1);
-    if (a.exact) hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, true, NT, KS>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, false, NT, KS>), grid, dim3(256), 0, st, a);
-    return hipGetLastError();
-}
-template <bool GATED>
+template <int FROM, bool GATED, int KS>
 static hipError_t launch_stream(const Fp8Args &a, hipStream_t st) {
-    const int rows = a.M / a.E;                         // of an expert, about
-    return rows <= 16 ? launch_stream_n<OF_DISPATCH, GATED, 1, 1>(a, st) : rows <= 32 ? launch_stream_n<OF_DISPATCH, GATED, 2, 1>(a, st)
-                                                                           : launch_stream_n<OF_DISPATCH, GATED, 4, 1>(a, st);
+    const int rows = KS > 1 ? 16 : 64;
+    const dim3 grid((unsigned)((a.N + rows - 1) / rows), FROM == OF_ALL ? 1 : (unsigned)a.E);
+    if (a.exact) hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, true, KS>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, false, KS>), grid, dim3(256), 0, st, a);
+    return hipGetLastError();
 }
 
 // ---- products of many rows: tiles through LDS --------------------------------------
@@ -1183,7 +1161,7 @@ static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
 
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
     if (!a.offsets) {
-        if (a.M <= 16) return launch_stream_n<OF_ALL, false, 1, 4>(a, st);
+        if (a.M <= 16) return launch_stream<OF_ALL, false, 4>(a, st);
         // 256 x 128 tiles where they are many enough for every compute unit; else 64 x 64; else 32 x 64 with K shared by four (64 rows
         // through 2,048 x 4,096: 13.8 us, 64 x 64 21.4; 500 through 2,500 x 2,000 in f32: 18.5 of 64 x 64, 31.7 shared)
         auto tiles = [&](int n, int m) { return (int64_t)((a.N + n - 1) / n) * ((a.M + m - 1) / m); };
@@ -1191,8 +1169,8 @@ hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
         if (tiles(64, 64) >= 200) return a.exact ? launch_tile_d<false, true, 3, 1, 2, 2, 2, 2>(a, st) : launch_tile_d<false, false, 3, 1, 2, 2, 2, 2>(a, st);
         return a.exact ? launch_tile_d<false, true, 3, 4, 2, 2, 1, 2>(a, st) : launch_tile_d<false, false, 3, 4, 2, 2, 1, 2>(a, st);
     }
-    if (a.M >= FP8_TILE_ROWS * a.E) return a.gated ? launch_tile<true>(a, st) : launch_tile<false>(a, st);
-    return a.gated ? launch_stream<true>(a, st) : launch_stream<false>(a, st);
+    if (a.tiles) return a.gated ? launch_tile<true>(a, st) : launch_tile<false>(a, st);
+    return a.gated ? launch_stream<OF_DISPATCH, true, 1>(a, st) : launch_stream<OF_DISPATCH, false, 1>(a, st);
 }
 
 // out[t] = the sum over k, in order, of the rows of t's pairs; a pair whose id is no expert's has none.  Four columns a thread, four rows on

@@ -397,6 +397,7 @@ struct Fp8Args {
     int64_t ldh;
     float *hs;
     int64_t ldhs;
+    int tiles;                    // a dispatch: by tiles (fp8_tile_rows)
     const int32_t *ids;           // few tokens: their experts [M], in place of a dispatch
     int cols;                     // set by the launcher
 };
@@ -413,12 +414,11 @@ struct Fp8FewArgs {
     int out_type;
     int parts;                    // set by the launcher
 };
-bool fp8_few_layer(int64_t P, int E, int H, int I);
+int fp8_tile_rows(const Fp8Mat &gate, const Fp8Mat &up, const Fp8Mat &down);
+bool fp8_few_layer(int64_t P, int E, int H, int I, int tile_rows);
 bool fp8_few_product(int M, int K);
 hipError_t launch_fp8_few_layer(Fp8Args a, int x_type, Fp8FewArgs f, float *rows, hipStream_t st);      // rows: [n_tok * K][H]
 hipError_t launch_fp8_few_product(const Fp8Args &a, int x_type, hipStream_t st);
-// rows of x for each expert from which products run on tiles
-constexpr int FP8_TILE_ROWS = 48;
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st);
 struct Fp8CombineArgs {
     const float *rows;            // [n_tok * K][H]

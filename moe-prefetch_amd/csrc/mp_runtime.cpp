@@ -4362,7 +4362,9 @@ int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream) {
     a.M = P; a.N = d->I; a.K = d->H; a.E = d->E;
     a.y = ws + l.act; a.ldy = d->I; a.y_type = MOE_DTYPE_F32;
     a.exact = d->out_type != MOE_DTYPE_BF16;
-    if (mp::fp8_few_layer(P, d->E, d->H, d->I)) {
+    const int tile_rows = mp::fp8_tile_rows(a.m[0], a.m[1], fp8_mat(d->down));
+    a.tiles = P >= tile_rows * d->E;
+    if (mp::fp8_few_layer(P, d->E, d->H, d->I, tile_rows)) {
         a.x = (const uint8_t *)d->x; a.ldx = d->x_stride;
         a.ids = d->ids;
         HIPCHK(mp::launch_fp8_few_layer(a, d->x_type, {fp8_mat(d->down), (const float *)(ws + l.act), d->ids, d->w, d->n_tok, d->E, d->K, d->H,
@@ -4376,7 +4378,7 @@ int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream) {
     a.offsets = offsets; a.perm = perm;
     a.hq = ws + l.h.q; a.ldh = l.h.ld; a.hs = (float *)(ws + l.h.s); a.ldhs = l.h.nb;
     HIPCHK(mp::launch_fp8_product(a, st));
-    if (P < mp::FP8_TILE_ROWS * d->E)                   // (the tiles quantize h themselves)
+    if (!a.tiles)                                       // (the tiles quantize h themselves)
         HIPCHK(mp::launch_fp8_quant({ws + l.act, d->I, MOE_DTYPE_F32, 1, P, d->I, ws + l.h.q, l.h.ld, (float *)(ws + l.h.s), l.h.nb}, st));
     a.m[0] = fp8_mat(d->down); a.gated = 0;
     a.x = ws + l.h.q; a.ldx = l.h.ld; a.xs = (const float *)(ws + l.h.s); a.ldxs = l.h.nb;
