@@ -880,7 +880,10 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
             const int at = (b + tid / BM + PER * i) * KG + kg;
             held_x[i] = KG > 1 && at >= whole ? 0.0f : from_x[min(at, nb - 1)];
         }
-        if (tid < SB * 2 * WN) held_w = from_w[min((b + tid / (2 * WN)) * KG + kg, nb - 1)];
+        if (tid < SB * 2 * WN) {
+            const int at = (b + tid / (2 * WN)) * KG + kg;
+            held_w = KG > 1 && at >= whole ? 0.0f : from_w[min(at, nb - 1)];
+        }
     };
     auto put_scales = [&](int par) FP8_INLINE {
 #pragma unroll
