@@ -74,7 +74,7 @@ extern "C" {
 
 #define MOE_DTYPE_F32  0    /* activation element types */
 #define MOE_DTYPE_BF16 1
-#define MOE_DTYPE_F16  2   /* moe_route_scored, moe_block_norm and moe_sample only */
+#define MOE_DTYPE_F16  2   /* moe_route_scored, moe_block_norm, moe_sample and moe_fp8_* only */
 
 const char *moe_last_error(void);   /* message of the last failure on this thread */
 int moe_abi_version(void);
@@ -888,8 +888,8 @@ int moe_fp8_product(const moe_fp8_product_desc *d, void *stream);
  *   ids, w   moe_route_scored's of route.logits, or given
  *   h        silu(gate_e . x) * (up_e . x), products as moe_fp8_product's, silu(g) = g / (1 + exp(-g))
  *   out[t]   sum over k, in order, of w[t][k] * (down_e . h), e = ids[t][k]
- * with h f32 until it is quantized for the product with down; the products with gate and up, whose small errors the
- * quantizer turns into steps of e4m3, are f32 throughout unless out is bf16.  A pair whose id is outside [0, E) adds nothing;
+ * with h f32 until it is quantized for the product with down; the products with gate and up are f32 throughout, for the
+ * quantizer turns small errors into steps of e4m3; that with down as for a y of out's type.  A pair whose id is outside [0, E) adds nothing;
  * an id may stand twice for one token.  n_tok * K <= 65535. */
 #define MOE_FP8_MAX_E 256
 typedef struct {

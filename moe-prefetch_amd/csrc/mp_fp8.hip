@@ -6,10 +6,12 @@
 // dot runs on the matrix cores, and one fma adds it, scaled, to the f32 sum of the row.  The weight's 16 rows are the A
 // operand, so that a lane holds four of them for one row of x: one scale a lane and block.
 //
-// The codes become fp16 for the matrix cores (exactly), whose fp16 products are exact and their sums f32.  The cores' own e4m3
+// EXACT: the codes become fp16 for the matrix cores (exactly), whose fp16 products are exact and their sums f32.  The cores' own e4m3
 // instructions add eight neighbouring products at 13 bits below the largest of them, what is below cut off (found by
 // products of powers of two: 2^-13 of the largest stays, 2^-14 does not): 1.4e-5 of the result for normal numbers, where f32 sums
-// have 1e-8.
+// have 1e-8.  They take half the time (2,048 rows of 8 of 128 experts, gate and up by tiles: 153 us, fp16 200 to 215), and y in 16 bits
+// does not show it: those products use them.  Those with gate and up do not, for h lies by a tie of e4m3 often enough that a
+// layer's error doubled (of bf16: 0.0036 of out instead of 0.0017).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -670,8 +672,8 @@ static hipError_t launch_few_t(Fp8Args a, hipStream_t st) {
     a.cols = std::min(a.M, lds_rows(a.K));
     const dim3 grid((unsigned)((a.N + 15) / 16), GATED ? (unsigned)a.M : 1);
     const size_t lds = (size_t)a.cols * (lds_stride(a.K) + 4 * ((a.K + FB - 1) / FB));
-    if (a.exact) hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED, true>), grid, dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED, false>), grid, dim3(256), lds, st, a);
+    if (GATED || a.exact) hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED, true>), grid, dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED, GATED>), grid, dim3(256), lds, st, a);
     return hipGetLastError();
 }
 template <bool GATED>
@@ -696,8 +698,8 @@ static hipError_t launch_mid_t(Fp8Args a, hipStream_t st) {
     a.cols = std::min(a.M, lds_rows(a.K));
     const dim3 grid((unsigned)((a.N + 63) / 64), (unsigned)std::min(a.E, a.M));
     const size_t lds = (size_t)a.cols * (lds_stride(a.K) + 4 * ((a.K + FB - 1) / FB));
-    if (a.exact) hipLaunchKernelGGL((fp8_mid_kernel<T, GATED, true>), grid, dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((fp8_mid_kernel<T, GATED, false>), grid, dim3(256), lds, st, a);
+    if (GATED || a.exact) hipLaunchKernelGGL((fp8_mid_kernel<T, GATED, true>), grid, dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((fp8_mid_kernel<T, GATED, GATED>), grid, dim3(256), lds, st, a);
     return hipGetLastError();
 }
 // Gate and up: as many pairs as a wave has lanes by one kernel, more by the other (64 pairs of 256 experts, 512 of 2,048: 26 us and 30).
@@ -727,8 +729,8 @@ template <int FROM, bool GATED, int KS>
 static hipError_t launch_stream(const Fp8Args &a, hipStream_t st) {
     const int rows = KS > 1 ? 16 : 64;
     const dim3 grid((unsigned)((a.N + rows - 1) / rows), FROM == OF_ALL ? 1 : (unsigned)a.E);
-    if (a.exact) hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, true, KS>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, false, KS>), grid, dim3(256), 0, st, a);
+    if (GATED || a.exact) hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, true, KS>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, GATED, KS>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
@@ -1159,7 +1161,7 @@ static hipError_t launch_tile_d(const Fp8Args &a, hipStream_t st) {
 }
 template <bool GATED>
 static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
-    return a.exact ? launch_tile_d<GATED, true, 3, 1, 4, 2, 4, 4>(a, st) : launch_tile_d<GATED, false, 3, 1, 4, 2, 4, 4>(a, st);
+    return GATED || a.exact ? launch_tile_d<GATED, true, 3, 1, 4, 2, 4, 4>(a, st) : launch_tile_d<GATED, GATED, 3, 1, 4, 2, 4, 4>(a, st);
 }
 
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {

@@ -4361,7 +4361,7 @@ int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream) {
     a.top = d->K;
     a.M = P; a.N = d->I; a.K = d->H; a.E = d->E;
     a.y = ws + l.act; a.ldy = d->I; a.y_type = MOE_DTYPE_F32;
-    a.exact = d->out_type != MOE_DTYPE_BF16;
+    a.exact = 1;
     const int tile_rows = mp::fp8_tile_rows(a.m[0], a.m[1], fp8_mat(d->down));
     a.tiles = P >= tile_rows * d->E;
     if (mp::fp8_few_layer(P, d->E, d->H, d->I, tile_rows)) {
