@@ -96,7 +96,8 @@ __device__ inline float without_inf(float *v, float m) {
 }
 
 // Sixteen lanes a block of one row, eight neighbouring elements each in one load; NB blocks a lane, sixteen apart, whose loads are on their
-// way together.  magic, shift: the division by the blocks of a row.
+// way together.  magic, shift: the division by the blocks of a row.  Memory bounds many rows (8,192 of 4,096 in bf16: 20.7 us, 4.9 TB/s, as a
+// copy), the launch few (64 of 2,048: 2.5 us).
 template <int T, int NB>
 __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a, uint32_t nb, uint32_t total, uint32_t magic, int shift) {
     const uint32_t g0 = blockIdx.x * (16 * NB) + threadIdx.x / 16;
@@ -270,7 +271,7 @@ constexpr int OF_DISPATCH = 1;    // an expert's pairs from a dispatch
 // sixteen rows of its own.  A wave's loads of DEEP blocks are on their way together.
 template <int FROM, bool GATED, bool EXACT, int KS>
 __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
-    // (two blocks of gate and up, three of down: 64 tokens of 128 experts 141 us; one and two 145, four and six 147: waves count, too)
+    // (two blocks of gate and up, three of down: 512 pairs of 128 experts 141 us for the layer; one and two 145, four and six 147: waves count, too)
     constexpr int DEEP = GATED ? 2 : 3, MATS = GATED ? 2 : 1;
     __shared__ float s_acc[KS > 1 ? MATS : 1][KS][KS > 1 ? 16 : 1][17];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
@@ -401,6 +402,7 @@ __device__ inline void list_bits(uint64_t m, uint8_t *list) {
 // launch, and nothing between.  Four waves share K.
 // GATED: workgroup y has the expert of pair y, where that is the expert's first pair, and all of its pairs among the ids
 // (at most 64); h goes out in f32 in the order of pairs.  Else rows 0 .. M - 1 of x.
+// One row through 2,048 x 2,048: 3.9 us, a launch and a trip to memory; gate and up of 512 x 2,048 of 64 pairs' experts, 57 of 256: 27 us, 4.4 TB/s.
 template <int T, bool GATED, bool EXACT>
 __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
     constexpr int WAVES = 4, DEEP = 4, MATS = GATED ? 2 : 1;
@@ -484,7 +486,9 @@ __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
 constexpr int MID_PAIRS = 512;
 // The same for up to MID_PAIRS pairs: workgroup y has expert y (where experts are more than pairs: the expert of pair y, if that is its first one),
 // whose pairs every wave finds among the ids, and each of its four waves sixteen rows of the weights.  The expert's rows of x (GATED; else of h: in f32 and in the order of pairs, as GATED leaves them) are quantized into LDS
-// by the workgroup, a wave's weights of DEEP blocks on their way while those before are multiplied.
+// by the workgroup, a wave's weights of DEEP blocks on their way while those before are multiplied (one of gate and up, two of down: 8 tokens of
+// 256 experts 59.8 us for the layer, 37 of 60 27.2; two and three 63.0 and 30.6, four and six 68.0 and 31.1: waves count more).
+// Memory bounds it: 64 tokens of 128 experts of 768 of 2,048 75 us (5.3 TB/s), down 43.7 (4.6).
 template <int T, bool GATED, bool EXACT>
 __global__ __launch_bounds__(256) void fp8_mid_kernel(Fp8Args a) {
     constexpr int DEEP = GATED ? 1 : 2, MATS = GATED ? 2 : 1;
@@ -740,10 +744,15 @@ static hipError_t launch_stream(const Fp8Args &a, hipStream_t st) {
 // without registers, are on their way while this one is multiplied.
 // The eight 16-byte chunks of a row lie in LDS at chunk ^ (row & 7): the lanes that read one chunk of eight rows then touch
 // all banks once.
+// 256 x 128 tiles, three stages, eight waves of 64 x 64: 4,096^3 78 to 95 us by box (1.45 to 1.76 PFLOP/s), 1.0 us a step of K and 6 a tile beside
+// them (K 256 to 8,192).  A step's products take 0.43 us of the matrix cores at most, its reads of LDS and the loads into it 0.6.
+// Loads of the weight to registers, past LDS, took 144 us, not 79 (16 rows of 64 bytes cost more than 8 of 128); 256 x 256 in two stages the
+// same 79.  Waves of a higher priority while they multiply: 95 us for the call, not 92; workgroups that walk over tiles, the next one's
+// first loads before this one's sums are stored: 97, not 91 (they spill).  A dispatch's, 2,048 tokens of 128 experts of 768 of 2,048: gate and up 195 to 215 us, down 103 to 108.
 // Workgroups go round the eight XCDs: each has a run of the tiles, so that those at work at once share what they read in its L2.
 __device__ inline int xcd_tile(int id, int total) { return id < total / 8 * 8 ? (id % 8) * (total / 8) + id / 8 : id; }
 // A workgroup's tile of a dispatch's products: its expert and first row (in the dispatch's order) of a run of bm, and its place among the
-// run's n_tiles, which follow one another (2,048 tokens of 128 experts: gate and up XXX us, YYY round the XCDs); false: there is none
+// run's n_tiles, which follow one another (2,048 tokens of 128 experts: 287 us for the layer, 294 round the XCDs); false: there is none
 __device__ inline bool find_run(const int32_t *offsets, int E, int bm, int n_tiles, int &n_tile, int &e, int &p0, int &end, int *s_run) {
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x;
@@ -1179,7 +1188,7 @@ hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
 }
 
 // out[t] = the sum over k, in order, of the rows of t's pairs; a pair whose id is no expert's has none.  Four columns a thread, four rows on
-// their way at once.
+// their way at once: 22 us for 2,048 tokens of eight rows of 2,048 (6.5 TB/s).
 __global__ __launch_bounds__(256) void fp8_combine_kernel(Fp8CombineArgs a) {
     const int h = 4 * (blockIdx.x * 256 + threadIdx.x), n = a.H - h;
     const int64_t t = blockIdx.y + (int64_t)gridDim.y * blockIdx.z;
