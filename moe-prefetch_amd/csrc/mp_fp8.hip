@@ -919,8 +919,8 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
 #pragma unroll
         for (int j = 0; j < TM; ++j) o.fx[j] = s_sx[kg][par][u][(wm * TM + j) * 16 + c];
     };
-    // A stage's products, a row of tiles' while the row before is scaled and added (EXACT: products take four times as long, and their
-    // operands the registers of that) and the row after is read; before the last row, when every read of the stage is done, then(); in each
+    // A stage's products, a row of tiles' while the row before is scaled and added (EXACT of four tiles a row: products take twice as long,
+    // and their operands the registers of that) and the row after is read; before the last row, when every read of the stage is done, then(); in each
     // row, after its products, along(row).
     auto multiply = [&](const int4_v *s, const Operands &o, auto then, auto along) FP8_INLINE {
         half8_v xh[TM][4];
@@ -929,7 +929,7 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
             for (int j = 0; j < TM; ++j)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) xh[j][k] = halves(o.x[j][2 * k], o.x[j][2 * k + 1]);
-        constexpr int LAG = EXACT ? 0 : 1;
+        constexpr int LAG = EXACT && TM > 2 ? 0 : 1;
         int8_v wf = o.w;
         float4_v d[LAG + 1][TM];
 #pragma unroll
@@ -948,7 +948,7 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
                         float4_v t = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                         for (int k = 0; k < 4; ++k) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[k], xh[j][k], t, 0, 0, 0);
-                        d[0][j] = t;
+                        d[i & LAG][j] = t;
                     } else {
                         d[i & LAG][j] = mfma_e4m3(wf, o.x[j]);
                     }
@@ -1170,7 +1170,14 @@ static hipError_t launch_tile_d(const Fp8Args &a, hipStream_t st) {
 }
 template <bool GATED>
 static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
-    return GATED || a.exact ? launch_tile_d<GATED, true, 3, 1, 4, 2, 4, 4>(a, st) : launch_tile_d<GATED, GATED, 3, 1, 4, 2, 4, 4>(a, st);
+    if constexpr (GATED) {
+        // 64 rows of x a tile up to 128 of an expert, then 128 (experts of 768 of 2,048, the layer: 12 rows 159 us and 176, 64 235 and 249,
+        // 128 330 and 334, 256 555 and 538; of down 128 rows always: 12 rows 157 us with 64, 159; 64 235 and 236; 128 352 and 333)
+        if (a.M <= 128ll * a.E) return launch_tile_d<true, true, 3, 1, 4, 2, 4, 2>(a, st);
+        return launch_tile_d<true, true, 3, 1, 4, 2, 4, 4>(a, st);
+    } else {
+        return a.exact ? launch_tile_d<false, true, 3, 1, 4, 2, 4, 4>(a, st) : launch_tile_d<false, false, 3, 1, 4, 2, 4, 4>(a, st);
+    }
 }
 
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {

@@ -76,17 +76,20 @@ def fp8_quantize(x, rows=1, q=None, scale=None, stream=None):
     K = x.shape[1]
     T, ld, dev = _first(x, K, "x")
     kind = _kind(x.dtype, "x")
-    s_shape = (-(-T // rows), _blocks(K))
+    s_rows, nb = -(-T // rows), -(-K // BLOCK)
     if q is None:
-        q = _empty((T, K), _F8, dev, stream)
+        q, ldq = _empty((T, K), _F8, dev, stream), K
     elif q.dtype is not _F8:
         raise ValueError(f"q must be {_F8}, not {q.dtype}")
+    else:
+        ldq = _rows(q, T, K, dev, "q")
     if scale is None:
-        scale = _empty(s_shape, _F32, dev, stream)
+        scale, lds = _empty((s_rows, nb), _F32, dev, stream), nb
     elif scale.dtype is not _F32:
         raise ValueError(f"scale must be {_F32}, not {scale.dtype}")
-    desc = _quantize[0](x.data_ptr(), ld, kind, rows, T, K, q.data_ptr(), _rows(q, T, K, dev, "q"), scale.data_ptr(),
-                        _rows(scale, *s_shape, dev, "scale"))
+    else:
+        lds = _rows(scale, s_rows, nb, dev, "scale")
+    desc = _quantize[0](x.data_ptr(), ld, kind, rows, T, K, q.data_ptr(), ldq, scale.data_ptr(), lds)
     _call(_quantize[1], desc, dev, stream, "moe_fp8_quantize")
     return q, scale
 
@@ -129,13 +132,14 @@ class Fp8Linear:
         if out is None:
             if out_dtype is None:
                 out_dtype = torch.bfloat16 if x.dtype is _F8 else x.dtype
-            _kind(out_dtype, "out_dtype")
-            out = _empty((M, N), out_dtype, dev, stream)
+            to = _kind(out_dtype, "out_dtype")
+            out, ldo = _empty((M, N), out_dtype, dev, stream), N
         elif out_dtype is not None and out.dtype is not out_dtype:
             raise ValueError(f"out is {out.dtype}, not {out_dtype}")
+        else:
+            ldo, to = _rows(out, M, N, dev, "out"), _kind(out.dtype, "out")
         ws, _keep = _workspace(size, dev, stream)
-        desc = self._pack(x.data_ptr(), ld, xs, lds, kind, M, N, K, *self._w, out.data_ptr(), _rows(out, M, N, dev, "out"),
-                          _kind(out.dtype, "out"), ws)
+        desc = self._pack(x.data_ptr(), ld, xs, lds, kind, M, N, K, *self._w, out.data_ptr(), ldo, to, ws)
         _call(self._fn, desc, dev, stream, "moe_fp8_product")
         return out
 
@@ -194,15 +198,17 @@ class Fp8Moe:
         pair = (T, K)
         if out is None:
             out_dtype = x.dtype if out_dtype is None else out_dtype
-            _kind(out_dtype, "out_dtype")
-            out = _empty((T, H), out_dtype, dev, stream)
+            to = _kind(out_dtype, "out_dtype")
+            out, ldo = _empty((T, H), out_dtype, dev, stream), H
         elif out_dtype is not None and out.dtype is not out_dtype:
             raise ValueError(f"out is {out.dtype}, not {out_dtype}")
+        else:
+            ldo, to = _rows(out, T, H, dev, "out"), _kind(out.dtype, "out")
         size = self._ws.get(pair)
         if size is None:
             size = self._ws[pair] = lib().moe_fp8_layer_workspace_bytes(T, E, K, H, self.I)
         ws, _keep = _workspace(size, dev, stream)
         desc = self._pack(x.data_ptr(), ld, kind, T, E, K, H, self.I, *self._w, _out(ids, pair, _I32, dev, "ids"),
-                          _out(w, pair, _F32, dev, "w"), out.data_ptr(), _rows(out, T, H, dev, "out"), _kind(out.dtype, "out"), ws)
+                          _out(w, pair, _F32, dev, "w"), out.data_ptr(), ldo, to, ws)
         _call(self._fn, desc + route, dev, stream, "moe_fp8_layer")
         return out, ids, w
