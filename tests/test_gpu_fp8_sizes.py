@@ -15,7 +15,8 @@ pytestmark = pytest.mark.gpu
 LAYERS = [(1, 60, 3, 512, 1000), (1, 60, 4, 640, 1000), (1, 60, 5, 512, 1000), (2, 5, 2, 384, 7168), (1, 16, 4, 6000, 300), (2, 3, 2, 64, 14400),
           (20, 256, 4, 256, 128), (60, 20, 2, 7168, 128), (30, 4, 2, 7168, 64), (3, 40, 1, 20000, 40), (2, 3, 2, 64, 30000), (80, 128, 8, 128, 128),
           (150, 60, 4, 128, 256), (100, 60, 6, 200, 120), (64, 40, 4, 256, 256), (40, 8, 2, 272, 128), (65, 8, 2, 256, 128), (128, 64, 4, 130, 64),
-          (129, 64, 4, 256, 64), (2, 256, 32, 128, 128), (4369, 20, 15, 32, 16), (700, 1, 1, 160, 144)]
+          (129, 64, 4, 256, 64), (2, 256, 32, 128, 128), (4369, 20, 15, 32, 16), (700, 1, 1, 160, 144),
+          (3, 2, 1, 1, 1), (40, 2, 2, 1, 5), (300, 2, 2, 5, 1), (600, 3, 2, 40, 130), (400, 2, 2, 256, 200)]
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
