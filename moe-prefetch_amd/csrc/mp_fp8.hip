@@ -919,9 +919,10 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
 #pragma unroll
         for (int j = 0; j < TM; ++j) o.fx[j] = s_sx[kg][par][u][(wm * TM + j) * 16 + c];
     };
-    // A stage's products, a row of tiles' while the row before is scaled and added (EXACT: products take twice as long, and their
-    // operands the registers of that; 4 x 2 tiles have room; 2 x 2 gain nothing: 500 rows of 2,000 by 2,500 18.3 us, 18.6 so) and the row after is read; before the last row, when every read of the stage is done, then(); in each
-    // row, after its products, along(row).
+    // A stage's products, a row of tiles' while the row before is scaled and added and the row after is read; before the last row, when every
+    // read of the stage is done, then(); in each row, after its products, along(row).
+    // EXACT: products take twice as long, and their operands the registers that a row's sums would wait in; 4 x 2 tiles have room for
+    // both, 2 x 2 gain nothing (500 rows of 2,000 by 2,500 18.3 us, 18.6 so).
     auto multiply = [&](const int4_v *s, const Operands &o, auto then, auto along) FP8_INLINE {
         half8_v xh[TM][4];
         if (EXACT)
