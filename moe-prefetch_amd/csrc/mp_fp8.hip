@@ -6,12 +6,10 @@
 // dot runs on the matrix cores, and one fma adds it, scaled, to the f32 sum of the row.  The weight's 16 rows are the A
 // operand, so that a lane holds four of them for one row of x: one scale a lane and block.
 //
-// EXACT: the codes become fp16 for the matrix cores (exactly), whose fp16 products are exact and their sums f32.  The cores' own e4m3
-// instructions add eight neighbouring products at 13 bits below the largest of them, what is below cut off (found by
-// products of powers of two: 2^-13 of the largest stays, 2^-14 does not): 1.4e-5 of the result for normal numbers, where f32 sums
-// have 1e-8.  They take half the time (2,048 rows of 8 of 128 experts, gate and up by tiles: 153 us, fp16 195 to 207), and y in 16 bits
-// does not show it: those products use them.  Those with gate and up do not, for h lies by a tie of e4m3 often enough that a
-// layer's error doubled (of bf16: 0.0036 of out instead of 0.0017).
+// The codes become fp16 for the matrix cores (exactly), whose fp16 products are exact and their sums f32.  The cores' own e4m3
+// instructions (16x16x128 and 16x16x32 alike) add eight neighbouring products at 13 bits below the largest of them, what is below cut
+// off (found by products of powers of two: 2^-13 of the largest stays, 2^-14 does not).  They take half the time, but that is 1.4e-5
+// of a sum of normal numbers, where f32 sums have 1e-8, and all of a sum whose large products cancel.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -192,14 +190,8 @@ __device__ inline half8_v halves(uint32_t lo, uint32_t hi) {
     const half2_v c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
     return half8_v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-// A block's dot from the cores' own e4m3 products.
-__device__ inline float4_v mfma_e4m3(int8_v w, int8_v x) {
-    const float4_v z = {0.0f, 0.0f, 0.0f, 0.0f};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, z, 0, 0, 0, 0, 0, 0);
-}
-template <bool EXACT>
+// a block's dot
 __device__ inline float4_v mfma_block(int8_v w, int8_v x) {
-    if (!EXACT) return mfma_e4m3(w, x);
     float4_v d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 8; i += 2) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(w[i], w[i + 1]), halves(x[i], x[i + 1]), d, 0, 0, 0);
@@ -208,9 +200,8 @@ __device__ inline float4_v mfma_block(int8_v w, int8_v x) {
 
 // acc += s * (w . x over a block).  The sum is done here: without the empty statement the compiler moves it behind a branch that follows, and there
 // it reads the product too early (it waits after the first of the four reads).
-template <bool EXACT>
 __device__ inline void add_block(float4_v &acc, int8_v w, int8_v x, float s) {
-    const float4_v d = mfma_block<EXACT>(w, x);
+    const float4_v d = mfma_block(w, x);
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] = fmaf(d[k], s, acc[k]);
     asm volatile("" : "+v"(acc));
@@ -269,7 +260,7 @@ constexpr int OF_DISPATCH = 1;    // an expert's pairs from a dispatch
 // Sixteen rows of a weight (of gate and up: GATED) for sixteen rows of codes at a time: every weight is read once for them, and memory bounds the
 // call.  KS waves share K, a block each in turn, and their sums are added in their order; with KS 1 each of the workgroup's four has
 // sixteen rows of its own.  A wave's loads of DEEP blocks are on their way together.
-template <int FROM, bool GATED, bool EXACT, int KS>
+template <int FROM, bool GATED, int KS>
 __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
     // (two blocks of gate and up, three of down: 512 pairs of 128 experts 141 us for the layer; one and two 145, four and six 147: waves count, too)
     constexpr int DEEP = GATED ? 2 : 3, MATS = GATED ? 2 : 1;
@@ -308,13 +299,13 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
             for (int i = 0; i < DEEP; ++i) {
                 if (b0 + i * KS >= whole) break;
 #pragma unroll
-                for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m], wf[i][m], xf[i], s[i] * f[i][m]);
+                for (int m = 0; m < MATS; ++m) add_block(acc[m], wf[i][m], xf[i], s[i] * f[i][m]);
             }
         }
         if (a.K % FB && whole % KS == first) {          // the last block
             const int8_v xt = load_last(x, a.K, g);
 #pragma unroll
-            for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m], load_last(w[m], a.K, g), xt, xs[whole] * ws[m][whole]);
+            for (int m = 0; m < MATS; ++m) add_block(acc[m], load_last(w[m], a.K, g), xt, xs[whole] * ws[m][whole]);
         }
         // (y, or h, of row p0 + col) -> where it goes, and its weight
         auto out_of = [&](int col, float &weight) FP8_INLINE {
@@ -403,7 +394,7 @@ __device__ inline void list_bits(uint64_t m, uint8_t *list) {
 // GATED: workgroup y has the expert of pair y, where that is the expert's first pair, and all of its pairs among the ids
 // (at most 64); h goes out in f32 in the order of pairs.  Else rows 0 .. M - 1 of x.
 // One row through 2,048 x 2,048: 3.9 us, a launch and a trip to memory; gate and up of 512 x 2,048 of 64 pairs' experts, 57 of 256: 27 us, 4.4 TB/s.
-template <int T, bool GATED, bool EXACT>
+template <int T, bool GATED>
 __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
     constexpr int WAVES = 4, DEEP = 4, MATS = GATED ? 2 : 1;
     extern __shared__ __align__(16) uint8_t s_q[];      // [16][stride] codes, [16][nb] scales
@@ -449,7 +440,7 @@ __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
         const uint8_t *q = s_q + min(c, cols - 1) * stride;
         const float *s = s_s + min(c, cols - 1) * nb;
         float4_v acc[2] = {};
-        auto add = [&](int8_v w, float f, int b, int m) FP8_INLINE { add_block<EXACT>(acc[m], w, lds_frag(q, b, g), s[b] * f); };
+        auto add = [&](int8_v w, float f, int b, int m) FP8_INLINE { add_block(acc[m], w, lds_frag(q, b, g), s[b] * f); };
         for (int b0 = wave; b0 < whole; b0 += WAVES * DEEP) {
             if (!loaded) load_w(b0);
             loaded = false;
@@ -489,7 +480,7 @@ constexpr int MID_PAIRS = 512;
 // by the workgroup, a wave's weights of DEEP blocks on their way while those before are multiplied (one of gate and up, two of down: 8 tokens of
 // 256 experts 59.8 us for the layer, 37 of 60 27.2; two and three 63.0 and 30.6, four and six 68.0 and 31.1: waves count more).
 // Memory bounds it: 64 tokens of 128 experts of 768 of 2,048 75 us (5.3 TB/s), down 43.7 (4.6).
-template <int T, bool GATED, bool EXACT>
+template <int T, bool GATED>
 __global__ __launch_bounds__(256) void fp8_mid_kernel(Fp8Args a) {
     constexpr int DEEP = GATED ? 1 : 2, MATS = GATED ? 2 : 1;
     extern __shared__ __align__(16) uint8_t s_q[];      // [cols][stride] codes, [cols][nb] scales
@@ -547,7 +538,7 @@ __global__ __launch_bounds__(256) void fp8_mid_kernel(Fp8Args a) {
             for (int i = 0; i < DEEP; ++i)
                 if (b0 + i < whole)
 #pragma unroll
-                    for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m], t.w[i][m], lds_frag(q, b0 + i, g), s[b0 + i] * t.s[i][m]);
+                    for (int m = 0; m < MATS; ++m) add_block(acc[m], t.w[i][m], lds_frag(q, b0 + i, g), s[b0 + i] * t.s[i][m]);
         };
         for (int b0 = 0; b0 < whole; b0 += 2 * DEEP) {
             load_w(w1, b0 + DEEP);
@@ -557,7 +548,7 @@ __global__ __launch_bounds__(256) void fp8_mid_kernel(Fp8Args a) {
         }
         if (whole < nb)                                 // the last block
 #pragma unroll
-            for (int m = 0; m < MATS; ++m) add_block<EXACT>(acc[m], load_last(w[m], a.K, g), lds_frag(q, whole, g), s[whole] * ws[m][whole]);
+            for (int m = 0; m < MATS; ++m) add_block(acc[m], load_last(w[m], a.K, g), lds_frag(q, whole, g), s[whole] * ws[m][whole]);
         const int n1 = n0 + 4 * g;
         if (c < cols && n1 < a.N) {
             const int pair = s_list[p0 + c];
@@ -575,7 +566,6 @@ __global__ __launch_bounds__(256) void fp8_mid_kernel(Fp8Args a) {
 // quantized into LDS while the weights are on their way; eight waves share the experts in use, and K.  The pairs' rows meet in LDS,
 // where each token's are added in order.
 constexpr int DOWN_PAIRS = 4;
-template <bool EXACT>
 __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
     constexpr int WAVES = 8, DEEP = 6;
     extern __shared__ __align__(16) uint8_t s_q[];      // [P][stride] codes, [P][nb] scales, [parts][P][17] rows
@@ -617,7 +607,7 @@ __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
     if (live) {
         const uint8_t *q = s_q + pair * stride;
         float4_v acc = {};
-        auto add = [&](int8_v w, int b, float sw) FP8_INLINE { add_block<EXACT>(acc, w, lds_frag(q, b, g), s_s[pair * nb + b] * sw); };
+        auto add = [&](int8_v w, int b, float sw) FP8_INLINE { add_block(acc, w, lds_frag(q, b, g), s_s[pair * nb + b] * sw); };
 #pragma unroll
         for (int i = 0; i < DEEP; ++i)
             if (part + i * a.parts < whole) add(wf[i], part + i * a.parts, f[i]);
@@ -676,8 +666,7 @@ static hipError_t launch_few_t(Fp8Args a, hipStream_t st) {
     a.cols = std::min(a.M, lds_rows(a.K));
     const dim3 grid((unsigned)((a.N + 15) / 16), GATED ? (unsigned)a.M : 1);
     const size_t lds = (size_t)a.cols * (lds_stride(a.K) + 4 * ((a.K + FB - 1) / FB));
-    if (GATED || a.exact) hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED, true>), grid, dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED, GATED>), grid, dim3(256), lds, st, a);
+    hipLaunchKernelGGL((fp8_few_up_kernel<T, GATED>), grid, dim3(256), lds, st, a);
     return hipGetLastError();
 }
 template <bool GATED>
@@ -692,8 +681,7 @@ static hipError_t launch_few_down(Fp8FewArgs a, hipStream_t st) {
     while (2 * a.parts * P <= 8 && 2 * a.parts <= nb) a.parts *= 2;
     const dim3 grid((unsigned)((a.H + 15) / 16));
     const size_t lds = (size_t)P * (lds_stride(a.I) + 4 * nb) + (size_t)a.parts * P * 17 * 4;
-    if (a.exact) hipLaunchKernelGGL((fp8_few_down_kernel<true>), grid, dim3(512), lds, st, a);
-    else hipLaunchKernelGGL((fp8_few_down_kernel<false>), grid, dim3(512), lds, st, a);
+    hipLaunchKernelGGL(fp8_few_down_kernel, grid, dim3(512), lds, st, a);
     return hipGetLastError();
 }
 
@@ -702,8 +690,7 @@ static hipError_t launch_mid_t(Fp8Args a, hipStream_t st) {
     a.cols = std::min(a.M, lds_rows(a.K));
     const dim3 grid((unsigned)((a.N + 63) / 64), (unsigned)std::min(a.E, a.M));
     const size_t lds = (size_t)a.cols * (lds_stride(a.K) + 4 * ((a.K + FB - 1) / FB));
-    if (GATED || a.exact) hipLaunchKernelGGL((fp8_mid_kernel<T, GATED, true>), grid, dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((fp8_mid_kernel<T, GATED, GATED>), grid, dim3(256), lds, st, a);
+    hipLaunchKernelGGL((fp8_mid_kernel<T, GATED>), grid, dim3(256), lds, st, a);
     return hipGetLastError();
 }
 // Gate and up: as many pairs as a wave has lanes by one kernel, more by the other (64 pairs of 256 experts, 512 of 2,048: 26 us and 30).
@@ -721,7 +708,6 @@ hipError_t launch_fp8_few_layer(Fp8Args a, int x_type, Fp8FewArgs f, float *rows
     a.m[0] = f.down; a.gated = 0;
     a.x = (const uint8_t *)f.h; a.ldx = f.I;
     a.N = f.H; a.K = f.I;
-    a.exact = f.exact;
     a.pair_w = f.w;
     a.y = rows; a.ldy = f.H;
     err = launch_mid_t<T_F32, false>(a, st);
@@ -733,8 +719,7 @@ template <int FROM, bool GATED, int KS>
 static hipError_t launch_stream(const Fp8Args &a, hipStream_t st) {
     const int rows = KS > 1 ? 16 : 64;
     const dim3 grid((unsigned)((a.N + rows - 1) / rows), FROM == OF_ALL ? 1 : (unsigned)a.E);
-    if (GATED || a.exact) hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, true, KS>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, GATED, KS>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((fp8_stream_kernel<FROM, GATED, KS>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
@@ -807,7 +792,7 @@ __device__ inline void barrier() {
 
 // NS: stages of loads to LDS without registers (rows on 16 bytes, near one another); 1: through registers.  KG groups of waves share K, a block
 // each in turn, and their sums are added in their order.
-template <bool GATED, bool EXACT, int NS, int KG, int WN, int WM, int TN, int TM>
+template <bool GATED, int NS, int KG, int WN, int WM, int TN, int TM>
 __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, int n_tiles, int m_tiles) {
     constexpr int THREADS = 64 * WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, CH = (BN + BM) * 8 / THREADS, SB = 6;
     static_assert(KG == 1 || (NS > 1 && !GATED && (KG - 1) * THREADS * TN * TM <= KG * (BN + BM) * 8), "sums fit a stage");
@@ -921,16 +906,15 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
     };
     // A stage's products, a row of tiles' while the row before is scaled and added and the row after is read; before the last row, when every
     // read of the stage is done, then(); in each row, after its products, along(row).
-    // EXACT: products take twice as long, and their operands the registers that a row's sums would wait in; 4 x 2 tiles have room for
-    // both, 2 x 2 gain nothing (500 rows of 2,000 by 2,500 18.3 us, 18.6 so).
+    // (The fp16 operands take the registers that a row's sums would wait in: 4 x 2 tiles have room for both, 2 x 2 gain nothing: 500 rows of
+    // 2,000 by 2,500 18.3 us, 18.6 so.)
     auto multiply = [&](const int4_v *s, const Operands &o, auto then, auto along) FP8_INLINE {
         half8_v xh[TM][4];
-        if (EXACT)
 #pragma unroll
-            for (int j = 0; j < TM; ++j)
+        for (int j = 0; j < TM; ++j)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) xh[j][k] = halves(o.x[j][2 * k], o.x[j][2 * k + 1]);
-        constexpr int LAG = EXACT && (TM > 2 || TN < 4) ? 0 : 1;
+            for (int k = 0; k < 4; ++k) xh[j][k] = halves(o.x[j][2 * k], o.x[j][2 * k + 1]);
+        constexpr int LAG = TM > 2 || TN < 4 ? 0 : 1;
         int8_v wf = o.w;
         float4_v d[LAG + 1][TM];
 #pragma unroll
@@ -940,19 +924,14 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
             if (i == TN - 1) then();
             if (i < TN) {
                 half8_v wh[4];
-                if (EXACT)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) wh[k] = halves(wf[2 * k], wf[2 * k + 1]);
+                for (int k = 0; k < 4; ++k) wh[k] = halves(wf[2 * k], wf[2 * k + 1]);
 #pragma unroll
                 for (int j = 0; j < TM; ++j) {
-                    if (EXACT) {
-                        float4_v t = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float4_v t = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[k], xh[j][k], t, 0, 0, 0);
-                        d[i & LAG][j] = t;
-                    } else {
-                        d[i & LAG][j] = mfma_e4m3(wf, o.x[j]);
-                    }
+                    for (int k = 0; k < 4; ++k) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[k], xh[j][k], t, 0, 0, 0);
+                    d[i & LAG][j] = t;
                 }
             }
             if (LAG) __builtin_amdgcn_sched_barrier(0);     // first the products
@@ -1150,34 +1129,34 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
     }
 }
 
-template <bool GATED, bool EXACT, int NS, int KG, int WN, int WM, int TN, int TM>
+template <bool GATED, int NS, int KG, int WN, int WM, int TN, int TM>
 static hipError_t launch_tile_n(const Fp8Args &a, hipStream_t st) {
     constexpr int ROWS = 16 * TN * WN / (GATED ? 2 : 1), BM = 16 * TM * WM;
     const int64_t n_tiles = (a.N + ROWS - 1) / ROWS;
     // (a dispatch: whole runs, and one for each used expert that is not whole)
     const int64_t runs = a.offsets ? a.M / BM + std::min(a.E, a.M) : (a.M + BM - 1) / BM;
-    hipLaunchKernelGGL((fp8_tile_kernel<GATED, EXACT, NS, KG, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM * KG), 0,
+    hipLaunchKernelGGL((fp8_tile_kernel<GATED, NS, KG, WN, WM, TN, TM>), dim3((unsigned)(n_tiles * runs)), dim3(64 * WN * WM * KG), 0,
                        st, a, (int)n_tiles, (int)runs);
     return hipGetLastError();
 }
-template <bool GATED, bool EXACT, int NS, int KG, int WN, int WM, int TN, int TM>
+template <bool GATED, int NS, int KG, int WN, int WM, int TN, int TM>
 static hipError_t launch_tile_d(const Fp8Args &a, hipStream_t st) {
     // rows on 16 bytes, and a workgroup's within 4 GiB (those of x from a dispatch: all)
     auto near = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0 && 256 * m.ld < 1ll << 32; };
     const int64_t rows = a.top ? (a.M + a.top - 1) / a.top : 256;
     if (!near(a.m[0]) || (GATED && !near(a.m[1])) || ((uintptr_t)a.x | a.ldx) % 16 || a.ldx * rows >= 1ll << 32)
-        return launch_tile_n<GATED, EXACT, 1, 1, WN, WM, TN, TM>(a, st);
-    return launch_tile_n<GATED, EXACT, NS, KG, WN, WM, TN, TM>(a, st);
+        return launch_tile_n<GATED, 1, 1, WN, WM, TN, TM>(a, st);
+    return launch_tile_n<GATED, NS, KG, WN, WM, TN, TM>(a, st);
 }
 template <bool GATED>
 static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
     if constexpr (GATED) {
         // 64 rows of x a tile up to 128 of an expert, then 128 (experts of 768 of 2,048, the layer: 12 rows 159 us and 176, 64 235 and 249,
         // 128 330 and 334, 256 555 and 538; of down 128 rows always: 12 rows 157 us with 64, 159; 64 235 and 236; 128 352 and 333)
-        if (a.M <= 128ll * a.E) return launch_tile_d<true, true, 3, 1, 4, 2, 4, 2>(a, st);
-        return launch_tile_d<true, true, 3, 1, 4, 2, 4, 4>(a, st);
+        if (a.M <= 128ll * a.E) return launch_tile_d<true, 3, 1, 4, 2, 4, 2>(a, st);
+        return launch_tile_d<true, 3, 1, 4, 2, 4, 4>(a, st);
     } else {
-        return a.exact ? launch_tile_d<false, true, 3, 1, 4, 2, 4, 4>(a, st) : launch_tile_d<false, false, 3, 1, 4, 2, 4, 4>(a, st);
+        return launch_tile_d<false, 3, 1, 4, 2, 4, 4>(a, st);
     }
 }
 
@@ -1188,8 +1167,8 @@ hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
         // through 2,048 x 4,096: 13.8 us, 64 x 64 21.4; 500 through 2,500 x 2,000 in f32: 18.5 of 64 x 64, 31.7 shared)
         auto tiles = [&](int n, int m) { return (int64_t)((a.N + n - 1) / n) * ((a.M + m - 1) / m); };
         if (tiles(256, 128) >= 200) return launch_tile<false>(a, st);
-        if (tiles(64, 64) >= 200) return a.exact ? launch_tile_d<false, true, 3, 1, 2, 2, 2, 2>(a, st) : launch_tile_d<false, false, 3, 1, 2, 2, 2, 2>(a, st);
-        return a.exact ? launch_tile_d<false, true, 3, 4, 2, 2, 1, 2>(a, st) : launch_tile_d<false, false, 3, 4, 2, 2, 1, 2>(a, st);
+        if (tiles(64, 64) >= 200) return launch_tile_d<false, 3, 1, 2, 2, 2, 2>(a, st);
+        return launch_tile_d<false, 3, 4, 2, 2, 1, 2>(a, st);
     }
     if (a.tiles) return a.gated ? launch_tile<true>(a, st) : launch_tile<false>(a, st);
     return a.gated ? launch_stream<OF_DISPATCH, true, 1>(a, st) : launch_stream<OF_DISPATCH, false, 1>(a, st);

@@ -392,7 +392,6 @@ struct Fp8Args {
     void *y;
     int64_t ldy;
     int y_type;
-    int exact;                    // sums of products in f32 throughout (see mp_fp8.hip)
     uint8_t *hq;                  // gated, many rows: y's codes and scales instead of y
     int64_t ldh;
     float *hs;
@@ -408,7 +407,7 @@ struct Fp8FewArgs {
     const float *h;               // [n_tok * K][I]
     const int32_t *ids;
     const float *w;
-    int n_tok, E, K, H, I, exact;
+    int n_tok, E, K, H, I;
     void *out;
     int64_t ldo;
     int out_type;

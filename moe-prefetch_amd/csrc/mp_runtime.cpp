@@ -4285,7 +4285,6 @@ int moe_fp8_product(const moe_fp8_product_desc *d, void *stream) {
     a.m[0] = fp8_mat(d->weight);
     a.x = (const uint8_t *)d->x; a.ldx = d->x_stride; a.xs = d->x_scale; a.ldxs = d->x_scale_stride;
     a.M = d->n_tok; a.N = d->N; a.K = d->K; a.E = 1;
-    a.exact = d->y_type == MOE_DTYPE_F32;
     a.y = d->y; a.ldy = d->y_stride; a.y_type = d->y_type;
     if (few) {
         HIPCHK(mp::launch_fp8_few_product(a, d->x_type, (hipStream_t)stream));
@@ -4361,14 +4360,13 @@ int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream) {
     a.top = d->K;
     a.M = P; a.N = d->I; a.K = d->H; a.E = d->E;
     a.y = ws + l.act; a.ldy = d->I; a.y_type = MOE_DTYPE_F32;
-    a.exact = 1;
     const int tile_rows = mp::fp8_tile_rows(a.m[0], a.m[1], fp8_mat(d->down));
     a.tiles = P >= tile_rows * d->E;
     if (mp::fp8_few_layer(P, d->E, d->H, d->I, tile_rows)) {
         a.x = (const uint8_t *)d->x; a.ldx = d->x_stride;
         a.ids = d->ids;
         HIPCHK(mp::launch_fp8_few_layer(a, d->x_type, {fp8_mat(d->down), (const float *)(ws + l.act), d->ids, d->w, d->n_tok, d->E, d->K, d->H,
-                                                       d->I, d->out_type == MOE_DTYPE_F32, d->out, d->out_stride, d->out_type},
+                                                       d->I, d->out, d->out_stride, d->out_type},
                                         (float *)(ws + l.rows), st));
         return MOE_OK;
     }
@@ -4383,7 +4381,6 @@ int moe_fp8_layer(const moe_fp8_layer_desc *d, void *stream) {
     a.m[0] = fp8_mat(d->down); a.gated = 0;
     a.x = ws + l.h.q; a.ldx = l.h.ld; a.xs = (const float *)(ws + l.h.s); a.ldxs = l.h.nb;
     a.top = 0; a.N = d->H; a.K = d->I;
-    a.exact = d->out_type == MOE_DTYPE_F32;
     a.pair_w = d->w;
     a.y = ws + l.rows; a.ldy = d->H;
     HIPCHK(mp::launch_fp8_product(a, st));
