@@ -910,10 +910,13 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
     // 2,000 by 2,500 18.3 us, 18.6 so.)
     auto multiply = [&](const int4_v *s, const Operands &o, auto then, auto along) FP8_INLINE {
         half8_v xh[TM][4];
+        auto convert_x = [&]() FP8_INLINE {
 #pragma unroll
-        for (int j = 0; j < TM; ++j)
+            for (int j = 0; j < TM; ++j)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) xh[j][k] = halves(o.x[j][2 * k], o.x[j][2 * k + 1]);
+                for (int k = 0; k < 4; ++k) xh[j][k] = halves(o.x[j][2 * k], o.x[j][2 * k + 1]);
+        };
+        if (TN > 1) convert_x();
         constexpr int LAG = TM > 2 || TN < 4 ? 0 : 1;
         int8_v wf = o.w;
         float4_v d[LAG + 1][TM];
@@ -924,6 +927,7 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
             if (i == TN - 1) then();
             if (i < TN) {
                 half8_v wh[4];
+                if (TN == 1) convert_x();               // (one row of tiles: the registers are the next stage's operands' until here)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) wh[k] = halves(wf[2 * k], wf[2 * k + 1]);
 #pragma unroll
@@ -1163,12 +1167,14 @@ static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
 hipError_t launch_fp8_product(const Fp8Args &a, hipStream_t st) {
     if (!a.offsets) {
         if (a.M <= 16) return launch_stream<OF_ALL, false, 4>(a, st);
-        // 256 x 128 tiles where they are many enough for every compute unit; else 64 x 64; else 32 x 64 with K shared by four (64 rows
-        // through 2,048 x 4,096: 13.8 us, 64 x 64 21.4; 500 through 2,500 x 2,000 in f32: 18.5 of 64 x 64, 31.7 shared)
+        // 256 x 128 tiles where they are many enough for every compute unit (1,800 rows through 3,600 x 2,048: 42.4 us, 64 x 64 51; 1,024 through
+        // 4,096 x 2,048 40.3 and 35); else 64 x 64 (128 through 8,192 x 2,048: 15.0, 32 x 64 18.8); else 32 x 64 with K shared, by two groups of
+        // waves or from 32 blocks on by four, which are held to 128 registers and spill 24 bytes a lane (64 rows through 2,048 x 2,048: two
+        // groups 10.9 us, four 11.8; 2,048 x 3,328 14.2 and 14.4; 2,048 x 4,096 16.1 and 15.6; 24 through 2,048 x 7,168 21.2 and 18.9)
         auto tiles = [&](int n, int m) { return (int64_t)((a.N + n - 1) / n) * ((a.M + m - 1) / m); };
         if (tiles(256, 128) >= 200) return launch_tile<false>(a, st);
         if (tiles(64, 64) >= 200) return launch_tile_d<false, 3, 1, 2, 2, 2, 2>(a, st);
-        return launch_tile_d<false, 3, 4, 2, 2, 1, 2>(a, st);
+        return a.K < 32 * FB ? launch_tile_d<false, 3, 2, 2, 2, 1, 2>(a, st) : launch_tile_d<false, 3, 4, 2, 2, 1, 2>(a, st);
     }
     if (a.tiles) return a.gated ? launch_tile<true>(a, st) : launch_tile<false>(a, st);
     return a.gated ? launch_stream<OF_DISPATCH, true, 1>(a, st) : launch_stream<OF_DISPATCH, false, 1>(a, st);
