@@ -474,7 +474,7 @@ __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
     }
 }
 
-constexpr int MID_PAIRS = 512;
+constexpr int MID_PAIRS = FP8_MID_PAIRS;
 // The same for up to MID_PAIRS pairs: workgroup y has expert y (where experts are more than pairs: the expert of pair y, if that is its first one),
 // whose pairs every wave finds among the ids, and each of its four waves sixteen rows of the weights.  The expert's rows of x (GATED; else of h: in f32 and in the order of pairs, as GATED leaves them) are quantized into LDS
 // by the workgroup, a wave's weights of DEEP blocks on their way while those before are multiplied (one of gate and up, two of down: 8 tokens of

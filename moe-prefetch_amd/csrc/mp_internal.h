@@ -361,6 +361,7 @@ hipError_t launch_sample(SampleArgs a, void *ws, hipStream_t st);
 
 // e4m3 weights with block scales (mp_fp8.hip); strides of codes count bytes, those of scales elements
 constexpr int FP8_BLOCK = 128;
+constexpr int FP8_MID_PAIRS = 512;    // a layer of more pairs goes by a dispatch (fp8_few_layer)
 struct Fp8QuantArgs {
     const void *x;
     int64_t ldx;

@@ -4314,8 +4314,13 @@ static Fp8LayerWs fp8_layer_ws(int64_t n_tok, int E, int K, int H, int I) {
     w.counts = take(w.total, (size_t)E * 4);
     w.offsets = take(w.total, (size_t)(E + 1) * 4);
     w.perm = take(w.total, (size_t)P * 4);
-    w.act = take(w.total, (size_t)(P * I) * 4);
-    w.rows = take(w.total, (size_t)(P * H) * 4);
+    // h in f32 and the pairs' rows.  After a dispatch h's codes are made of it (tiles never write it) before a row is written: one place for both.
+    if (P > mp::FP8_MID_PAIRS) {
+        w.act = w.rows = take(w.total, (size_t)(P * std::max(H, I)) * 4);
+    } else {
+        w.act = take(w.total, (size_t)(P * I) * 4);
+        w.rows = take(w.total, (size_t)(P * H) * 4);
+    }
     return w;
 }
 static bool fp8_layer_shape(int n_tok, int E, int K, int H, int I) {

@@ -108,7 +108,7 @@ def test_product_within_f32_sums(M, N, K, given, dt):
 
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 @pytest.mark.parametrize("T, E, K, H, I", [(1, 8, 2, 256, 128), (7, 60, 6, 1000, 200), (64, 16, 4, 256, 384), (150, 80, 4, 128, 256), (130, 4, 1, 257, 100),
-                                           (700, 3, 2, 256, 640)])
+                                           (700, 3, 2, 256, 640), (150, 80, 4, 160, 700), (150, 80, 4, 700, 160), (300, 4, 2, 144, 720)])
 def test_layer_within_f32_sums(T, E, K, H, I, dt):
     g = gen(T + 10 * E + H + 1)
     m, up, gate, down = moe(g, E, K, H, I)
