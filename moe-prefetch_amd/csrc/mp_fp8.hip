@@ -392,7 +392,7 @@ __device__ inline void list_bits(uint64_t m, uint8_t *list) {
 // Sixteen rows of a weight (of gate and up: GATED) for few rows of x, which are quantized into LDS while the weight is on its way: one
 // launch, and nothing between.  Four waves share K.
 // GATED: workgroup y has the expert of pair y, where that is the expert's first pair, and all of its pairs among the ids
-// (at most 64); h goes out in f32 in the order of pairs.  Else rows 0 .. M - 1 of x.
+// (at most 64, a wave's lanes); h goes out in f32 in the order of pairs.  Else rows 0 .. M - 1 of x.
 // One row through 2,048 x 2,048: 3.9 us, a launch and a trip to memory; gate and up of 512 x 2,048 of 64 pairs' experts, 57 of 256: 27 us, 4.4 TB/s.
 template <int T, bool GATED>
 __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
@@ -565,7 +565,7 @@ __global__ __launch_bounds__(256) void fp8_mid_kernel(Fp8Args a) {
 // The down product of DOWN_PAIRS pairs at most and the sum over a token's experts: sixteen columns of out for all tokens.  h of all pairs is
 // quantized into LDS while the weights are on their way; eight waves share the experts in use, and K.  The pairs' rows meet in LDS,
 // where each token's are added in order.
-constexpr int DOWN_PAIRS = 4;
+constexpr int DOWN_PAIRS = 8;
 __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
     constexpr int WAVES = 8, DEEP = 6;
     extern __shared__ __align__(16) uint8_t s_q[];      // [P][stride] codes, [P][nb] scales, [parts][P][17] rows
@@ -693,14 +693,17 @@ static hipError_t launch_mid_t(Fp8Args a, hipStream_t st) {
     hipLaunchKernelGGL((fp8_mid_kernel<T, GATED>), grid, dim3(256), lds, st, a);
     return hipGetLastError();
 }
-// Gate and up: as many pairs as a wave has lanes by one kernel, more by the other (64 pairs of 256 experts, 512 of 2,048: 26 us and 30).
+// Gate and up: up to 32 pairs with K shared by four waves, more with sixteen rows a wave (experts of 768 of 2,048, the layer: 8 pairs 22.7 us and
+// 27.3, 16 29.6 and 31.4, 32 46.8 and 46.4; of 512, 24 pairs of 256 29.9 and 32.1, 64 55.9 and 54.7; 64 of 16 of 1,024 43.1 and 40.0).
+constexpr int FEW_PAIRS = 32;
+static_assert(FEW_PAIRS <= 64, "fp8_few_up_kernel finds pairs by the lanes of a wave");
 static hipError_t launch_few_gated(const Fp8Args &a, int x_type, hipStream_t st) {
-    if (a.M <= 64) return launch_few<true>(a, x_type, st);
+    if (a.M <= FEW_PAIRS) return launch_few<true>(a, x_type, st);
     return x_type == T_F32 ? launch_mid_t<T_F32, true>(a, st) : x_type == T_BF16 ? launch_mid_t<T_BF16, true>(a, st) : launch_mid_t<T_F16, true>(a, st);
 }
-// Down with the sum over a token's experts where pairs are DOWN_PAIRS at most (a layer of one token, two experts of 2,048 of 1,024: 14.0 us,
-// through pair rows 18.0; one of 8,192 of 5,120: 40.6 and 50.7; but eight of 768 of 2,048: 21.0 and 21.4, sixteen 30.3 and 27.7), else into
-// pair rows.
+// Down with the sum over a token's experts where pairs are DOWN_PAIRS at most, a wave each, else into pair rows (a layer of one token, two
+// experts of 2,048 of 1,024: 15.1 us, through pair rows 19.2; one of 8,192 of 5,120: 41.1 and 55.4; four of 768 of 2,048 16.1 and 18.7, eight 21.5
+// and 22.8, eight of 1,536 30.8 and 30.1, of 2,048 of 7,168 84.7 and 85.2).
 hipError_t launch_fp8_few_layer(Fp8Args a, int x_type, Fp8FewArgs f, float *rows, hipStream_t st) {
     hipError_t err = launch_few_gated(a, x_type, st);
     if (err != hipSuccess) return err;
