@@ -262,8 +262,9 @@ constexpr int OF_DISPATCH = 1;    // an expert's pairs from a dispatch
 // sixteen rows of its own.  A wave's loads of DEEP blocks are on their way together.
 template <int FROM, bool GATED, int KS>
 __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args a) {
-    // (two blocks of gate and up, three of down: 512 pairs of 128 experts 141 us for the layer; one and two 145, four and six 147: waves count, too)
-    constexpr int DEEP = GATED ? 2 : 3, MATS = GATED ? 2 : 1;
+    // (one block of gate and up, two of down: 640 pairs of 128 experts 144 us for the layer, 960 158, 600 of 60 off 16 bytes 42.9; two and three
+    // 145, 160 and 45.6; four and six 146, 162 and 46.5: waves count more)
+    constexpr int DEEP = GATED ? 1 : 2, MATS = GATED ? 2 : 1;
     __shared__ float s_acc[KS > 1 ? MATS : 1][KS][KS > 1 ? 16 : 1][17];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     const int n0 = (KS > 1 ? blockIdx.x : blockIdx.x * 4 + wave) * 16, whole = a.K / FB, first = KS > 1 ? wave : 0;
