@@ -94,7 +94,7 @@ __device__ inline float without_inf(float *v, float m) {
 }
 
 // Sixteen lanes a block of one row, eight neighbouring elements each in one load; NB blocks a lane, sixteen apart, whose loads are on their
-// way together.  magic, shift: the division by the blocks of a row.  Memory bounds many rows (8,192 of 4,096 in bf16: 20.7 us, 4.9 TB/s, as a
+// way together.  magic, shift: the division by the blocks of a row.  Memory bounds many rows (8,192 of 4,096 in bf16: 20.8 us, 4.9 TB/s, as a
 // copy), the launch few (64 of 2,048: 2.5 us).
 template <int T, int NB>
 __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a, uint32_t nb, uint32_t total, uint32_t magic, int shift) {
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a, uin
     }
 }
 
-// a workgroup a block of 128 rows
+// a workgroup a block of 128 rows: memory bounds it, too (98,304 of 2,048 in bf16: 123 us, 4.9 TB/s; 768 of 2,048 4.7 us)
 template <int T>
 __global__ __launch_bounds__(256) void fp8_quant_block_kernel(Fp8QuantArgs a) {
     __shared__ float s_max[4];
@@ -394,7 +394,7 @@ __device__ inline void list_bits(uint64_t m, uint8_t *list) {
 // launch, and nothing between.  Four waves share K.
 // GATED: workgroup y has the expert of pair y, where that is the expert's first pair, and all of its pairs among the ids
 // (at most 64, a wave's lanes); h goes out in f32 in the order of pairs.  Else rows 0 .. M - 1 of x.
-// One row through 2,048 x 2,048: 3.9 us, a launch and a trip to memory; gate and up of 512 x 2,048 of 64 pairs' experts, 57 of 256: 27 us, 4.4 TB/s.
+// One row through 2,048 x 2,048: 4.0 us, a launch and a trip to memory; gate and up of 768 x 2,048 of eight pairs' experts 10.9 us, 2.3 TB/s.
 template <int T, bool GATED>
 __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
     constexpr int WAVES = 4, DEEP = 4, MATS = GATED ? 2 : 1;
@@ -478,9 +478,9 @@ __global__ __launch_bounds__(256) void fp8_few_up_kernel(Fp8Args a) {
 constexpr int MID_PAIRS = FP8_MID_PAIRS;
 // The same for up to MID_PAIRS pairs: workgroup y has expert y (where experts are more than pairs: the expert of pair y, if that is its first one),
 // whose pairs every wave finds among the ids, and each of its four waves sixteen rows of the weights.  The expert's rows of x (GATED; else of h: in f32 and in the order of pairs, as GATED leaves them) are quantized into LDS
-// by the workgroup, a wave's weights of DEEP blocks on their way while those before are multiplied (one of gate and up, two of down: 8 tokens of
-// 256 experts 59.8 us for the layer, 37 of 60 27.2; two and three 63.0 and 30.6, four and six 68.0 and 31.1: waves count more).
-// Memory bounds it: 64 tokens of 128 experts of 768 of 2,048 75 us (5.3 TB/s), down 43.7 (4.6).
+// by the workgroup, a wave's weights of DEEP blocks on their way while those before are multiplied (one of gate and up, two of down: 10 tokens of
+// 256 experts 63.6 us for the layer, 37 of 60 27.9, 64 of 128 134; two and three 69.5, 30.9 and 140, four and six 74.0, 32.2 and 147: waves
+// count more).  Memory bounds it: 64 tokens of 128 experts of 768 of 2,048 75 us (5.4 TB/s), down 44.3 (4.5).
 template <int T, bool GATED>
 __global__ __launch_bounds__(256) void fp8_mid_kernel(Fp8Args a) {
     constexpr int DEEP = GATED ? 1 : 2, MATS = GATED ? 2 : 1;
@@ -648,15 +648,15 @@ __global__ __launch_bounds__(512) void fp8_few_down_kernel(Fp8FewArgs a) {
 static int lds_rows(int K) { return std::min(16, 54 * 1024 / (lds_stride(K) + 4 * ((K + FB - 1) / FB))); }
 bool fp8_few_product(int M, int K) { return M <= lds_rows(K); }
 // From how many rows an expert (on average) a layer's products run on tiles.  Weights on 16 bytes: 8 (128 experts of 768 of 2,048, 960 pairs:
-// 157.1 us for the layer, from codes sixteen rows at a time 157.4; 640: 155 and 147; 1,536: 159 and 192).  Others: 16 (60 of 200 of 1,000, 1,920
-// pairs: 63 and 67; 600: 58 and 43).
+// 160 us for the layer, from codes sixteen rows at a time 158; 640: 156 and 144; 1,536: 165 and 197).  Others: 16 (60 of 200 of 1,000, 960 pairs:
+// 52 and 51; 600: 52 and 43; 1,920: 55 and 73).
 int fp8_tile_rows(const Fp8Mat &gate, const Fp8Mat &up, const Fp8Mat &down) {
     auto on16 = [](const Fp8Mat &m) { return ((uintptr_t)m.w | m.ld | m.ex) % 16 == 0; };
     return on16(gate) && on16(up) && on16(down) ? 8 : 16;
 }
 // Which layers take the kernels above: few pairs, fewer than tiles have, and of an expert as many as LDS holds, for else its weights are read
-// again (80 pairs of 8 experts of 2,048 of 1,024: 35 us, tiles 43; 256 of 32 of 768 of 2,048: 78 and 64; 128 of 8 of 14,336 of 4,096: 870 and
-// 368).
+// again (80 pairs of 8 experts of 2,048 of 1,024: 37 us, tiles 49; 512 of 128 of 768 of 2,048: 134 and 162; 256 of 32 57.5 and 58.2; 128 of 8 of
+// 14,336 of 4,096: 910 and 363).
 bool fp8_few_layer(int64_t P, int E, int H, int I, int tile_rows) {
     const int64_t fit = lds_rows(std::max(H, I));
     return P <= MID_PAIRS && (P <= 128 || P < (int64_t)tile_rows * E) && P <= fit * E && std::min(P, (int64_t)2) <= fit;
@@ -733,15 +733,17 @@ static hipError_t launch_stream(const Fp8Args &a, hipStream_t st) {
 // without registers, are on their way while this one is multiplied.
 // The eight 16-byte chunks of a row lie in LDS at chunk ^ (row & 7): the lanes that read one chunk of eight rows then touch
 // all banks once.
-// 256 x 128 tiles, three stages, eight waves of 64 x 64: 4,096^3 78 to 95 us by box (1.45 to 1.76 PFLOP/s), 1.0 us a step of K and 6 a tile beside
-// them (K 256 to 8,192).  A step's products take 0.43 us of the matrix cores at most, its reads of LDS and the loads into it 0.6.
-// Loads of the weight to registers, past LDS, took 144 us, not 79 (16 rows of 64 bytes cost more than 8 of 128); 256 x 256 in two stages the
-// same 79.  Waves of a higher priority while they multiply: 95 us for the call, not 92; workgroups that walk over tiles, the next one's
-// first loads before this one's sums are stored: 97, not 91 (they spill).  A dispatch's, 2,048 tokens of 128 experts of 768 of 2,048: gate and up 195 to 207 us, down 103 to 109.
+// 256 x 128 tiles, three stages, eight waves of 64 x 64: 4,096^3 of given codes 131 us (1.05 PFLOP/s; traced behind a quantizer 137 to 155), 1.65
+// us a step of K and 9 a tile and launch beside them (2,048 rows through 4,096 rows of K 256 to 8,192: 12.8 to 118 us).  A step's products take 0.86
+// us of the matrix cores at least, its reads of LDS and the loads into it 0.6, its conversions to fp16 are 128 a wave for 64 products.
+// 128 x 128 or 256 x 64 tiles took 165 us for the call, not 145.  With the cores' e4m3 products 256 x 256 in two stages, waves of a higher
+// priority, the weight loaded to registers past LDS and workgroups that walk over tiles gained nothing or lost.
+// This form spills 20 bytes a lane, and that of gate and up of 128 rows 28, none of them within the loop over six steps.
+// A dispatch's, 2,048 tokens of 128 experts of 768 of 2,048: gate and up 197 to 203 us, down 123 to 131.
 // Workgroups go round the eight XCDs: each has a run of the tiles, so that those at work at once share what they read in its L2.
 __device__ inline int xcd_tile(int id, int total) { return id < total / 8 * 8 ? (id % 8) * (total / 8) + id / 8 : id; }
 // A workgroup's tile of a dispatch's products: its expert and first row (in the dispatch's order) of a run of bm, and its place among the
-// run's n_tiles, which follow one another (2,048 tokens of 128 experts: 287 us for the layer, 294 round the XCDs); false: there is none
+// run's n_tiles, which follow one another (2,048 tokens of 128 experts: 341 us for the layer, 363 round the XCDs); false: there is none
 __device__ inline bool find_run(const int32_t *offsets, int E, int bm, int n_tiles, int &n_tile, int &e, int &p0, int &end, int *s_run) {
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x;
@@ -910,8 +912,9 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
     };
     // A stage's products, a row of tiles' while the row before is scaled and added and the row after is read; before the last row, when every
     // read of the stage is done, then(); in each row, after its products, along(row).
-    // (The fp16 operands take the registers that a row's sums would wait in: 4 x 2 tiles have room for both, 2 x 2 gain nothing: 500 rows of
-    // 2,000 by 2,500 18.3 us, 18.6 so.)
+    // (The fp16 operands take the registers that a row's sums would wait in: 4 x 2 tiles have room for both (2,048 tokens of 128 experts 341 us,
+    // 343 without), 2 x 2 lose by it (500 rows through 2,500 x 2,000 20.6 us, 21.5 so), and so does one row of tiles (64 through 4,096 x 4,096 16.3,
+    // 17.3).)
     auto multiply = [&](const int4_v *s, const Operands &o, auto then, auto along) FP8_INLINE {
         half8_v xh[TM][4];
         auto convert_x = [&]() FP8_INLINE {
@@ -967,8 +970,8 @@ __global__ __launch_bounds__(64 * WN * WM * KG) void fp8_tile_kernel(Fp8Args a, 
         // Steps stand in the code one by one, each with its own places in LDS, so that reads wait for the loads to their own place alone; at
         // the loop's head they wait for all.  At the end of K the loads are of its last block again, so that every step is alike.
         // One stage is multiplied while the loads of the NS - 1 after it are on their way.  Before its last row of tiles, when every
-        // wave has read all of it, the next stage's first operands are read.  The loads stand between the rows of tiles: all at once
-        // they would hold up the reads and products behind them (4096^3: 96 us, 79 so).
+        // wave has read all of it, the next stage's first operands are read.  The loads stand between the rows of tiles; all of
+        // them after the first take the same time (4096^3 143 us, the layer of 2,048 tokens 338, 341 so).
         constexpr int ROWS_LOAD = TN > 1 ? TN - 1 : 1, EACH_ROW = (CH + ROWS_LOAD - 1) / ROWS_LOAD, BEHIND = NS - 2 - (TN == 1);
         auto run = [&](auto live) FP8_INLINE {
             constexpr bool LIVE = decltype(live)::value;
@@ -1159,8 +1162,8 @@ static hipError_t launch_tile_d(const Fp8Args &a, hipStream_t st) {
 template <bool GATED>
 static hipError_t launch_tile(const Fp8Args &a, hipStream_t st) {
     if constexpr (GATED) {
-        // 64 rows of x a tile up to 128 of an expert, then 128 (experts of 768 of 2,048, the layer: 12 rows 159 us and 176, 64 235 and 249,
-        // 128 330 and 334, 256 555 and 538; of down 128 rows always: 12 rows 157 us with 64, 159; 64 235 and 236; 128 352 and 333)
+        // 64 rows of x a tile up to 128 of an expert, then 128 (experts of 768 of 2,048, the layer: 12 rows 165 us and 183, 64 239 and 253,
+        // 128 341 and 343, 256 573 and 556; of down 128 rows always: 12 rows 160 us with 64, 165; 64 238 and 239; 128 358 and 341)
         if (a.M <= 128ll * a.E) return launch_tile_d<true, 3, 1, 4, 2, 4, 2>(a, st);
         return launch_tile_d<true, 3, 1, 4, 2, 4, 4>(a, st);
     } else {
