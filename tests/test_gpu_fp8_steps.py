@@ -51,7 +51,7 @@ def test_product_of_256_x_128(K, dt):
 
 # 70 x 300: 32 x 64 tiles, K shared by two groups of waves, from 32 blocks on by four
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("K", [*DEPTHS, 128, 256, 272, 1664, 3200, 3968, 4000, 4080, 4096, 4112, 4224, 4240, 4352, 4608, 6400, 6528, 8000, 4100, 7000])
+@pytest.mark.parametrize("K", [*DEPTHS, 1, 16, 48, 100, 127, 128, 130, 144, 256, 272, 1664, 3200, 3968, 4000, 4080, 4096, 4112, 4224, 4240, 4352, 4608, 6400, 6528, 8000, 4100, 7000])
 def test_product_with_k_shared(K, dt):
     check_exact(70, 300, K, dt)
 
